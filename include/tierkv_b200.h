@@ -97,6 +97,8 @@ extern "C" {
 /* Device-side error bits, reported through tkv_read_device_errors(). */
 #define TKV_DEVERR_BAD_SLOT  0x1u  /* HOT/WARM block whose slot is outside its pool */
 #define TKV_DEVERR_TIMEOUT   0x2u  /* a bounded pipeline wait gave up            */
+#define TKV_DEVERR_NO_BLOCKS 0x4u  /* a planned request found no free block or no table room */
+#define TKV_DEVERR_BAD_POS   0x8u  /* rotary position outside the cos / sin table (clamped) */
 
 /* tkv_decode_args.flags: blocks per work chunk (0 = chosen by the planner) */
 #define TKV_FLAG_CHUNK_MASK  0xff
@@ -370,6 +372,178 @@ int32_t tkv_noalloc_prepare(int32_t device);
  * counterpart of tkv_read_device_errors for a caller workspace).
  * Synchronizes the stream.  No counterpart in the reference. */
 int32_t tkv_noalloc_read_device_errors(uint32_t* bits_out, void* stream);
+
+/* ---- serving steps over an 8-bit paged cache -------------------------------
+ * No counterpart in the reference: its 8-bit blocks are filled by demotion and
+ * read by one query token.  Here a layer's whole cache is 8-bit (Format S
+ * codes, or e4m3) with one fp32 scale per (block, kv head) and tensor, and a
+ * batch of requests of any query lengths is planned, rotated, written and
+ * attended in one launch each:
+ *
+ *   tkv_kv8_plan_step  block tables, slot maps and write lists from lengths
+ *   tkv_rotary         rotary positions with up to four axes
+ *   tkv_kv8_append     (rotary and) quantized write into the cache
+ *   tkv_kv8_attention  causal attention of the new tokens over the cache
+ *
+ * `error_word` of each call is a device word that collects TKV_DEVERR_* bits
+ * (the first word of a decode workspace, so tkv_read_device_errors reads it).
+ */
+#define TKV_KV8_INT8  0  /* int8 codes, |code| <= 127: Format S's WARM layout */
+#define TKV_KV8_E4M3  1  /* 8-bit floats, 4 exponent and 3 mantissa bits, |code| <= 448 */
+
+#define TKV_KV8_MAX_REQUESTS 8192
+
+/* One layer's cache; value = code * scale[block, kv head]. */
+typedef struct tkv_kv8_cache {
+    void*   k_codes;      /* [blocks, kv_heads, block_size, head_dim], 16-byte aligned */
+    void*   v_codes;
+    float*  k_scale;      /* [blocks, kv_heads] */
+    float*  v_scale;
+    int64_t blocks;       /* blocks * kv_heads * block_size < 2^31 */
+    int32_t kv_heads;
+    int32_t block_size;   /* 16, 32 or 64 */
+    int32_t head_dim;     /* 64 or 128 */
+    int32_t format;       /* TKV_KV8_INT8 / TKV_KV8_E4M3 */
+} tkv_kv8_cache;
+
+/* One step of `requests` requests whose new tokens are packed one request
+ * after the other.  Request i holds context_lens[i] tokens and gets
+ * new_lens[i] more (negative lengths count as 0).  need(i) = ceil((context +
+ * new) / block_size) - ceil(context / block_size) blocks are taken from the
+ * end of the free list in request order: with C the running sum of need, new
+ * block j of request i is free_blocks[free_count - 1 - (C(i-1) + j)].  A
+ * request is admitted when its row has room for all its blocks and need(i) is
+ * 0 or C(i) <= free_count; a row without room counts need 0.  A request that
+ * is not admitted keeps its context, its tokens get slot -1, and the launch
+ * records TKV_DEVERR_NO_BLOCKS.  Nothing is written to table cells other than
+ * those of the new blocks.
+ * Inputs may alias the outputs of the same meaning (context_lens / kv_lens,
+ * free_count / free_count_out). */
+typedef struct tkv_kv8_plan_args {
+    const int32_t* context_lens;   /* [requests] */
+    const int32_t* new_lens;       /* [requests] */
+    int32_t*       block_table;    /* [requests, table_stride], in and out */
+    int64_t        table_stride;
+    const int32_t* free_blocks;    /* [free_capacity] */
+    const int32_t* free_count;     /* [1] entries of free_blocks that are free */
+    int32_t*       kv_lens;        /* [requests] tokens after the step */
+    int32_t*       cu_q;           /* [requests + 1] first packed token of each request */
+    int32_t*       admitted;       /* [requests] 1 / 0 */
+    int32_t*       slot_map;       /* [tokens] block * block_size + offset, -1 = none */
+    int32_t*       token_request;  /* [tokens] request, -1 past the last token */
+    int32_t*       positions;      /* [tokens] position in the request, -1 past the last token */
+    int32_t*       units;          /* [units_cap][4] (block, first packed token, row offset,
+                                      rows): the blocks that the step writes; -1 past the last */
+    int32_t*       num_units;      /* [1] */
+    int32_t*       free_count_out; /* [1] */
+    uint32_t*      error_word;     /* optional */
+    int32_t        requests;       /* 1 .. TKV_KV8_MAX_REQUESTS */
+    int32_t        tokens;         /* capacity of the token outputs; tokens past it are dropped */
+    int32_t        units_cap;      /* min(tokens, tokens / block_size + 2 * requests) suffices */
+    int32_t        table_width;    /* cells of a row that may be used */
+    int32_t        free_capacity;
+    int32_t        block_size;     /* 16, 32 or 64 */
+} tkv_kv8_plan_args;
+
+int32_t tkv_kv8_plan_step(const tkv_kv8_plan_args* args, void* stream);
+
+/* Rotary positions.  Frequency f (of rot_dim / 2) turns the pair (x1, x2) of
+ * every head by (c, s) = (cos_sin[p, f], cos_sin[p, rot_dim / 2 + f]) with p
+ * the token's position on the frequency's axis: y1 = x1 c - x2 s, y2 = x2 c +
+ * x1 s, in fp32 with every product and sum rounded, then rounded once to the
+ * tensor's type.  The pair is (x[f], x[f + rot_dim / 2]), or (x[2 f], x[2 f +
+ * 1]) with `pairs`.  Axes: sections[a] frequencies belong to axis a, one run
+ * after the other, or with `interleave` f belongs to axis f % axes while f /
+ * axes < sections[f % axes] and to axis 0 otherwise.  Elements past rot_dim
+ * pass through.  Positions outside [0, rows) are clamped and recorded
+ * (TKV_DEVERR_BAD_POS). */
+typedef struct tkv_rotary {
+    const float* cos_sin;          /* [rows, rot_dim], 16-byte aligned */
+    const void*  positions;        /* [axes, tokens] int32 or int64 */
+    int64_t      rows;
+    int64_t      axis_stride;      /* elements between the axes' rows */
+    int32_t      positions_bytes;  /* 4 or 8 */
+    int32_t      rot_dim;          /* multiple of 16, <= head_dim */
+    int32_t      axes;             /* 1 .. 4 */
+    int32_t      sections[4];      /* sum = rot_dim / 2 */
+    int32_t      interleave;
+    int32_t      pairs;
+} tkv_rotary;
+
+/* A [tokens, heads, head_dim] view: strides in elements, multiples of 8; the
+ * base 16-byte aligned; head_dim contiguous. */
+typedef struct tkv_token_view {
+    const void* data;
+    int64_t     token_stride;
+    int64_t     head_stride;
+} tkv_token_view;
+
+/* Rotates q (heads) and k (kv_heads) of `tokens` tokens into q_out / k_out;
+ * either may be absent (heads or kv_heads 0), and an output may be its input.
+ * head_dim: a multiple of 16 up to 256.  dtype: TKV_DTYPE_F16 / BF16. */
+int32_t tkv_rotary_embed(const tkv_rotary* rotary, const tkv_token_view* q, const tkv_token_view* k,
+                         const tkv_token_view* q_out, const tkv_token_view* k_out, int32_t tokens,
+                         int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype,
+                         uint32_t* error_word, void* stream);
+
+/* Writes the rows of k / v ([tokens, kv_heads, head_dim]) that `units` names
+ * into the cache and, with `rotary`, rotates k on the way (in fp32, not
+ * rounded in between) and q into q_out.  Unit (block, first, offset, rows):
+ * rows [offset, offset + rows) of the block get tokens [first, first + rows).
+ * Per kv head and tensor: s_new = max |x| / qmax (127 or 448) over the new
+ * rows; with offset 0 the scale is s_new, else max(old scale, s_new), and when
+ * that is larger than the old scale the codes of rows [0, offset) become
+ * round(code * (old / new)).  Codes are round(x / scale), to the nearest, ties
+ * to even, clamped; a scale of 0 becomes 1.  A block whose new rows or whose
+ * old scale hold a NaN or an infinity gets scale NaN and, in those rows, code
+ * 0.  Rows past offset + rows are left alone.  No two units may name one
+ * block; a unit outside the cache, the block or the tokens is skipped and
+ * recorded (TKV_DEVERR_BAD_SLOT). */
+typedef struct tkv_kv8_append_args {
+    tkv_token_view k, v, q, q_out;  /* q: heads 0 = none */
+    const int32_t* units;           /* [units_cap][4] */
+    const int32_t* num_units;       /* [1] device */
+    const tkv_rotary* rotary;       /* optional; NULL: k as is, no q */
+    uint32_t*      error_word;      /* optional */
+    int32_t        units_cap;
+    int32_t        tokens;
+    int32_t        heads;
+    int32_t        dtype;           /* of k, v, q: TKV_DTYPE_F16 / BF16 */
+} tkv_kv8_append_args;
+
+int32_t tkv_kv8_append(const tkv_kv8_cache* cache, const tkv_kv8_append_args* args, void* stream);
+
+/* Attention of a packed batch over the cache.  Query token t of request i
+ * (cu_q[i] <= t < cu_q[i + 1]) sits at position kv_lens[i] - (cu_q[i + 1] - t)
+ * and sees keys j <= position, with a window only those j > position - window.
+ * out = sum_j p_j v_j, p the softmax of (q . k_j) * scaling; a token that sees
+ * no key gets 0 and LSE -inf.  Table cells outside the cache read as zeros and
+ * are recorded (TKV_DEVERR_BAD_SLOT); kv_lens are clamped to the table.
+ * Tokens outside [cu_q[0], cu_q[requests]) are not written. */
+typedef struct tkv_kv8_attention_args {
+    tkv_token_view q;               /* [tokens, heads, head_dim] */
+    void*          out;             /* [tokens, heads, head_dim], q's dtype, contiguous */
+    float*         out_lse;         /* optional [tokens, heads] natural log */
+    const int32_t* block_table;     /* [requests, table_stride] */
+    int64_t        table_stride;
+    const int32_t* kv_lens;         /* [requests] */
+    const int32_t* cu_q;            /* [requests + 1], not decreasing */
+    int32_t        requests;        /* 1 .. TKV_KV8_MAX_REQUESTS */
+    int32_t        tokens;
+    int32_t        heads;           /* a multiple of the cache's kv_heads, up to 64 each */
+    int32_t        dtype;           /* TKV_DTYPE_F16 / BF16 */
+    int32_t        table_width;     /* cells of a row */
+    int32_t        max_q_len;       /* upper bound of the requests' query tokens */
+    int32_t        window;          /* 0 = none */
+    float          scaling;         /* finite, > 0 */
+    void*          workspace;       /* as tkv_decode_args.workspace */
+    size_t         workspace_bytes;
+} tkv_kv8_attention_args;
+
+int32_t tkv_kv8_attention_workspace(const tkv_kv8_cache* cache, const tkv_kv8_attention_args* args,
+                                    size_t* workspace_bytes_out);
+int32_t tkv_kv8_attention(const tkv_kv8_cache* cache, const tkv_kv8_attention_args* args,
+                          void* stream);
 
 #ifdef __cplusplus
 }

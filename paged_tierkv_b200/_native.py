@@ -29,6 +29,12 @@ TKV_DTYPE_F32 = 2
 
 TKV_DEVERR_BAD_SLOT = 0x1
 TKV_DEVERR_TIMEOUT = 0x2
+TKV_DEVERR_NO_BLOCKS = 0x4
+TKV_DEVERR_BAD_POS = 0x8
+
+TKV_KV8_INT8 = 0
+TKV_KV8_E4M3 = 1
+TKV_KV8_MAX_REQUESTS = 8192
 
 EXPORTED_SYMBOLS = (
     "tkv_get_version",
@@ -55,6 +61,11 @@ EXPORTED_SYMBOLS = (
     "tkv_prefill_block_scores",
     "tkv_prefill_read_errors",
     "tkv_store_prefill_blocks",
+    "tkv_kv8_plan_step",
+    "tkv_rotary_embed",
+    "tkv_kv8_append",
+    "tkv_kv8_attention_workspace",
+    "tkv_kv8_attention",
 )
 
 TKV_EXCHANGE_MAX_RANKS = 8
@@ -131,6 +142,109 @@ class TkvExchange(ctypes.Structure):
     ]
 
 
+class TkvKv8Cache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("blocks", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("format", ctypes.c_int32),
+    ]
+
+
+class TkvKv8PlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("context_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("free_blocks", ctypes.c_void_p),
+        ("free_count", ctypes.c_void_p),
+        ("kv_lens", ctypes.c_void_p),
+        ("cu_q", ctypes.c_void_p),
+        ("admitted", ctypes.c_void_p),
+        ("slot_map", ctypes.c_void_p),
+        ("token_request", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("units", ctypes.c_void_p),
+        ("num_units", ctypes.c_void_p),
+        ("free_count_out", ctypes.c_void_p),
+        ("error_word", ctypes.c_void_p),
+        ("requests", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("units_cap", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
+        ("free_capacity", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+    ]
+
+
+class TkvRotary(ctypes.Structure):
+    _fields_ = [
+        ("cos_sin", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("axis_stride", ctypes.c_int64),
+        ("positions_bytes", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 4),
+        ("interleave", ctypes.c_int32),
+        ("pairs", ctypes.c_int32),
+    ]
+
+
+class TkvTokenView(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class TkvKv8AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("k", TkvTokenView),
+        ("v", TkvTokenView),
+        ("q", TkvTokenView),
+        ("q_out", TkvTokenView),
+        ("units", ctypes.c_void_p),
+        ("num_units", ctypes.c_void_p),
+        ("rotary", ctypes.POINTER(TkvRotary)),
+        ("error_word", ctypes.c_void_p),
+        ("units_cap", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class TkvKv8AttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", TkvTokenView),
+        ("out", ctypes.c_void_p),
+        ("out_lse", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("kv_lens", ctypes.c_void_p),
+        ("cu_q", ctypes.c_void_p),
+        ("requests", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
+        ("max_q_len", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scaling", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 _LIB = None
 
 
@@ -184,6 +298,13 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
                                       i32, vp, vp, vp], i32),
         "tkv_prefill_read_errors": ([ctypes.POINTER(ctypes.c_uint32), vp], i32),
         "tkv_store_prefill_blocks": ([ctypes.POINTER(TkvPools), vp, vp, i32, vp, i32, vp], i32),
+        "tkv_kv8_plan_step": ([ctypes.POINTER(TkvKv8PlanArgs), vp], i32),
+        "tkv_rotary_embed": ([ctypes.POINTER(TkvRotary)] + [ctypes.POINTER(TkvTokenView)] * 4
+                             + [i32] * 5 + [vp, vp], i32),
+        "tkv_kv8_append": ([ctypes.POINTER(TkvKv8Cache), ctypes.POINTER(TkvKv8AppendArgs), vp], i32),
+        "tkv_kv8_attention_workspace": ([ctypes.POINTER(TkvKv8Cache), ctypes.POINTER(TkvKv8AttentionArgs),
+                                         ctypes.POINTER(ctypes.c_size_t)], i32),
+        "tkv_kv8_attention": ([ctypes.POINTER(TkvKv8Cache), ctypes.POINTER(TkvKv8AttentionArgs), vp], i32),
     }
     for name, (argtypes, restype) in sigs.items():
         fn = getattr(lib, name)

@@ -19,7 +19,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIBNAME = "libtierkv_b200.so"
-SOURCES = ["tkv_api.cu", "tkv_decode.cu", "tkv_quant.cu", "tkv_prefill.cu"]
+SOURCES = ["tkv_api.cu", "tkv_decode.cu", "tkv_quant.cu", "tkv_prefill.cu", "tkv_kv8.cu",
+           "tkv_kv8_attn.cu", "tkv_kv8_api.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -57,14 +58,17 @@ def build(verbose_ptxas: bool = False, force: bool = False, defines: tuple[str, 
     if verbose_ptxas:
         common += ["-Xptxas", "-v"]
     common += [f"-D{d}" for d in defines]
-    objs = []
+    objs, running = [], []
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(objdir, src.replace(".cu", ".o"))
         objs.append(o)
         if force or verbose_ptxas or _stale(o, [s] + headers):
             cmd = [nvcc, *common, "-c", s, "-o", o]
-            subprocess.run(cmd, check=True)
+            running.append((cmd, subprocess.Popen(cmd)))
+    for code, cmd in [(proc.wait(), cmd) for cmd, proc in running]:  # they compile side by side
+        if code != 0:
+            raise subprocess.CalledProcessError(code, cmd)
     out = out or lib_path()
     if force or _stale(out, objs):
         tmp = out + ".tmp"

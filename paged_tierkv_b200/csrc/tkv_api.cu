@@ -301,6 +301,10 @@ bool tkv::encode_head_rows_map(CUtensorMap* map, const void* base, int64_t heads
   return r == CUDA_SUCCESS;
 }
 
+bool tkv::encode_code_map(CUtensorMap* map, const void* base, int64_t rows, int head_dim, int box_rows) {
+  return encode_pool_map(map, const_cast<void*>(base), false, rows, head_dim, head_dim, box_rows);
+}
+
 extern "C" {
 
 int32_t tkv_get_version(void) { return TKV_ABI_VERSION; }

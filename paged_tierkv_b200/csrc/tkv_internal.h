@@ -216,6 +216,10 @@ cudaError_t prefill_error_word(uint32_t** out);
 bool encode_head_rows_map(CUtensorMap* map, const void* base, int64_t heads, int64_t rows,
                           int head_dim);
 
+// 2-D tiled map over rows of head_dim bytes (8-bit codes), box_rows rows a box,
+// 128- or 64-byte swizzle.
+bool encode_code_map(CUtensorMap* map, const void* base, int64_t rows, int head_dim, int box_rows);
+
 cudaError_t launch_demote(const DemoteParams& p, int format, cudaStream_t stream);
 cudaError_t launch_append(const AppendParams& p, cudaStream_t stream);
 

@@ -1,0 +1,615 @@
+// tkv_kv8.cu -- step planning, rotary positions and the quantizing append of
+// the 8-bit paged cache (tkv_kv8_* in include/tierkv_b200.h).
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "tierkv_b200.h"
+#include "tkv_kv8.h"
+
+namespace cg = cooperative_groups;
+
+namespace tkv {
+
+// ---------------------------------------------------------------- step planning
+//
+// need(i) = ceil((c + n) / bs) - ceil(c / bs) new blocks, C their running sum;
+// the k-th block of the step is the k-th from the end of the free list.  One
+// cluster plans the step: every CTA scans the requests' lengths into shared
+// memory (an 8-byte load per request, so repeating it per CTA costs nothing
+// next to a second launch), then the cluster's threads share the tokens, table
+// cells and write units and find each one's request by bisection of the
+// scanned sums.  A cluster barrier between the last read of an input and the
+// first write lets kv_lens / free_count be updated in place.  Latency bound:
+// a launch, one round of loads, two block scans.
+constexpr int kPlanCluster = 8;
+constexpr int kPlanThreads = 1024;
+
+struct Scan {
+  int32_t warp_sum[2][32];
+  int32_t carry[2];
+};
+
+// Exclusive sums over the CTA's threads of (a, b); every thread also gets the totals.
+__device__ __forceinline__ void scan2(Scan& s, int32_t a, int32_t b, int32_t& ea, int32_t& eb,
+                                      int32_t& ta, int32_t& tb) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int32_t ia = a, ib = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int32_t xa = __shfl_up_sync(~0u, ia, o), xb = __shfl_up_sync(~0u, ib, o);
+    if (lane >= o) {
+      ia += xa;
+      ib += xb;
+    }
+  }
+  __syncthreads();  // the previous scan's readers are done
+  if (lane == 31) {
+    s.warp_sum[0][warp] = ia;
+    s.warp_sum[1][warp] = ib;
+  }
+  __syncthreads();
+  int32_t wa = s.warp_sum[0][lane], wb = s.warp_sum[1][lane];  // kPlanThreads / 32 == 32 warps
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int32_t xa = __shfl_up_sync(~0u, wa, o), xb = __shfl_up_sync(~0u, wb, o);
+    if (lane >= o) {
+      wa += xa;
+      wb += xb;
+    }
+  }
+  ta = __shfl_sync(~0u, wa, 31);
+  tb = __shfl_sync(~0u, wb, 31);
+  const int32_t before_a = __shfl_sync(~0u, wa, warp ? warp - 1 : 0);
+  const int32_t before_b = __shfl_sync(~0u, wb, warp ? warp - 1 : 0);
+  ea = (warp ? before_a : 0) + ia - a;
+  eb = (warp ? before_b : 0) + ib - b;
+}
+
+// Largest i with first[i] <= x, for a non-decreasing first[0 .. n] with first[0] = 0 <= x < first[n].
+__device__ __forceinline__ int find(const int32_t* first, int n, int32_t x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int32_t ceil_div(int32_t x, int bs) {
+  return (int32_t)(((int64_t)x + bs - 1) / bs);
+}
+
+__global__ void __launch_bounds__(kPlanThreads, 1)
+    plan_step_kernel(const tkv_kv8_plan_args p) {
+  extern __shared__ int32_t plan_smem[];
+  __shared__ Scan scan;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int n = p.requests, bs = p.block_size, tid = threadIdx.x;
+  int32_t* ctx = plan_smem;            // [n]      cached tokens, bit 31: not admitted
+  int32_t* cu = ctx + n;               // [n + 1]  first packed token
+  int32_t* need = cu + n + 1;          // [n + 1]  running sum of new blocks
+  int32_t* cu_unit = need + n + 1;     // [n + 1]  first write unit
+  const int32_t free_count = max(0, min(*p.free_count, p.free_capacity));
+
+  // lengths -> running sums of the new tokens and the new blocks; a thread
+  // owns n / 1024 consecutive requests
+  const int per = (n + kPlanThreads - 1) / kPlanThreads;
+  const int r0 = min(n, tid * per), r1 = min(n, r0 + per);
+  int32_t sum_new = 0, sum_need = 0;
+  for (int i = r0; i < r1; ++i) {
+    const int32_t c = max(0, p.context_lens[i]), m = max(0, p.new_lens[i]);
+    const int32_t want = ceil_div(c + m, bs);
+    ctx[i] = c;
+    cu[i] = m;
+    need[i] = want <= p.table_width ? want - ceil_div(c, bs) : -1;
+    sum_new += m;
+    sum_need += max(0, need[i]);
+  }
+  int32_t at_new, at_need, total_new, total_need;
+  scan2(scan, sum_new, sum_need, at_new, at_need, total_new, total_need);
+  int32_t sum_units = 0, taken = 0;
+  bool refused = false;
+  for (int i = r0; i < r1; ++i) {
+    const int32_t m = cu[i], k = need[i], c = ctx[i];
+    const bool ok = k >= 0 && (k == 0 || at_need + k <= free_count);
+    if (!ok) ctx[i] = c | (int32_t)0x80000000;
+    if (!ok && m > 0) refused = true;
+    cu[i] = at_new;
+    need[i] = at_need;
+    cu_unit[i] = ok && m > 0 ? ceil_div(c + m, bs) - c / bs : 0;
+    sum_units += cu_unit[i];
+    at_new += m;
+    at_need += max(0, k);
+    if (ok) taken += k;
+  }
+  int32_t at_unit, at_taken, total_units, total_taken;
+  scan2(scan, sum_units, taken, at_unit, at_taken, total_units, total_taken);
+  for (int i = r0; i < r1; ++i) {
+    const int32_t u = cu_unit[i];
+    cu_unit[i] = at_unit;
+    at_unit += u;
+  }
+  if (tid == 0) {
+    cu[n] = total_new;
+    need[n] = total_need;
+    cu_unit[n] = total_units;
+  }
+  cluster.sync();  // every CTA has read its inputs; shared memory is complete
+
+  const int rank = (int)cluster.block_rank();
+  const int gtid = rank * kPlanThreads + tid;
+  constexpr int kStride = kPlanCluster * kPlanThreads;
+  if (rank == 0) {
+    for (int i = r0; i < r1; ++i) {
+      const int32_t c = ctx[i] & 0x7fffffff;
+      p.kv_lens[i] = ctx[i] >= 0 ? c + (cu[i + 1] - cu[i]) : c;
+      p.cu_q[i] = cu[i];
+      p.admitted[i] = ctx[i] >= 0;
+    }
+    if (tid == 0) {
+      p.cu_q[n] = total_new;
+      *p.num_units = min(total_units, p.units_cap);
+      *p.free_count_out = free_count - total_taken;
+    }
+    if (refused && p.error_word) atomicOr(p.error_word, TKV_DEVERR_NO_BLOCKS);
+  }
+
+  // new table cells
+  for (int u = gtid; u < total_need; u += kStride) {
+    const int i = find(need, n, u);
+    if (ctx[i] < 0) continue;
+    p.block_table[i * p.table_stride + ceil_div(ctx[i], bs) + (u - need[i])] =
+        p.free_blocks[free_count - 1 - u];
+  }
+  // block of request i's cell j: one this step takes, or one it already held
+  auto block_of = [&](int i, int32_t c, int32_t j) -> int32_t {
+    const int32_t held = ceil_div(c, bs);
+    return j >= held ? p.free_blocks[free_count - 1 - (need[i] + j - held)]
+                     : p.block_table[i * p.table_stride + j];
+  };
+  // write units
+  for (int u = gtid; u < p.units_cap; u += kStride) {
+    int4 out = make_int4(-1, -1, -1, -1);
+    if (u < total_units) {
+      const int i = find(cu_unit, n, u);
+      const int32_t c = ctx[i], end = c + (cu[i + 1] - cu[i]);
+      const int32_t j = c / bs + (u - cu_unit[i]);
+      const int32_t lo = max(c, j * bs), hi = min(end, (j + 1) * bs);
+      out = make_int4(block_of(i, c, j), cu[i] + (lo - c), lo - j * bs, hi - lo);
+    }
+    reinterpret_cast<int4*>(p.units)[u] = out;
+  }
+  // tokens
+  for (int t = gtid; t < p.tokens; t += kStride) {
+    int32_t slot = -1, req = -1, pos = -1;
+    if (t < total_new) {
+      req = find(cu, n, t);
+      const int32_t c = ctx[req];
+      pos = (c & 0x7fffffff) + (t - cu[req]);
+      if (c >= 0) slot = block_of(req, c, pos / bs) * bs + pos % bs;
+    }
+    p.slot_map[t] = slot;
+    p.token_request[t] = req;
+    p.positions[t] = pos;
+  }
+}
+
+cudaError_t launch_plan_step(const tkv_kv8_plan_args& p, cudaStream_t stream) {
+  const size_t smem = sizeof(int32_t) * (4 * (size_t)p.requests + 3);
+  if (smem > 40 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(plan_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)(sizeof(int32_t) * (4 * TKV_KV8_MAX_REQUESTS + 3)));
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kPlanCluster);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = kPlanCluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, plan_step_kernel, p);
+}
+
+// ---------------------------------------------------------------- element types
+template <typename T>
+struct Pack;  // 8 elements in 16 bytes
+template <>
+struct Pack<__half> {
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+    uint4 v;
+    __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    return v;
+  }
+};
+template <>
+struct Pack<__nv_bfloat16> {
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+    uint4 v;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    return v;
+  }
+};
+
+// ---------------------------------------------------------------- rotation
+// A rotation item is 16 elements of one head: 8 frequencies f0 .. f0 + 7 and
+// both elements of their pairs, held as x[0..7] (x1) and x[8..15] (x2).  Items
+// past rot_dim / 16 are 16 consecutive elements that pass through.
+struct ItemPlace {
+  int lo, hi;  // element offsets of the item's two 16-byte halves
+  int f0;      // first frequency, -1: passes through
+};
+__device__ __forceinline__ ItemPlace item_place(const RotaryArgs& r, int item) {
+  ItemPlace w;
+  if (item < r.rot_dim / 16) {
+    w.f0 = item * 8;
+    w.lo = r.pairs ? item * 16 : item * 8;
+    w.hi = r.pairs ? item * 16 + 8 : r.rot_dim / 2 + item * 8;
+  } else {
+    w.f0 = -1;
+    w.lo = item * 16;
+    w.hi = w.lo + 8;
+  }
+  return w;
+}
+
+// Axis of frequency f.
+__device__ __forceinline__ int freq_axis(const RotaryArgs& r, int f) {
+  if (r.axes == 1) return 0;
+  if (r.interleave) {
+    const int a = f % r.axes;
+    return f / r.axes < r.sections[a] ? a : 0;
+  }
+  int a = 0, end = r.sections[0];
+  while (f >= end && a + 1 < r.axes) end += r.sections[++a];
+  return a;
+}
+
+__device__ __forceinline__ int64_t load_position(const RotaryArgs& r, int axis, int64_t token,
+                                                 uint32_t* err) {
+  const int64_t at = axis * r.axis_stride + token;
+  const int64_t p = r.positions_bytes == 8 ? reinterpret_cast<const int64_t*>(r.positions)[at]
+                                           : (int64_t)reinterpret_cast<const int32_t*>(r.positions)[at];
+  if (p >= 0 && p < r.rows) return p;
+  if (err) atomicOr(err, TKV_DEVERR_BAD_POS);
+  return p < 0 ? 0 : r.rows - 1;
+}
+
+// y1 = x1 c - x2 s, y2 = x2 c + x1 s; every product and sum rounded by itself,
+// so that codes quantized from the result equal an unfused pipeline's.
+__device__ __forceinline__ void turn(float& x1, float& x2, float c, float s) {
+  const float y1 = __fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s));
+  x2 = __fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s));
+  x1 = y1;
+}
+
+// The pair order of `pairs` (x1, x2 adjacent) <-> the split order (all x1, all x2).
+__device__ __forceinline__ void split_pairs(float (&x)[16]) {
+  float y[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    y[i] = x[2 * i];
+    y[8 + i] = x[2 * i + 1];
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = y[i];
+}
+__device__ __forceinline__ void join_pairs(float (&x)[16]) {
+  float y[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    y[2 * i] = x[i];
+    y[2 * i + 1] = x[8 + i];
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = y[i];
+}
+
+template <typename T>
+__device__ __forceinline__ void load_item(const T* row, const ItemPlace& w, float (&x)[16]) {
+  float a[8], b[8];
+  Pack<T>::unpack(*reinterpret_cast<const uint4*>(row + w.lo), a);
+  Pack<T>::unpack(*reinterpret_cast<const uint4*>(row + w.hi), b);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = a[i];
+    x[8 + i] = b[i];
+  }
+}
+
+// One CTA rotates every head of one token: (c, s) of its rot_dim / 2
+// frequencies go to shared memory once (the table row is 4 rot_dim bytes
+// against 2 head_dim bytes of each head), then the threads share the (head,
+// item) pairs.  Bound by HBM: every element is read once and written once.
+constexpr int kRotThreads = 128;
+constexpr int kMaxRotDim = 256;
+
+template <typename T>
+__device__ __forceinline__ void rotate_token(const RotaryArgs& r, int64_t token, const T* q, const T* k,
+                                             T* qo, T* ko, int64_t qs, int64_t ks, int64_t qos,
+                                             int64_t kos, int heads, int kv_heads, int head_dim,
+                                             float* cs, uint32_t* err) {
+  const int half = r.rot_dim / 2;
+  for (int f = threadIdx.x; f < half; f += kRotThreads) {
+    const int64_t p = load_position(r, freq_axis(r, f), token, err);
+    cs[f] = r.cos_sin[p * r.rot_dim + f];
+    cs[half + f] = r.cos_sin[p * r.rot_dim + half + f];
+  }
+  __syncthreads();
+  const int per = head_dim / 16;
+  const int total = (heads + kv_heads) * per;
+  for (int i = threadIdx.x; i < total; i += kRotThreads) {
+    const int h = i / per;
+    const ItemPlace w = item_place(r, i - h * per);
+    const T* src = h < heads ? q + h * qs : k + (h - heads) * ks;
+    T* dst = h < heads ? qo + h * qos : ko + (h - heads) * kos;
+    float x[16];
+    load_item<T>(src, w, x);
+    if (w.f0 >= 0) {
+      if (r.pairs) split_pairs(x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) turn(x[j], x[8 + j], cs[w.f0 + j], cs[half + w.f0 + j]);
+      if (r.pairs) join_pairs(x);
+    }
+    float a[8], b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      a[j] = x[j];
+      b[j] = x[8 + j];
+    }
+    *reinterpret_cast<uint4*>(dst + w.lo) = Pack<T>::pack(a);
+    *reinterpret_cast<uint4*>(dst + w.hi) = Pack<T>::pack(b);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  __shared__ float cs[kMaxRotDim];
+  const int64_t t = blockIdx.x;
+  rotate_token<T>(p.rot, t, (const T*)p.q.data + t * p.q.token_stride,
+                  (const T*)p.k.data + t * p.k.token_stride,
+                  (T*)const_cast<void*>(p.q_out.data) + t * p.q_out.token_stride,
+                  (T*)const_cast<void*>(p.k_out.data) + t * p.k_out.token_stride, p.q.head_stride,
+                  p.k.head_stride, p.q_out.head_stride, p.k_out.head_stride, p.heads, p.kv_heads,
+                  p.head_dim, cs, p.err);
+}
+
+cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream) {
+  if (p.tokens == 0 || p.heads + p.kv_heads == 0) return cudaSuccess;
+  if (dtype == kDtF16) rotary_kernel<__half><<<p.tokens, kRotThreads, 0, stream>>>(p);
+  else rotary_kernel<__nv_bfloat16><<<p.tokens, kRotThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+// ---------------------------------------------------------------- append
+// Quantization to a code byte, to the nearest (ties to even), saturating.
+template <int FMT>
+__device__ __forceinline__ uint32_t encode(float x) {
+  if (FMT == TKV_KV8_INT8) {
+    const float q = fminf(fmaxf(rintf(x), -127.f), 127.f);
+    return (uint32_t)(int32_t)q & 0xffu;
+  }
+  return (uint32_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+}
+template <int FMT>
+__device__ __forceinline__ float decode(uint32_t b) {
+  if (FMT == TKV_KV8_INT8) return (float)(int8_t)b;
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
+}
+template <int FMT>
+constexpr float kQMax = FMT == TKV_KV8_INT8 ? 127.f : 448.f;
+
+template <int FMT>
+__device__ __forceinline__ uint2 encode8(const float* x, float s) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i >> 2] |= encode<FMT>(__fdiv_rn(x[i], s)) << (8 * (i & 3));
+  return make_uint2(w[0], w[1]);
+}
+
+// A tile is one (write unit, K or V, kv head): BS rows of D codes and one
+// scale, owned by WPT warps.  Thread layout: D / 16 rotation items per row;
+// a warp covers 32 / (D / 16) rows at once and keeps its kItems items (16 fp32
+// each) in registers between the maximum and the quantization, so the new rows
+// are read once.  Old rows are touched only when the scale grows.
+template <int D, int BS>
+struct AppendShape {
+  static constexpr int kPerRow = D / 16;
+  static constexpr int kTileItems = BS * kPerRow;
+  static constexpr int kWarps = kTileItems / 32 >= 16 ? 4 : (kTileItems / 32 >= 8 ? 2 : 1);
+  static constexpr int kItems = kTileItems / (32 * kWarps);
+  static constexpr int kTiles = 4 / kWarps;  // per CTA of 128 threads
+};
+
+template <typename T, int D, int BS, int FMT>
+__global__ void __launch_bounds__(128) append_kernel8(const __grid_constant__ AppendParams8 p) {
+  using S = AppendShape<D, BS>;
+  __shared__ float cs[kMaxRotDim];
+  __shared__ float warp_max[4];
+  const int tiles_per_unit = 2 * p.kv_heads;
+  const int ctas_per_unit = (tiles_per_unit + S::kTiles - 1) / S::kTiles;
+  const int64_t unit_ctas = (int64_t)p.units_cap * ctas_per_unit;
+  if ((int64_t)blockIdx.x >= unit_ctas) {
+    // ---- the query's rotation, one token a CTA
+    const int64_t t = (int64_t)blockIdx.x - unit_ctas;
+    rotate_token<T>(p.rot, t, (const T*)p.q.data + t * p.q.token_stride, (const T*)nullptr,
+                    (T*)const_cast<void*>(p.q_out.data) + t * p.q_out.token_stride, (T*)nullptr,
+                    p.q.head_stride, 0, p.q_out.head_stride, 0, p.heads, 0, D, cs, p.err);
+    return;
+  }
+  const int u = (int)(blockIdx.x / ctas_per_unit);
+  if (u >= min(*p.num_units, p.units_cap)) return;
+  const int4 unit = reinterpret_cast<const int4*>(p.units)[u];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = warp / S::kWarps;             // tile of the CTA
+  const int part = warp % S::kWarps;            // warp of the tile
+  const int tile = (int)(blockIdx.x % ctas_per_unit) * S::kTiles + sub;
+  const int off = unit.z, rows = unit.w;
+  const bool good = unit.x >= 0 && unit.x < p.blocks && off >= 0 && rows >= 1 && rows <= BS - off &&
+                    unit.y >= 0 && unit.y <= p.tokens - rows;
+  if (!good) {  // the unit's CTAs agree
+    if (threadIdx.x == 0 && p.err) atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
+    return;
+  }
+  const bool live = tile < tiles_per_unit;
+  const bool is_v = tile >= p.kv_heads;
+  const int h = is_v ? tile - p.kv_heads : tile;
+  const int item = lane % S::kPerRow;
+  const int row0 = part * (S::kItems * 32 / S::kPerRow) + lane / S::kPerRow;
+  constexpr int kRowStep = 32 / S::kPerRow;
+  const bool rotate = !is_v && p.has_rot;
+  RotaryArgs plain = {};
+  const ItemPlace w = item_place(rotate ? p.rot : plain, item);
+  const tkv_token_view& view = is_v ? p.v : p.k;
+  const T* src = (const T*)view.data + h * view.head_stride;
+
+  float x[S::kItems][16];
+  float amax = 0.f;
+  bool odd = false;  // a NaN or an infinity among the new rows
+#pragma unroll
+  for (int i = 0; i < S::kItems; ++i) {
+    const int row = row0 + i * kRowStep;
+    if (live && row >= off && row < off + rows) {
+      const int64_t token = unit.y + (row - off);
+      load_item<T>(src + token * view.token_stride, w, x[i]);
+      if (rotate && w.f0 >= 0) {
+        const int half = p.rot.rot_dim / 2;
+        if (p.rot.pairs) split_pairs(x[i]);
+        if (p.rot.axes == 1) {
+          const float* c = p.rot.cos_sin + load_position(p.rot, 0, token, p.err) * p.rot.rot_dim + w.f0;
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            const float4 c4 = *reinterpret_cast<const float4*>(c + j);
+            const float4 s4 = *reinterpret_cast<const float4*>(c + half + j);
+            turn(x[i][j], x[i][8 + j], c4.x, s4.x);
+            turn(x[i][j + 1], x[i][9 + j], c4.y, s4.y);
+            turn(x[i][j + 2], x[i][10 + j], c4.z, s4.z);
+            turn(x[i][j + 3], x[i][11 + j], c4.w, s4.w);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int f = w.f0 + j;
+            const int64_t pos = load_position(p.rot, freq_axis(p.rot, f), token, p.err);
+            turn(x[i][j], x[i][8 + j], p.rot.cos_sin[pos * p.rot.rot_dim + f],
+                 p.rot.cos_sin[pos * p.rot.rot_dim + half + f]);
+          }
+        }
+        if (p.rot.pairs) join_pairs(x[i]);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        amax = fmaxf(amax, fabsf(x[i][j]));
+        odd |= !(fabsf(x[i][j]) <= 3.402823466e38f);
+      }
+    }
+  }
+  if (odd) amax = INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+  if (S::kWarps > 1) {
+    if (lane == 0) warp_max[warp] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S::kWarps; ++i) amax = fmaxf(amax, warp_max[sub * S::kWarps + i]);
+  }
+  if (!live) return;
+  float* scale = (is_v ? p.v_scale : p.k_scale) + (int64_t)unit.x * p.kv_heads + h;
+  const float s_old = off > 0 ? *scale : 0.f;
+  float s = fmaxf(__fdiv_rn(amax, kQMax<FMT>), s_old);
+  if (s == 0.f) s = 1.f;
+  const bool poisoned = !(amax < INFINITY) || !(s_old < INFINITY);
+  uint8_t* codes = (is_v ? p.v_codes : p.k_codes) + ((int64_t)unit.x * p.kv_heads + h) * (BS * D);
+  if (S::kWarps > 1) __syncthreads();  // every warp has read the old scale
+  if (part == 0 && lane == 0) *scale = poisoned ? __int_as_float(0x7fc00000) : s;
+  const float shrink = __fdiv_rn(s_old, s);
+#pragma unroll
+  for (int i = 0; i < S::kItems; ++i) {
+    const int row = row0 + i * kRowStep;
+    uint8_t* dst = codes + row * D;
+    if (row >= off && row < off + rows) {
+      uint2 a = make_uint2(0, 0), b = a;
+      if (!poisoned) {
+        a = encode8<FMT>(x[i], s);
+        b = encode8<FMT>(x[i] + 8, s);
+      }
+      *reinterpret_cast<uint2*>(dst + w.lo) = a;
+      *reinterpret_cast<uint2*>(dst + w.hi) = b;
+    } else if (row < off && s > s_old && !poisoned) {
+      uint4 v = *reinterpret_cast<const uint4*>(dst + item * 16);
+      uint32_t* c = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t y = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          y |= encode<FMT>(__fmul_rn(decode<FMT>((c[j] >> (8 * k)) & 0xffu), shrink)) << (8 * k);
+        c[j] = y;
+      }
+      *reinterpret_cast<uint4*>(dst + item * 16) = v;
+    }
+  }
+}
+
+template <typename T, int D, int BS, int FMT>
+static cudaError_t launch_append8(const AppendParams8& p, cudaStream_t stream) {
+  using S = AppendShape<D, BS>;
+  const int64_t ctas = (int64_t)p.units_cap * ((2 * p.kv_heads + S::kTiles - 1) / S::kTiles) +
+                       (p.heads > 0 ? p.tokens : 0);
+  if (ctas == 0) return cudaSuccess;
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
+  append_kernel8<T, D, BS, FMT><<<(unsigned)ctas, 128, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int FMT>
+static cudaError_t pick_append(const AppendParams8& p, int d, int bs, cudaStream_t stream) {
+  if (d == 128) {
+    if (bs == 16) return launch_append8<T, 128, 16, FMT>(p, stream);
+    if (bs == 32) return launch_append8<T, 128, 32, FMT>(p, stream);
+    return launch_append8<T, 128, 64, FMT>(p, stream);
+  }
+  if (bs == 16) return launch_append8<T, 64, 16, FMT>(p, stream);
+  if (bs == 32) return launch_append8<T, 64, 32, FMT>(p, stream);
+  return launch_append8<T, 64, 64, FMT>(p, stream);
+}
+
+cudaError_t launch_kv8_append(const AppendParams8& p, int d, int bs, int format, int dtype,
+                              cudaStream_t stream) {
+  if (dtype == kDtF16)
+    return format == TKV_KV8_INT8 ? pick_append<__half, TKV_KV8_INT8>(p, d, bs, stream)
+                                  : pick_append<__half, TKV_KV8_E4M3>(p, d, bs, stream);
+  return format == TKV_KV8_INT8 ? pick_append<__nv_bfloat16, TKV_KV8_INT8>(p, d, bs, stream)
+                                : pick_append<__nv_bfloat16, TKV_KV8_E4M3>(p, d, bs, stream);
+}
+
+}  // namespace tkv

@@ -1,0 +1,76 @@
+// tkv_kv8.h -- parameter blocks and launchers of the 8-bit paged cache's
+// kernels (not part of the public ABI).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "tierkv_b200.h"
+#include "tkv_internal.h"
+
+namespace tkv {
+
+using RotaryArgs = tkv_rotary;
+
+struct RotaryParams {
+  RotaryArgs rot;
+  tkv_token_view q, k, q_out, k_out;
+  uint32_t* err;
+  int32_t tokens, heads, kv_heads, head_dim;
+};
+
+struct AppendParams8 {
+  RotaryArgs rot;
+  tkv_token_view k, v, q, q_out;
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* units;
+  const int32_t* num_units;
+  uint32_t* err;
+  int64_t blocks;
+  int32_t units_cap, tokens, heads, kv_heads;
+  int32_t has_rot;
+};
+
+struct AttnParams8 {
+  tkv_token_view q;
+  void* out;
+  float* out_lse;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* kv_lens;
+  const int32_t* cu_q;
+  const uint8_t* k_codes;
+  const uint8_t* v_codes;
+  const float* k_scale;
+  const float* v_scale;
+  uint32_t* err;
+  uint32_t* counters;
+  uint8_t* data;
+  int64_t blocks;
+  int32_t requests, tokens, heads, kv_heads, group;
+  int32_t table_width, max_q_len, window, block_size;
+  int32_t bf16;          // q and out are bf16 (else fp16)
+  int32_t few_rows_max;  // rows per kv head of the requests that few_rows_kernel takes
+  float scale_log2;
+};
+
+cudaError_t launch_plan_step(const tkv_kv8_plan_args& p, cudaStream_t stream);
+cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream);
+cudaError_t launch_kv8_append(const AppendParams8& p, int head_dim, int block_size, int format,
+                              int dtype, cudaStream_t stream);
+
+// Scratch of an attention call: counters (returned to zero by the launch) and
+// partial results.
+void kv8_attention_scratch(int sms, int head_dim, int group, int max_q_len, int requests,
+                           int kv_heads, size_t* counters, size_t* data);
+cudaError_t launch_kv8_attention(const AttnParams8& p, int sms, int head_dim, int format,
+                                 cudaStream_t stream);
+// Tensor maps of the K and V codes as [blocks * kv_heads * block_size][head_dim]
+// bytes, boxes of min(block_size, 32) rows, swizzled by the row's width.
+bool kv8_code_maps(const AttnParams8& p, int head_dim, CUtensorMap maps[2]);
+
+}  // namespace tkv

@@ -1,0 +1,470 @@
+"""Serving steps over an 8-bit paged cache.
+
+One layer's cache (:class:`Kv8Cache`) is 8-bit throughout -- Format S int8
+codes, or e4m3 -- with one fp32 scale per (block, kv head) and tensor.  A batch
+of requests with any query lengths (single tokens, drafted tokens, prompt
+chunks, whole prompts) takes one step in four calls:
+
+* :func:`plan_step`     block tables, slot maps and write lists from the
+  requests' lengths, on the GPU (one plan serves every layer);
+* :func:`rotary_embed`  rotary positions with up to four axes, or fused into
+* :func:`append`        the quantizing write of the new keys and values;
+* :func:`attention`     causal attention of the new tokens over the cache.
+
+Every computation is one call into the C-ABI library (``tkv_kv8_*`` and
+``tkv_rotary_embed`` in include/tierkv_b200.h).  Errors the device finds
+(out-of-cache slots, exhausted free blocks, positions outside the cos / sin
+table) go to the stream's error word, ``ops.read_device_errors``.  The
+reference has no counterpart: its 8-bit blocks are filled by demotion only.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+from dataclasses import dataclass
+
+import torch
+
+from . import _native as N
+from . import ops
+
+_FORMAT = {torch.int8: N.TKV_KV8_INT8, torch.float8_e4m3fn: N.TKV_KV8_E4M3}
+_FLOATS = {torch.float16: N.TKV_DTYPE_F16, torch.bfloat16: N.TKV_DTYPE_BF16}
+MAX_REQUESTS = N.TKV_KV8_MAX_REQUESTS
+
+
+# ---------------------------------------------------------------------------
+# handles
+# ---------------------------------------------------------------------------
+
+class Kv8Cache:
+    """One layer's 8-bit cache: k_codes / v_codes [blocks, kv_heads, block_size,
+    head_dim] int8 or float8_e4m3fn, k_scale / v_scale [blocks, kv_heads] fp32;
+    value = code * scale.  block_size 16, 32 or 64; head_dim 64 or 128."""
+
+    def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
+                 v_scale: torch.Tensor):
+        if k_codes.ndim != 4 or k_codes.dtype not in _FORMAT:
+            raise ValueError("cache codes must be int8 or float8_e4m3fn [blocks, kv_heads, block_size, head_dim].")
+        if not k_codes.is_cuda:
+            raise ValueError("cache tensors must be CUDA tensors.")
+        for t, like in ((v_codes, k_codes), (v_scale, k_scale)):
+            if t.shape != like.shape or t.dtype != like.dtype:
+                raise ValueError("the value tensors must match the key tensors in shape and dtype.")
+        if k_scale.dtype != torch.float32 or tuple(k_scale.shape) != tuple(k_codes.shape[:2]):
+            raise ValueError("cache scales must be fp32 [blocks, kv_heads].")
+        for t in (k_codes, v_codes, k_scale, v_scale):
+            if not t.is_contiguous() or t.device != k_codes.device:
+                raise ValueError("cache tensors must be contiguous and on one device.")
+        self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
+        self.blocks, self.kv_heads, self.block_size, self.head_dim = (int(x) for x in k_codes.shape)
+        self.device = k_codes.device
+        self._struct = N.TkvKv8Cache(k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
+                                     v_scale.data_ptr(), self.blocks, self.kv_heads, self.block_size,
+                                     self.head_dim, _FORMAT[k_codes.dtype])
+
+    @classmethod
+    def allocate(cls, blocks: int, kv_heads: int, block_size: int, head_dim: int, device,
+                 dtype: torch.dtype = torch.int8) -> "Kv8Cache":
+        """A cache of zero codes with scale 1."""
+        if dtype not in _FORMAT:
+            raise ValueError("an 8-bit cache is int8 or float8_e4m3fn.")
+        shape = (blocks, kv_heads, block_size, head_dim)
+        codes = [torch.zeros(shape, dtype=torch.int8, device=device).view(dtype) for _ in range(2)]
+        return cls(*codes, *(torch.ones(shape[:2], device=device) for _ in range(2)))
+
+    @classmethod
+    def of_pools(cls, pools: ops.TieredPools) -> "Kv8Cache":
+        """The WARM pools of Format S, shared: blocks that demotion filled can be
+        attended by any number of query tokens."""
+        if pools.fmt != ops.FORMAT_S:
+            raise ValueError("an 8-bit cache shares Format S pools only.")
+        return cls(pools.warm_k, pools.warm_v, pools.k_scale, pools.v_scale)
+
+
+class StepPlan:
+    """What one step's launches share.  :func:`plan_step` fills a plan made by
+    :meth:`allocate`; a program that keeps its own tables passes them here:
+    ``units`` / ``num_units`` for :func:`append`, ``block_table`` / ``kv_lens``
+    / ``cu_q`` for :func:`attention`.
+
+    kv_lens [requests], cu_q [requests + 1], admitted [requests], slot_map /
+    token_request / positions [tokens] (-1 past the last token), units [cap, 4]
+    (block, first token, row offset, rows; -1 past the last), num_units [1],
+    free_count [1]; all int32."""
+
+    def __init__(self, *, block_size: int, units=None, num_units=None, block_table=None, kv_lens=None,
+                 cu_q=None):
+        self.block_size = int(block_size)
+        self.units, self.num_units = units, num_units
+        self.block_table, self.kv_lens, self.cu_q = block_table, kv_lens, cu_q
+        self.admitted = self.slot_map = self.token_request = self.positions = self.free_count = None
+        self.requests = 0
+        self._args = None
+        for name in ("units", "num_units", "kv_lens", "cu_q"):
+            t = getattr(self, name)
+            if t is not None and (t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous int32 CUDA tensor.")
+        if units is not None and (units.ndim != 2 or units.shape[1] != 4 or num_units is None):
+            raise ValueError("units must be [count, 4] beside num_units [1].")
+        if block_table is not None:
+            if kv_lens is None or cu_q is None:
+                raise ValueError("a block_table needs kv_lens and cu_q.")
+            self.requests = int(kv_lens.numel())
+            if cu_q.numel() != self.requests + 1:
+                raise ValueError("cu_q must have one entry more than kv_lens.")
+            _check_table(block_table, self.requests)
+
+    @classmethod
+    def allocate(cls, max_requests: int, max_tokens: int, block_size: int, device) -> "StepPlan":
+        """Buffers for steps of up to max_requests requests and max_tokens tokens."""
+        if not 1 <= max_requests <= MAX_REQUESTS:
+            raise ValueError(f"a step plans 1 to {MAX_REQUESTS} requests.")
+        if max_tokens < 0:
+            raise ValueError("max_tokens must not be negative.")
+        r, t = int(max_requests), int(max_tokens)
+        cap = _units_cap(r, t, block_size)
+        # one buffer: [units | slot_map | token_request | positions | kv_lens | admitted | cu_q | counts]
+        sizes = (4 * cap, t, t, t, r, r, r + 1, 1, 1)
+        buf = torch.full((sum((n + 3) // 4 * 4 for n in sizes),), -1, dtype=torch.int32, device=device)
+        at, parts = 0, []
+        for n in sizes:
+            parts.append(buf[at:at + n])
+            at += (n + 3) // 4 * 4
+        units, slot, req, pos, kv, adm, cu, num, free = parts
+        plan = cls(block_size=block_size, units=units.view(cap, 4), num_units=num)
+        plan.kv_lens, plan.cu_q = kv, cu
+        plan.slot_map, plan.token_request, plan.positions = slot, req, pos
+        plan.admitted, plan.free_count = adm, free
+        plan._args = N.TkvKv8PlanArgs(
+            None, None, None, 0, None, None, kv.data_ptr(), cu.data_ptr(), adm.data_ptr(),
+            slot.data_ptr(), req.data_ptr(), pos.data_ptr(), units.data_ptr(), num.data_ptr(),
+            free.data_ptr(), None, 0, 0, 0, 0, 0, plan.block_size)
+        return plan
+
+
+@dataclass(frozen=True)
+class Rotary:
+    """Rotary positions: cos_sin [rows, rot_dim] fp32 (the cosines of the rot_dim
+    / 2 frequencies, then their sines); ``sections`` frequencies for each of up
+    to four axes (None: one axis), one run after the other or, with
+    ``interleave``, axis f % axes for frequency f while that axis has any left
+    (axis 0 afterwards).  ``pairs``: a pair is two adjacent elements; otherwise
+    element f and f + rot_dim / 2."""
+
+    cos_sin: torch.Tensor
+    sections: tuple | None = None
+    interleave: bool = False
+    pairs: bool = False
+
+    def __post_init__(self):
+        t = self.cos_sin
+        if t.ndim != 2 or t.dtype != torch.float32 or not t.is_cuda or not t.is_contiguous():
+            raise ValueError("cos_sin must be a contiguous fp32 CUDA tensor [rows, rot_dim].")
+        if t.data_ptr() % 16:
+            raise ValueError("cos_sin must be 16-byte aligned.")
+        half = int(t.shape[1]) // 2
+        sec = (half,) if self.sections is None else tuple(int(x) for x in self.sections)
+        if not 1 <= len(sec) <= 4 or any(x < 0 for x in sec) or sum(sec) != half:
+            raise ValueError("sections must be 1 to 4 counts that add up to rot_dim / 2.")
+        object.__setattr__(self, "_struct", N.TkvRotary(
+            t.data_ptr(), None, int(t.shape[0]), 0, 4, int(t.shape[1]), len(sec),
+            (ctypes.c_int32 * 4)(*sec), int(bool(self.interleave)), int(bool(self.pairs))))
+        object.__setattr__(self, "axes", len(sec))
+
+    def _at(self, positions: torch.Tensor, tokens: int):
+        """(the C struct with these positions, the tensor that backs them)."""
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != self.cos_sin.device:
+            raise ValueError("positions must be int32 or int64 on the table's device.")
+        if positions.ndim == 1 and self.axes == 1:
+            positions = positions.unsqueeze(0)
+        if positions.ndim != 2 or positions.shape[0] != self.axes or positions.shape[1] < tokens:
+            raise ValueError("positions must have shape [axes, tokens] (or [tokens] for one axis).")
+        if positions.shape[1] > 1 and positions.stride(1) != 1:
+            positions = positions.contiguous()
+        st = N.TkvRotary.from_buffer_copy(self._struct)
+        st.positions = positions.data_ptr()
+        st.positions_bytes = positions.element_size()
+        st.axis_stride = positions.stride(0)
+        return st, positions
+
+
+# ---------------------------------------------------------------------------
+# shared checks
+# ---------------------------------------------------------------------------
+
+def _units_cap(requests: int, tokens: int, block_size: int) -> int:
+    return min(tokens, tokens // block_size + 2 * requests)
+
+
+def _check_table(table: torch.Tensor, requests: int) -> None:
+    if table.dtype != torch.int32 or not table.is_cuda or table.ndim != 2 or table.shape[0] < requests:
+        raise ValueError("block_table must be an int32 CUDA tensor [requests, width].")
+    if table.shape[1] > 1 and table.stride(1) != 1 or table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError("block_table rows must be contiguous and must not overlap.")
+
+
+def _table_stride(table: torch.Tensor) -> int:
+    return int(table.stride(0)) if table.shape[0] > 1 else int(table.shape[1])
+
+
+def _view(t: torch.Tensor) -> N.TkvTokenView | None:
+    """The strided view of [tokens, heads, head_dim], None if it is not 16-byte aligned throughout."""
+    n, h, d = t.shape
+    s0, s1, s2 = t.stride()
+    s0, s1 = s0 if n > 1 else 0, s1 if h > 1 else 0
+    if (d > 1 and s2 != 1) or s0 % 8 or s1 % 8 or t.data_ptr() % 16:
+        return None
+    return N.TkvTokenView(t.data_ptr(), s0, s1)
+
+
+def _input_view(t: torch.Tensor):
+    """(view, tensor that backs it): strided as it is, or through a compact copy."""
+    v = _view(t)
+    if v is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        v = _view(t)
+    return v, t
+
+
+def _output_view(t: torch.Tensor, like: torch.Tensor, name: str) -> N.TkvTokenView:
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must match its input in shape, dtype and device.")
+    v = _view(t)
+    if v is None:
+        raise ValueError(f"{name} must be 16-byte aligned with head_dim contiguous.")
+    return v
+
+
+def _heads3(t: torch.Tensor, name: str) -> None:
+    if t.ndim != 3 or t.dtype not in _FLOATS:
+        raise ValueError(f"{name} must be an fp16 or bf16 tensor [tokens, heads, head_dim].")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor.")
+
+
+def _streamed(fn):
+    """``stream=``: the whole call -- its copies, outputs and workspace too -- runs
+    on that stream, and the caching allocator learns that its inputs are used
+    there.  Ordering it after the inputs' producers is the caller's part."""
+
+    @functools.wraps(fn)
+    def call(*args, stream=None, **kwargs):
+        if stream is None:
+            return fn(*args, **kwargs)
+        for x in (*args, *kwargs.values()):
+            for t in (x,) if isinstance(x, torch.Tensor) else getattr(x, "__dict__", {}).values():
+                if isinstance(t, torch.Tensor) and t.is_cuda:
+                    t.record_stream(stream)
+        with torch.cuda.stream(stream):
+            return fn(*args, **kwargs)
+
+    return call
+
+
+def _call(device: torch.device, launch) -> None:
+    """Runs ``launch(current stream of device, its workspace)`` with ``device`` current."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _call(device, launch)
+    st = ops._stream(None, index)
+    launch(st, ops.workspace_for(device, st.value or 0, 1 << 16))
+
+
+# ---------------------------------------------------------------------------
+# the operators
+# ---------------------------------------------------------------------------
+
+@_streamed
+def plan_step(plan: StepPlan, context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+              free_blocks: torch.Tensor, free_count: torch.Tensor, *, tokens: int | None = None) -> StepPlan:
+    """Plans one step on the GPU: request i holds context_lens[i] tokens and gets
+    new_lens[i] more, packed one request after the other.
+
+    New blocks come from the end of the free list (free_blocks [capacity],
+    free_count [1]) in request order and are written into block_table
+    [requests, width]; every other table cell stays.  A request whose row or
+    whose share of the free list does not suffice is not admitted: its context
+    stays, its tokens get slot -1 and ``TKV_DEVERR_NO_BLOCKS`` is recorded.
+    Fills ``plan`` (its buffers' first entries, for fewer requests than it was
+    allocated for) and returns it.  ``plan.kv_lens`` and ``plan.free_count`` may
+    be passed back as the next step's context_lens and free_count.  ``tokens``:
+    how many entries of the token outputs to write (default: all)."""
+    a = plan._args
+    if a is None:
+        raise ValueError("plan_step fills a plan made by StepPlan.allocate.")
+    n = int(context_lens.numel())
+    for t, name in ((context_lens, "context_lens"), (new_lens, "new_lens"), (free_blocks, "free_blocks"),
+                    (free_count, "free_count")):
+        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 CUDA tensor.")
+    if not 1 <= n <= plan.admitted.numel() or new_lens.numel() != n or free_count.numel() != 1:
+        raise ValueError("context_lens and new_lens must have 1 to the plan's max_requests entries, free_count one.")
+    _check_table(block_table, n)
+    cap = int(plan.slot_map.numel())
+    tokens = cap if tokens is None else int(tokens)
+    if not 0 <= tokens <= cap:
+        raise ValueError("tokens must be between 0 and the plan's max_tokens.")
+    a.context_lens = context_lens.data_ptr()
+    a.new_lens = new_lens.data_ptr()
+    a.block_table = block_table.data_ptr()
+    a.table_stride = _table_stride(block_table)
+    a.free_blocks = free_blocks.data_ptr()
+    a.free_count = free_count.data_ptr()
+    a.requests, a.tokens, a.table_width = n, tokens, int(block_table.shape[1])
+    a.units_cap = min(_units_cap(n, tokens, plan.block_size), int(plan.units.shape[0]))
+    a.free_capacity = int(free_blocks.numel())
+
+    def launch(st, ws):
+        a.error_word = ws.data_ptr()
+        N.check(N.load().tkv_kv8_plan_step(ctypes.byref(a), st), "tkv_kv8_plan_step")
+
+    _call(plan.kv_lens.device, launch)
+    plan.block_table, plan.requests = block_table, n
+    return plan
+
+
+@_streamed
+def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary, *,
+                 q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """Rotates q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim]
+    (fp16 / bf16, any 16-byte aligned token and head strides; either may be
+    None) by their tokens' positions [axes, tokens]; returns (q_out, k_out).
+    An output may be its input."""
+    x = q if q is not None else k
+    if x is None:
+        raise ValueError("rotary_embed needs q or k.")
+    tokens, _, d = x.shape if x.ndim == 3 else (0, 0, 0)
+    views, outs, inputs = [], [], []
+    for t, out, name in ((q, q_out, "q"), (k, k_out, "k")):
+        if t is None:
+            views += [None, None]
+            outs.append(None)
+            continue
+        _heads3(t, name)
+        if t.shape[0] != tokens or t.shape[2] != d or t.dtype != x.dtype or t.device != x.device:
+            raise ValueError("q and k must agree in tokens, head_dim, dtype and device.")
+        if out is None:
+            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        v, t = _input_view(t)
+        views += [v, _output_view(out, t, name + "_out")]
+        outs.append(out)
+        inputs.append(t)  # a copy lives until the launch
+    rot, positions = rotary._at(positions, tokens)
+    qv, qov, kv, kov = (None if v is None else ctypes.byref(v) for v in views)
+
+    def launch(st, ws):
+        N.check(N.load().tkv_rotary_embed(
+            ctypes.byref(rot), qv, kv, qov, kov, tokens, 0 if q is None else q.shape[1],
+            0 if k is None else k.shape[1], d, _FLOATS[x.dtype], ws.data_ptr(), st), "tkv_rotary_embed")
+
+    _call(x.device, launch)
+    return outs[0], outs[1]
+
+
+@_streamed
+def append(cache: Kv8Cache, plan: StepPlan, k: torch.Tensor, v: torch.Tensor, *, q: torch.Tensor | None = None,
+           positions: torch.Tensor | None = None, rotary: Rotary | None = None,
+           q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Quantizes the step's new keys and values [tokens, kv_heads, head_dim] into
+    the blocks of ``plan.units``; with ``rotary``, k is rotated on the way (in
+    fp32) and q, when given, into q_out, which is returned.
+
+    A block's scale is max |x| / 127 (448 for e4m3) of its rows; when a block
+    that already holds rows gets larger ones, its scale grows and its codes are
+    rounded again.  A block with a NaN or an infinity gets scale NaN."""
+    _heads3(k, "k")
+    _heads3(v, "v")
+    tokens = int(k.shape[0])
+    if tuple(k.shape) != (tokens, cache.kv_heads, cache.head_dim) or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("k and v must have shape [tokens, kv_heads, head_dim] of the cache and one dtype.")
+    if k.device != cache.device or v.device != cache.device:
+        raise ValueError("k and v must be on the cache's device.")
+    if plan.units is None or plan.block_size != cache.block_size:
+        raise ValueError("append needs a plan with write units of the cache's block size.")
+    if rotary is None and q is not None:
+        raise ValueError("q is rotated only: pass rotary and positions beside it.")
+    if rotary is not None and positions is None:
+        raise ValueError("rotary needs the tokens' positions.")
+    kv_view, k = _input_view(k)
+    v_view, v = _input_view(v)
+    args = N.TkvKv8AppendArgs()
+    args.k, args.v = kv_view, v_view
+    rot = None
+    if rotary is not None:
+        rot, positions = rotary._at(positions, tokens)
+        args.rotary = ctypes.pointer(rot)
+    if q is not None:
+        _heads3(q, "q")
+        if q.shape[0] != tokens or q.shape[2] != cache.head_dim or q.dtype != k.dtype or q.device != k.device:
+            raise ValueError("q must agree with k in tokens, head_dim, dtype and device.")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        args.q, q = _input_view(q)
+        args.q_out = _output_view(q_out, q, "q_out")
+        args.heads = int(q.shape[1])
+    args.units, args.num_units = plan.units.data_ptr(), plan.num_units.data_ptr()
+    # no step writes more units than tokens
+    args.units_cap = min(int(plan.units.shape[0]), tokens)
+    args.tokens, args.dtype = tokens, _FLOATS[k.dtype]
+
+    def launch(st, ws):
+        args.error_word = ws.data_ptr()
+        N.check(N.load().tkv_kv8_append(ctypes.byref(cache._struct), ctypes.byref(args), st), "tkv_kv8_append")
+
+    _call(cache.device, launch)
+    return q_out if q is not None else None
+
+
+@_streamed
+def attention(q: torch.Tensor, cache: Kv8Cache, plan: StepPlan, scaling: float, *,
+              max_q_len: int | None = None, window: int = 0, out: torch.Tensor | None = None,
+              return_lse: bool = False):
+    """Causal attention of the step's query tokens q [tokens, heads, head_dim]
+    over the cache: request i's tokens are q[cu_q[i]:cu_q[i + 1]], the last of
+    its kv_lens[i] tokens; each sees the keys up to its own position, with
+    ``window`` only the last ``window`` of them.  heads: a multiple of
+    kv_heads, up to 64 per kv head.  ``max_q_len``: an upper bound of the
+    requests' query tokens (default: tokens).
+
+    Returns out (q's dtype), with return_lse (out, lse [tokens, heads] fp32,
+    natural log).  A token that sees nothing gets 0 and -inf; tokens that belong
+    to no request are not written.  A request whose table names a block outside
+    the cache reads zeros there (``TKV_DEVERR_BAD_SLOT``)."""
+    _heads3(q, "q")
+    tokens, heads, d = (int(x) for x in q.shape)
+    if d != cache.head_dim or q.device != cache.device or heads % cache.kv_heads:
+        raise ValueError("q must match the cache in head_dim and device, and heads be a multiple of kv_heads.")
+    if plan.block_table is None or plan.block_size != cache.block_size:
+        raise ValueError("attention needs a plan with block tables of the cache's block size.")
+    if out is None:
+        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() \
+            or out.data_ptr() % 16:
+        raise ValueError("out must be a contiguous, 16-byte aligned tensor like q.")
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    view, q = _input_view(q)
+    table = plan.block_table
+    args = N.TkvKv8AttentionArgs(
+        view, out.data_ptr(), None if lse is None else lse.data_ptr(), table.data_ptr(), _table_stride(table),
+        plan.kv_lens.data_ptr(), plan.cu_q.data_ptr(), plan.requests, tokens, heads, _FLOATS[q.dtype],
+        int(table.shape[1]), min(tokens, tokens if max_q_len is None else int(max_q_len)), int(window),
+        float(scaling), None, 0)
+
+    def launch(st, ws):
+        lib = N.load()
+        for attempt in range(2):
+            args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
+            status = lib.tkv_kv8_attention(ctypes.byref(cache._struct), ctypes.byref(args), st)
+            if status != N.TKV_ERR_WORKSPACE or attempt:
+                break
+            nbytes = ctypes.c_size_t()
+            N.check(lib.tkv_kv8_attention_workspace(ctypes.byref(cache._struct), ctypes.byref(args),
+                                                    ctypes.byref(nbytes)), "tkv_kv8_attention_workspace")
+            ws = ops.workspace_for(cache.device, st.value or 0, nbytes.value)
+        N.check(status, "tkv_kv8_attention")
+
+    _call(cache.device, launch)
+    return (out, lse) if return_lse else out

@@ -334,7 +334,10 @@ class TierKVDeviceError(N.TierKVError):
         self.bits = int(bits)
         self.call = int(call)
         names = [n for b, n in ((N.TKV_DEVERR_BAD_SLOT, "out-of-pool slot"),
-                                (N.TKV_DEVERR_TIMEOUT, "bounded wait timed out")) if self.bits & b]
+                                (N.TKV_DEVERR_TIMEOUT, "bounded wait timed out"),
+                                (N.TKV_DEVERR_NO_BLOCKS, "request without free blocks or table room"),
+                                (N.TKV_DEVERR_BAD_POS, "rotary position outside its table"))
+                 if self.bits & b]
         super().__init__(f"{what} call {self.call} recorded device error 0x{self.bits:x} "
                          f"({', '.join(names) or 'unknown'})")
 
