@@ -1,93 +1,728 @@
-// tkv_kv8_attn.cu -- attention of a packed batch over the 8-bit paged cache.
+// tkv_kv8_attn.cu -- attention over the 8-bit paged cache for requests with
+// few query rows (single tokens, drafted tokens, short chunks).
+//
+// A row is one (query token, query head); the rows of a kv head share its K/V,
+// so they are packed into tiles of 8 * NT rows and every code is read once per
+// tile.  At few rows the kernel is bound by HBM: 2 head_dim bytes per token and
+// kv head against 4 head_dim rows flops.
+//
+// Work is a flat list of steps -- 128 tokens (4 warps x 32) of one (request, kv
+// head, row tile) unit, units in order -- cut into one contiguous range per
+// resident CTA, so ragged batches and single long contexts load every SM
+// alike.  A CTA that covers a whole unit writes the output; otherwise it
+// leaves (max, sum, accumulator) partials in the workspace and the last CTA of
+// the unit to arrive merges them in CTA order (the result does not depend on
+// which one is last).
+//
+// Inside a CTA every warp runs by itself: it streams its 32-token tiles (TMA
+// boxes of K and V codes, scales by 4-byte asynchronous copies) through its own
+// ring of stages, computes S^T = K Q^T and O^T += V^T P^T with mma.m16n8k16 on
+// codes expanded to fp16 (exact for int8 and e4m3), and keeps its own softmax
+// statistics; the warps meet only at the end of a unit.  A warp's issue cursor
+// runs ahead over unit boundaries, so the ring stays full across them.
+//
+// Scales: K's multiplies the logits in fp32.  V's is folded into P, normalised
+// by a power of two (vinv) so that P stays in fp16's normal range for any
+// scale; queries in bf16 become fp16 through a power of two per row, which
+// only drops bits 2^-28 below the row's maximum.  fp16 P (11 bits) rounds 8
+// times finer than the bf16 of the usual fused kernels; sums, maxima and
+// accumulators are fp32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
+#include <math.h>
+
+#include <cstring>
 
 #include "tkv_kv8.h"
 #include "tkv_kv8_common.cuh"
+#include "tkv_ptx.cuh"
 
 namespace tkv {
 
-template <int FMT>
-__device__ __forceinline__ float code_value(uint8_t b) {
-  if (FMT == TKV_KV8_INT8) return (float)(int8_t)b;
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
+// Row tiles of 8 that an instance of the kernel holds, by the most rows a
+// request may have.
+static int few_row_tiles(int group, int max_q_len) {
+  const int64_t rows = (int64_t)group * max_q_len;
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+}
+constexpr int few_ctas_per_sm(int nt) { return nt == 4 ? 1 : 2; }
+
+constexpr int kFewWarps = 4;
+constexpr int kFewThreads = 32 * kFewWarps;
+constexpr int kTileTok = 32;                          // tokens of a warp's tile
+constexpr int kStepTok = kTileTok * kFewWarps;        // tokens of a step
+
+template <int D, int NT>
+struct FewLayout {
+  static constexpr int kStages = 3;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kHalf = kTileTok * D;           // codes of K (or V) in a stage
+  static constexpr int kStage = 2 * kHalf;
+  static constexpr int kRing = kFewWarps * kStages * kStage;
+  static constexpr int kQOff = kRing;                  // fp16 [rows][D + 16]
+  static constexpr int kQStride = D + 16;   // 8-byte fragment reads of 4 rows hit 32 banks
+  static constexpr int kMergeOff = kQOff + kRows * kQStride * 2;   // fp32 [2][rows][D + 4]
+  static constexpr int kMergeStride = D + 4;
+  static constexpr int kStatOff = kMergeOff + 2 * kRows * kMergeStride * 4;  // [warps][rows][2], row scales
+  static constexpr int kScaleOff = kStatOff + (kFewWarps + 1) * kRows * 8;   // [warps][stages][4]
+  static constexpr int kBarOff = kScaleOff + kFewWarps * kStages * 16;
+  static constexpr int kMiscOff = kBarOff + kFewWarps * kStages * 8;
+  static constexpr int kBytes = kMiscOff + 64 + 1024;  // + slack to align the ring to 1024
+};
+
+// Where a walk over the units stands.
+struct UnitPos {
+  int req;        // request
+  int head;       // kv head
+  int rt;         // row tile
+  int q0, q_len;  // first packed token, query tokens
+  int kv;         // keys
+  int tiles_r;    // row tiles of the request
+  int step0;      // first step (of 128 tokens) of the request's units
+  int steps;      // steps of each of its units
+};
+
+template <int RT>
+__device__ __forceinline__ bool load_request(const AttnParams8& p, int bs, int req, UnitPos& u) {
+  u.req = req;
+  const RequestLens n = request_lens(p, bs, req);
+  u.q0 = n.q0;
+  u.q_len = n.q_len;
+  u.kv = n.kv;
+  if (!n.few_rows(p)) {
+    u.steps = 0;
+    u.tiles_r = 0;
+    return false;
+  }
+  u.tiles_r = (n.q_len * p.group + RT - 1) / RT;
+  const int lo = n.first_key(p);
+  u.step0 = lo / kStepTok;
+  // a request without keys keeps one empty step, which writes its zeros
+  u.steps = max(1, (n.kv + kStepTok - 1) / kStepTok - u.step0);
+  return u.tiles_r > 0;
 }
 
-// One warp per (token, query head), one key at a time, online softmax.
-template <int D, int FMT>
-__global__ void __launch_bounds__(128) attention_simple_kernel(const AttnParams8 p) {
-  const int lane = threadIdx.x & 31, bs = p.block_size;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= (int64_t)p.tokens * p.heads) return;
-  const int t = (int)(w / p.heads), h = (int)(w % p.heads), kh = h / p.group;
-  if (t < p.cu_q[0] || t >= p.cu_q[p.requests]) return;
-  int lo = 0, hi = p.requests;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_q[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  const RequestLens n = request_lens(p, bs, lo);
-  const int pos = n.kv - (n.q0 + n.q_len - t);
-  constexpr int E = D / 64;
-  float2 q[E], o[E] = {};
-  const uint32_t* qp = reinterpret_cast<const uint32_t*>((const uint16_t*)p.q.data + t * p.q.token_stride +
-                                                         h * p.q.head_stride) + lane * E;
-#pragma unroll
-  for (int i = 0; i < E; ++i) q[i] = unpack_in(p.bf16, qp[i]);
-  float m = -INFINITY, l = 0.f;
-  const int first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-  for (int j = first; j <= pos; ++j) {
-    int64_t b = p.table[lo * p.table_stride + j / bs];
-    float ks = 0.f, vs = 0.f;
-    if (b < 0 || b >= p.blocks) {
-      b = 0;
-      if (lane == 0) atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
-    } else {
-      ks = p.k_scale[b * p.kv_heads + kh];
-      vs = p.v_scale[b * p.kv_heads + kh];
+template <int RT>
+__device__ __forceinline__ int64_t request_steps(const AttnParams8& p, int bs, int req) {
+  UnitPos u;
+  return load_request<RT>(p, bs, req, u) ? (int64_t)u.steps * u.tiles_r * p.kv_heads : 0;
+}
+
+// Next unit in order; false past the last request.
+template <int RT>
+__device__ __forceinline__ bool next_unit(const AttnParams8& p, int bs, UnitPos& u) {
+  if (++u.rt < u.tiles_r) return true;
+  u.rt = 0;
+  if (++u.head < p.kv_heads) return true;
+  u.head = 0;
+  for (int r = u.req + 1; r < p.requests; ++r)
+    if (load_request<RT>(p, bs, r, u)) return true;
+  return false;
+}
+
+template <int D, int BOXES, int FMT, int NT>
+__global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
+    few_rows_kernel(const __grid_constant__ AttnParams8 p, const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v) {
+  using L = FewLayout<D, NT>;
+  constexpr int RT = L::kRows;
+  constexpr int S = L::kStages;
+  constexpr int kBoxes = BOXES;                         // TMA boxes of a tile (K; V alike)
+  constexpr int kBox = kTileTok / kBoxes;               // rows of a box
+  const int bs = p.block_size;
+  const bool bf16 = p.bf16 != 0;
+  constexpr int kBatch = 32 / kBoxes;                   // tiles whose table cells a warp holds
+  constexpr int kSwz = D == 128 ? 7 : 3;
+  extern __shared__ uint8_t few_raw[];
+  const uint32_t raw = smem_u32(few_raw);
+  uint8_t* smem = few_raw + (((raw + 1023u) & ~1023u) - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  uint8_t* ring = smem + warp * S * L::kStage;
+  __half* q_s = reinterpret_cast<__half*>(smem + L::kQOff);
+  float* merge_s = reinterpret_cast<float*>(smem + L::kMergeOff);
+  float* stat_s = reinterpret_cast<float*>(smem + L::kStatOff);
+  float* rscale_s = stat_s + kFewWarps * RT * 2;         // [RT] logit scale of each row
+  float* scale_s = reinterpret_cast<float*>(smem + L::kScaleOff) + warp * S * 4;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff) + warp * S;
+  int64_t* range_s = reinterpret_cast<int64_t*>(smem + L::kMiscOff);   // scan scratch
+  int* flag_s = reinterpret_cast<int*>(smem + L::kMiscOff + 56);
+
+  if (lane == 0) {
+    // one expect_tx arrival and one per scale-copying lane
+    for (int s = 0; s < S; ++s) mbar_init(full + s, 1 + 2 * kBoxes);
+    fence_mbar_init();
+    if (warp == 0) {
+      prefetch_tensormap(&tm_k);
+      prefetch_tensormap(&tm_v);
     }
-    const int64_t at = ((b * p.kv_heads + kh) * bs + j % bs) * D + lane * 2 * E;
-    float s = 0.f;
+  }
+
+  // ---- this CTA's range of the flat step list
+  UnitPos unit;
+  int64_t total, ctas, begin, end, unit_at;   // unit_at: flat index of the unit's first step
+  {
+    const int per = (p.requests + kFewThreads - 1) / kFewThreads;
+    const int r0 = min(p.requests, (int)threadIdx.x * per), r1 = min(p.requests, r0 + per);
+    int64_t sum = 0;
+    for (int r = r0; r < r1; ++r) sum += request_steps<RT>(p, bs, r);
+    int64_t inc = sum;
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-      s += q[i].x * code_value<FMT>(p.k_codes[at + 2 * i]) + q[i].y * code_value<FMT>(p.k_codes[at + 2 * i + 1]);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(~0u, inc, o);
+      if (lane >= o) inc += x;
+    }
+    if (lane == 31) range_s[warp] = inc;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
-    s *= ks * p.scale_log2;
-    const float mn = fmaxf(m, s);
-    const float a = exp2f(m - mn), e = exp2f(s - mn);
-    m = mn;
-    l = l * a + e;
+    for (int w = 0; w < kFewWarps; ++w) {
+      if (w < warp) before += range_s[w];
+      total += range_s[w];
+    }
+    ctas = min((int64_t)gridDim.x, total);   // every range holds a step
+    if (blockIdx.x >= ctas) return;
+    begin = total * blockIdx.x / ctas;
+    end = total * (blockIdx.x + 1) / ctas;
+    int64_t at = before + inc - sum;
+    __syncthreads();
+    if (at <= begin && begin < at + sum) {
+      int r = r0;
+      for (;; ++r) {
+        const int64_t n = request_steps<RT>(p, bs, r);
+        if (begin < at + n) break;
+        at += n;
+      }
+      range_s[0] = at;
+      range_s[1] = r;
+    }
+    __syncthreads();
+    load_request<RT>(p, bs, (int)range_s[1], unit);
+    const int64_t in = (begin - range_s[0]) / unit.steps;   // unit of the request
+    unit.head = (int)(in / unit.tiles_r);
+    unit.rt = (int)(in % unit.tiles_r);
+    unit_at = range_s[0] + in * unit.steps;
+  }
+
+  // ---- the warp's issue cursor: tile `warp` of every step of the range, S ahead
+  UnitPos iu = unit;
+  int64_t i_at = unit_at;               // flat index of iu's first step
+  int64_t i_pos = begin;                // next step to issue
+  int64_t issued = 0;
+  int32_t cells = 0;                    // lane: table cell (batch tile lane / kBoxes, box lane % kBoxes)
+  int64_t cells_at = -1;                // flat step of the batch's first tile
+  bool ok = true;
+  auto issue = [&]() {
+    if (i_pos >= end || !ok) return;
+    if (i_pos >= i_at + iu.steps) {
+      i_at += iu.steps;
+      next_unit<RT>(p, bs, iu);
+      cells_at = -1;
+    }
+    const int step = iu.step0 + (int)(i_pos - i_at);
+    if (cells_at < 0 || i_pos - cells_at >= kBatch) {
+      cells_at = i_pos;
+      const int tok = (step + lane / kBoxes) * kStepTok + warp * kTileTok + (lane % kBoxes) * kBox;
+      cells = -1;
+      if (tok < iu.kv) cells = p.table[iu.req * p.table_stride + tok / bs];
+    }
+    const int s = (int)(issued % S);
+    const int tok0 = step * kStepTok + warp * kTileTok;
+    const int b = (int)(i_pos - cells_at) * kBoxes;
+    uint8_t* st = ring + s * L::kStage;
+    // lanes [0, kBoxes): K boxes, [kBoxes, 2 kBoxes): V boxes
+    const int box = lane % kBoxes;
+    const int cell = __shfl_sync(~0u, cells, b + box);
+    const int tok = tok0 + box * kBox;
+    const bool in_keys = tok < iu.kv && tok + kBox > (p.window > 0 ? iu.kv - iu.q_len - p.window + 1 : 0);
+    const bool good = in_keys && cell >= 0 && cell < p.blocks;
+    if (lane == 0) {
+      int n = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      o[i].x = o[i].x * a + e * vs * code_value<FMT>(p.v_codes[at + 2 * i]);
-      o[i].y = o[i].y * a + e * vs * code_value<FMT>(p.v_codes[at + 2 * i + 1]);
+      for (int x = 0; x < kBoxes; ++x) {
+        const int tx = tok0 + x * kBox;
+        n += tx < iu.kv && tx + kBox > (p.window > 0 ? iu.kv - iu.q_len - p.window + 1 : 0);
+      }
+      mbar_arrive_expect_tx(full + s, n * 2 * kBox * D);
+    }
+    __syncwarp();
+    if (lane < 2 * kBoxes) {
+      const bool is_v = lane >= kBoxes;
+      const int64_t blk = good ? cell : 0;   // a bad slot loads block 0 under scale 0: zeros
+      if (in_keys) {
+        tma_load_2d(st + (is_v ? L::kHalf : 0) + box * kBox * D, is_v ? &tm_v : &tm_k, 0,
+                    (int)((blk * p.kv_heads + iu.head) * bs + tok % bs), full + s);
+        if (!good) atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
+      }
+      float* dst = scale_s + s * 4 + lane;
+      if (good) cp_async4(dst, (is_v ? p.v_scale : p.k_scale) + blk * p.kv_heads + iu.head);
+      else *dst = 0.f;
+      cp_async_mbar_arrive(full + s);
+    }
+    __syncwarp();
+    ++issued;
+    ++i_pos;
+  };
+  __syncwarp();
+#pragma unroll 1
+  for (int s = 0; s < S; ++s) issue();
+
+  // ---- units
+  const int lm_row = (lane & 7) + ((lane >> 3) & 1) * 8;   // ldmatrix: row and 16-byte chunk of this lane
+  const int lm_chunk = lane >> 4;
+  int64_t consumed = 0;
+  int64_t pos = begin;
+  while (pos < end) {
+    const int64_t seg_end = min(end, unit_at + unit.steps);
+    const int rows = min(RT, unit.q_len * p.group - unit.rt * RT);
+    const int nact = (rows + 7) / 8;
+    const int row0 = unit.rt * RT;       // first row of the tile within the request
+    // the rows' queries as fp16, and their logit scales
+    for (int r = warp; r < RT; r += kFewWarps) {
+      constexpr int E = D / 64;            // words per lane
+      float2 x[E];
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = make_float2(0.f, 0.f);
+      if (r < rows) {
+        const int tok = unit.q0 + (row0 + r) / p.group, h = unit.head * p.group + (row0 + r) % p.group;
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(
+            (const uint16_t*)p.q.data + tok * p.q.token_stride + h * p.q.head_stride);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          x[i] = unpack_in(bf16, src[lane + 32 * i]);
+          amax = fmaxf(amax, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+        }
+      }
+      float up = 1.f, down = 1.f;
+      if (bf16) fp16_scale(warp_max(amax), up, down);
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        *reinterpret_cast<uint32_t*>(q_s + r * L::kQStride + 2 * (lane + 32 * i)) =
+            pack_half2(x[i].x * up, x[i].y * up);
+      if (lane == 0) rscale_s[r] = p.scale_log2 * down;
+    }
+    __syncthreads();
+    constexpr bool kQRegs = NT <= 2;     // few rows: their fragments stay in registers
+    uint2 qf[kQRegs ? NT : 1][kQRegs ? D / 16 : 1];
+    if constexpr (kQRegs) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c)
+          qf[n][c] = *reinterpret_cast<const uint2*>(q_s + (n * 8 + g) * L::kQStride + c * 16 + 4 * t4);
+    }
+    float rs[NT][2];
+    int limit[NT][2];                     // keys below limit are visible (and at or above limit - window)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = n * 8 + 2 * t4 + c;
+        rs[n][c] = rscale_s[r];
+        limit[n][c] = unit.kv - unit.q_len + (row0 + min(r, rows - 1)) / p.group + 1;
+      }
+    // every row sees keys [all_lo, all_hi)
+    const int all_hi = unit.kv - unit.q_len + row0 / p.group + 1;
+    const int all_lo = p.window > 0 ? unit.kv - unit.q_len + (row0 + rows - 1) / p.group + 1 - p.window : 0;
+    const int any_lo = p.window > 0 ? unit.kv - unit.q_len - p.window + 1 : 0;
+
+    float m[NT][2], l[NT][2], acc[NT][D / 16][4];
+    float vinv = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u) acc[n][u][0] = acc[n][u][1] = acc[n][u][2] = acc[n][u][3] = 0.f;
+    }
+
+#pragma unroll 1
+    for (; pos < seg_end; ++pos) {
+      const int s = (int)(consumed % S);
+      if (ok && !mbar_wait(full + s, (uint32_t)((consumed / S) & 1))) {
+        ok = false;
+        if (lane == 0) atomicOr(p.err, TKV_DEVERR_TIMEOUT);
+      }
+      __syncwarp();
+      const uint32_t tok_ = wait_token();
+      const int tok0 = (unit.step0 + (int)(pos - unit_at)) * kStepTok + warp * kTileTok;
+      uint8_t* st = ring + s * L::kStage;
+      if (tok0 < unit.kv && tok0 + kTileTok > any_lo) {
+        const uint32_t kaddr = after(smem_u32(st), tok_);
+        const bool edge = tok0 + kTileTok > all_hi || tok0 < all_lo;
+        if (tok0 + kTileTok > unit.kv || tok0 < any_lo) {
+          // rows nobody sees may hold anything: their values must not reach the MMA
+          for (int i = lane; i < kTileTok * D / 16; i += 32) {
+            const int tk = tok0 + i / (D / 16);
+            if (tk >= unit.kv || tk < any_lo) *reinterpret_cast<uint4*>(st + L::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();   // the stage's next TMA write comes after these stores
+          __syncwarp();
+        }
+        const uint32_t vaddr = after(kaddr + L::kHalf, wait_token());
+        float ks[kBoxes], vs[kBoxes];
+#pragma unroll
+        for (int b = 0; b < kBoxes; ++b) {
+          ks[b] = scale_s[s * 4 + b];
+          vs[b] = scale_s[s * 4 + kBoxes + b];
+        }
+        // S^T: 2 x 16 tokens, 8 NT rows
+        float sc[NT][2][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) sc[n][h][0] = sc[n][h][1] = sc[n][h][2] = sc[n][h][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 16; c += 2) {
+          uint32_t a[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t off = (uint32_t)((h * 16 + lm_row) * D + (c + lm_chunk) * 16);
+            ldsm_x4(kaddr + swz<kSwz>(off), a[h][0], a[h][1], a[h][2], a[h][3]);
+          }
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            uint32_t f[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              expand4<FMT>(a[h][2 * cc], f[h][0], f[h][2]);
+              expand4<FMT>(a[h][2 * cc + 1], f[h][1], f[h][3]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              if (n < nact) {
+                uint2 b;
+                if constexpr (kQRegs) b = qf[n][c + cc];
+                else b = *reinterpret_cast<const uint2*>(q_s + (n * 8 + g) * L::kQStride + (c + cc) * 16 + 4 * t4);
+                mma_16816(sc[n][0], f[0][0], f[0][1], f[0][2], f[0][3], b.x, b.y);
+                mma_16816(sc[n][1], f[1][0], f[1][1], f[1][2], f[1][3], b.x, b.y);
+              }
+          }
+        }
+        // V's scale relative to the power of two the accumulators carry
+        float vn[kBoxes];
+#pragma unroll
+        for (int b = 0; b < kBoxes; ++b) {
+          if (vs[b] > 0.f && vs[b] < 3e38f && (vinv == 0.f || vs[b] * vinv > 32768.f)) {
+            const float nv = scale_inverse(vs[b]);
+            const float r = vinv == 0.f ? 0.f : nv / vinv;
+            vinv = nv;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int u = 0; u < D / 16; ++u)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[n][u][x] *= r;
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kBoxes; ++b) vn[b] = vs[b] * vinv;
+        uint32_t pb[NT][2][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (n >= nact) continue;
+          float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int c = x & 1;
+              float v = sc[n][h][x] * (ks[h * kBoxes / 2] * rs[n][c]);
+              if (edge) {
+                const int tk = tok0 + h * 16 + g + (x >> 1) * 8;
+                if (tk >= limit[n][c] || (p.window > 0 && tk < limit[n][c] - p.window)) v = -INFINITY;
+              }
+              sc[n][h][x] = v;
+              mx[c] = fmaxf(mx[c], v);
+            }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            mx[0] = fmaxf(mx[0], __shfl_xor_sync(~0u, mx[0], o));
+            mx[1] = fmaxf(mx[1], __shfl_xor_sync(~0u, mx[1], o));
+          }
+          if (__any_sync(~0u, mx[0] > m[n][0] || mx[1] > m[n][1])) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float mn = fmaxf(m[n][c], mx[c]);
+              const float r = mn == -INFINITY ? 1.f : ex2(m[n][c] - mn);
+              m[n][c] = mn;
+              l[n][c] *= r;
+#pragma unroll
+              for (int u = 0; u < D / 16; ++u) {
+                acc[n][u][c] *= r;
+                acc[n][u][2 + c] *= r;
+              }
+            }
+          }
+          const float base[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float e[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float w = ex2(sc[n][h][x] - base[x & 1]);
+              l[n][x & 1] += w;
+              e[x] = w * vn[h * kBoxes / 2];
+              if (edge && sc[n][h][x] == -INFINITY) e[x] = 0.f;   // also under a NaN scale
+            }
+            pb[n][h][0] = movmatrix_t(pack_half2(e[0], e[1]));
+            pb[n][h][1] = movmatrix_t(pack_half2(e[2], e[3]));
+          }
+        }
+        // O^T += V^T P^T: lane (g, t4) owns head_dim elements [g D / 8, (g + 1) D / 8)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          constexpr int W = D / 32;   // words of codes per token and lane
+          uint32_t w[4][W];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int tk = h * 16 + 2 * t4 + (i & 1) + (i >> 1) * 8;
+            const uint32_t ad = vaddr + swz<kSwz>((uint32_t)(tk * D + g * (D / 8)));
+            if constexpr (W == 4) {
+              const uint4 v = lds128(ad);
+              w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
+            } else {
+              const uint2 v = lds64(ad);
+              w[i][0] = v.x, w[i][1] = v.y;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < W; ++j) {
+            uint32_t a0[4], a1[4];   // tokens (2t, 2t+1), (2t+8, 2t+9) of elements 4j .. 4j+3
+            expand_pairs<FMT>(w[0][j], w[1][j], a0);
+            expand_pairs<FMT>(w[2][j], w[3][j], a1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              if (n < nact) {
+                mma_16816(acc[n][2 * j], a0[0], a0[1], a1[0], a1[1], pb[n][h][0], pb[n][h][1]);
+                mma_16816(acc[n][2 * j + 1], a0[2], a0[3], a1[2], a1[3], pb[n][h][0], pb[n][h][1]);
+              }
+          }
+        }
+      }
+      // the fragments' loads come before the stage's reuse: every one of them
+      // feeds the first row tile's accumulators
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u) hold(acc[0][u][0]);
+      ++consumed;
+      __syncwarp();   // every lane has read the stage
+      issue();
+    }
+
+    // ---- the CTA's share of the unit: merge the warps' statistics and accumulators
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(~0u, l[n][c], o);
+        if (g == 0) {
+          stat_s[(warp * RT + n * 8 + 2 * t4 + c) * 2] = m[n][c];
+          stat_s[(warp * RT + n * 8 + 2 * t4 + c) * 2 + 1] = l[n][c];
+        }
+      }
+    __syncthreads();
+    float mm[NT][2], ll[NT][2];
+    const float back = vinv == 0.f ? 0.f : 1.f / vinv;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = n * 8 + 2 * t4 + c;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) mx = fmaxf(mx, stat_s[(w * RT + r) * 2]);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) {
+          const float mw = stat_s[(w * RT + r) * 2], lw = stat_s[(w * RT + r) * 2 + 1];
+          sum += mx == -INFINITY ? lw : lw * ex2(mw - mx);   // no key seen: 0, or NaN logits' sum
+        }
+        mm[n][c] = mx;
+        ll[n][c] = sum;
+        const float f = back * (mx == -INFINITY ? 1.f : ex2(m[n][c] - mx));
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) {
+          acc[n][u][c] *= f;
+          acc[n][u][2 + c] *= f;
+        }
+      }
+    // warps 3 and 2 hand their accumulators to 1 and 0, then 1 to 0
+    auto put = [&](float* dst) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (n < nact)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float* d = dst + (n * 8 + 2 * t4 + c) * L::kMergeStride + g * (D / 8);
+#pragma unroll
+            for (int u = 0; u < D / 16; u += 2)
+              *reinterpret_cast<float4*>(d + 2 * u) =
+                  make_float4(acc[n][u][c], acc[n][u][2 + c], acc[n][u + 1][c], acc[n][u + 1][2 + c]);
+          }
+    };
+    auto add = [&](const float* src) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (n < nact)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float* d = src + (n * 8 + 2 * t4 + c) * L::kMergeStride + g * (D / 8);
+#pragma unroll
+            for (int u = 0; u < D / 16; u += 2) {
+              const float4 v = *reinterpret_cast<const float4*>(d + 2 * u);
+              acc[n][u][c] += v.x;
+              acc[n][u][2 + c] += v.y;
+              acc[n][u + 1][c] += v.z;
+              acc[n][u + 1][2 + c] += v.w;
+            }
+          }
+    };
+    float* buf = merge_s + (warp & 1) * RT * L::kMergeStride;
+    if (warp >= 2) put(buf);
+    __syncthreads();
+    if (warp < 2) add(buf);
+    __syncwarp();
+    if (warp == 1) put(buf);
+    __syncthreads();
+    const int64_t u0 = unit_at, u1 = unit_at + unit.steps;
+    const bool whole = begin <= u0 && end >= u1;
+    const int slot = begin >= u0 ? 0 : 1;
+    float* part = reinterpret_cast<float*>(p.data) + ((int64_t)blockIdx.x * 2 + slot) * RT * (D + 2);
+    if (warp == 0) {
+      add(merge_s + RT * L::kMergeStride);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int r = n * 8 + 2 * t4 + c;
+          if (r >= rows) continue;
+          if (whole) {
+            const float sum = ll[n][c], inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int64_t orow = (int64_t)(unit.q0 + (row0 + r) / p.group) * p.heads + unit.head * p.group +
+                                 (row0 + r) % p.group;
+            uint16_t* o = (uint16_t*)p.out + orow * D + g * (D / 8);
+#pragma unroll
+            for (int u = 0; u < D / 16; u += 4) {
+              uint32_t w[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                w[x] = pack_out(bf16, acc[n][u + x][c] * inv, acc[n][u + x][2 + c] * inv);
+              *reinterpret_cast<uint4*>(o + 2 * u) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            if (g == 0 && p.out_lse) p.out_lse[orow] = sum == 0.f ? -INFINITY : row_lse(mm[n][c], sum);
+          } else {
+            float* d = part + r * D + g * (D / 8);
+#pragma unroll
+            for (int u = 0; u < D / 16; u += 2)
+              *reinterpret_cast<float4*>(d + 2 * u) =
+                  make_float4(acc[n][u][c], acc[n][u][2 + c], acc[n][u + 1][c], acc[n][u + 1][2 + c]);
+            if (g == 0) *reinterpret_cast<float2*>(part + RT * D + r * 2) = make_float2(mm[n][c], ll[n][c]);
+          }
+        }
+    }
+    if (!whole) {
+      // CTAs whose ranges meet this unit: start(c) = total c / ctas
+      const int c0 = (int)(((u0 + 1) * ctas - 1) / total);
+      const int c1 = (int)((u1 * ctas - 1) / total);
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        const uint32_t n = atom_add_acq_rel_gpu(p.counters + c0, 1u);
+        *flag_s = n == (uint32_t)(c1 - c0);
+        if (*flag_s) p.counters[c0] = 0;
+      }
+      __syncthreads();
+      if (*flag_s) {
+        const int64_t stride = (int64_t)2 * RT * (D + 2);
+        // CTA c0's share sits in slot 0 when its range starts at the unit, else in slot 1
+        const float* first = reinterpret_cast<const float*>(p.data) +
+                             ((int64_t)c0 * 2 + (total * c0 / ctas >= u0 ? 0 : 1)) * RT * (D + 2);
+        const float* rest = reinterpret_cast<const float*>(p.data) + (int64_t)c0 * stride;
+        const int parts = c1 - c0 + 1;
+        constexpr int kLanes = D / 4;    // threads of a row
+        for (int r = threadIdx.x / kLanes; r < rows; r += kFewThreads / kLanes) {
+          const int d4 = (threadIdx.x % kLanes) * 4;
+          float mx = -INFINITY;
+          for (int i = 0; i < parts; ++i)
+            mx = fmaxf(mx, __ldcg((i ? rest + i * stride : first) + RT * D + r * 2));
+          float sum = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
+#pragma unroll 4
+          for (int i = 0; i < parts; ++i) {
+            const float* src = i ? rest + i * stride : first;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + RT * D + r * 2));
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(src + r * D + d4));
+            const float f = mx == -INFINITY ? 1.f : ex2(ml.x - mx);
+            sum += ml.y * f;
+            o0 += v.x * f, o1 += v.y * f, o2 += v.z * f, o3 += v.w * f;
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const int64_t orow = (int64_t)(unit.q0 + (row0 + r) / p.group) * p.heads + unit.head * p.group +
+                               (row0 + r) % p.group;
+          *reinterpret_cast<uint2*>((uint16_t*)p.out + orow * D + d4) =
+              make_uint2(pack_out(bf16, o0 * inv, o1 * inv), pack_out(bf16, o2 * inv, o3 * inv));
+          if (d4 == 0 && p.out_lse) p.out_lse[orow] = sum == 0.f ? -INFINITY : row_lse(mx, sum);
+        }
+      }
+    }
+    __syncthreads();   // the shared buffers are free for the next unit
+    if (pos < end) {
+      unit_at += unit.steps;
+      next_unit<RT>(p, bs, unit);
     }
   }
-  uint32_t* op = reinterpret_cast<uint32_t*>((uint16_t*)p.out + w * D) + lane * E;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int i = 0; i < E; ++i) op[i] = pack_out(p.bf16, o[i].x * inv, o[i].y * inv);
-  if (p.out_lse && lane == 0) p.out_lse[w] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  // after a timeout: no copy may still be landing when the CTA exits
+  if (!ok)
+    for (int64_t i = max((int64_t)0, issued - S); i < issued; ++i)
+      mbar_wait(full + i % S, (uint32_t)((i / S) & 1));
 }
 
-void kv8_attention_scratch(int, int, int, int, int, int, size_t* counters, size_t* data) {
-  *counters = 0;
-  *data = 0;
-}
+// ---------------------------------------------------------------- host side
+namespace {
 
-cudaError_t launch_kv8_attention(const AttnParams8& p, int, int d, int format, cudaStream_t stream) {
-  const unsigned grid = (unsigned)(((int64_t)p.tokens * p.heads + 3) / 4);
-  if (d == 128) {
-    if (format == TKV_KV8_INT8) attention_simple_kernel<128, TKV_KV8_INT8><<<grid, 128, 0, stream>>>(p);
-    else attention_simple_kernel<128, TKV_KV8_E4M3><<<grid, 128, 0, stream>>>(p);
-  } else {
-    if (format == TKV_KV8_INT8) attention_simple_kernel<64, TKV_KV8_INT8><<<grid, 128, 0, stream>>>(p);
-    else attention_simple_kernel<64, TKV_KV8_E4M3><<<grid, 128, 0, stream>>>(p);
-  }
+template <int D, int BOXES, int FMT, int NT>
+cudaError_t launch_few(const AttnParams8& p, const CUtensorMap* maps, int sms, cudaStream_t stream) {
+  using L = FewLayout<D, NT>;
+  auto kern = few_rows_kernel<D, BOXES, FMT, NT>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  if (e != cudaSuccess) return e;
+  kern<<<sms * few_ctas_per_sm(NT), kFewThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
   return cudaGetLastError();
+}
+
+template <int D, int BOXES, int FMT>
+cudaError_t few_nt(const AttnParams8& p, const CUtensorMap* maps, int sms, cudaStream_t s) {
+  const int nt = few_row_tiles(p.group, p.max_q_len);
+  if (nt == 1) return launch_few<D, BOXES, FMT, 1>(p, maps, sms, s);
+  if (nt == 2) return launch_few<D, BOXES, FMT, 2>(p, maps, sms, s);
+  return launch_few<D, BOXES, FMT, 4>(p, maps, sms, s);
+}
+
+template <int D>
+cudaError_t few_format(const AttnParams8& p, const CUtensorMap* maps, int sms, int format, cudaStream_t s) {
+  if (p.block_size == 16)
+    return format == TKV_KV8_INT8 ? few_nt<D, 2, TKV_KV8_INT8>(p, maps, sms, s)
+                                  : few_nt<D, 2, TKV_KV8_E4M3>(p, maps, sms, s);
+  return format == TKV_KV8_INT8 ? few_nt<D, 1, TKV_KV8_INT8>(p, maps, sms, s)
+                                : few_nt<D, 1, TKV_KV8_E4M3>(p, maps, sms, s);
+}
+
+}  // namespace
+
+void kv8_attention_scratch(int sms, int d, int group, int max_q_len, int, int, size_t* counters,
+                           size_t* data) {
+  const int nt = few_row_tiles(group, max_q_len);
+  const size_t ctas = (size_t)sms * few_ctas_per_sm(nt);
+  *counters = ctas * sizeof(uint32_t);
+  *data = ctas * 2 * 8 * nt * (d + 2) * sizeof(float);
+}
+
+cudaError_t launch_kv8_attention(const AttnParams8& p, int sms, int d, int format, cudaStream_t stream) {
+  CUtensorMap maps[2];
+  if (!kv8_code_maps(p, d, maps)) return cudaErrorInvalidValue;
+  return d == 128 ? few_format<128>(p, maps, sms, format, stream)
+                  : few_format<64>(p, maps, sms, format, stream);
 }
 
 }  // namespace tkv
