@@ -20,7 +20,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIBNAME = "libtierkv_b200.so"
 SOURCES = ["tkv_api.cu", "tkv_decode.cu", "tkv_quant.cu", "tkv_prefill.cu", "tkv_kv8.cu",
-           "tkv_kv8_attn.cu", "tkv_kv8_api.cu"]
+           "tkv_kv8_attn.cu", "tkv_kv8_umma.cu", "tkv_kv8_api.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -35,6 +35,12 @@ struct AppendParams8 {
   int32_t has_rot;
 };
 
+// A unit of many_rows_kernel split over `parts` CTAs; parts 0: none.
+struct MergeUnit {
+  int32_t parts, slot0;   // the first part's slot in its CTA
+  int32_t q0, row0, head, rows;
+};
+
 struct AttnParams8 {
   tkv_token_view q;
   void* out;
@@ -50,6 +56,9 @@ struct AttnParams8 {
   uint32_t* err;
   uint32_t* counters;
   uint8_t* data;
+  float4* part_o;         // many_rows_kernel: [ctas][2][head_dim / 4][256]
+  float* part_lse;        // [ctas][2][256], log2
+  MergeUnit* merges;      // [ctas]
   int64_t blocks;
   int32_t requests, tokens, heads, kv_heads, group;
   int32_t table_width, max_q_len, window, block_size;
@@ -65,10 +74,12 @@ cudaError_t launch_kv8_append(const AppendParams8& p, int head_dim, int block_si
 
 // Scratch of an attention call: counters (returned to zero by the launch) and
 // partial results.
-void kv8_attention_scratch(int sms, int head_dim, int group, int max_q_len, int requests,
-                           int kv_heads, size_t* counters, size_t* data);
+void kv8_attention_scratch(int sms, int head_dim, int group, int max_q_len, size_t* counters,
+                           size_t* data);
 cudaError_t launch_kv8_attention(const AttnParams8& p, int sms, int head_dim, int format,
                                  cudaStream_t stream);
+cudaError_t launch_many_rows(const AttnParams8& p, int sms, int head_dim, int format, cudaStream_t stream);
+size_t many_rows_scratch(int sms, int head_dim);
 // Tensor maps of the K and V codes as [blocks * kv_heads * block_size][head_dim]
 // bytes, boxes of min(block_size, 32) rows, swizzled by the row's width.
 bool kv8_code_maps(const AttnParams8& p, int head_dim, CUtensorMap maps[2]);

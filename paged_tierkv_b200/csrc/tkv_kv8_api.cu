@@ -211,8 +211,8 @@ int32_t tkv_kv8_attention_workspace(const tkv_kv8_cache* cache, const tkv_kv8_at
   int sms = 0;
   if ((st = device_sms(&sms)) != TKV_OK) return st;
   size_t counters = 0, data = 0;
-  kv8_attention_scratch(sms, cache->head_dim, a->heads / cache->kv_heads, a->max_q_len, a->requests,
-                        cache->kv_heads, &counters, &data);
+  kv8_attention_scratch(sms, cache->head_dim, a->heads / cache->kv_heads, a->max_q_len,
+                        &counters, &data);
   size_t w = 8 * ((counters + kAlign - 1) / kAlign * kAlign);
   const size_t by_data = (data + 2 * kAlign) * 8 / 7 + 8 * kAlign;
   if (by_data > w) w = by_data;
@@ -232,8 +232,7 @@ int32_t tkv_kv8_attention(const tkv_kv8_cache* cache, const tkv_kv8_attention_ar
   if ((st = device_sms(&sms)) != TKV_OK) return st;
   size_t counters = 0, data = 0;
   const int group = a->heads / cache->kv_heads;
-  kv8_attention_scratch(sms, cache->head_dim, group, a->max_q_len, a->requests, cache->kv_heads,
-                        &counters, &data);
+  kv8_attention_scratch(sms, cache->head_dim, group, a->max_q_len, &counters, &data);
   if (!a->workspace || !aligned(a->workspace, 256) || !fits(a->workspace_bytes, counters, data))
     return TKV_ERR_WORKSPACE;
   uint8_t* ws = reinterpret_cast<uint8_t*>(a->workspace);
@@ -265,7 +264,6 @@ int32_t tkv_kv8_attention(const tkv_kv8_cache* cache, const tkv_kv8_attention_ar
   p.scale_log2 = a->scaling * kLog2e;
   p.block_size = cache->block_size;
   p.bf16 = a->dtype == TKV_DTYPE_BF16;
-  p.few_rows_max = 0x7fffffff;
   return cuda_status(launch_kv8_attention(p, sms, cache->head_dim, cache->format,
                                           reinterpret_cast<cudaStream_t>(stream)));
 }

@@ -31,7 +31,7 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
-#include <cstring>
+#include <algorithm>
 
 #include "tkv_kv8.h"
 #include "tkv_kv8_common.cuh"
@@ -39,10 +39,13 @@
 
 namespace tkv {
 
+// Rows per kv head up to which a request runs here.
+constexpr int kFewRowsMax = 64;
+
 // Row tiles of 8 that an instance of the kernel holds, by the most rows a
-// request may have.
+// request of this kernel may have.
 static int few_row_tiles(int group, int max_q_len) {
-  const int64_t rows = (int64_t)group * max_q_len;
+  const int64_t rows = std::min<int64_t>((int64_t)group * max_q_len, kFewRowsMax);
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
 constexpr int few_ctas_per_sm(int nt) { return nt == 4 ? 1 : 2; }
@@ -710,19 +713,27 @@ cudaError_t few_format(const AttnParams8& p, const CUtensorMap* maps, int sms, i
 
 }  // namespace
 
-void kv8_attention_scratch(int sms, int d, int group, int max_q_len, int, int, size_t* counters,
-                           size_t* data) {
+void kv8_attention_scratch(int sms, int d, int group, int max_q_len, size_t* counters, size_t* data) {
   const int nt = few_row_tiles(group, max_q_len);
   const size_t ctas = (size_t)sms * few_ctas_per_sm(nt);
   *counters = ctas * sizeof(uint32_t);
   *data = ctas * 2 * 8 * nt * (d + 2) * sizeof(float);
+  if ((int64_t)group * max_q_len > kFewRowsMax) *data = std::max(*data, many_rows_scratch(sms, d));
 }
 
-cudaError_t launch_kv8_attention(const AttnParams8& p, int sms, int d, int format, cudaStream_t stream) {
-  CUtensorMap maps[2];
-  if (!kv8_code_maps(p, d, maps)) return cudaErrorInvalidValue;
-  return d == 128 ? few_format<128>(p, maps, sms, format, stream)
-                  : few_format<64>(p, maps, sms, format, stream);
+cudaError_t launch_kv8_attention(const AttnParams8& args, int sms, int d, int format, cudaStream_t stream) {
+  AttnParams8 p = args;
+  const bool many = (int64_t)p.group * p.max_q_len > kFewRowsMax;
+  // a lone request needs one kernel: the one for its largest possible size
+  p.few_rows_max = many && p.requests == 1 ? 0 : kFewRowsMax;
+  if (p.few_rows_max > 0) {
+    CUtensorMap maps[2];
+    if (!kv8_code_maps(p, d, maps)) return cudaErrorInvalidValue;
+    const cudaError_t e = d == 128 ? few_format<128>(p, maps, sms, format, stream)
+                                   : few_format<64>(p, maps, sms, format, stream);
+    if (e != cudaSuccess || !many) return e;
+  }
+  return launch_many_rows(p, sms, d, format, stream);
 }
 
 }  // namespace tkv

@@ -1,0 +1,777 @@
+// tkv_kv8_umma.cu -- attention over the 8-bit paged cache for requests with
+// many query rows (prompts, prompt chunks), on the tcgen05 tensor cores.
+//
+// Rows (query token, query head of a kv head's group) are packed into units of
+// 256, two 128-row query tiles that share every K/V tile of 128 tokens.  Per
+// tile the CTA does S_i = Q_i K^T and O_i += P_i V (i = 0, 1), fp16 in, fp32
+// out, all four accumulators in tensor memory:
+//   columns [0, 128) S0, [128, 256) S1, [256, 256 + D) O0, [256 + D, 256 + 2 D) O1,
+// P_i overwriting the first half of S_i as fp16 and feeding the MMA from there.
+// While the tensor core works for one query tile the other one's softmax runs.
+//
+//   warps 0-3, 4-7   softmax of query tile 0, 1: one thread per row, no
+//                    cross-thread reduction; also load Q and write the output
+//   warps 8-11       read K and V codes (16 bytes a lane, one tile ahead),
+//                    expand them to fp16 (exact) and store them in the
+//                    128-byte-swizzled layout that the MMA descriptors name:
+//                    K as K-major rows, V as rows of the MN-major B operand
+//   warp 12          issues the MMAs
+//
+// Scales.  A tile's K scales multiply the logits of their 16 columns in fp32.
+// V's go into the exponent: P' = exp2(s - m + log2(vs vinv)), vinv a power of
+// two that keeps P' in fp16's normal range, and the row sum gets p back by one
+// multiplication with 1 / vs per 16 columns.  m follows the running maximum
+// lazily: O is only rescaled when it has grown by more than 8 (a factor 2^8
+// that fp16 holds).  bf16 queries become fp16 by a power of two per row.
+//
+// Work is a flat list of (unit, K/V tile), cut evenly over the CTAs, so that
+// causal and ragged batches and few rows over a long cache load every SM
+// alike.  A unit that ends up on several CTAs leaves its partial rows (max,
+// sum, accumulator) in the workspace, and merge_rows_kernel joins them.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "tkv_kv8_common.cuh"
+
+namespace tkv {
+
+constexpr int kManyThreads = 416;
+constexpr int kUnitRows = 256;
+constexpr int kTok = 128;                 // tokens of a K/V tile
+constexpr int kGroups = kTok / 16;        // scale groups of a tile
+constexpr uint32_t kManyTmem = 512;
+constexpr float kTinyScale = 7.8886091e-31f;   // 2^-100
+constexpr float kLazy = 8.f;              // growth of the maximum (log2) that P absorbs
+
+template <int D>
+struct ManyLayout {
+  static constexpr int kTile = kTok * D * 2;              // fp16 tile: [D / 64][128][64]
+  static constexpr int kQOff = 0;                         // [2]
+  static constexpr int kKOff = 2 * kTile;                 // [2] stages
+  static constexpr int kVOff = 4 * kTile;                 // [2] stages
+  static constexpr int kScOff = 6 * kTile;                // [4][kGroups] float4 (ks, vs, log2 vs, 1 / vs)
+  static constexpr int kBarOff = kScOff + 4 * kGroups * 16;
+  static constexpr int kNumBars = 32;
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+  static constexpr int kBytes = kMiscOff + 512 + 1024;    // + slack to align the base to 1024
+};
+
+// ---- the flat list of (request, row tile, kv head) units and their K/V tiles
+struct ManyUnit {
+  int req, rt, head;
+  int q0, q_len, kv;
+  int rts;          // row tiles of the request
+  int tile0, n;     // first K/V tile, tiles of the unit
+};
+
+__device__ __forceinline__ void unit_tiles(const AttnParams8& p, ManyUnit& u) {
+  const int first = u.rt * kUnitRows / p.group;
+  const int last = min(u.q_len - 1, (u.rt * kUnitRows + kUnitRows - 1) / p.group);
+  const int hi = max(0, u.kv - u.q_len + last + 1);
+  const int lo = p.window > 0 ? min(max(0, u.kv - u.q_len + first + 1 - p.window), hi) : 0;
+  u.tile0 = lo / kTok;
+  u.n = max(1, (hi + kTok - 1) / kTok - u.tile0);   // one empty tile writes the zeros of unseen rows
+}
+
+__device__ __forceinline__ bool load_many(const AttnParams8& p, int req, ManyUnit& u) {
+  const RequestLens n = request_lens(p, p.block_size, req);
+  u.req = req;
+  u.q0 = n.q0;
+  u.q_len = n.q_len;
+  u.kv = n.kv;
+  u.rts = n.q_len == 0 || n.few_rows(p) ? 0 : (int)(((int64_t)n.q_len * p.group + kUnitRows - 1) / kUnitRows);
+  return u.rts > 0;
+}
+
+__device__ __forceinline__ int64_t many_tiles(const AttnParams8& p, int req) {
+  ManyUnit u;
+  if (!load_many(p, req, u)) return 0;
+  int64_t sum = 0;
+  for (u.rt = 0; u.rt < u.rts; ++u.rt) {
+    unit_tiles(p, u);
+    sum += u.n;
+  }
+  return sum * p.kv_heads;
+}
+
+__device__ __forceinline__ void next_many(const AttnParams8& p, ManyUnit& u) {
+  if (++u.head < p.kv_heads) return;
+  u.head = 0;
+  if (++u.rt < u.rts) {
+    unit_tiles(p, u);
+    return;
+  }
+  u.rt = 0;
+  for (int r = u.req + 1; r < p.requests; ++r)
+    if (load_many(p, r, u)) break;
+  unit_tiles(p, u);
+}
+
+// A CTA's walk: segment after segment of its range, each inside one unit.
+struct Walk {
+  ManyUnit u;
+  int64_t u_at, pos, end;   // flat index of the unit's first tile; of the next tile; of the range's end
+  __device__ __forceinline__ bool more() const { return pos < end; }
+  __device__ __forceinline__ int first() const { return u.tile0 + (int)(pos - u_at); }
+  __device__ __forceinline__ int count() const { return (int)(min(end, u_at + u.n) - pos); }
+  __device__ __forceinline__ int rows(const AttnParams8& p) const {
+    return min(kUnitRows, u.q_len * p.group - u.rt * kUnitRows);
+  }
+  __device__ __forceinline__ void next(const AttnParams8& p) {
+    pos = min(end, u_at + u.n);
+    if (pos < end) {
+      u_at += u.n;
+      next_many(p, u);
+    }
+  }
+};
+
+// ---- tcgen05 helpers
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[32]) {
+  tmem_ld32(taddr, v);
+  // the wait "rewrites" the registers, so no use of them moves above it
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]),
+                 "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]),
+                 "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]),
+                 "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+               :
+               : "memory");
+}
+
+// D[tmem] (+)= A[tmem, fp16 pairs along the columns] * B[smem].
+__device__ __forceinline__ void umma_ts_f16(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Descriptor of the MN-major B operand V: rows of 128 bytes (64 fp16 of N) with
+// 128-byte swizzle, groups of 8 rows (K) 1024 bytes apart (stride offset), the
+// next 64 of N a whole [128][64] panel further (leading offset).
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(kTok * 128 >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kManyThreads, 1)
+    many_rows_kernel(const __grid_constant__ AttnParams8 p) {
+  using L = ManyLayout<D>;
+  extern __shared__ uint8_t many_raw[];
+  const uint32_t raw = smem_u32(many_raw);
+  uint8_t* smem = many_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* q_full = bars;          // [2] 128 arrivals
+  uint64_t* s_full = bars + 2;      // [2] S_i written (commit)
+  uint64_t* p_full = bars + 4;      // [2] 128 arrivals: P_i stored, S_i read
+  uint64_t* o_full = bars + 6;      // [2] O_i updated (commit)
+  uint64_t* k_full = bars + 8;      // [2] 128 arrivals
+  uint64_t* k_empty = bars + 10;    // [2] commit
+  uint64_t* v_full = bars + 12;     // [2] 128 arrivals
+  uint64_t* v_empty = bars + 14;    // [2] commit
+  uint64_t* sc_full = bars + 16;    // [4] 8 arrivals: a tile's scales (reused 4 tiles later)
+  uint64_t* done = bars + 20;
+  float4* scales = reinterpret_cast<float4*>(smem + L::kScOff);
+  int64_t* misc = reinterpret_cast<int64_t*>(smem + L::kMiscOff);
+  MergeUnit* merge_s = reinterpret_cast<MergeUnit*>(smem + L::kMiscOff + 64);
+  uint32_t* taddr_s = reinterpret_cast<uint32_t*>(smem + L::kMiscOff + 256);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 128);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 128);
+      mbar_init(o_full + i, 1);
+      mbar_init(k_full + i, 128);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, 128);
+      mbar_init(v_empty + i, 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(sc_full + i, kGroups);
+    mbar_init(done, 1);
+    fence_mbar_init();
+    *merge_s = MergeUnit{};
+  }
+
+  // ---- this CTA's range of the flat list
+  Walk walk;
+  int64_t total, ctas, begin;
+  {
+    constexpr int kScan = 128;      // threads that own requests
+    const int tid = threadIdx.x;
+    const int per = (p.requests + kScan - 1) / kScan;
+    const int r0 = min(p.requests, tid * per), r1 = tid < kScan ? min(p.requests, r0 + per) : r0;
+    int64_t sum = 0;
+    for (int r = r0; r < r1; ++r) sum += many_tiles(p, r);
+    int64_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(~0u, inc, o);
+      if (lane >= o) inc += x;
+    }
+    if (lane == 31) misc[warp] = inc;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+    for (int w = 0; w < kScan / 32; ++w) {
+      if (w < warp) before += misc[w];
+      total += misc[w];
+    }
+    ctas = min((int64_t)gridDim.x, total);
+    if (blockIdx.x >= ctas) {
+      if (tid == 0) p.merges[blockIdx.x].parts = 0;
+      return;                       // CTA-uniform
+    }
+    begin = total * blockIdx.x / ctas;
+    int64_t at = before + inc - sum;
+    __syncthreads();
+    if (at <= begin && begin < at + sum) {
+      int r = r0;
+      for (;; ++r) {
+        const int64_t n = many_tiles(p, r);
+        if (begin < at + n) break;
+        at += n;
+      }
+      ManyUnit u;
+      load_many(p, r, u);
+      for (u.rt = 0;; ++u.rt) {
+        unit_tiles(p, u);
+        if (begin < at + (int64_t)u.n * p.kv_heads) break;
+        at += (int64_t)u.n * p.kv_heads;
+      }
+      misc[0] = at;
+      misc[1] = r;
+      misc[2] = u.rt;
+    }
+    __syncthreads();
+    load_many(p, (int)misc[1], walk.u);
+    walk.u.rt = (int)misc[2];
+    unit_tiles(p, walk.u);
+    walk.u.head = (int)((begin - misc[0]) / walk.u.n);
+    walk.u_at = misc[0] + (int64_t)walk.u.head * walk.u.n;
+    walk.pos = begin;
+    walk.end = total * (blockIdx.x + 1) / ctas;
+  }
+  if (warp == 12) tmem_alloc(taddr_s, kManyTmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *taddr_s;
+  bool ok = true;
+
+  if (warp >= 8 && warp < 12) {
+    // ---- K and V: codes -> fp16 tiles
+    constexpr int kPerRow = D / 16;              // 16-byte chunks of a row of codes
+    constexpr int kPasses = kPerRow;             // 128 threads x 16 bytes cover 128 / kPerRow rows
+    constexpr int kPassRows = 128 / kPerRow;
+    const int t = threadIdx.x - 256;
+    const int row = t / kPerRow, c16 = t % kPerRow;
+    const int bs = p.block_size;
+    // fp16 chunks 2 c16, 2 c16 + 1 of the row: panel c16 / 4, 16-byte chunk 2 (c16 % 4)
+    // within its 128-byte line; lanes of the second panel store in the other
+    // order so that one row's eight lanes hit all banks
+    const int swap = kPerRow == 8 ? c16 >> 2 : 0;
+    uint4 kc[kPasses], vc[kPasses];
+    int32_t cell[kPasses];
+    int32_t s_cell = -1;
+    float s_k = 0.f, s_v = 0.f;
+    Walk ahead = walk;                           // the tile whose cells are loaded next
+    int a_i = 0;
+    int req_kv = 0, req_lo = 0, head = 0;        // of the tile in `cell`
+    int tok_base = 0;
+    auto load_cells = [&]() {
+      if (!ahead.more()) {
+        req_kv = 0;
+        req_lo = 0;
+        tok_base = 0;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) cell[i] = -1;
+        s_cell = -1;
+        return;
+      }
+      tok_base = (ahead.first() + a_i) * kTok;
+      req_kv = ahead.u.kv;
+      head = ahead.u.head;
+      req_lo = p.window > 0 ? max(0, ahead.u.kv - ahead.u.q_len - p.window + 1) : 0;
+      const int32_t* tab = p.table + ahead.u.req * p.table_stride;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int tok = tok_base + i * kPassRows + row;
+        cell[i] = tok >= req_lo && tok < req_kv ? tab[tok / bs] : -1;
+      }
+      const int tok = tok_base + t * 16;
+      s_cell = t < kGroups && tok + 15 >= req_lo && tok < req_kv ? tab[tok / bs] : -1;
+      if (++a_i == ahead.count()) {
+        ahead.next(p);
+        a_i = 0;
+      }
+    };
+    auto load_codes = [&](const uint8_t* codes, uint4 (&x)[kPasses]) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int tok = tok_base + i * kPassRows + row;
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (cell[i] >= 0 && cell[i] < p.blocks)
+          x[i] = __ldg(reinterpret_cast<const uint4*>(
+              codes + (((int64_t)cell[i] * p.kv_heads + head) * bs + tok % bs) * D + c16 * 16));
+      }
+    };
+    auto store_tile = [&](uint8_t* tile, const uint4 (&x)[kPasses]) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kPassRows + row;
+        uint4 f[2];
+        expand4<FMT>(x[i].x, f[0].x, f[0].y);
+        expand4<FMT>(x[i].y, f[0].z, f[0].w);
+        expand4<FMT>(x[i].z, f[1].x, f[1].y);
+        expand4<FMT>(x[i].w, f[1].z, f[1].w);
+        uint8_t* line = tile + ((c16 >> 2) * kTok + r) * 128;
+        const int c = 2 * (c16 & 3);
+        const uint4 first = swap ? f[1] : f[0], second = swap ? f[0] : f[1];
+        *reinterpret_cast<uint4*>(line + (((c + swap) ^ (r & 7)) << 4)) = first;
+        *reinterpret_cast<uint4*>(line + (((c + 1 - swap) ^ (r & 7)) << 4)) = second;
+      }
+    };
+    auto load_scales = [&]() {
+      s_k = s_v = 0.f;
+      if (s_cell >= 0 && s_cell < p.blocks) {
+        s_k = p.k_scale[(int64_t)s_cell * p.kv_heads + head];
+        s_v = p.v_scale[(int64_t)s_cell * p.kv_heads + head];
+      } else if (t < kGroups && tok_base + t * 16 + 15 >= req_lo && tok_base + t * 16 < req_kv) {
+        atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
+      }
+    };
+    load_cells();
+    load_codes(p.k_codes, kc);
+    load_codes(p.v_codes, vc);
+    load_scales();
+    const int64_t n = walk.end - walk.pos;
+    for (int64_t j = 0; j < n; ++j) {
+      const int s = (int)(j & 1);
+      const uint32_t ph = (uint32_t)((j >> 1) & 1);
+      if (t < kGroups) {
+        // a V scale of 0 counts as 2^-100: its values stay below any output's
+        // last bit, and the row sum gets the group's p back
+        const float vs = s_v < kTinyScale ? kTinyScale : s_v;
+        scales[(j & 3) * kGroups + t] = make_float4(s_k, vs, lg2(vs), 1.f / vs);
+        mbar_arrive(sc_full + (j & 3));
+      }
+      if (ok && !mbar_wait(k_empty + s, ph ^ 1)) ok = false;
+      store_tile(smem + L::kKOff + s * L::kTile, kc);
+      fence_proxy_async();
+      mbar_arrive(k_full + s);
+      load_cells();                              // tile j + 1
+      load_codes(p.k_codes, kc);
+      if (ok && !mbar_wait(v_empty + s, ph ^ 1)) ok = false;
+      store_tile(smem + L::kVOff + s * L::kTile, vc);
+      fence_proxy_async();
+      mbar_arrive(v_full + s);
+      load_codes(p.v_codes, vc);
+      load_scales();
+    }
+  } else if (warp == 12) {
+    // ---- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t kIdescQK = umma_idesc_f16_f32(128, kTok);
+      constexpr uint32_t kIdescPV = umma_idesc_f16_f32(128, D) | (1u << 16);   // B is MN-major
+      const uint32_t base = smem_u32(smem);
+      int64_t g = 0;                             // tiles done before this segment
+      int64_t g1 = 0;                            // the same, counting query tile 1's only
+      int seg = 0, seg1 = 0;
+      auto qk = [&](int i, int s) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (uint32_t)((ks >> 2) * kTok * 128 + (ks & 3) * 32);
+          umma_f16(tmem + i * kTok, umma_desc_k_sw128(base + L::kQOff + i * L::kTile + off),
+                   umma_desc_k_sw128(base + L::kKOff + s * L::kTile + off), kIdescQK, ks > 0);
+        }
+        umma_commit(s_full + i);
+      };
+      auto pv = [&](int i, int s, bool first) {
+#pragma unroll
+        for (int ks = 0; ks < kTok / 16; ++ks)
+          umma_ts_f16(tmem + 256 + i * D, tmem + i * kTok + ks * 8,
+                      umma_desc_mn_sw128(base + L::kVOff + s * L::kTile + ks * 2048), kIdescPV,
+                      ks > 0 || !first);
+        umma_commit(o_full + i);
+      };
+      auto wait = [&](uint64_t* bar, int64_t phase) {
+        if (ok && !mbar_wait(bar, (uint32_t)(phase & 1))) ok = false;
+      };
+      for (Walk w = walk; w.more(); w.next(p)) {
+        const int n = w.count();
+        const bool two = w.rows(p) > 128;
+        wait(q_full, seg);
+        if (two) wait(q_full + 1, seg1);
+        wait(k_full + (g & 1), g >> 1);
+        tc_fence_after();
+        if (!ok) break;
+        qk(0, (int)(g & 1));
+        if (two) qk(1, (int)(g & 1));
+        umma_commit(k_empty + (g & 1));
+        for (int j = 0; j < n; ++j) {
+          const int64_t at = g + j;
+          const int s = (int)(at & 1), s2 = s ^ 1;
+          if (j + 1 < n) wait(k_full + s2, (at + 1) >> 1);
+          wait(v_full + s, at >> 1);
+          wait(p_full, at);
+          tc_fence_after();
+          if (!ok) break;
+          pv(0, s, j == 0);
+          if (j + 1 < n) qk(0, s2);
+          if (two) {
+            wait(p_full + 1, g1 + j);
+            tc_fence_after();
+            if (!ok) break;
+            pv(1, s, j == 0);
+          }
+          umma_commit(v_empty + s);
+          if (j + 1 < n) {
+            if (two) qk(1, s2);
+            umma_commit(k_empty + s2);
+          }
+        }
+        if (!ok) break;
+        g += n;
+        ++seg;
+        if (two) {
+          g1 += n;
+          ++seg1;
+        }
+      }
+      umma_commit(done);            // every MMA issued above has completed once this phase does
+      ok = mbar_wait(done, 0) && ok;
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: thread t owns row t of query tile i
+    const int i = warp >> 2;
+    const int t = threadIdx.x & 127;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const uint32_t s_col = lane_base + i * kTok, o_col = lane_base + 256 + i * D;
+    const bool bf16 = p.bf16 != 0;
+    int64_t sc_at = 0;              // tiles of the walk before this segment (scale slots)
+    int64_t at = 0;                 // tiles this query tile has done
+    for (Walk w = walk; w.more(); w.next(p)) {
+      const int n = w.count(), rows = w.rows(p);
+      if (i * 128 >= rows) {        // tile 1 of a unit of up to 128 rows
+        sc_at += n;
+        continue;
+      }
+      const int r = i * 128 + t;
+      const bool live = r < rows;
+      const int urow = w.u.rt * kUnitRows + min(r, rows - 1);
+      const int tok = urow / p.group;               // query token within the request
+      const int64_t orow = (int64_t)(w.u.q0 + tok) * p.heads + w.u.head * p.group + urow % p.group;
+      float rscale = p.scale_log2;
+      {
+        // Q row -> fp16, K-major 128-byte-swizzled
+        const uint16_t* src = (const uint16_t*)p.q.data + (w.u.q0 + tok) * p.q.token_stride +
+                              (int64_t)(w.u.head * p.group + urow % p.group) * p.q.head_stride;
+        uint8_t* tile = smem + L::kQOff + i * L::kTile;
+        float up = 1.f, down = 1.f;
+        if (bf16) {
+          float amax = 0.f;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src + c * 8);
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = unpack_in(true, x[k]);
+              amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+          fp16_scale(amax, up, down);
+        }
+        rscale *= down;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 v = *reinterpret_cast<const uint4*>(src + c * 8);
+          if (bf16) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = unpack_in(true, x[k]);
+              x[k] = pack_half2(f.x * up, f.y * up);
+            }
+          }
+          *reinterpret_cast<uint4*>(tile + ((c >> 3) * kTok + t) * 128 + (((c & 7) ^ (t & 7)) << 4)) = v;
+        }
+        fence_proxy_async();
+        mbar_arrive(q_full + i);
+      }
+      const int hi = w.u.kv - w.u.q_len + tok + 1;            // keys [lo, hi) are visible
+      const int lo = p.window > 0 ? hi - p.window : 0;
+      // the tile's rows all see keys [all_lo, all_hi)
+      const int all_hi = w.u.kv - w.u.q_len + (w.u.rt * kUnitRows + i * 128) / p.group + 1;
+      const int all_lo = p.window > 0 ? w.u.kv - w.u.q_len + (w.u.rt * kUnitRows + min(rows, i * 128 + 128) - 1) /
+                                                                 p.group + 1 - p.window : 0;
+      float m = -INFINITY, l = 0.f;       // reference of the exponents (log2), sum in units of vinv
+      float vlog = 0.f;                   // log2 vinv
+      bool vset = false;
+      const int tile0 = w.first();
+      for (int j = 0; j < n; ++j, ++at, ++sc_at) {
+        const float4* sc = scales + (sc_at & 3) * kGroups;
+        if (ok && !mbar_wait(s_full + i, (uint32_t)(at & 1))) ok = false;
+        // complete by now; the wait orders the scales' reads
+        if (ok && !mbar_wait(sc_full + (sc_at & 3), (uint32_t)((sc_at >> 2) & 1))) ok = false;
+        __syncwarp();
+        tc_fence_after();
+        const int k0 = (tile0 + j) * kTok;
+        const bool edge = k0 + kTok > all_hi || k0 < all_lo;
+        // pass 1: the row's maximum
+        float mx = -INFINITY;
+        float vmax = kTinyScale;
+#pragma unroll
+        for (int c = 0; c < kTok / 32; ++c) {
+          uint32_t v[32];
+          tmem_load(s_col + c * 32, v);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float a = -INFINITY;
+            if (edge) {
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                const int key = k0 + c * 32 + h * 16 + x;
+                a = fmaxf(a, key < hi && key >= lo ? __uint_as_float(v[h * 16 + x]) : -INFINITY);
+              }
+            } else {
+#pragma unroll
+              for (int x = 0; x < 16; ++x) a = fmaxf(a, __uint_as_float(v[h * 16 + x]));
+            }
+            const float4 g = sc[c * 2 + h];
+            // no key of the group: -inf whatever its scale (0 where nothing is stored)
+            mx = fmaxf(mx, a == -INFINITY ? a : a * g.x);
+            if (g.y < 3e38f) vmax = fmaxf(vmax, g.y);
+          }
+        }
+        mx *= rscale;
+        // V's power of two: set by the first tile, moved when a scale outgrows it
+        float shift = 0.f;                            // log2 of the factor O and l take
+        if (!vset || lg2(vmax) + vlog > 7.f) {
+          const float nv = 6.f - ceilf(lg2(vmax));
+          shift = vset ? nv - vlog : 0.f;
+          vlog = nv;
+          vset = true;
+        }
+        if (mx > m + kLazy || (m == -INFINITY && mx > -INFINITY)) {
+          shift += m == -INFINITY ? 0.f : m - mx;     // nothing summed yet: nothing to rescale
+          m = mx;
+        }
+        if (__any_sync(~0u, shift != 0.f)) {
+          const float f = ex2(shift);
+          l *= f;
+          if (j > 0) {
+            if (ok && !mbar_wait(o_full + i, (uint32_t)((at - 1) & 1))) ok = false;
+            __syncwarp();
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t v[32], a[16], b[16];
+              tmem_load(o_col + c * 32, v);
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                a[x] = __float_as_uint(__uint_as_float(v[x]) * f);
+                b[x] = __float_as_uint(__uint_as_float(v[16 + x]) * f);
+              }
+              tmem_st16(o_col + c * 32, a);
+              tmem_st16(o_col + c * 32 + 16, b);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        // pass 2: P' and the sum
+#pragma unroll
+        for (int c = 0; c < kTok / 32; ++c) {
+          uint32_t v[32], pk[16];
+          tmem_load(s_col + c * 32, v);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 g = sc[c * 2 + h];
+            const float mul = g.x * rscale, add = (g.z + vlog) - base;
+            float sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 16; x += 2) {
+              float e0 = ex2(fmaf(__uint_as_float(v[h * 16 + x]), mul, add));
+              float e1 = ex2(fmaf(__uint_as_float(v[h * 16 + x + 1]), mul, add));
+              if (edge) {
+                const int key = k0 + c * 32 + h * 16 + x;
+                e0 = key < hi && key >= lo ? e0 : 0.f;
+                e1 = key + 1 < hi && key + 1 >= lo ? e1 : 0.f;
+              }
+              sum += e0 + e1;
+              pk[h * 8 + x / 2] = pack_half2(e0, e1);
+            }
+            if (sum != 0.f) l = fmaf(sum, g.w, l);    // a masked group's scale does not count
+          }
+          tmem_st16(s_col + c * 16, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_full + i);
+      }
+      // ---- the segment's rows
+      if (ok && !mbar_wait(o_full + i, (uint32_t)((at - 1) & 1))) ok = false;
+      __syncwarp();
+      tc_fence_after();
+      const int64_t u1 = w.u_at + w.u.n;
+      const bool whole = w.pos == w.u_at && w.end >= u1;
+      const int slot = begin >= w.u_at ? 0 : 1;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float4* part = p.part_o + ((int64_t)blockIdx.x * 2 + slot) * (D / 4) * kUnitRows + r;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t v[32];
+        tmem_load(o_col + c * 32, v);
+        if (whole && live) {
+          uint4* dst = reinterpret_cast<uint4*>((uint16_t*)p.out + orow * D + c * 32);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              o[k] = pack_out(bf16, __uint_as_float(v[x * 8 + 2 * k]) * inv,
+                              __uint_as_float(v[x * 8 + 2 * k + 1]) * inv);
+            dst[x] = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        } else if (live) {
+          // partials as shares of the row's mass: scale-free across CTAs
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            part[(c * 8 + x) * kUnitRows] =
+                make_float4(__uint_as_float(v[4 * x]) * inv, __uint_as_float(v[4 * x + 1]) * inv,
+                            __uint_as_float(v[4 * x + 2]) * inv, __uint_as_float(v[4 * x + 3]) * inv);
+        }
+      }
+      if (live) {
+        // l = sum of p * vinv
+        const float lse2 = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + lg2(l) - vlog;
+        if (whole) {
+          if (p.out_lse) p.out_lse[orow] = lse2 * kLn2;
+        } else {
+          p.part_lse[((int64_t)blockIdx.x * 2 + slot) * kUnitRows + r] = lse2;
+        }
+      }
+      if (i == 0 && t == 0 && !whole && w.pos == w.u_at) {
+        // the unit's first CTA names the merge, over CTAs up to the one whose
+        // range (start(c) = total c / ctas) holds the unit's last tile
+        MergeUnit mu;
+        mu.parts = (int)((u1 * ctas - 1) / total) - (int)blockIdx.x + 1;
+        mu.slot0 = slot;
+        mu.q0 = w.u.q0;
+        mu.row0 = w.u.rt * kUnitRows;
+        mu.head = w.u.head;
+        mu.rows = rows;
+        *merge_s = mu;
+      }
+      tc_fence_before();
+    }
+  }
+  if (!ok) atomicOr(p.err, TKV_DEVERR_TIMEOUT);
+  // every TMEM access and MMA of the CTA has completed
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0)
+    p.merges[blockIdx.x] = *merge_s;
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_free(tmem, kManyTmem);
+  }
+}
+
+// Joins the partial rows of a split unit: CTA (c, y) takes 32 elements of every
+// row of the unit that starts in CTA c of many_rows_kernel and ends in a later one.
+template <int D>
+__global__ void __launch_bounds__(kUnitRows) merge_rows_kernel(const __grid_constant__ AttnParams8 p) {
+  const MergeUnit u = p.merges[blockIdx.x];
+  const int r = threadIdx.x;
+  if (u.parts == 0 || r >= u.rows) return;
+  // part 0 sits in slot0 of CTA c, the others in slot 0 of theirs
+  auto at = [&](int i) { return ((int64_t)(blockIdx.x + i) * 2 + (i ? 0 : u.slot0)); };
+  float mx = -INFINITY;
+  for (int i = 0; i < u.parts; ++i) mx = fmaxf(mx, p.part_lse[at(i) * kUnitRows + r]);
+  float4 o[8] = {};
+  float sum = 0.f;
+  for (int i = 0; i < u.parts; ++i) {
+    const float lse = p.part_lse[at(i) * kUnitRows + r];
+    const float f = lse == -INFINITY ? 0.f : ex2(lse - mx);
+    sum += f;
+    if (f == 0.f) continue;       // also skips NaN-free empties; a NaN weight is not 0
+    const float4* src = p.part_o + (at(i) * (D / 4) + blockIdx.y * 8) * kUnitRows + r;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float4 v = src[x * kUnitRows];
+      o[x].x += v.x * f;
+      o[x].y += v.y * f;
+      o[x].z += v.z * f;
+      o[x].w += v.w * f;
+    }
+  }
+  const int urow = u.row0 + r;
+  const int64_t orow = (int64_t)(u.q0 + urow / p.group) * p.heads + u.head * p.group + urow % p.group;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const bool bf16 = p.bf16 != 0;
+  uint4* dst = reinterpret_cast<uint4*>((uint16_t*)p.out + orow * D + blockIdx.y * 32);
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    dst[x] = make_uint4(pack_out(bf16, o[2 * x].x * inv, o[2 * x].y * inv),
+                        pack_out(bf16, o[2 * x].z * inv, o[2 * x].w * inv),
+                        pack_out(bf16, o[2 * x + 1].x * inv, o[2 * x + 1].y * inv),
+                        pack_out(bf16, o[2 * x + 1].z * inv, o[2 * x + 1].w * inv));
+  if (blockIdx.y == 0 && p.out_lse) p.out_lse[orow] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
+}
+
+// ---------------------------------------------------------------- host side
+size_t many_rows_scratch(int sms, int d) {
+  return (size_t)sms * 2 * kUnitRows * (d + 1) * sizeof(float) + (size_t)sms * sizeof(MergeUnit) + 512;
+}
+
+namespace {
+template <int D, int FMT>
+cudaError_t launch_many(AttnParams8 p, int sms, cudaStream_t stream) {
+  using L = ManyLayout<D>;
+  uint8_t* at = p.data;
+  p.part_o = reinterpret_cast<float4*>(at);
+  at += (size_t)sms * 2 * kUnitRows * D * sizeof(float);
+  p.part_lse = reinterpret_cast<float*>(at);
+  at += (size_t)sms * 2 * kUnitRows * sizeof(float);
+  p.merges = reinterpret_cast<MergeUnit*>(at);
+  auto kern = many_rows_kernel<D, FMT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  if (e != cudaSuccess) return e;
+  kern<<<sms, kManyThreads, L::kBytes, stream>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  merge_rows_kernel<D><<<dim3(sms, D / 32), kUnitRows, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+}  // namespace
+
+cudaError_t launch_many_rows(const AttnParams8& p, int sms, int d, int format, cudaStream_t stream) {
+  if (d == 128)
+    return format == TKV_KV8_INT8 ? launch_many<128, TKV_KV8_INT8>(p, sms, stream)
+                                  : launch_many<128, TKV_KV8_E4M3>(p, sms, stream);
+  return format == TKV_KV8_INT8 ? launch_many<64, TKV_KV8_INT8>(p, sms, stream)
+                                : launch_many<64, TKV_KV8_E4M3>(p, sms, stream);
+}
+
+}  // namespace tkv
