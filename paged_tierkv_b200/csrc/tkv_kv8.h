@@ -65,6 +65,13 @@ struct AttnParams8 {
   int32_t bf16;          // q and out are bf16 (else fp16)
   int32_t few_rows_max;  // rows per kv head of the requests that few_rows_kernel takes
   float scale_log2;
+  uint32_t group_inv;    // ceil(2^32 / group) for 1 < group <= 64
+#ifdef __CUDACC__
+  // row / group for a row of a request: exact for row < 2^26
+  __device__ __forceinline__ int token_of(int row) const {
+    return group == 1 ? row : (int)__umulhi((uint32_t)row, group_inv);
+  }
+#endif
 };
 
 cudaError_t launch_plan_step(const tkv_kv8_plan_args& p, cudaStream_t stream);

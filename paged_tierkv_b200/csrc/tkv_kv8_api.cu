@@ -73,6 +73,7 @@ int32_t check_attention(const tkv_kv8_cache* c, const tkv_kv8_attention_args* a)
   if (a->requests < 1 || a->requests > TKV_KV8_MAX_REQUESTS) return TKV_ERR_INVALID;
   if (a->tokens < 0 || a->heads <= 0 || a->heads % c->kv_heads) return TKV_ERR_INVALID;
   if (a->heads / c->kv_heads > 64) return TKV_ERR_UNSUPPORTED;
+  if ((int64_t)a->tokens * (a->heads / c->kv_heads) >= (int64_t(1) << 26)) return TKV_ERR_UNSUPPORTED;
   if (a->dtype != TKV_DTYPE_F16 && a->dtype != TKV_DTYPE_BF16) return TKV_ERR_UNSUPPORTED;
   if (a->max_q_len < 0 || a->window < 0) return TKV_ERR_INVALID;
   if (a->table_width < 0 || a->table_stride < a->table_width ||
@@ -262,6 +263,7 @@ int32_t tkv_kv8_attention(const tkv_kv8_cache* cache, const tkv_kv8_attention_ar
   p.max_q_len = a->max_q_len;
   p.window = a->window;
   p.scale_log2 = a->scaling * kLog2e;
+  p.group_inv = group > 1 ? (uint32_t)(((uint64_t(1) << 32) + group - 1) / group) : 0;
   p.block_size = cache->block_size;
   p.bf16 = a->dtype == TKV_DTYPE_BF16;
   return cuda_status(launch_kv8_attention(p, sms, cache->head_dim, cache->format,

@@ -724,8 +724,9 @@ void kv8_attention_scratch(int sms, int d, int group, int max_q_len, size_t* cou
 cudaError_t launch_kv8_attention(const AttnParams8& args, int sms, int d, int format, cudaStream_t stream) {
   AttnParams8 p = args;
   const bool many = (int64_t)p.group * p.max_q_len > kFewRowsMax;
-  // a lone request needs one kernel: the one for its largest possible size
-  p.few_rows_max = many && p.requests == 1 ? 0 : kFewRowsMax;
+  // a lone request needs one kernel: the one for its largest possible size; and
+  // without a request that max_q_len calls long, this kernel takes all
+  p.few_rows_max = !many ? 0x7fffffff : p.requests == 1 ? 0 : kFewRowsMax;
   if (p.few_rows_max > 0) {
     CUtensorMap maps[2];
     if (!kv8_code_maps(p, d, maps)) return cudaErrorInvalidValue;

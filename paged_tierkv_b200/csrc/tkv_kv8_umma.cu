@@ -10,12 +10,14 @@
 // While the tensor core works for one query tile the other one's softmax runs.
 //
 //   warps 0-3, 4-7   softmax of query tile 0, 1: one thread per row, no
-//                    cross-thread reduction; also load Q and write the output
-//   warps 8-11       read K and V codes (16 bytes a lane, one tile ahead),
+//                    cross-thread reduction; also load Q, write the output, and
+//                    one thread of each issues its tile's MMAs (twelve warps
+//                    leave 168 registers a thread; a thirteenth for the MMAs
+//                    would leave 128)
+//   warps 8-11       read K and V codes (16 bytes a lane, a tile ahead),
 //                    expand them to fp16 (exact) and store them in the
 //                    128-byte-swizzled layout that the MMA descriptors name:
 //                    K as K-major rows, V as rows of the MN-major B operand
-//   warp 12          issues the MMAs
 //
 // Scales.  A tile's K scales multiply the logits of their 16 columns in fp32.
 // V's go into the exponent: P' = exp2(s - m + log2(vs vinv)), vinv a power of
@@ -24,9 +26,10 @@
 // lazily: O is only rescaled when it has grown by more than 8 (a factor 2^8
 // that fp16 holds).  bf16 queries become fp16 by a power of two per row.
 //
-// Work is a flat list of (unit, K/V tile), cut evenly over the CTAs, so that
-// causal and ragged batches and few rows over a long cache load every SM
-// alike.  A unit that ends up on several CTAs leaves its partial rows (max,
+// Work is a flat list of (unit, K/V tile), where a unit counts kUnitCost tiles
+// more than it has (loading Q, writing the output), cut evenly over the CTAs,
+// so that causal and ragged batches and few rows over a long cache load every
+// SM alike.  A unit that ends up on several CTAs leaves its partial rows (max,
 // sum, accumulator) in the workspace, and merge_rows_kernel joins them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,10 +39,11 @@
 
 namespace tkv {
 
-constexpr int kManyThreads = 416;
+constexpr int kManyThreads = 384;
 constexpr int kUnitRows = 256;
 constexpr int kTok = 128;                 // tokens of a K/V tile
 constexpr int kGroups = kTok / 16;        // scale groups of a tile
+constexpr int kUnitCost = 2;              // a unit's fixed cost in tiles
 constexpr uint32_t kManyTmem = 512;
 constexpr float kTinyScale = 7.8886091e-31f;   // 2^-100
 constexpr float kLazy = 8.f;              // growth of the maximum (log2) that P absorbs
@@ -52,8 +56,9 @@ struct ManyLayout {
   static constexpr int kVOff = 4 * kTile;                 // [2] stages
   static constexpr int kScOff = 6 * kTile;                // [4][kGroups] float4 (ks, vs, log2 vs, 1 / vs)
   static constexpr int kBarOff = kScOff + 4 * kGroups * 16;
-  static constexpr int kNumBars = 32;
-  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+  static constexpr int kNumBars = 16;
+  static constexpr int kRowOff = kBarOff + kNumBars * 8;  // [256] logit scale of each row
+  static constexpr int kMiscOff = kRowOff + kUnitRows * 4;
   static constexpr int kBytes = kMiscOff + 512 + 1024;    // + slack to align the base to 1024
 };
 
@@ -62,12 +67,13 @@ struct ManyUnit {
   int req, rt, head;
   int q0, q_len, kv;
   int rts;          // row tiles of the request
+  int req_lo;       // first key that any of its tokens sees
   int tile0, n;     // first K/V tile, tiles of the unit
 };
 
 __device__ __forceinline__ void unit_tiles(const AttnParams8& p, ManyUnit& u) {
-  const int first = u.rt * kUnitRows / p.group;
-  const int last = min(u.q_len - 1, (u.rt * kUnitRows + kUnitRows - 1) / p.group);
+  const int first = p.token_of(u.rt * kUnitRows);
+  const int last = min(u.q_len - 1, p.token_of(u.rt * kUnitRows + kUnitRows - 1));
   const int hi = max(0, u.kv - u.q_len + last + 1);
   const int lo = p.window > 0 ? min(max(0, u.kv - u.q_len + first + 1 - p.window), hi) : 0;
   u.tile0 = lo / kTok;
@@ -80,6 +86,7 @@ __device__ __forceinline__ bool load_many(const AttnParams8& p, int req, ManyUni
   u.q0 = n.q0;
   u.q_len = n.q_len;
   u.kv = n.kv;
+  u.req_lo = n.first_key(p);
   u.rts = n.q_len == 0 || n.few_rows(p) ? 0 : (int)(((int64_t)n.q_len * p.group + kUnitRows - 1) / kUnitRows);
   return u.rts > 0;
 }
@@ -90,7 +97,7 @@ __device__ __forceinline__ int64_t many_tiles(const AttnParams8& p, int req) {
   int64_t sum = 0;
   for (u.rt = 0; u.rt < u.rts; ++u.rt) {
     unit_tiles(p, u);
-    sum += u.n;
+    sum += u.n + kUnitCost;
   }
   return sum * p.kv_heads;
 }
@@ -108,22 +115,25 @@ __device__ __forceinline__ void next_many(const AttnParams8& p, ManyUnit& u) {
   unit_tiles(p, u);
 }
 
-// A CTA's walk: segment after segment of its range, each inside one unit.
+// A CTA's walk over the segments of its range, each inside one unit.  A unit
+// takes kUnitCost + n places of the flat list: its tiles are the last n, so a
+// range that ends before them has none of the unit.
 struct Walk {
   ManyUnit u;
-  int64_t u_at, pos, end;   // flat index of the unit's first tile; of the next tile; of the range's end
-  __device__ __forceinline__ bool more() const { return pos < end; }
-  __device__ __forceinline__ int first() const { return u.tile0 + (int)(pos - u_at); }
-  __device__ __forceinline__ int count() const { return (int)(min(end, u_at + u.n) - pos); }
+  int64_t u_at, begin, end;   // flat place of the unit, and the CTA's range
+  __device__ __forceinline__ int64_t u_end() const { return u_at + kUnitCost + u.n; }
+  __device__ __forceinline__ int64_t tiles_at() const { return u_at + kUnitCost; }
+  __device__ __forceinline__ bool more() const { return tiles_at() < end; }
+  __device__ __forceinline__ int skipped() const { return (int)max((int64_t)0, begin - tiles_at()); }
+  __device__ __forceinline__ int first() const { return u.tile0 + skipped(); }
+  __device__ __forceinline__ int count() const { return (int)(min(end, u_end()) - tiles_at()) - skipped(); }
+  __device__ __forceinline__ bool whole() const { return begin <= tiles_at() && end >= u_end(); }
   __device__ __forceinline__ int rows(const AttnParams8& p) const {
     return min(kUnitRows, u.q_len * p.group - u.rt * kUnitRows);
   }
   __device__ __forceinline__ void next(const AttnParams8& p) {
-    pos = min(end, u_at + u.n);
-    if (pos < end) {
-      u_at += u.n;
-      next_many(p, u);
-    }
+    u_at = u_end();
+    if (u_at < end) next_many(p, u);
   }
 };
 
@@ -138,8 +148,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[32]) {
-  tmem_ld32(taddr, v);
+__device__ __forceinline__ void tmem_wait_into(uint32_t (&v)[32]) {
   // the wait "rewrites" the registers, so no use of them moves above it
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
@@ -149,6 +158,11 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[32]) {
                  "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
                :
                : "memory");
+}
+
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[32]) {
+  tmem_ld32(taddr, v);
+  tmem_wait_into(v);
 }
 
 // D[tmem] (+)= A[tmem, fp16 pairs along the columns] * B[smem].
@@ -170,6 +184,20 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr) {
          ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+// Read-only loads that stay where they are written, ahead of the barrier waits.
+__device__ __forceinline__ int32_t ld_nc(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_nc16(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
 template <int D, int FMT>
 __global__ void __launch_bounds__(kManyThreads, 1)
     many_rows_kernel(const __grid_constant__ AttnParams8 p) {
@@ -178,16 +206,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   const uint32_t raw = smem_u32(many_raw);
   uint8_t* smem = many_raw + (((raw + 1023u) & ~1023u) - raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
-  uint64_t* q_full = bars;          // [2] 128 arrivals
-  uint64_t* s_full = bars + 2;      // [2] S_i written (commit)
-  uint64_t* p_full = bars + 4;      // [2] 128 arrivals: P_i stored, S_i read
-  uint64_t* o_full = bars + 6;      // [2] O_i updated (commit)
-  uint64_t* k_full = bars + 8;      // [2] 128 arrivals
-  uint64_t* k_empty = bars + 10;    // [2] commit
-  uint64_t* v_full = bars + 12;     // [2] 128 arrivals
-  uint64_t* v_empty = bars + 14;    // [2] commit
-  uint64_t* sc_full = bars + 16;    // [4] 8 arrivals: a tile's scales (reused 4 tiles later)
-  uint64_t* done = bars + 20;
+  uint64_t* s_full = bars;          // [2] S_i written (commit)
+  uint64_t* o_full = bars + 2;      // [2] O_i updated (commit)
+  uint64_t* k_full = bars + 4;      // [2] 128 arrivals
+  uint64_t* k_empty = bars + 6;     // [2] one per query tile: its S MMA is done (commit)
+  uint64_t* v_full = bars + 8;      // [2] 128 arrivals
+  uint64_t* v_empty = bars + 10;    // [2] one per query tile: its O MMA is done (commit)
+  uint64_t* sc_full = bars + 12;    // [4] 8 arrivals: a tile's scales (reused 4 tiles later)
+  float* row_s = reinterpret_cast<float*>(smem + L::kRowOff);
   float4* scales = reinterpret_cast<float4*>(smem + L::kScOff);
   int64_t* misc = reinterpret_cast<int64_t*>(smem + L::kMiscOff);
   MergeUnit* merge_s = reinterpret_cast<MergeUnit*>(smem + L::kMiscOff + 64);
@@ -196,24 +222,21 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + i, 128);
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 128);
       mbar_init(o_full + i, 1);
       mbar_init(k_full + i, 128);
-      mbar_init(k_empty + i, 1);
+      mbar_init(k_empty + i, 2);
       mbar_init(v_full + i, 128);
-      mbar_init(v_empty + i, 1);
+      mbar_init(v_empty + i, 2);
     }
     for (int i = 0; i < 4; ++i) mbar_init(sc_full + i, kGroups);
-    mbar_init(done, 1);
     fence_mbar_init();
     *merge_s = MergeUnit{};
   }
 
   // ---- this CTA's range of the flat list
   Walk walk;
-  int64_t total, ctas, begin;
+  int64_t total, ctas;
   {
     constexpr int kScan = 128;      // threads that own requests
     const int tid = threadIdx.x;
@@ -240,7 +263,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       if (tid == 0) p.merges[blockIdx.x].parts = 0;
       return;                       // CTA-uniform
     }
-    begin = total * blockIdx.x / ctas;
+    walk.begin = total * blockIdx.x / ctas;
+    walk.end = total * (blockIdx.x + 1) / ctas;
+    const int64_t begin = walk.begin;
     int64_t at = before + inc - sum;
     __syncthreads();
     if (at <= begin && begin < at + sum) {
@@ -254,8 +279,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       load_many(p, r, u);
       for (u.rt = 0;; ++u.rt) {
         unit_tiles(p, u);
-        if (begin < at + (int64_t)u.n * p.kv_heads) break;
-        at += (int64_t)u.n * p.kv_heads;
+        const int64_t n = (int64_t)(u.n + kUnitCost) * p.kv_heads;
+        if (begin < at + n) break;
+        at += n;
       }
       misc[0] = at;
       misc[1] = r;
@@ -265,76 +291,86 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     load_many(p, (int)misc[1], walk.u);
     walk.u.rt = (int)misc[2];
     unit_tiles(p, walk.u);
-    walk.u.head = (int)((begin - misc[0]) / walk.u.n);
-    walk.u_at = misc[0] + (int64_t)walk.u.head * walk.u.n;
-    walk.pos = begin;
-    walk.end = total * (blockIdx.x + 1) / ctas;
+    walk.u.head = (int)((begin - misc[0]) / (walk.u.n + kUnitCost));
+    walk.u_at = misc[0] + (int64_t)walk.u.head * (walk.u.n + kUnitCost);
   }
-  if (warp == 12) tmem_alloc(taddr_s, kManyTmem);
+  if (warp == 8) tmem_alloc(taddr_s, kManyTmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *taddr_s;
   bool ok = true;
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= 8) {
     // ---- K and V: codes -> fp16 tiles
     constexpr int kPerRow = D / 16;              // 16-byte chunks of a row of codes
     constexpr int kPasses = kPerRow;             // 128 threads x 16 bytes cover 128 / kPerRow rows
     constexpr int kPassRows = 128 / kPerRow;
     const int t = threadIdx.x - 256;
     const int row = t / kPerRow, c16 = t % kPerRow;
-    const int bs = p.block_size;
     // fp16 chunks 2 c16, 2 c16 + 1 of the row: panel c16 / 4, 16-byte chunk 2 (c16 % 4)
     // within its 128-byte line; lanes of the second panel store in the other
     // order so that one row's eight lanes hit all banks
     const int swap = kPerRow == 8 ? c16 >> 2 : 0;
+    const int bs_log2 = 31 - __clz(p.block_size);
     uint4 kc[kPasses], vc[kPasses];
-    int32_t cell[kPasses];
-    int32_t s_cell = -1;
+    // Three tiles are in flight: tile j in kc / vc, the table cells of tile j + 1
+    // in `cell`, those of tile j + 2 being loaded.  Rows outside the keys that
+    // the unit sees read some valid block and are zeroed when they are stored.
+    int32_t cell[kPasses], s_cell = 0;
+    int tok_base = 0, key_lo = 0, key_hi = 0, head = 0;       // of the tile in `cell`
+    int c_base = 0, c_lo = 0, c_hi = 0;                       // of the tile in kc / vc
     float s_k = 0.f, s_v = 0.f;
-    Walk ahead = walk;                           // the tile whose cells are loaded next
+    Walk ahead = walk;
     int a_i = 0;
-    int req_kv = 0, req_lo = 0, head = 0;        // of the tile in `cell`
-    int tok_base = 0;
     auto load_cells = [&]() {
-      if (!ahead.more()) {
-        req_kv = 0;
-        req_lo = 0;
-        tok_base = 0;
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) cell[i] = -1;
-        s_cell = -1;
-        return;
-      }
+      key_lo = key_hi = 0;
+      if (!ahead.more()) return;
       tok_base = (ahead.first() + a_i) * kTok;
-      req_kv = ahead.u.kv;
+      key_hi = ahead.u.kv;
       head = ahead.u.head;
-      req_lo = p.window > 0 ? max(0, ahead.u.kv - ahead.u.q_len - p.window + 1) : 0;
+      key_lo = ahead.u.req_lo;
       const int32_t* tab = p.table + ahead.u.req * p.table_stride;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int tok = tok_base + i * kPassRows + row;
-        cell[i] = tok >= req_lo && tok < req_kv ? tab[tok / bs] : -1;
-      }
-      const int tok = tok_base + t * 16;
-      s_cell = t < kGroups && tok + 15 >= req_lo && tok < req_kv ? tab[tok / bs] : -1;
       if (++a_i == ahead.count()) {
         ahead.next(p);
         a_i = 0;
       }
+      if (key_hi == 0) return;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+        cell[i] = ld_nc(tab + (min(max(tok_base + i * kPassRows + row, key_lo), key_hi - 1) >> bs_log2));
+      s_cell = ld_nc(tab + (min(max(tok_base + t * 16, key_lo), key_hi - 1) >> bs_log2));
     };
     auto load_codes = [&](const uint8_t* codes, uint4 (&x)[kPasses]) {
+      if (key_hi == 0) return;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
         const int tok = tok_base + i * kPassRows + row;
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (cell[i] >= 0 && cell[i] < p.blocks)
-          x[i] = __ldg(reinterpret_cast<const uint4*>(
-              codes + (((int64_t)cell[i] * p.kv_heads + head) * bs + tok % bs) * D + c16 * 16));
+        const int blk = cell[i] >= 0 && cell[i] < p.blocks ? cell[i] : 0;
+        const int line = ((blk * p.kv_heads + head) << bs_log2) + (tok & (p.block_size - 1));
+        x[i] = ld_nc16(codes + (int64_t)line * D + c16 * 16);
       }
     };
-    auto store_tile = [&](uint8_t* tile, const uint4 (&x)[kPasses]) {
+    auto load_scales = [&]() {
+      s_k = s_v = 0.f;
+      const int tok = tok_base + t * 16;
+      if (t >= kGroups || tok + 15 < key_lo || tok >= key_hi) return;
+      if (s_cell < 0 || s_cell >= p.blocks) {
+        atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
+        return;
+      }
+      s_k = p.k_scale[(int64_t)s_cell * p.kv_heads + head];
+      s_v = p.v_scale[(int64_t)s_cell * p.kv_heads + head];
+    };
+    // A bad slot's rows keep block 0's codes: their scale is 0 (V: 2^-100).
+    auto store_tile = [&](uint8_t* tile, uint4 (&x)[kPasses]) {
+      if (c_base < c_lo || c_base + kTok > c_hi) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+          const int tok = c_base + i * kPassRows + row;
+          if (tok < c_lo || tok >= c_hi) x[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
         const int r = i * kPassRows + row;
@@ -350,20 +386,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         *reinterpret_cast<uint4*>(line + (((c + 1 - swap) ^ (r & 7)) << 4)) = second;
       }
     };
-    auto load_scales = [&]() {
-      s_k = s_v = 0.f;
-      if (s_cell >= 0 && s_cell < p.blocks) {
-        s_k = p.k_scale[(int64_t)s_cell * p.kv_heads + head];
-        s_v = p.v_scale[(int64_t)s_cell * p.kv_heads + head];
-      } else if (t < kGroups && tok_base + t * 16 + 15 >= req_lo && tok_base + t * 16 < req_kv) {
-        atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
-      }
+    auto take = [&]() {   // the tile in `cell` becomes the one in kc / vc
+      c_base = tok_base;
+      c_lo = key_lo;
+      c_hi = key_hi;
     };
     load_cells();
     load_codes(p.k_codes, kc);
     load_codes(p.v_codes, vc);
     load_scales();
-    const int64_t n = walk.end - walk.pos;
+    take();
+    load_cells();
+    int64_t n = 0;
+    for (Walk w = walk; w.more(); w.next(p)) n += w.count();
     for (int64_t j = 0; j < n; ++j) {
       const int s = (int)(j & 1);
       const uint32_t ph = (uint32_t)((j >> 1) & 1);
@@ -378,186 +413,148 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       store_tile(smem + L::kKOff + s * L::kTile, kc);
       fence_proxy_async();
       mbar_arrive(k_full + s);
-      load_cells();                              // tile j + 1
-      load_codes(p.k_codes, kc);
+      load_codes(p.k_codes, kc);                 // tile j + 1
       if (ok && !mbar_wait(v_empty + s, ph ^ 1)) ok = false;
       store_tile(smem + L::kVOff + s * L::kTile, vc);
       fence_proxy_async();
       mbar_arrive(v_full + s);
       load_codes(p.v_codes, vc);
       load_scales();
+      take();
+      load_cells();                              // tile j + 2
     }
-  } else if (warp == 12) {
-    // ---- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t kIdescQK = umma_idesc_f16_f32(128, kTok);
-      constexpr uint32_t kIdescPV = umma_idesc_f16_f32(128, D) | (1u << 16);   // B is MN-major
-      const uint32_t base = smem_u32(smem);
-      int64_t g = 0;                             // tiles done before this segment
-      int64_t g1 = 0;                            // the same, counting query tile 1's only
-      int seg = 0, seg1 = 0;
-      auto qk = [&](int i, int s) {
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (uint32_t)((ks >> 2) * kTok * 128 + (ks & 3) * 32);
-          umma_f16(tmem + i * kTok, umma_desc_k_sw128(base + L::kQOff + i * L::kTile + off),
-                   umma_desc_k_sw128(base + L::kKOff + s * L::kTile + off), kIdescQK, ks > 0);
-        }
-        umma_commit(s_full + i);
-      };
-      auto pv = [&](int i, int s, bool first) {
-#pragma unroll
-        for (int ks = 0; ks < kTok / 16; ++ks)
-          umma_ts_f16(tmem + 256 + i * D, tmem + i * kTok + ks * 8,
-                      umma_desc_mn_sw128(base + L::kVOff + s * L::kTile + ks * 2048), kIdescPV,
-                      ks > 0 || !first);
-        umma_commit(o_full + i);
-      };
-      auto wait = [&](uint64_t* bar, int64_t phase) {
-        if (ok && !mbar_wait(bar, (uint32_t)(phase & 1))) ok = false;
-      };
-      for (Walk w = walk; w.more(); w.next(p)) {
-        const int n = w.count();
-        const bool two = w.rows(p) > 128;
-        wait(q_full, seg);
-        if (two) wait(q_full + 1, seg1);
-        wait(k_full + (g & 1), g >> 1);
-        tc_fence_after();
-        if (!ok) break;
-        qk(0, (int)(g & 1));
-        if (two) qk(1, (int)(g & 1));
-        umma_commit(k_empty + (g & 1));
-        for (int j = 0; j < n; ++j) {
-          const int64_t at = g + j;
-          const int s = (int)(at & 1), s2 = s ^ 1;
-          if (j + 1 < n) wait(k_full + s2, (at + 1) >> 1);
-          wait(v_full + s, at >> 1);
-          wait(p_full, at);
-          tc_fence_after();
-          if (!ok) break;
-          pv(0, s, j == 0);
-          if (j + 1 < n) qk(0, s2);
-          if (two) {
-            wait(p_full + 1, g1 + j);
-            tc_fence_after();
-            if (!ok) break;
-            pv(1, s, j == 0);
-          }
-          umma_commit(v_empty + s);
-          if (j + 1 < n) {
-            if (two) qk(1, s2);
-            umma_commit(k_empty + s2);
-          }
-        }
-        if (!ok) break;
-        g += n;
-        ++seg;
-        if (two) {
-          g1 += n;
-          ++seg1;
-        }
-      }
-      umma_commit(done);            // every MMA issued above has completed once this phase does
-      ok = mbar_wait(done, 0) && ok;
-    }
-    __syncwarp();
   } else {
     // ---- softmax: thread t owns row t of query tile i
     const int i = warp >> 2;
     const int t = threadIdx.x & 127;
+    const bool leader = t == 0;     // issues the query tile's MMAs
     const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     const uint32_t s_col = lane_base + i * kTok, o_col = lane_base + 256 + i * D;
+    const uint32_t base = smem_u32(smem);
+    uint8_t* q_tile = smem + L::kQOff + i * L::kTile;
     const bool bf16 = p.bf16 != 0;
-    int64_t sc_at = 0;              // tiles of the walk before this segment (scale slots)
+    constexpr uint32_t kIdescQK = umma_idesc_f16_f32(128, kTok);
+    constexpr uint32_t kIdescPV = umma_idesc_f16_f32(128, D) | (1u << 16);   // B is MN-major
+    auto wait = [&](uint64_t* bar, int64_t phase) {
+      if (ok && !mbar_wait(bar, (uint32_t)(phase & 1))) ok = false;
+    };
+    auto qk = [&](int64_t tile) {   // S_i of the walk's tile
+      const int s = (int)(tile & 1);
+      wait(k_full + s, tile >> 1);
+      tc_fence_after();
+      if (!ok) return;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint32_t off = (uint32_t)((ks >> 2) * kTok * 128 + (ks & 3) * 32);
+        umma_f16(tmem + i * kTok, umma_desc_k_sw128(base + L::kQOff + i * L::kTile + off),
+                 umma_desc_k_sw128(base + L::kKOff + s * L::kTile + off), kIdescQK, ks > 0);
+      }
+      umma_commit(s_full + i);
+      umma_commit(k_empty + s);
+    };
+    auto pv = [&](int64_t tile, bool first) {
+      const int s = (int)(tile & 1);
+      wait(v_full + s, tile >> 1);
+      tc_fence_after();
+      if (!ok) return;
+#pragma unroll
+      for (int ks = 0; ks < kTok / 16; ++ks)
+        umma_ts_f16(tmem + 256 + i * D, tmem + i * kTok + ks * 8,
+                    umma_desc_mn_sw128(base + L::kVOff + s * L::kTile + ks * 2048), kIdescPV, ks > 0 || !first);
+      umma_commit(o_full + i);
+      umma_commit(v_empty + s);
+    };
+    int64_t tile = 0;               // tiles of the walk before this one (stages, scale slots)
     int64_t at = 0;                 // tiles this query tile has done
     for (Walk w = walk; w.more(); w.next(p)) {
       const int n = w.count(), rows = w.rows(p);
-      if (i * 128 >= rows) {        // tile 1 of a unit of up to 128 rows
-        sc_at += n;
+      if (i * 128 >= rows) {        // tile 1 of a unit of up to 128 rows: hand the stages on
+        if (leader)
+          for (int j = 0; j < n; ++j) {
+            wait(k_full + ((tile + j) & 1), (tile + j) >> 1);
+            mbar_arrive(k_empty + ((tile + j) & 1));
+            wait(v_full + ((tile + j) & 1), (tile + j) >> 1);
+            mbar_arrive(v_empty + ((tile + j) & 1));
+          }
+        __syncwarp();
+        tile += n;
         continue;
       }
+      // Q rows of this warp -> fp16, K-major 128-byte-swizzled; kRowLanes lanes a row
+      constexpr int kRowLanes = D / 8;
+      const int row0 = w.u.rt * kUnitRows + i * 128;   // the tile's first row within the request
+#pragma unroll 4
+      for (int c = 0; c < kRowLanes; ++c) {
+        const int tr = (warp & 3) * 32 + c * (32 / kRowLanes) + lane / kRowLanes;
+        const int ch = lane % kRowLanes;
+        const int urow = min(row0 + tr, w.u.q_len * p.group - 1);
+        const int tok = p.token_of(urow);
+        uint4 v = *reinterpret_cast<const uint4*>(
+            (const uint16_t*)p.q.data + (w.u.q0 + tok) * p.q.token_stride +
+            (int64_t)(w.u.head * p.group + urow - tok * p.group) * p.q.head_stride + ch * 8);
+        float down = 1.f;
+        if (bf16) {
+          uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+          float2 f[4];
+          float amax = 0.f, up;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            f[k] = unpack_in(true, x[k]);
+            amax = fmaxf(amax, fmaxf(fabsf(f[k].x), fabsf(f[k].y)));
+          }
+#pragma unroll
+          for (int o = kRowLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+          fp16_scale(amax, up, down);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] = pack_half2(f[k].x * up, f[k].y * up);
+        }
+        *reinterpret_cast<uint4*>(q_tile + ((ch >> 3) * kTok + tr) * 128 + (((ch & 7) ^ (tr & 7)) << 4)) = v;
+        if (ch == 0) row_s[i * 128 + tr] = p.scale_log2 * down;
+      }
+      fence_proxy_async();
+      tc_fence_before();
+      named_barrier(1 + i, 128);
+      if (leader) qk(tile);
+      __syncwarp();
       const int r = i * 128 + t;
       const bool live = r < rows;
-      const int urow = w.u.rt * kUnitRows + min(r, rows - 1);
-      const int tok = urow / p.group;               // query token within the request
-      const int64_t orow = (int64_t)(w.u.q0 + tok) * p.heads + w.u.head * p.group + urow % p.group;
-      float rscale = p.scale_log2;
-      {
-        // Q row -> fp16, K-major 128-byte-swizzled
-        const uint16_t* src = (const uint16_t*)p.q.data + (w.u.q0 + tok) * p.q.token_stride +
-                              (int64_t)(w.u.head * p.group + urow % p.group) * p.q.head_stride;
-        uint8_t* tile = smem + L::kQOff + i * L::kTile;
-        float up = 1.f, down = 1.f;
-        if (bf16) {
-          float amax = 0.f;
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src + c * 8);
-            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = unpack_in(true, x[k]);
-              amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-          }
-          fp16_scale(amax, up, down);
-        }
-        rscale *= down;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          uint4 v = *reinterpret_cast<const uint4*>(src + c * 8);
-          if (bf16) {
-            uint32_t* x = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = unpack_in(true, x[k]);
-              x[k] = pack_half2(f.x * up, f.y * up);
-            }
-          }
-          *reinterpret_cast<uint4*>(tile + ((c >> 3) * kTok + t) * 128 + (((c & 7) ^ (t & 7)) << 4)) = v;
-        }
-        fence_proxy_async();
-        mbar_arrive(q_full + i);
-      }
+      const int urow = min(row0 + t, w.u.q_len * p.group - 1);
+      const int tok = p.token_of(urow);
+      const float rscale = row_s[r];
       const int hi = w.u.kv - w.u.q_len + tok + 1;            // keys [lo, hi) are visible
       const int lo = p.window > 0 ? hi - p.window : 0;
-      // the tile's rows all see keys [all_lo, all_hi)
-      const int all_hi = w.u.kv - w.u.q_len + (w.u.rt * kUnitRows + i * 128) / p.group + 1;
-      const int all_lo = p.window > 0 ? w.u.kv - w.u.q_len + (w.u.rt * kUnitRows + min(rows, i * 128 + 128) - 1) /
-                                                                 p.group + 1 - p.window : 0;
+      // every row of the warp sees keys [all_lo, all_hi); none sees any outside [any_lo, any_hi)
+      const int all_hi = __shfl_sync(~0u, hi, 0), any_hi = __shfl_sync(~0u, hi, 31);
+      const int all_lo = __shfl_sync(~0u, lo, 31), any_lo = __shfl_sync(~0u, lo, 0);
       float m = -INFINITY, l = 0.f;       // reference of the exponents (log2), sum in units of vinv
       float vlog = 0.f;                   // log2 vinv
-      bool vset = false;
       const int tile0 = w.first();
-      for (int j = 0; j < n; ++j, ++at, ++sc_at) {
-        const float4* sc = scales + (sc_at & 3) * kGroups;
-        if (ok && !mbar_wait(s_full + i, (uint32_t)(at & 1))) ok = false;
-        // complete by now; the wait orders the scales' reads
-        if (ok && !mbar_wait(sc_full + (sc_at & 3), (uint32_t)((sc_at >> 2) & 1))) ok = false;
+      for (int j = 0; j < n; ++j, ++at, ++tile) {
+        const float4* sc = scales + (tile & 3) * kGroups;
+        wait(s_full + i, at);
+        wait(sc_full + (tile & 3), tile >> 2);   // complete by now: orders the scales' reads
         __syncwarp();
         tc_fence_after();
         const int k0 = (tile0 + j) * kTok;
-        const bool edge = k0 + kTok > all_hi || k0 < all_lo;
-        // pass 1: the row's maximum
-        float mx = -INFINITY;
-        float vmax = kTinyScale;
+        // pass 1: the row's maximum and the largest V scale
+        float mx = -INFINITY, vmax = kTinyScale;
 #pragma unroll
         for (int c = 0; c < kTok / 32; ++c) {
+          const int kc = k0 + c * 32;
+          if (kc >= any_hi || kc + 32 <= any_lo) continue;
           uint32_t v[32];
           tmem_load(s_col + c * 32, v);
+          if (kc + 32 > all_hi || kc < all_lo) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (kc + x >= hi || kc + x < lo) v[x] = 0xff800000u;
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float a = -INFINITY;
-            if (edge) {
+            float a = fmaxf(__uint_as_float(v[h * 16]), __uint_as_float(v[h * 16 + 1]));
 #pragma unroll
-              for (int x = 0; x < 16; ++x) {
-                const int key = k0 + c * 32 + h * 16 + x;
-                a = fmaxf(a, key < hi && key >= lo ? __uint_as_float(v[h * 16 + x]) : -INFINITY);
-              }
-            } else {
-#pragma unroll
-              for (int x = 0; x < 16; ++x) a = fmaxf(a, __uint_as_float(v[h * 16 + x]));
-            }
+            for (int x = 2; x < 16; x += 2)
+              a = fmaxf(fmaxf(a, __uint_as_float(v[h * 16 + x])), __uint_as_float(v[h * 16 + x + 1]));
             const float4 g = sc[c * 2 + h];
             // no key of the group: -inf whatever its scale (0 where nothing is stored)
             mx = fmaxf(mx, a == -INFINITY ? a : a * g.x);
@@ -567,83 +564,106 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         mx *= rscale;
         // V's power of two: set by the first tile, moved when a scale outgrows it
         float shift = 0.f;                            // log2 of the factor O and l take
-        if (!vset || lg2(vmax) + vlog > 7.f) {
-          const float nv = 6.f - ceilf(lg2(vmax));
-          shift = vset ? nv - vlog : 0.f;
-          vlog = nv;
-          vset = true;
+        const float vtop = lg2(vmax);
+        if (j == 0) {
+          vlog = 6.f - ceilf(vtop);
+        } else if (vtop + vlog > 7.f) {
+          shift = 6.f - ceilf(vtop) - vlog;
+          vlog += shift;
         }
-        if (mx > m + kLazy || (m == -INFINITY && mx > -INFINITY)) {
-          shift += m == -INFINITY ? 0.f : m - mx;     // nothing summed yet: nothing to rescale
+        if (mx > m + kLazy) {
+          if (m != -INFINITY) shift += m - mx;        // nothing summed yet: nothing to rescale
           m = mx;
         }
         if (__any_sync(~0u, shift != 0.f)) {
           const float f = ex2(shift);
           l *= f;
-          if (j > 0) {
-            if (ok && !mbar_wait(o_full + i, (uint32_t)((at - 1) & 1))) ok = false;
-            __syncwarp();
-            tc_fence_after();
+          wait(o_full + i, at - 1);
+          __syncwarp();
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t v[32], a[16], b[16];
+            tmem_load(o_col + c * 32, v);
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t v[32], a[16], b[16];
-              tmem_load(o_col + c * 32, v);
-#pragma unroll
-              for (int x = 0; x < 16; ++x) {
-                a[x] = __float_as_uint(__uint_as_float(v[x]) * f);
-                b[x] = __float_as_uint(__uint_as_float(v[16 + x]) * f);
-              }
-              tmem_st16(o_col + c * 32, a);
-              tmem_st16(o_col + c * 32 + 16, b);
+            for (int x = 0; x < 16; ++x) {
+              a[x] = __float_as_uint(__uint_as_float(v[x]) * f);
+              b[x] = __float_as_uint(__uint_as_float(v[16 + x]) * f);
             }
+            tmem_st16(o_col + c * 32, a);
+            tmem_st16(o_col + c * 32 + 16, b);
           }
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        // pass 2: P' and the sum
+        const float off = vlog - (m == -INFINITY ? 0.f : m);
+        // pass 2: P' and the sum; the next chunk's logits load while this one's are used
+        uint32_t v[2][32];
+        tmem_ld32(s_col, v[0]);
 #pragma unroll
         for (int c = 0; c < kTok / 32; ++c) {
-          uint32_t v[32], pk[16];
-          tmem_load(s_col + c * 32, v);
+          uint32_t(&x)[32] = v[c & 1];
+          tmem_wait_into(x);
+          if (c + 1 < kTok / 32) tmem_ld32(s_col + (c + 1) * 32, v[(c + 1) & 1]);
+          const int kc = k0 + c * 32;
+          uint32_t pk[16];
+          if (kc >= any_hi || kc + 32 <= any_lo) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 g = sc[c * 2 + h];
-            const float mul = g.x * rscale, add = (g.z + vlog) - base;
-            float sum = 0.f;
+            for (int k = 0; k < 16; ++k) pk[k] = 0;
+          } else {
+            const bool edge = kc + 32 > all_hi || kc < all_lo;
 #pragma unroll
-            for (int x = 0; x < 16; x += 2) {
-              float e0 = ex2(fmaf(__uint_as_float(v[h * 16 + x]), mul, add));
-              float e1 = ex2(fmaf(__uint_as_float(v[h * 16 + x + 1]), mul, add));
+            for (int h = 0; h < 2; ++h) {
+              const float4 g = sc[c * 2 + h];
+              const float mul = g.x * rscale, add = g.z + off;
+              float e[16];
+#pragma unroll
+              for (int k = 0; k < 16; ++k) e[k] = ex2(fmaf(__uint_as_float(x[h * 16 + k]), mul, add));
               if (edge) {
-                const int key = k0 + c * 32 + h * 16 + x;
-                e0 = key < hi && key >= lo ? e0 : 0.f;
-                e1 = key + 1 < hi && key + 1 >= lo ? e1 : 0.f;
+                const int key = kc + h * 16;
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                  if (key + k >= hi || key + k < lo) e[k] = 0.f;
               }
-              sum += e0 + e1;
-              pk[h * 8 + x / 2] = pack_half2(e0, e1);
+              float s0 = e[0] + e[1], s1 = e[2] + e[3];
+#pragma unroll
+              for (int k = 4; k < 16; k += 4) {
+                s0 += e[k] + e[k + 1];
+                s1 += e[k + 2] + e[k + 3];
+              }
+#pragma unroll
+              for (int k = 0; k < 8; ++k) pk[h * 8 + k] = pack_half2(e[2 * k], e[2 * k + 1]);
+              s0 += s1;
+              if (s0 != 0.f) l = fmaf(s0, g.w, l);    // a masked group's scale does not count
             }
-            if (sum != 0.f) l = fmaf(sum, g.w, l);    // a masked group's scale does not count
           }
           tmem_st16(s_col + c * 16, pk);
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(p_full + i);
+        named_barrier(1 + i, 128);    // the whole tile's P is stored
+        if (leader) {
+          pv(tile, j == 0);
+          if (j + 1 < n) qk(tile + 1);
+        }
+        __syncwarp();
       }
       // ---- the segment's rows
-      if (ok && !mbar_wait(o_full + i, (uint32_t)((at - 1) & 1))) ok = false;
+      wait(o_full + i, at - 1);
       __syncwarp();
       tc_fence_after();
-      const int64_t u1 = w.u_at + w.u.n;
-      const bool whole = w.pos == w.u_at && w.end >= u1;
-      const int slot = begin >= w.u_at ? 0 : 1;
+      const bool whole = w.whole();
+      const int slot = w.begin >= w.u_at ? 0 : 1;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      float4* part = p.part_o + ((int64_t)blockIdx.x * 2 + slot) * (D / 4) * kUnitRows + r;
+      if (whole) {
+        // through the warp's own rows of the Q tile (its last MMA is done), so
+        // that whole rows leave together
+        uint8_t* stage = q_tile + (warp & 3) * 32 * 128;
+        auto staged = [&](int wr, int ch) {
+          return reinterpret_cast<uint4*>(stage + ((ch >> 3) * kTok + wr) * 128 + (((ch & 7) ^ (wr & 7)) << 4));
+        };
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t v[32];
-        tmem_load(o_col + c * 32, v);
-        if (whole && live) {
-          uint4* dst = reinterpret_cast<uint4*>((uint16_t*)p.out + orow * D + c * 32);
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t v[32];
+          tmem_load(o_col + c * 32, v);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             uint32_t o[4];
@@ -651,10 +671,29 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             for (int k = 0; k < 4; ++k)
               o[k] = pack_out(bf16, __uint_as_float(v[x * 8 + 2 * k]) * inv,
                               __uint_as_float(v[x * 8 + 2 * k + 1]) * inv);
-            dst[x] = make_uint4(o[0], o[1], o[2], o[3]);
+            *staged(lane, c * 4 + x) = make_uint4(o[0], o[1], o[2], o[3]);
           }
-        } else if (live) {
-          // partials as shares of the row's mass: scale-free across CTAs
+        }
+        __syncwarp();
+#pragma unroll 4
+        for (int c = 0; c < kRowLanes; ++c) {
+          const int wr = c * (32 / kRowLanes) + lane / kRowLanes, ch = lane % kRowLanes;
+          const int tr = (warp & 3) * 32 + wr;
+          const uint4 v = *staged(wr, ch);
+          if (i * 128 + tr < rows) {
+            const int ur = row0 + tr, tk = p.token_of(ur);
+            *reinterpret_cast<uint4*>((uint16_t*)p.out + ((int64_t)(w.u.q0 + tk) * p.heads + w.u.head * p.group +
+                                                          ur - tk * p.group) * D + ch * 8) = v;
+          }
+        }
+        __syncwarp();
+      } else {
+        // partials as shares of the row's mass: free of vinv and of the reference
+        float4* part = p.part_o + ((int64_t)blockIdx.x * 2 + slot) * (D / 4) * kUnitRows + r;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t v[32];
+          tmem_load(o_col + c * 32, v);
 #pragma unroll
           for (int x = 0; x < 8; ++x)
             part[(c * 8 + x) * kUnitRows] =
@@ -662,20 +701,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                             __uint_as_float(v[4 * x + 2]) * inv, __uint_as_float(v[4 * x + 3]) * inv);
         }
       }
-      if (live) {
-        // l = sum of p * vinv
-        const float lse2 = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + lg2(l) - vlog;
-        if (whole) {
-          if (p.out_lse) p.out_lse[orow] = lse2 * kLn2;
-        } else {
-          p.part_lse[((int64_t)blockIdx.x * 2 + slot) * kUnitRows + r] = lse2;
-        }
+      const float lse2 = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + lg2(l) - vlog;
+      if (!whole) {
+        p.part_lse[((int64_t)blockIdx.x * 2 + slot) * kUnitRows + r] = lse2;
+      } else if (live && p.out_lse) {
+        p.out_lse[(int64_t)(w.u.q0 + tok) * p.heads + w.u.head * p.group + urow - tok * p.group] = lse2 * kLn2;
       }
-      if (i == 0 && t == 0 && !whole && w.pos == w.u_at) {
-        // the unit's first CTA names the merge, over CTAs up to the one whose
-        // range (start(c) = total c / ctas) holds the unit's last tile
+      if (i == 0 && leader && !whole && w.skipped() == 0) {
+        // the CTA with the unit's first tile names the merge, over the CTAs up to
+        // the one whose range (start(c) = total c / ctas) holds its last tile
         MergeUnit mu;
-        mu.parts = (int)((u1 * ctas - 1) / total) - (int)blockIdx.x + 1;
+        mu.parts = (int)((w.u_end() * ctas - 1) / total) - (int)blockIdx.x + 1;
         mu.slot0 = slot;
         mu.q0 = w.u.q0;
         mu.row0 = w.u.rt * kUnitRows;
@@ -692,7 +728,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __syncthreads();
   if (threadIdx.x == 0)
     p.merges[blockIdx.x] = *merge_s;
-  if (warp == 12) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_free(tmem, kManyTmem);
   }
@@ -726,8 +762,8 @@ __global__ void __launch_bounds__(kUnitRows) merge_rows_kernel(const __grid_cons
       o[x].w += v.w * f;
     }
   }
-  const int urow = u.row0 + r;
-  const int64_t orow = (int64_t)(u.q0 + urow / p.group) * p.heads + u.head * p.group + urow % p.group;
+  const int urow = u.row0 + r, tok = p.token_of(urow);
+  const int64_t orow = (int64_t)(u.q0 + tok) * p.heads + u.head * p.group + urow - tok * p.group;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const bool bf16 = p.bf16 != 0;
   uint4* dst = reinterpret_cast<uint4*>((uint16_t*)p.out + orow * D + blockIdx.y * 32);
