@@ -10,14 +10,17 @@
 // While the tensor core works for one query tile the other one's softmax runs.
 //
 //   warps 0-3, 4-7   softmax of query tile 0, 1: one thread per row, no
-//                    cross-thread reduction; also load Q, write the output, and
-//                    one thread of each issues its tile's MMAs (twelve warps
-//                    leave 168 registers a thread; a thirteenth for the MMAs
-//                    would leave 128)
+//                    cross-thread reduction; also load Q and write the output
 //   warps 8-11       read K and V codes (16 bytes a lane, a tile ahead),
 //                    expand them to fp16 (exact) and store them in the
 //                    128-byte-swizzled layout that the MMA descriptors name:
 //                    K as K-major rows, V as rows of the MN-major B operand
+//   warp 12          issues the MMAs
+//
+// Three kinds of code share the SM's instruction caches, and each tile passes
+// through all of it: the loops over a tile's columns and over the MMAs of a
+// product stay rolled (unrolled, the instruction fetch of every role stalled:
+// 1530 us against BELOW for the 8192-token prompt).
 //
 // Scales.  A tile's K scales multiply the logits of their 16 columns in fp32.
 // V's go into the exponent: P' = exp2(s - m + log2(vs vinv)), vinv a power of
@@ -39,10 +42,11 @@
 
 namespace tkv {
 
-constexpr int kManyThreads = 384;
+constexpr int kManyThreads = 416;
 constexpr int kUnitRows = 256;
 constexpr int kTok = 128;                 // tokens of a K/V tile
 constexpr int kGroups = kTok / 16;        // scale groups of a tile
+constexpr int kScStride = kGroups + 1;    // and the log2 of the tile's largest V scale
 constexpr int kUnitCost = 2;              // a unit's fixed cost in tiles
 constexpr uint32_t kManyTmem = 512;
 constexpr float kTinyScale = 7.8886091e-31f;   // 2^-100
@@ -54,9 +58,9 @@ struct ManyLayout {
   static constexpr int kQOff = 0;                         // [2]
   static constexpr int kKOff = 2 * kTile;                 // [2] stages
   static constexpr int kVOff = 4 * kTile;                 // [2] stages
-  static constexpr int kScOff = 6 * kTile;                // [4][kGroups] float4 (ks, vs, log2 vs, 1 / vs)
-  static constexpr int kBarOff = kScOff + 4 * kGroups * 16;
-  static constexpr int kNumBars = 16;
+  static constexpr int kScOff = 6 * kTile;                // [4][kScStride] float4 (ks, vs, log2 vs, 1 / vs)
+  static constexpr int kBarOff = kScOff + 4 * kScStride * 16;
+  static constexpr int kNumBars = 24;
   static constexpr int kRowOff = kBarOff + kNumBars * 8;  // [256] logit scale of each row
   static constexpr int kMiscOff = kRowOff + kUnitRows * 4;
   static constexpr int kBytes = kMiscOff + 512 + 1024;    // + slack to align the base to 1024
@@ -118,16 +122,18 @@ __device__ __forceinline__ void next_many(const AttnParams8& p, ManyUnit& u) {
 // A CTA's walk over the segments of its range, each inside one unit.  A unit
 // takes kUnitCost + n places of the flat list: its tiles are the last n, so a
 // range that ends before them has none of the unit.
+// Places are relative to the start of the CTA's range, [0, end).
 struct Walk {
   ManyUnit u;
-  int64_t u_at, begin, end;   // flat place of the unit, and the CTA's range
-  __device__ __forceinline__ int64_t u_end() const { return u_at + kUnitCost + u.n; }
-  __device__ __forceinline__ int64_t tiles_at() const { return u_at + kUnitCost; }
+  int u_at, end;
+  __device__ __forceinline__ int tiles_at() const { return u_at + kUnitCost; }
+  __device__ __forceinline__ int u_end() const { return tiles_at() + u.n; }
   __device__ __forceinline__ bool more() const { return tiles_at() < end; }
-  __device__ __forceinline__ int skipped() const { return (int)max((int64_t)0, begin - tiles_at()); }
+  __device__ __forceinline__ int skipped() const { return max(0, -tiles_at()); }
   __device__ __forceinline__ int first() const { return u.tile0 + skipped(); }
-  __device__ __forceinline__ int count() const { return (int)(min(end, u_end()) - tiles_at()) - skipped(); }
-  __device__ __forceinline__ bool whole() const { return begin <= tiles_at() && end >= u_end(); }
+  __device__ __forceinline__ int count() const { return min(end, u_end()) - tiles_at() - skipped(); }
+  __device__ __forceinline__ bool whole() const { return tiles_at() >= 0 && end >= u_end(); }
+  __device__ __forceinline__ int slot() const { return u_at <= 0 ? 0 : 1; }
   __device__ __forceinline__ int rows(const AttnParams8& p) const {
     return min(kUnitRows, u.q_len * p.group - u.rt * kUnitRows);
   }
@@ -146,6 +152,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_wait_into(uint32_t (&v)[32]) {
@@ -160,6 +171,15 @@ __device__ __forceinline__ void tmem_wait_into(uint32_t (&v)[32]) {
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[32]) {
   tmem_ld32(taddr, v);
   tmem_wait_into(v);
@@ -184,6 +204,41 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr) {
          ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+// Exponentials of each 16 that run on the FMA pipe instead of the MUFU unit
+// (16 a clock per SM, which 128 x 128 logits keep busy for as long as the tile's
+// two MMAs take the tensor core).
+constexpr int kFmaExps = 0;
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// 32 logits of a row: those at or past `over` or below `under` become -inf, the
+// others take their 16-column group's factor.
+__device__ __forceinline__ void hide(uint32_t (&v)[32], int over, int under, float f0, float f1) {
+#pragma unroll
+  for (int x = 0; x < 32; ++x)
+    v[x] = x < over && x >= under ? __float_as_uint(__uint_as_float(v[x]) * (x < 16 ? f0 : f1)) : 0xff800000u;
+}
+
 // Read-only loads that stay where they are written, ahead of the barrier waits.
 __device__ __forceinline__ int32_t ld_nc(const int32_t* p) {
   int32_t v;
@@ -206,13 +261,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   const uint32_t raw = smem_u32(many_raw);
   uint8_t* smem = many_raw + (((raw + 1023u) & ~1023u) - raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
-  uint64_t* s_full = bars;          // [2] S_i written (commit)
-  uint64_t* o_full = bars + 2;      // [2] O_i updated (commit)
-  uint64_t* k_full = bars + 4;      // [2] 128 arrivals
-  uint64_t* k_empty = bars + 6;     // [2] one per query tile: its S MMA is done (commit)
-  uint64_t* v_full = bars + 8;      // [2] 128 arrivals
-  uint64_t* v_empty = bars + 10;    // [2] one per query tile: its O MMA is done (commit)
-  uint64_t* sc_full = bars + 12;    // [4] 8 arrivals: a tile's scales (reused 4 tiles later)
+  uint64_t* q_full = bars;          // [2] 4 warps: Q_i stored
+  uint64_t* s_full = bars + 2;      // [2] S_i written (commit)
+  uint64_t* p_full = bars + 4;      // [2] 4 warps: P_i stored, S_i read, O_i rescaled
+  uint64_t* o_full = bars + 6;      // [2] O_i updated (commit)
+  uint64_t* k_full = bars + 8;      // [2] 4 warps
+  uint64_t* k_empty = bars + 10;    // [2] commit
+  uint64_t* v_full = bars + 12;     // [2] 4 warps
+  uint64_t* v_empty = bars + 14;    // [2] commit
+  uint64_t* sc_full = bars + 16;    // [4] a tile's scales (reused 4 tiles later)
+  uint64_t* done = bars + 20;
   float* row_s = reinterpret_cast<float*>(smem + L::kRowOff);
   float4* scales = reinterpret_cast<float4*>(smem + L::kScOff);
   int64_t* misc = reinterpret_cast<int64_t*>(smem + L::kMiscOff);
@@ -222,21 +280,23 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 4);
       mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
       mbar_init(o_full + i, 1);
-      mbar_init(k_full + i, 128);
-      mbar_init(k_empty + i, 2);
-      mbar_init(v_full + i, 128);
-      mbar_init(v_empty + i, 2);
+      mbar_init(k_full + i, 4);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, 4);
+      mbar_init(v_empty + i, 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(sc_full + i, kGroups);
+    for (int i = 0; i < 4; ++i) mbar_init(sc_full + i, 1);
+    mbar_init(done, 1);
     fence_mbar_init();
     *merge_s = MergeUnit{};
   }
 
   // ---- this CTA's range of the flat list
   Walk walk;
-  int64_t total, ctas;
   {
     constexpr int kScan = 128;      // threads that own requests
     const int tid = threadIdx.x;
@@ -252,20 +312,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
     if (lane == 31) misc[warp] = inc;
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
+    int64_t before = 0, total = 0;
     for (int w = 0; w < kScan / 32; ++w) {
       if (w < warp) before += misc[w];
       total += misc[w];
     }
-    ctas = min((int64_t)gridDim.x, total);
+    const int64_t ctas = min((int64_t)gridDim.x, total);
     if (blockIdx.x >= ctas) {
       if (tid == 0) p.merges[blockIdx.x].parts = 0;
       return;                       // CTA-uniform
     }
-    walk.begin = total * blockIdx.x / ctas;
-    walk.end = total * (blockIdx.x + 1) / ctas;
-    const int64_t begin = walk.begin;
+    const int64_t begin = total * blockIdx.x / ctas;
+    walk.end = (int)(total * (blockIdx.x + 1) / ctas - begin);
     int64_t at = before + inc - sum;
     __syncthreads();
     if (at <= begin && begin < at + sum) {
@@ -286,32 +344,103 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       misc[0] = at;
       misc[1] = r;
       misc[2] = u.rt;
+      misc[3] = total;
     }
     __syncthreads();
     load_many(p, (int)misc[1], walk.u);
     walk.u.rt = (int)misc[2];
     unit_tiles(p, walk.u);
     walk.u.head = (int)((begin - misc[0]) / (walk.u.n + kUnitCost));
-    walk.u_at = misc[0] + (int64_t)walk.u.head * (walk.u.n + kUnitCost);
+    walk.u_at = (int)(misc[0] + (int64_t)walk.u.head * (walk.u.n + kUnitCost) - begin);
   }
-  if (warp == 8) tmem_alloc(taddr_s, kManyTmem);
+  if (warp == 12) tmem_alloc(taddr_s, kManyTmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *taddr_s;
   bool ok = true;
 
-  if (warp >= 8) {
+  if (warp >= 12) {
+    if (warp == 12 && lane == 0) {
+      // ---- MMA issuer
+      constexpr uint32_t kIdescQK = umma_idesc_f16_f32(128, kTok);
+      constexpr uint32_t kIdescPV = umma_idesc_f16_f32(128, D) | (1u << 16);   // B is MN-major
+      const uint32_t base = smem_u32(smem);
+      auto wait = [&](uint64_t* bar, int phase) {
+        if (ok && !mbar_wait(bar, (uint32_t)(phase & 1))) ok = false;
+      };
+      // descriptors of the first K step; steps of 16 elements move the start
+      // address (16-byte units) by 2 inside a 64-element panel (K-major Q, K) and
+      // by 128 (16 rows of the MN-major V)
+      const uint64_t q_desc = umma_desc_k_sw128(base + L::kQOff), k_desc = umma_desc_k_sw128(base + L::kKOff);
+      const uint64_t v_desc = umma_desc_mn_sw128(base + L::kVOff);
+      auto qk = [&](int i, int s) {
+        uint64_t a = q_desc + (uint32_t)(i * (L::kTile >> 4)), b = k_desc + (uint32_t)(s * (L::kTile >> 4));
+#pragma unroll 1
+        for (int ks = 0; ks < D / 16; ++ks) {
+          umma_f16(tmem + i * kTok, a, b, kIdescQK, ks > 0);
+          const uint32_t step = (ks & 3) == 3 ? (kTok * 128 - 96) >> 4 : 2;
+          a += step;
+          b += step;
+        }
+        umma_commit(s_full + i);
+      };
+      auto pv = [&](int i, int s, bool first) {
+        uint64_t b = v_desc + (uint32_t)(s * (L::kTile >> 4));
+#pragma unroll 1
+        for (int ks = 0; ks < kTok / 16; ++ks, b += 2048 >> 4)
+          umma_ts_f16(tmem + 256 + i * D, tmem + i * kTok + ks * 8, b, kIdescPV, ks > 0 || !first);
+        umma_commit(o_full + i);
+      };
+      int g = 0, g1 = 0;            // tiles done before this segment; query tile 1's
+      int seg = 0, seg1 = 0;
+      for (Walk w = walk; w.more() && ok; w.next(p)) {
+        const int n = w.count();
+        const int tiles = w.rows(p) > 128 ? 2 : 1;
+        // step j: O_i of tile j - 1, then S_i of tile j, for both query tiles
+#pragma unroll 1
+        for (int j = 0; j <= n && ok; ++j) {
+          const int at = g + j;
+#pragma unroll 1
+          for (int i = 0; i < tiles && ok; ++i) {
+            if (j > 0) {
+              wait(v_full + ((at - 1) & 1), (at - 1) >> 1);
+              wait(p_full + i, (i ? g1 : g) + j - 1);
+            } else {
+              wait(q_full + i, i ? seg1 : seg);
+            }
+            if (j < n) wait(k_full + (at & 1), at >> 1);
+            tc_fence_after();
+            if (!ok) break;
+            if (j > 0) pv(i, (at - 1) & 1, j == 1);
+            if (j < n) qk(i, at & 1);
+          }
+          if (!ok) break;
+          if (j > 0) umma_commit(v_empty + ((at - 1) & 1));
+          if (j < n) umma_commit(k_empty + (at & 1));
+        }
+        g += n;
+        ++seg;
+        if (tiles == 2) {
+          g1 += n;
+          ++seg1;
+        }
+      }
+      umma_commit(done);            // every MMA issued above has completed once this phase does
+      ok = mbar_wait(done, 0) && ok;
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
     // ---- K and V: codes -> fp16 tiles
     constexpr int kPerRow = D / 16;              // 16-byte chunks of a row of codes
     constexpr int kPasses = kPerRow;             // 128 threads x 16 bytes cover 128 / kPerRow rows
     constexpr int kPassRows = 128 / kPerRow;
     const int t = threadIdx.x - 256;
-    const int row = t / kPerRow, c16 = t % kPerRow;
-    // fp16 chunks 2 c16, 2 c16 + 1 of the row: panel c16 / 4, 16-byte chunk 2 (c16 % 4)
-    // within its 128-byte line; lanes of the second panel store in the other
-    // order so that one row's eight lanes hit all banks
-    const int swap = kPerRow == 8 ? c16 >> 2 : 0;
+    // chunk of the row and row of the pass: the eight lanes of a store phase hold
+    // four chunks of two neighbouring rows of one 64-element panel, which the
+    // swizzle spreads over all banks
+    const int c16 = (t & 3) + (kPerRow == 8 ? ((t >> 4) & 1) * 4 : 0);
+    const int row = kPerRow == 8 ? ((t >> 2) & 3) + (t >> 5) * 4 : t >> 2;
     const int bs_log2 = 31 - __clz(p.block_size);
     uint4 kc[kPasses], vc[kPasses];
     // Three tiles are in flight: tile j in kc / vc, the table cells of tile j + 1
@@ -337,18 +466,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
       if (key_hi == 0) return;
 #pragma unroll
-      for (int i = 0; i < kPasses; ++i)
+      for (int i = 0; i < kPasses; ++i)   // 16-row groups never straddle a block
         cell[i] = ld_nc(tab + (min(max(tok_base + i * kPassRows + row, key_lo), key_hi - 1) >> bs_log2));
       s_cell = ld_nc(tab + (min(max(tok_base + t * 16, key_lo), key_hi - 1) >> bs_log2));
     };
+    const int64_t block_bytes = (int64_t)p.block_size * D;
+    const uint32_t blocks = (uint32_t)p.blocks;
     auto load_codes = [&](const uint8_t* codes, uint4 (&x)[kPasses]) {
       if (key_hi == 0) return;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
-        const int tok = tok_base + i * kPassRows + row;
-        const int blk = cell[i] >= 0 && cell[i] < p.blocks ? cell[i] : 0;
-        const int line = ((blk * p.kv_heads + head) << bs_log2) + (tok & (p.block_size - 1));
-        x[i] = ld_nc16(codes + (int64_t)line * D + c16 * 16);
+        const uint32_t blk = (uint32_t)cell[i] < blocks ? (uint32_t)cell[i] : 0u;
+        const int in_block = ((i * kPassRows + row) & (p.block_size - 1)) * D + c16 * 16;
+        x[i] = ld_nc16(codes + (int64_t)(blk * p.kv_heads + head) * block_bytes + in_block);
       }
     };
     auto load_scales = [&]() {
@@ -381,9 +511,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         expand4<FMT>(x[i].w, f[1].z, f[1].w);
         uint8_t* line = tile + ((c16 >> 2) * kTok + r) * 128;
         const int c = 2 * (c16 & 3);
-        const uint4 first = swap ? f[1] : f[0], second = swap ? f[0] : f[1];
-        *reinterpret_cast<uint4*>(line + (((c + swap) ^ (r & 7)) << 4)) = first;
-        *reinterpret_cast<uint4*>(line + (((c + 1 - swap) ^ (r & 7)) << 4)) = second;
+        *reinterpret_cast<uint4*>(line + ((c ^ (row & 7)) << 4)) = f[0];
+        *reinterpret_cast<uint4*>(line + (((c + 1) ^ (row & 7)) << 4)) = f[1];
       }
     };
     auto take = [&]() {   // the tile in `cell` becomes the one in kc / vc
@@ -397,27 +526,35 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     load_scales();
     take();
     load_cells();
-    int64_t n = 0;
+    int n = 0;
     for (Walk w = walk; w.more(); w.next(p)) n += w.count();
-    for (int64_t j = 0; j < n; ++j) {
-      const int s = (int)(j & 1);
+    for (int j = 0; j < n; ++j) {
+      const int s = j & 1;
       const uint32_t ph = (uint32_t)((j >> 1) & 1);
-      if (t < kGroups) {
+      if (t < 32) {
         // a V scale of 0 counts as 2^-100: its values stay below any output's
         // last bit, and the row sum gets the group's p back
         const float vs = s_v < kTinyScale ? kTinyScale : s_v;
-        scales[(j & 3) * kGroups + t] = make_float4(s_k, vs, lg2(vs), 1.f / vs);
-        mbar_arrive(sc_full + (j & 3));
+        float top = vs < 3e38f ? vs : kTinyScale;        // a NaN does not move vinv
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+        if (t < kGroups) scales[(j & 3) * kScStride + t] = make_float4(s_k, vs, lg2(vs), 1.f / vs);
+        if (t == 0) scales[(j & 3) * kScStride + kGroups].x = lg2(top);
       }
+      __syncwarp();
+      if (t == 0) mbar_arrive(sc_full + (j & 3));
       if (ok && !mbar_wait(k_empty + s, ph ^ 1)) ok = false;
       store_tile(smem + L::kKOff + s * L::kTile, kc);
       fence_proxy_async();
-      mbar_arrive(k_full + s);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(k_full + s);
       load_codes(p.k_codes, kc);                 // tile j + 1
       if (ok && !mbar_wait(v_empty + s, ph ^ 1)) ok = false;
       store_tile(smem + L::kVOff + s * L::kTile, vc);
       fence_proxy_async();
-      mbar_arrive(v_full + s);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_full + s);
       load_codes(p.v_codes, vc);
       load_scales();
       take();
@@ -427,95 +564,64 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     // ---- softmax: thread t owns row t of query tile i
     const int i = warp >> 2;
     const int t = threadIdx.x & 127;
-    const bool leader = t == 0;     // issues the query tile's MMAs
     const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     const uint32_t s_col = lane_base + i * kTok, o_col = lane_base + 256 + i * D;
-    const uint32_t base = smem_u32(smem);
     uint8_t* q_tile = smem + L::kQOff + i * L::kTile;
     const bool bf16 = p.bf16 != 0;
-    constexpr uint32_t kIdescQK = umma_idesc_f16_f32(128, kTok);
-    constexpr uint32_t kIdescPV = umma_idesc_f16_f32(128, D) | (1u << 16);   // B is MN-major
-    auto wait = [&](uint64_t* bar, int64_t phase) {
+    auto wait = [&](uint64_t* bar, int phase) {
       if (ok && !mbar_wait(bar, (uint32_t)(phase & 1))) ok = false;
     };
-    auto qk = [&](int64_t tile) {   // S_i of the walk's tile
-      const int s = (int)(tile & 1);
-      wait(k_full + s, tile >> 1);
-      tc_fence_after();
-      if (!ok) return;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint32_t off = (uint32_t)((ks >> 2) * kTok * 128 + (ks & 3) * 32);
-        umma_f16(tmem + i * kTok, umma_desc_k_sw128(base + L::kQOff + i * L::kTile + off),
-                 umma_desc_k_sw128(base + L::kKOff + s * L::kTile + off), kIdescQK, ks > 0);
-      }
-      umma_commit(s_full + i);
-      umma_commit(k_empty + s);
-    };
-    auto pv = [&](int64_t tile, bool first) {
-      const int s = (int)(tile & 1);
-      wait(v_full + s, tile >> 1);
-      tc_fence_after();
-      if (!ok) return;
-#pragma unroll
-      for (int ks = 0; ks < kTok / 16; ++ks)
-        umma_ts_f16(tmem + 256 + i * D, tmem + i * kTok + ks * 8,
-                    umma_desc_mn_sw128(base + L::kVOff + s * L::kTile + ks * 2048), kIdescPV, ks > 0 || !first);
-      umma_commit(o_full + i);
-      umma_commit(v_empty + s);
-    };
-    int64_t tile = 0;               // tiles of the walk before this one (stages, scale slots)
-    int64_t at = 0;                 // tiles this query tile has done
+    int tile = 0;                   // tiles of the walk before this one (scale slots)
+    int at = 0;                     // tiles this query tile has done
     for (Walk w = walk; w.more(); w.next(p)) {
       const int n = w.count(), rows = w.rows(p);
-      if (i * 128 >= rows) {        // tile 1 of a unit of up to 128 rows: hand the stages on
-        if (leader)
-          for (int j = 0; j < n; ++j) {
-            wait(k_full + ((tile + j) & 1), (tile + j) >> 1);
-            mbar_arrive(k_empty + ((tile + j) & 1));
-            wait(v_full + ((tile + j) & 1), (tile + j) >> 1);
-            mbar_arrive(v_empty + ((tile + j) & 1));
-          }
-        __syncwarp();
+      if (i * 128 >= rows) {        // tile 1 of a unit of up to 128 rows
         tile += n;
         continue;
       }
       // Q rows of this warp -> fp16, K-major 128-byte-swizzled; kRowLanes lanes a row
       constexpr int kRowLanes = D / 8;
       const int row0 = w.u.rt * kUnitRows + i * 128;   // the tile's first row within the request
-#pragma unroll 4
-      for (int c = 0; c < kRowLanes; ++c) {
-        const int tr = (warp & 3) * 32 + c * (32 / kRowLanes) + lane / kRowLanes;
-        const int ch = lane % kRowLanes;
-        const int urow = min(row0 + tr, w.u.q_len * p.group - 1);
-        const int tok = p.token_of(urow);
-        uint4 v = *reinterpret_cast<const uint4*>(
-            (const uint16_t*)p.q.data + (w.u.q0 + tok) * p.q.token_stride +
-            (int64_t)(w.u.head * p.group + urow - tok * p.group) * p.q.head_stride + ch * 8);
-        float down = 1.f;
-        if (bf16) {
-          uint32_t* x = reinterpret_cast<uint32_t*>(&v);
-          float2 f[4];
-          float amax = 0.f, up;
+      {
+        uint4 qv[kRowLanes];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            f[k] = unpack_in(true, x[k]);
-            amax = fmaxf(amax, fmaxf(fabsf(f[k].x), fabsf(f[k].y)));
-          }
-#pragma unroll
-          for (int o = kRowLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
-          fp16_scale(amax, up, down);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = pack_half2(f[k].x * up, f[k].y * up);
+        for (int c = 0; c < kRowLanes; ++c) {
+          const int tr = (warp & 3) * 32 + c * (32 / kRowLanes) + lane / kRowLanes;
+          const int urow = min(row0 + tr, w.u.q_len * p.group - 1);
+          const int tok = p.token_of(urow);
+          qv[c] = *reinterpret_cast<const uint4*>(
+              (const uint16_t*)p.q.data + (w.u.q0 + tok) * p.q.token_stride +
+              (int64_t)(w.u.head * p.group + urow - tok * p.group) * p.q.head_stride + (lane % kRowLanes) * 8);
         }
-        *reinterpret_cast<uint4*>(q_tile + ((ch >> 3) * kTok + tr) * 128 + (((ch & 7) ^ (tr & 7)) << 4)) = v;
-        if (ch == 0) row_s[i * 128 + tr] = p.scale_log2 * down;
+#pragma unroll
+        for (int c = 0; c < kRowLanes; ++c) {
+          const int tr = (warp & 3) * 32 + c * (32 / kRowLanes) + lane / kRowLanes;
+          const int ch = lane % kRowLanes;
+          uint4 v = qv[c];
+          float down = 1.f;
+          if (bf16) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+            float2 f[4];
+            float amax = 0.f, up;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              f[k] = unpack_in(true, x[k]);
+              amax = fmaxf(amax, fmaxf(fabsf(f[k].x), fabsf(f[k].y)));
+            }
+#pragma unroll
+            for (int o = kRowLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+            fp16_scale(amax, up, down);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = pack_half2(f[k].x * up, f[k].y * up);
+          }
+          *reinterpret_cast<uint4*>(q_tile + ((ch >> 3) * kTok + tr) * 128 + (((ch & 7) ^ (tr & 7)) << 4)) = v;
+          if (ch == 0) row_s[i * 128 + tr] = p.scale_log2 * down;
+        }
       }
       fence_proxy_async();
       tc_fence_before();
-      named_barrier(1 + i, 128);
-      if (leader) qk(tile);
       __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + i);
       const int r = i * 128 + t;
       const bool live = r < rows;
       const int urow = min(row0 + t, w.u.q_len * p.group - 1);
@@ -523,48 +629,46 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const float rscale = row_s[r];
       const int hi = w.u.kv - w.u.q_len + tok + 1;            // keys [lo, hi) are visible
       const int lo = p.window > 0 ? hi - p.window : 0;
-      // every row of the warp sees keys [all_lo, all_hi); none sees any outside [any_lo, any_hi)
-      const int all_hi = __shfl_sync(~0u, hi, 0), any_hi = __shfl_sync(~0u, hi, 31);
-      const int all_lo = __shfl_sync(~0u, lo, 31), any_lo = __shfl_sync(~0u, lo, 0);
+      // every row of the warp sees keys [all_lo, all_hi)
+      const int all_hi = __shfl_sync(~0u, hi, 0), all_lo = __shfl_sync(~0u, lo, 31);
       float m = -INFINITY, l = 0.f;       // reference of the exponents (log2), sum in units of vinv
       float vlog = 0.f;                   // log2 vinv
       const int tile0 = w.first();
       for (int j = 0; j < n; ++j, ++at, ++tile) {
-        const float4* sc = scales + (tile & 3) * kGroups;
+        const float4* sc = scales + (tile & 3) * kScStride;
         wait(s_full + i, at);
         wait(sc_full + (tile & 3), tile >> 2);   // complete by now: orders the scales' reads
         __syncwarp();
         tc_fence_after();
         const int k0 = (tile0 + j) * kTok;
-        // pass 1: the row's maximum and the largest V scale
-        float mx = -INFINITY, vmax = kTinyScale;
-#pragma unroll
+        const bool edge = k0 + kTok > all_hi || k0 < all_lo;
+        // pass 1: the row's maximum
+        float mx = -INFINITY;
+        uint32_t dead = 0;                  // edge tiles: groups that the row does not see
+#pragma unroll 1
         for (int c = 0; c < kTok / 32; ++c) {
-          const int kc = k0 + c * 32;
-          if (kc >= any_hi || kc + 32 <= any_lo) continue;
           uint32_t v[32];
           tmem_load(s_col + c * 32, v);
-          if (kc + 32 > all_hi || kc < all_lo) {
-#pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (kc + x >= hi || kc + x < lo) v[x] = 0xff800000u;
-          }
+          if (edge) hide(v, hi - (k0 + c * 32), lo - (k0 + c * 32), 1.f, 1.f);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float a = fmaxf(__uint_as_float(v[h * 16]), __uint_as_float(v[h * 16 + 1]));
+            float a = __uint_as_float(v[h * 16]), a2 = __uint_as_float(v[h * 16 + 1]);
 #pragma unroll
-            for (int x = 2; x < 16; x += 2)
-              a = fmaxf(fmaxf(a, __uint_as_float(v[h * 16 + x])), __uint_as_float(v[h * 16 + x + 1]));
-            const float4 g = sc[c * 2 + h];
-            // no key of the group: -inf whatever its scale (0 where nothing is stored)
-            mx = fmaxf(mx, a == -INFINITY ? a : a * g.x);
-            if (g.y < 3e38f) vmax = fmaxf(vmax, g.y);
+            for (int x = 2; x < 14; x += 4) {
+              a = max3(a, __uint_as_float(v[h * 16 + x]), __uint_as_float(v[h * 16 + x + 1]));
+              a2 = max3(a2, __uint_as_float(v[h * 16 + x + 2]), __uint_as_float(v[h * 16 + x + 3]));
+            }
+            a = max3(a, __uint_as_float(v[h * 16 + 14]), __uint_as_float(v[h * 16 + 15]));
+            a = fmaxf(a, a2);
+            // an unseen group's scale does not count (0 or NaN where nothing is stored)
+            if (a == -INFINITY) dead |= 1u << (c * 2 + h);
+            else mx = fmaxf(mx, a * sc[c * 2 + h].x);
           }
         }
         mx *= rscale;
         // V's power of two: set by the first tile, moved when a scale outgrows it
         float shift = 0.f;                            // log2 of the factor O and l take
-        const float vtop = lg2(vmax);
+        const float vtop = sc[kGroups].x;
         if (j == 0) {
           vlog = 6.f - ceilf(vtop);
         } else if (vtop + vlog > 7.f) {
@@ -582,76 +686,59 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t v[32], a[16], b[16];
-            tmem_load(o_col + c * 32, v);
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_load16(o_col + c * 16, o);
 #pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              a[x] = __float_as_uint(__uint_as_float(v[x]) * f);
-              b[x] = __float_as_uint(__uint_as_float(v[16 + x]) * f);
-            }
-            tmem_st16(o_col + c * 32, a);
-            tmem_st16(o_col + c * 32 + 16, b);
+            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+            tmem_st16(o_col + c * 16, o);
           }
         }
         const float off = vlog - (m == -INFINITY ? 0.f : m);
-        // pass 2: P' and the sum; the next chunk's logits load while this one's are used
-        uint32_t v[2][32];
-        tmem_ld32(s_col, v[0]);
-#pragma unroll
+        // pass 2: P' and the sum
+#pragma unroll 1
         for (int c = 0; c < kTok / 32; ++c) {
-          uint32_t(&x)[32] = v[c & 1];
-          tmem_wait_into(x);
-          if (c + 1 < kTok / 32) tmem_ld32(s_col + (c + 1) * 32, v[(c + 1) & 1]);
-          const int kc = k0 + c * 32;
-          uint32_t pk[16];
-          if (kc >= any_hi || kc + 32 <= any_lo) {
+          uint32_t v[32], pk[16];
+          tmem_load(s_col + c * 32, v);
+          const float4 g[2] = {sc[c * 2], sc[c * 2 + 1]};
+          float mul[2] = {g[0].x * rscale, g[1].x * rscale};
+          float add[2] = {g[0].z + off, g[1].z + off};
+          if (edge) {
+            // K's scales go in here, so that a hidden logit is -inf whatever its
+            // group's scales are
+            hide(v, hi - (k0 + c * 32), lo - (k0 + c * 32), g[0].x, g[1].x);
+            mul[0] = mul[1] = rscale;
+            if (dead >> (c * 2) & 1) add[0] = 0.f;
+            if (dead >> (c * 2) & 2) add[1] = 0.f;
+          }
 #pragma unroll
-            for (int k = 0; k < 16; ++k) pk[k] = 0;
-          } else {
-            const bool edge = kc + 32 > all_hi || kc < all_lo;
+          for (int h = 0; h < 2; ++h) {
+            float2 s2;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float4 g = sc[c * 2 + h];
-              const float mul = g.x * rscale, add = g.z + off;
-              float e[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) e[k] = ex2(fmaf(__uint_as_float(x[h * 16 + k]), mul, add));
-              if (edge) {
-                const int key = kc + h * 16;
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                  if (key + k >= hi || key + k < lo) e[k] = 0.f;
-              }
-              float s0 = e[0] + e[1], s1 = e[2] + e[3];
-#pragma unroll
-              for (int k = 4; k < 16; k += 4) {
-                s0 += e[k] + e[k + 1];
-                s1 += e[k + 2] + e[k + 3];
-              }
-#pragma unroll
-              for (int k = 0; k < 8; ++k) pk[h * 8 + k] = pack_half2(e[2 * k], e[2 * k + 1]);
-              s0 += s1;
-              if (s0 != 0.f) l = fmaf(s0, g.w, l);    // a masked group's scale does not count
+            for (int k = 0; k < 8; ++k) {
+              const float2 x = fma2(make_float2(__uint_as_float(v[h * 16 + 2 * k]),
+                                                __uint_as_float(v[h * 16 + 2 * k + 1])),
+                                    make_float2(mul[h], mul[h]), make_float2(add[h], add[h]));
+              const float2 e = make_float2(ex2(x.x), k >= 8 - kFmaExps ? ex2_fma(x.y) : ex2(x.y));
+              s2 = k ? add2(s2, e) : e;
+              pk[h * 8 + k] = pack_half2(e.x, e.y);
             }
+            const float sum = s2.x + s2.y;
+            if (sum != 0.f) l = fmaf(sum, g[h].w, l);
           }
           tmem_st16(s_col + c * 16, pk);
         }
         tmem_wait_st();
         tc_fence_before();
-        named_barrier(1 + i, 128);    // the whole tile's P is stored
-        if (leader) {
-          pv(tile, j == 0);
-          if (j + 1 < n) qk(tile + 1);
-        }
         __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + i);
       }
       // ---- the segment's rows
       wait(o_full + i, at - 1);
       __syncwarp();
       tc_fence_after();
       const bool whole = w.whole();
-      const int slot = w.begin >= w.u_at ? 0 : 1;
+      const int slot = w.slot();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (whole) {
         // through the warp's own rows of the Q tile (its last MMA is done), so
@@ -707,11 +794,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       } else if (live && p.out_lse) {
         p.out_lse[(int64_t)(w.u.q0 + tok) * p.heads + w.u.head * p.group + urow - tok * p.group] = lse2 * kLn2;
       }
-      if (i == 0 && leader && !whole && w.skipped() == 0) {
+      if (threadIdx.x == 0 && !whole && w.skipped() == 0) {
         // the CTA with the unit's first tile names the merge, over the CTAs up to
         // the one whose range (start(c) = total c / ctas) holds its last tile
         MergeUnit mu;
-        mu.parts = (int)((w.u_end() * ctas - 1) / total) - (int)blockIdx.x + 1;
+        const int64_t total = misc[3], ctas = min((int64_t)gridDim.x, total);
+        const int64_t u_end = total * blockIdx.x / ctas + w.u_end();
+        mu.parts = (int)((u_end * ctas - 1) / total) - (int)blockIdx.x + 1;
         mu.slot0 = slot;
         mu.q0 = w.u.q0;
         mu.row0 = w.u.rt * kUnitRows;
@@ -728,7 +817,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __syncthreads();
   if (threadIdx.x == 0)
     p.merges[blockIdx.x] = *merge_s;
-  if (warp == 8) {
+  if (warp == 12) {
     tc_fence_after();
     tmem_free(tmem, kManyTmem);
   }
