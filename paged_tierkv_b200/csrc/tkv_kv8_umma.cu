@@ -185,14 +185,24 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[32]) {
   tmem_wait_into(v);
 }
 
-// D[tmem] (+)= A[tmem, fp16 pairs along the columns] * B[smem].
-__device__ __forceinline__ void umma_ts_f16(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// D[tmem] (+)= A[smem] * B[smem]^T, the descriptors as their two words.
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                        uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem, fp16 pairs along the columns] * B[smem].
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -369,27 +379,27 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       auto wait = [&](uint64_t* bar, int phase) {
         if (ok && !mbar_wait(bar, (uint32_t)(phase & 1))) ok = false;
       };
-      // descriptors of the first K step; steps of 16 elements move the start
-      // address (16-byte units) by 2 inside a 64-element panel (K-major Q, K) and
-      // by 128 (16 rows of the MN-major V)
-      const uint64_t q_desc = umma_desc_k_sw128(base + L::kQOff), k_desc = umma_desc_k_sw128(base + L::kKOff);
-      const uint64_t v_desc = umma_desc_mn_sw128(base + L::kVOff);
+      // descriptors differ in their low words (start addresses in 16-byte units):
+      // steps of 16 elements move by 2 inside a 64-element panel (K-major Q, K)
+      // and by 128 (16 rows of the MN-major V)
+      const uint64_t k_major = umma_desc_k_sw128(base), mn_major = umma_desc_mn_sw128(base);
+      const uint32_t k_hi = (uint32_t)(k_major >> 32), mn_hi = (uint32_t)(mn_major >> 32);
+      const uint32_t q_lo = (uint32_t)k_major + (L::kQOff >> 4), k_lo = (uint32_t)k_major + (L::kKOff >> 4);
+      const uint32_t v_lo = (uint32_t)mn_major + (L::kVOff >> 4);
       auto qk = [&](int i, int s) {
-        uint64_t a = q_desc + (uint32_t)(i * (L::kTile >> 4)), b = k_desc + (uint32_t)(s * (L::kTile >> 4));
-#pragma unroll 1
+        const uint32_t a = q_lo + i * (L::kTile >> 4), b = k_lo + s * (L::kTile >> 4), d = tmem + i * kTok;
+#pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          umma_f16(tmem + i * kTok, a, b, kIdescQK, ks > 0);
-          const uint32_t step = (ks & 3) == 3 ? (kTok * 128 - 96) >> 4 : 2;
-          a += step;
-          b += step;
+          const uint32_t step = (ks >> 2) * (kTok * 128 >> 4) + (ks & 3) * 2;
+          umma_ss(d, a + step, k_hi, b + step, k_hi, kIdescQK, ks > 0);
         }
         umma_commit(s_full + i);
       };
       auto pv = [&](int i, int s, bool first) {
-        uint64_t b = v_desc + (uint32_t)(s * (L::kTile >> 4));
-#pragma unroll 1
-        for (int ks = 0; ks < kTok / 16; ++ks, b += 2048 >> 4)
-          umma_ts_f16(tmem + 256 + i * D, tmem + i * kTok + ks * 8, b, kIdescPV, ks > 0 || !first);
+        const uint32_t a = tmem + i * kTok, b = v_lo + s * (L::kTile >> 4), d = tmem + 256 + i * D;
+#pragma unroll
+        for (int ks = 0; ks < kTok / 16; ++ks)
+          umma_ts(d, a + ks * 8, b + ks * (2048 >> 4), mn_hi, kIdescPV, ks > 0 || !first);
         umma_commit(o_full + i);
       };
       int g = 0, g1 = 0;            // tiles done before this segment; query tile 1's
