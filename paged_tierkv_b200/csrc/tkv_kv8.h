@@ -85,7 +85,8 @@ void kv8_attention_scratch(int sms, int head_dim, int group, int max_q_len, size
                            size_t* data);
 cudaError_t launch_kv8_attention(const AttnParams8& p, int sms, int head_dim, int format,
                                  cudaStream_t stream);
-cudaError_t launch_many_rows(const AttnParams8& p, int sms, int head_dim, int format, cudaStream_t stream);
+cudaError_t launch_many_rows(const AttnParams8& p, const CUtensorMap* maps, int sms, int head_dim, int format,
+                             cudaStream_t stream);
 size_t many_rows_scratch(int sms, int head_dim);
 // Tensor maps of the K and V codes as [blocks * kv_heads * block_size][head_dim]
 // bytes, boxes of min(block_size, 32) rows, swizzled by the row's width.

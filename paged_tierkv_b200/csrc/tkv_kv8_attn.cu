@@ -727,14 +727,14 @@ cudaError_t launch_kv8_attention(const AttnParams8& args, int sms, int d, int fo
   // a lone request needs one kernel: the one for its largest possible size; and
   // without a request that max_q_len calls long, this kernel takes all
   p.few_rows_max = !many ? 0x7fffffff : p.requests == 1 ? 0 : kFewRowsMax;
+  CUtensorMap maps[2];
+  if (!kv8_code_maps(p, d, maps)) return cudaErrorInvalidValue;
   if (p.few_rows_max > 0) {
-    CUtensorMap maps[2];
-    if (!kv8_code_maps(p, d, maps)) return cudaErrorInvalidValue;
     const cudaError_t e = d == 128 ? few_format<128>(p, maps, sms, format, stream)
                                    : few_format<64>(p, maps, sms, format, stream);
     if (e != cudaSuccess || !many) return e;
   }
-  return launch_many_rows(p, sms, d, format, stream);
+  return launch_many_rows(p, maps, sms, d, format, stream);
 }
 
 }  // namespace tkv

@@ -121,6 +121,11 @@ __device__ __forceinline__ void expand_pairs(uint32_t wa, uint32_t wb, uint32_t 
 __device__ __forceinline__ void cp_async4(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
+// 16 bytes past L1; cp_async_wait_all waits for this thread's copies.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // One arrival (counted in the barrier's initial count) once this thread's
 // earlier cp.async copies have landed.
 __device__ __forceinline__ void cp_async_mbar_arrive(uint64_t* bar) {

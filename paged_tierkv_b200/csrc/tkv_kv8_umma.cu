@@ -11,11 +11,12 @@
 //
 //   warps 0-3, 4-7   softmax of query tile 0, 1: one thread per row, no
 //                    cross-thread reduction; also load Q and write the output
-//   warps 8-11       read K and V codes (16 bytes a lane, a tile ahead),
-//                    expand them to fp16 (exact) and store them in the
+//   warps 8-11       expand codes to fp16 (exact) and store them in the
 //                    128-byte-swizzled layout that the MMA descriptors name:
 //                    K as K-major rows, V as rows of the MN-major B operand
 //   warp 12          issues the MMAs
+//   warp 13          walks the block table: TMA boxes of codes and the scales,
+//                    a tile ahead of the expansion
 //
 // Three kinds of code share the SM's instruction caches, and each tile passes
 // through all of it: the loops over a tile's columns and over the MMAs of a
@@ -42,11 +43,11 @@
 
 namespace tkv {
 
-constexpr int kManyThreads = 416;
+constexpr int kManyThreads = 448;
 constexpr int kUnitRows = 256;
 constexpr int kTok = 128;                 // tokens of a K/V tile
 constexpr int kGroups = kTok / 16;        // scale groups of a tile
-constexpr int kScStride = kGroups + 1;    // and the log2 of the tile's largest V scale
+constexpr int kScStride = kGroups + 1;    // and (log2 of the largest V scale, first token, first and last key)
 constexpr int kUnitCost = 2;              // a unit's fixed cost in tiles
 constexpr uint32_t kManyTmem = 512;
 constexpr float kTinyScale = 7.8886091e-31f;   // 2^-100
@@ -58,13 +59,16 @@ struct ManyLayout {
   static constexpr int kQOff = 0;                         // [2]
   static constexpr int kKOff = 2 * kTile;                 // [2] stages
   static constexpr int kVOff = 4 * kTile;                 // [2] stages
-  static constexpr int kScOff = 6 * kTile;                // [4][kScStride] float4 (ks, vs, log2 vs, 1 / vs)
+  static constexpr int kCodes = kTok * D;                 // staged codes of a tile
+  static constexpr int kStOff = 6 * kTile;                // K, V
+  static constexpr int kScOff = kStOff + 2 * kCodes;      // [4][kScStride] float4 (ks, vs, log2 vs, 1 / vs)
   static constexpr int kBarOff = kScOff + 4 * kScStride * 16;
-  static constexpr int kNumBars = 24;
+  static constexpr int kNumBars = 26;
   static constexpr int kRowOff = kBarOff + kNumBars * 8;  // [256] logit scale of each row
   static constexpr int kMiscOff = kRowOff + kUnitRows * 4;
-  static constexpr int kBytes = kMiscOff + 512 + 1024;    // + slack to align the base to 1024
+  static constexpr int kBytes = kMiscOff + 128 + 1024;    // + slack to align the base to 1024
 };
+static_assert(ManyLayout<128>::kBytes <= 232448, "shared memory");
 
 // ---- the flat list of (request, row tile, kv head) units and their K/V tiles
 struct ManyUnit {
@@ -95,14 +99,17 @@ __device__ __forceinline__ bool load_many(const AttnParams8& p, int req, ManyUni
   return u.rts > 0;
 }
 
-__device__ __forceinline__ int64_t many_tiles(const AttnParams8& p, int req) {
+// A request's places in the flat list, evaluated by `lanes` threads (a power of
+// two, neighbours) together; every one of them gets the sum.
+__device__ __forceinline__ int64_t many_places(const AttnParams8& p, int req, int sub, int lanes) {
   ManyUnit u;
-  if (!load_many(p, req, u)) return 0;
   int64_t sum = 0;
-  for (u.rt = 0; u.rt < u.rts; ++u.rt) {
-    unit_tiles(p, u);
-    sum += u.n + kUnitCost;
-  }
+  if (req < p.requests && load_many(p, req, u))
+    for (u.rt = sub; u.rt < u.rts; u.rt += lanes) {
+      unit_tiles(p, u);
+      sum += u.n + kUnitCost;
+    }
+  for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
   return sum * p.kv_heads;
 }
 
@@ -249,23 +256,10 @@ __device__ __forceinline__ void hide(uint32_t (&v)[32], int over, int under, flo
     v[x] = x < over && x >= under ? __float_as_uint(__uint_as_float(v[x]) * (x < 16 ? f0 : f1)) : 0xff800000u;
 }
 
-// Read-only loads that stay where they are written, ahead of the barrier waits.
-__device__ __forceinline__ int32_t ld_nc(const int32_t* p) {
-  int32_t v;
-  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint4 ld_nc16(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-
 template <int D, int FMT>
 __global__ void __launch_bounds__(kManyThreads, 1)
-    many_rows_kernel(const __grid_constant__ AttnParams8 p) {
+    many_rows_kernel(const __grid_constant__ AttnParams8 p, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v) {
   using L = ManyLayout<D>;
   extern __shared__ uint8_t many_raw[];
   const uint32_t raw = smem_u32(many_raw);
@@ -281,11 +275,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   uint64_t* v_empty = bars + 14;    // [2] commit
   uint64_t* sc_full = bars + 16;    // [4] a tile's scales (reused 4 tiles later)
   uint64_t* done = bars + 20;
+  uint64_t* st_full = bars + 21;    // [2] K, V codes staged (TMA)
+  uint64_t* st_empty = bars + 23;   // [2] 4 warps
   float* row_s = reinterpret_cast<float*>(smem + L::kRowOff);
   float4* scales = reinterpret_cast<float4*>(smem + L::kScOff);
   int64_t* misc = reinterpret_cast<int64_t*>(smem + L::kMiscOff);
-  MergeUnit* merge_s = reinterpret_cast<MergeUnit*>(smem + L::kMiscOff + 64);
-  uint32_t* taddr_s = reinterpret_cast<uint32_t*>(smem + L::kMiscOff + 256);
+  MergeUnit* merge_s = reinterpret_cast<MergeUnit*>(smem + L::kMiscOff + 104);
+  uint32_t* taddr_s = reinterpret_cast<uint32_t*>(smem + L::kMiscOff + 96);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -298,35 +294,38 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       mbar_init(k_empty + i, 1);
       mbar_init(v_full + i, 4);
       mbar_init(v_empty + i, 1);
+      mbar_init(st_full + i, 1);
+      mbar_init(st_empty + i, 4);
     }
     for (int i = 0; i < 4; ++i) mbar_init(sc_full + i, 1);
     mbar_init(done, 1);
     fence_mbar_init();
     *merge_s = MergeUnit{};
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
   }
 
   // ---- this CTA's range of the flat list
   Walk walk;
   {
-    constexpr int kScan = 128;      // threads that own requests
+    // 256 threads, `lanes` of them for each request of a round
+    constexpr int kScan = 256;
     const int tid = threadIdx.x;
-    const int per = (p.requests + kScan - 1) / kScan;
-    const int r0 = min(p.requests, tid * per), r1 = tid < kScan ? min(p.requests, r0 + per) : r0;
+    int lanes = 32;
+    while (lanes > 1 && lanes * p.requests > kScan) lanes >>= 1;
+    const int sub = tid & (lanes - 1), per_round = kScan / lanes;
+    const bool scans = tid < kScan;
     int64_t sum = 0;
-    for (int r = r0; r < r1; ++r) sum += many_tiles(p, r);
-    int64_t inc = sum;
+    for (int r = tid / lanes; scans && r - tid / lanes < p.requests; r += per_round) {
+      const int64_t n = many_places(p, r, sub, lanes);
+      if (sub == 0) sum += n;
+    }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(~0u, inc, o);
-      if (lane >= o) inc += x;
-    }
-    if (lane == 31) misc[warp] = inc;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (scans && lane == 0) misc[warp] = sum;
     __syncthreads();
-    int64_t before = 0, total = 0;
-    for (int w = 0; w < kScan / 32; ++w) {
-      if (w < warp) before += misc[w];
-      total += misc[w];
-    }
+    int64_t total = 0;
+    for (int w = 0; w < kScan / 32; ++w) total += misc[w];
     const int64_t ctas = min((int64_t)gridDim.x, total);
     if (blockIdx.x >= ctas) {
       if (tid == 0) p.merges[blockIdx.x].parts = 0;
@@ -334,27 +333,56 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
     const int64_t begin = total * blockIdx.x / ctas;
     walk.end = (int)(total * (blockIdx.x + 1) / ctas - begin);
-    int64_t at = before + inc - sum;
+    // the request that holds `begin`, then its row tile
     __syncthreads();
-    if (at <= begin && begin < at + sum) {
-      int r = r0;
-      for (;; ++r) {
-        const int64_t n = many_tiles(p, r);
-        if (begin < at + n) break;
-        at += n;
+    int64_t at = 0;
+    for (int r0 = 0; r0 < p.requests; r0 += per_round) {
+      const int64_t n = scans ? many_places(p, r0 + tid / lanes, sub, lanes) : 0;
+      int64_t inc = sub == 0 && scans ? n : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(~0u, inc, o);
+        if (lane >= o) inc += x;
       }
+      if (scans && lane == 31) misc[warp] = inc;
+      __syncthreads();
+      int64_t first = at + inc - n, next = at;
+      for (int w = 0; w < kScan / 32; ++w) {
+        if (w < warp) first += misc[w];
+        next += misc[w];
+      }
+      if (scans && sub == 0 && first <= begin && begin < first + n) {
+        misc[8] = first;
+        misc[9] = r0 + tid / lanes;
+      }
+      __syncthreads();
+      at = next;
+      if (begin < at) break;        // CTA-uniform
+    }
+    if (warp == 0) {
       ManyUnit u;
-      load_many(p, r, u);
-      for (u.rt = 0;; ++u.rt) {
+      load_many(p, (int)misc[9], u);
+      int64_t first = misc[8];
+      for (int rt0 = 0;; rt0 += 32) {
+        u.rt = min(rt0 + lane, u.rts - 1);
         unit_tiles(p, u);
-        const int64_t n = (int64_t)(u.n + kUnitCost) * p.kv_heads;
-        if (begin < at + n) break;
-        at += n;
+        int64_t inc = rt0 + lane < u.rts ? (int64_t)(u.n + kUnitCost) * p.kv_heads : 0;
+        const int64_t n = inc;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t x = __shfl_up_sync(~0u, inc, o);
+          if (lane >= o) inc += x;
+        }
+        const int64_t mine = first + inc - n;
+        if (mine <= begin && begin < mine + n) {
+          misc[0] = mine;
+          misc[1] = u.req;
+          misc[2] = u.rt;
+          misc[3] = total;
+        }
+        first += __shfl_sync(~0u, inc, 31);
+        if (begin < first) break;
       }
-      misc[0] = at;
-      misc[1] = r;
-      misc[2] = u.rt;
-      misc[3] = total;
     }
     __syncthreads();
     load_many(p, (int)misc[1], walk.u);
@@ -370,8 +398,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   const uint32_t tmem = *taddr_s;
   bool ok = true;
 
-  if (warp >= 12) {
-    if (warp == 12 && lane == 0) {
+  if (warp == 12) {
+    if (lane == 0) {
       // ---- MMA issuer
       constexpr uint32_t kIdescQK = umma_idesc_f16_f32(128, kTok);
       constexpr uint32_t kIdescPV = umma_idesc_f16_f32(128, D) | (1u << 16);   // B is MN-major
@@ -440,135 +468,128 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       ok = mbar_wait(done, 0) && ok;
     }
     __syncwarp();
+  } else if (warp == 13) {
+    // ---- codes by TMA, scales through shared memory
+    const int bs_log2 = 31 - __clz(p.block_size);
+    const int box = min(p.block_size, 32), boxes = kTok / box;
+    const int grp = lane & (kGroups - 1);                 // this lane's 16-token group
+    const int box_grp = (lane & (boxes - 1)) * (box / 16);   // and its box's first group
+    Walk w = walk;
+    int j = 0, i = 0, cell = 0;
+    float ks = 0.f, vs = 0.f;
+    int tok0 = 0, lo = 0, hi = 0, head = 0;               // of the tile whose cells are held
+    bool seen = false;                                    // the lane's group holds keys of the unit
+    auto load = [&]() {
+      if (!w.more()) return;
+      tok0 = (w.first() + i) * kTok;
+      lo = w.u.req_lo;
+      hi = w.u.kv;
+      head = w.u.head;
+      const int tok = tok0 + grp * 16;
+      seen = tok + 15 >= lo && tok < hi;
+      cell = seen ? p.table[w.u.req * p.table_stride + (tok >> bs_log2)] : 0;
+      const bool good = cell >= 0 && cell < p.blocks;
+      if (seen && !good) atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
+      // a bad slot loads block 0's codes under scale 0
+      ks = vs = 0.f;
+      if (!good) cell = 0;
+      else if (seen) {
+        ks = p.k_scale[(int64_t)cell * p.kv_heads + head];
+        vs = p.v_scale[(int64_t)cell * p.kv_heads + head];
+      }
+      if (++i == w.count()) {
+        w.next(p);
+        i = 0;
+      }
+    };
+    bool more = w.more();
+    load();
+    for (; more; ++j) {
+      // a V scale of 0 counts as 2^-100: its values stay below any output's last
+      // bit, and the row sum gets the group's p back
+      const float v1 = vs < kTinyScale ? kTinyScale : vs;
+      float top = v1 < 3e38f ? v1 : kTinyScale;           // a NaN does not move vinv
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+      float4* sc = scales + (j & 3) * kScStride;
+      if (lane < kGroups) sc[lane] = make_float4(ks, v1, lg2(v1), 1.f / v1);
+      if (lane == 0)
+        sc[kGroups] = make_float4(lg2(top), __int_as_float(tok0), __int_as_float(lo), __int_as_float(hi));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sc_full + (j & 3));
+      const uint32_t live = __ballot_sync(~0u, seen) & ((1u << kGroups) - 1);
+      const uint32_t mask = ((1u << (box / 16)) - 1);
+      const bool load_box = lane < boxes && (live >> box_grp & mask);
+      const uint32_t bytes = __popc(__ballot_sync(~0u, load_box)) * box * D;
+      // a box's block: that of its first group with keys
+      const int src = box_grp + (load_box ? __ffs(live >> box_grp & mask) - 1 : 0);
+      const int blk = __shfl_sync(~0u, cell, src);
+      const int y = ((blk * p.kv_heads + head) << bs_log2) + ((box_grp * 16) & (p.block_size - 1));
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        if (ok && !mbar_wait(st_empty + kv, (uint32_t)(j & 1) ^ 1)) ok = false;
+        if (lane == 0 && ok) mbar_arrive_expect_tx(st_full + kv, bytes);
+        __syncwarp();
+        if (load_box && ok)
+          tma_load_2d(smem + L::kStOff + kv * L::kCodes + (box_grp * 16) * D, kv ? &tm_v : &tm_k, 0, y, st_full + kv);
+      }
+      more = w.more();
+      load();
+    }
+    // no copy may still be landing when the CTA exits
+    if (j > 0)
+      for (int kv = 0; kv < 2; ++kv)
+        if (!mbar_wait(st_full + kv, (uint32_t)((j - 1) & 1))) ok = false;
+    __syncwarp();
   } else if (warp >= 8) {
-    // ---- K and V: codes -> fp16 tiles
+    // ---- codes -> fp16 tiles
     constexpr int kPerRow = D / 16;              // 16-byte chunks of a row of codes
-    constexpr int kPasses = kPerRow;             // 128 threads x 16 bytes cover 128 / kPerRow rows
-    constexpr int kPassRows = 128 / kPerRow;
+    constexpr int kPassRows = 128 / kPerRow;     // rows that 128 threads x 16 bytes cover
     const int t = threadIdx.x - 256;
     // chunk of the row and row of the pass: the eight lanes of a store phase hold
     // four chunks of two neighbouring rows of one 64-element panel, which the
     // swizzle spreads over all banks
     const int c16 = (t & 3) + (kPerRow == 8 ? ((t >> 4) & 1) * 4 : 0);
     const int row = kPerRow == 8 ? ((t >> 2) & 3) + (t >> 5) * 4 : t >> 2;
-    const int bs_log2 = 31 - __clz(p.block_size);
-    uint4 kc[kPasses], vc[kPasses];
-    // Three tiles are in flight: tile j in kc / vc, the table cells of tile j + 1
-    // in `cell`, those of tile j + 2 being loaded.  Rows outside the keys that
-    // the unit sees read some valid block and are zeroed when they are stored.
-    int32_t cell[kPasses], s_cell = 0;
-    int tok_base = 0, key_lo = 0, key_hi = 0, head = 0;       // of the tile in `cell`
-    int c_base = 0, c_lo = 0, c_hi = 0;                       // of the tile in kc / vc
-    float s_k = 0.f, s_v = 0.f;
-    Walk ahead = walk;
-    int a_i = 0;
-    auto load_cells = [&]() {
-      key_lo = key_hi = 0;
-      if (!ahead.more()) return;
-      tok_base = (ahead.first() + a_i) * kTok;
-      key_hi = ahead.u.kv;
-      head = ahead.u.head;
-      key_lo = ahead.u.req_lo;
-      const int32_t* tab = p.table + ahead.u.req * p.table_stride;
-      if (++a_i == ahead.count()) {
-        ahead.next(p);
-        a_i = 0;
-      }
-      if (key_hi == 0) return;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i)   // 16-row groups never straddle a block
-        cell[i] = ld_nc(tab + (min(max(tok_base + i * kPassRows + row, key_lo), key_hi - 1) >> bs_log2));
-      s_cell = ld_nc(tab + (min(max(tok_base + t * 16, key_lo), key_hi - 1) >> bs_log2));
-    };
-    const int64_t block_bytes = (int64_t)p.block_size * D;
-    const uint32_t blocks = (uint32_t)p.blocks;
-    auto load_codes = [&](const uint8_t* codes, uint4 (&x)[kPasses]) {
-      if (key_hi == 0) return;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const uint32_t blk = (uint32_t)cell[i] < blocks ? (uint32_t)cell[i] : 0u;
-        const int in_block = ((i * kPassRows + row) & (p.block_size - 1)) * D + c16 * 16;
-        x[i] = ld_nc16(codes + (int64_t)(blk * p.kv_heads + head) * block_bytes + in_block);
-      }
-    };
-    auto load_scales = [&]() {
-      s_k = s_v = 0.f;
-      const int tok = tok_base + t * 16;
-      if (t >= kGroups || tok + 15 < key_lo || tok >= key_hi) return;
-      if (s_cell < 0 || s_cell >= p.blocks) {
-        atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
-        return;
-      }
-      s_k = p.k_scale[(int64_t)s_cell * p.kv_heads + head];
-      s_v = p.v_scale[(int64_t)s_cell * p.kv_heads + head];
-    };
-    // A bad slot's rows keep block 0's codes: their scale is 0 (V: 2^-100).
-    auto store_tile = [&](uint8_t* tile, uint4 (&x)[kPasses]) {
-      if (c_base < c_lo || c_base + kTok > c_hi) {
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-          const int tok = c_base + i * kPassRows + row;
-          if (tok < c_lo || tok >= c_hi) x[i] = make_uint4(0, 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int r = i * kPassRows + row;
-        uint4 f[2];
-        expand4<FMT>(x[i].x, f[0].x, f[0].y);
-        expand4<FMT>(x[i].y, f[0].z, f[0].w);
-        expand4<FMT>(x[i].z, f[1].x, f[1].y);
-        expand4<FMT>(x[i].w, f[1].z, f[1].w);
-        uint8_t* line = tile + ((c16 >> 2) * kTok + r) * 128;
-        const int c = 2 * (c16 & 3);
-        *reinterpret_cast<uint4*>(line + ((c ^ (row & 7)) << 4)) = f[0];
-        *reinterpret_cast<uint4*>(line + (((c + 1) ^ (row & 7)) << 4)) = f[1];
-      }
-    };
-    auto take = [&]() {   // the tile in `cell` becomes the one in kc / vc
-      c_base = tok_base;
-      c_lo = key_lo;
-      c_hi = key_hi;
-    };
-    load_cells();
-    load_codes(p.k_codes, kc);
-    load_codes(p.v_codes, vc);
-    load_scales();
-    take();
-    load_cells();
+    const uint32_t from = swz<kPerRow == 8 ? 7 : 3>((uint32_t)(row * D + c16 * 16));
+    const int c = 2 * (c16 & 3);
+    const uint32_t to0 = ((c16 >> 2) * kTok + row) * 128 + ((c ^ (row & 7)) << 4);
+    const uint32_t to1 = ((c16 >> 2) * kTok + row) * 128 + (((c + 1) ^ (row & 7)) << 4);
     int n = 0;
     for (Walk w = walk; w.more(); w.next(p)) n += w.count();
+#pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const int s = j & 1;
-      const uint32_t ph = (uint32_t)((j >> 1) & 1);
-      if (t < 32) {
-        // a V scale of 0 counts as 2^-100: its values stay below any output's
-        // last bit, and the row sum gets the group's p back
-        const float vs = s_v < kTinyScale ? kTinyScale : s_v;
-        float top = vs < 3e38f ? vs : kTinyScale;        // a NaN does not move vinv
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-        if (t < kGroups) scales[(j & 3) * kScStride + t] = make_float4(s_k, vs, lg2(vs), 1.f / vs);
-        if (t == 0) scales[(j & 3) * kScStride + kGroups].x = lg2(top);
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        if (ok && !mbar_wait(st_full + kv, (uint32_t)(j & 1))) ok = false;
+        if (ok && !mbar_wait((kv ? v_empty : k_empty) + s, (uint32_t)((j >> 1) & 1) ^ 1)) ok = false;
+        const float4 info = scales[(j & 3) * kScStride + kGroups];
+        const int tok = __float_as_int(info.y) + row, lo = __float_as_int(info.z), hi = __float_as_int(info.w);
+        const uint8_t* src = smem + L::kStOff + kv * L::kCodes + from;
+        uint8_t* dst = smem + (kv ? L::kVOff : L::kKOff) + s * L::kTile;
+        // rows of a pass are kPassRows (a multiple of 8) apart: the swizzles repeat
+#pragma unroll 2
+        for (int i = 0; i < kPerRow; ++i) {
+          uint4 x = *reinterpret_cast<const uint4*>(src + i * kPassRows * D);
+          // rows that nobody sees may hold anything
+          if (tok + i * kPassRows < lo || tok + i * kPassRows >= hi) x = make_uint4(0, 0, 0, 0);
+          uint4 f[2];
+          expand4<FMT>(x.x, f[0].x, f[0].y);
+          expand4<FMT>(x.y, f[0].z, f[0].w);
+          expand4<FMT>(x.z, f[1].x, f[1].y);
+          expand4<FMT>(x.w, f[1].z, f[1].w);
+          *reinterpret_cast<uint4*>(dst + to0 + i * kPassRows * 128) = f[0];
+          *reinterpret_cast<uint4*>(dst + to1 + i * kPassRows * 128) = f[1];
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive((kv ? v_full : k_full) + s);
+          mbar_arrive(st_empty + kv);
+        }
       }
-      __syncwarp();
-      if (t == 0) mbar_arrive(sc_full + (j & 3));
-      if (ok && !mbar_wait(k_empty + s, ph ^ 1)) ok = false;
-      store_tile(smem + L::kKOff + s * L::kTile, kc);
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(k_full + s);
-      load_codes(p.k_codes, kc);                 // tile j + 1
-      if (ok && !mbar_wait(v_empty + s, ph ^ 1)) ok = false;
-      store_tile(smem + L::kVOff + s * L::kTile, vc);
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(v_full + s);
-      load_codes(p.v_codes, vc);
-      load_scales();
-      take();
-      load_cells();                              // tile j + 2
     }
   } else {
     // ---- softmax: thread t owns row t of query tile i
@@ -592,24 +613,27 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       // Q rows of this warp -> fp16, K-major 128-byte-swizzled; kRowLanes lanes a row
       constexpr int kRowLanes = D / 8;
       const int row0 = w.u.rt * kUnitRows + i * 128;   // the tile's first row within the request
+      const int wrow = (warp & 3) * 32;
       {
-        uint4 qv[kRowLanes];
-#pragma unroll
-        for (int c = 0; c < kRowLanes; ++c) {
-          const int tr = (warp & 3) * 32 + c * (32 / kRowLanes) + lane / kRowLanes;
+        const int ch = lane % kRowLanes;
+        uint8_t* line = q_tile + (ch >> 3) * (kTok * 128);
+#pragma unroll 1
+        for (int c = 0; c < 32; c += 32 / kRowLanes) {
+          const int tr = wrow + c + lane / kRowLanes;
           const int urow = min(row0 + tr, w.u.q_len * p.group - 1);
           const int tok = p.token_of(urow);
-          qv[c] = *reinterpret_cast<const uint4*>(
-              (const uint16_t*)p.q.data + (w.u.q0 + tok) * p.q.token_stride +
-              (int64_t)(w.u.head * p.group + urow - tok * p.group) * p.q.head_stride + (lane % kRowLanes) * 8);
+          cp_async16(line + tr * 128 + (((ch & 7) ^ (tr & 7)) << 4),
+                     (const uint16_t*)p.q.data + (w.u.q0 + tok) * p.q.token_stride +
+                         (int64_t)(w.u.head * p.group + urow - tok * p.group) * p.q.head_stride + ch * 8);
         }
-#pragma unroll
-        for (int c = 0; c < kRowLanes; ++c) {
-          const int tr = (warp & 3) * 32 + c * (32 / kRowLanes) + lane / kRowLanes;
-          const int ch = lane % kRowLanes;
-          uint4 v = qv[c];
-          float down = 1.f;
-          if (bf16) {
+        cp_async_wait_all();
+        float down = 1.f;
+        if (bf16) {
+#pragma unroll 1
+          for (int c = 0; c < 32; c += 32 / kRowLanes) {
+            const int tr = wrow + c + lane / kRowLanes;
+            uint4* at = reinterpret_cast<uint4*>(line + tr * 128 + (((ch & 7) ^ (tr & 7)) << 4));
+            uint4 v = *at;             // this lane's own copy
             uint32_t* x = reinterpret_cast<uint32_t*>(&v);
             float2 f[4];
             float amax = 0.f, up;
@@ -623,9 +647,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             fp16_scale(amax, up, down);
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[k] = pack_half2(f[k].x * up, f[k].y * up);
+            *at = v;
+            if (ch == 0) row_s[i * 128 + tr] = p.scale_log2 * down;
           }
-          *reinterpret_cast<uint4*>(q_tile + ((ch >> 3) * kTok + tr) * 128 + (((ch & 7) ^ (tr & 7)) << 4)) = v;
-          if (ch == 0) row_s[i * 128 + tr] = p.scale_log2 * down;
+        } else {
+          row_s[i * 128 + wrow + lane] = p.scale_log2;
         }
       }
       fence_proxy_async();
@@ -757,7 +783,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         auto staged = [&](int wr, int ch) {
           return reinterpret_cast<uint4*>(stage + ((ch >> 3) * kTok + wr) * 128 + (((ch & 7) ^ (wr & 7)) << 4));
         };
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t v[32];
           tmem_load(o_col + c * 32, v);
@@ -772,7 +798,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
         }
         __syncwarp();
-#pragma unroll 4
+#pragma unroll 2
         for (int c = 0; c < kRowLanes; ++c) {
           const int wr = c * (32 / kRowLanes) + lane / kRowLanes, ch = lane % kRowLanes;
           const int tr = (warp & 3) * 32 + wr;
@@ -787,7 +813,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       } else {
         // partials as shares of the row's mass: free of vinv and of the reference
         float4* part = p.part_o + ((int64_t)blockIdx.x * 2 + slot) * (D / 4) * kUnitRows + r;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t v[32];
           tmem_load(o_col + c * 32, v);
@@ -882,7 +908,7 @@ size_t many_rows_scratch(int sms, int d) {
 
 namespace {
 template <int D, int FMT>
-cudaError_t launch_many(AttnParams8 p, int sms, cudaStream_t stream) {
+cudaError_t launch_many(AttnParams8 p, const CUtensorMap* maps, int sms, cudaStream_t stream) {
   using L = ManyLayout<D>;
   uint8_t* at = p.data;
   p.part_o = reinterpret_cast<float4*>(at);
@@ -893,7 +919,7 @@ cudaError_t launch_many(AttnParams8 p, int sms, cudaStream_t stream) {
   auto kern = many_rows_kernel<D, FMT>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   if (e != cudaSuccess) return e;
-  kern<<<sms, kManyThreads, L::kBytes, stream>>>(p);
+  kern<<<sms, kManyThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   merge_rows_kernel<D><<<dim3(sms, D / 32), kUnitRows, 0, stream>>>(p);
@@ -901,12 +927,13 @@ cudaError_t launch_many(AttnParams8 p, int sms, cudaStream_t stream) {
 }
 }  // namespace
 
-cudaError_t launch_many_rows(const AttnParams8& p, int sms, int d, int format, cudaStream_t stream) {
+cudaError_t launch_many_rows(const AttnParams8& p, const CUtensorMap* maps, int sms, int d, int format,
+                             cudaStream_t stream) {
   if (d == 128)
-    return format == TKV_KV8_INT8 ? launch_many<128, TKV_KV8_INT8>(p, sms, stream)
-                                  : launch_many<128, TKV_KV8_E4M3>(p, sms, stream);
-  return format == TKV_KV8_INT8 ? launch_many<64, TKV_KV8_INT8>(p, sms, stream)
-                                : launch_many<64, TKV_KV8_E4M3>(p, sms, stream);
+    return format == TKV_KV8_INT8 ? launch_many<128, TKV_KV8_INT8>(p, maps, sms, stream)
+                                  : launch_many<128, TKV_KV8_E4M3>(p, maps, sms, stream);
+  return format == TKV_KV8_INT8 ? launch_many<64, TKV_KV8_INT8>(p, maps, sms, stream)
+                                : launch_many<64, TKV_KV8_E4M3>(p, maps, sms, stream);
 }
 
 }  // namespace tkv
