@@ -48,7 +48,7 @@ constexpr int kUnitRows = 256;
 constexpr int kTok = 128;                 // tokens of a K/V tile
 constexpr int kGroups = kTok / 16;        // scale groups of a tile
 constexpr int kScStride = kGroups + 1;    // and (log2 of the largest V scale, first token, first and last key)
-constexpr int kUnitCost = 2;              // a unit's fixed cost in tiles
+constexpr int kUnitCost = 4;              // a unit's fixed cost in tiles
 constexpr uint32_t kManyTmem = 512;
 constexpr float kTinyScale = 7.8886091e-31f;   // 2^-100
 constexpr float kLazy = 8.f;              // growth of the maximum (log2) that P absorbs
@@ -441,13 +441,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           const int at = g + j;
 #pragma unroll 1
           for (int i = 0; i < tiles && ok; ++i) {
-            if (j > 0) {
-              wait(v_full + ((at - 1) & 1), (at - 1) >> 1);
-              wait(p_full + i, (i ? g1 : g) + j - 1);
-            } else {
-              wait(q_full + i, i ? seg1 : seg);
+            if (i == 0) {
+              if (j > 0) wait(v_full + ((at - 1) & 1), (at - 1) >> 1);
+              if (j < n) wait(k_full + (at & 1), at >> 1);
             }
-            if (j < n) wait(k_full + (at & 1), at >> 1);
+            if (j > 0) wait(p_full + i, (i ? g1 : g) + j - 1);
+            else wait(q_full + i, i ? seg1 : seg);
             tc_fence_after();
             if (!ok) break;
             if (j > 0) pv(i, (at - 1) & 1, j == 1);
@@ -629,7 +628,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         cp_async_wait_all();
         float down = 1.f;
         if (bf16) {
-#pragma unroll 1
+#pragma unroll 4
           for (int c = 0; c < 32; c += 32 / kRowLanes) {
             const int tr = wrow + c + lane / kRowLanes;
             uint4* at = reinterpret_cast<uint4*>(line + tr * 128 + (((ch & 7) ^ (tr & 7)) << 4));
@@ -682,22 +681,29 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         float mx = -INFINITY;
         uint32_t dead = 0;                  // edge tiles: groups that the row does not see
 #pragma unroll 1
-        for (int c = 0; c < kTok / 32; ++c) {
-          uint32_t v[32];
-          tmem_load(s_col + c * 32, v);
-          if (edge) hide(v, hi - (k0 + c * 32), lo - (k0 + c * 32), 1.f, 1.f);
+        for (int c = 0; c < kTok / 32; c += 2) {
+          uint32_t v[2][32];
+          tmem_ld32(s_col + c * 32, v[0]);
+          tmem_ld32(s_col + c * 32 + 32, v[1]);
+          tmem_wait_into(v[0]);
+          tmem_wait_into(v[1]);
+          if (edge) {
+            hide(v[0], hi - (k0 + c * 32), lo - (k0 + c * 32), 1.f, 1.f);
+            hide(v[1], hi - (k0 + c * 32 + 32), lo - (k0 + c * 32 + 32), 1.f, 1.f);
+          }
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float a = __uint_as_float(v[h * 16]), a2 = __uint_as_float(v[h * 16 + 1]);
+          for (int h = 0; h < 4; ++h) {
+            const uint32_t(&x)[32] = v[h >> 1];
+            const int o = (h & 1) * 16;
+            float a = __uint_as_float(x[o]), a2 = __uint_as_float(x[o + 1]);
 #pragma unroll
-            for (int x = 2; x < 14; x += 4) {
-              a = max3(a, __uint_as_float(v[h * 16 + x]), __uint_as_float(v[h * 16 + x + 1]));
-              a2 = max3(a2, __uint_as_float(v[h * 16 + x + 2]), __uint_as_float(v[h * 16 + x + 3]));
+            for (int k = 2; k < 14; k += 4) {
+              a = max3(a, __uint_as_float(x[o + k]), __uint_as_float(x[o + k + 1]));
+              a2 = max3(a2, __uint_as_float(x[o + k + 2]), __uint_as_float(x[o + k + 3]));
             }
-            a = max3(a, __uint_as_float(v[h * 16 + 14]), __uint_as_float(v[h * 16 + 15]));
-            a = fmaxf(a, a2);
+            a = fmaxf(max3(a, __uint_as_float(x[o + 14]), __uint_as_float(x[o + 15])), a2);
             // an unseen group's scale does not count (0 or NaN where nothing is stored)
-            if (a == -INFINITY) dead |= 1u << (c * 2 + h);
+            if (edge && a == -INFINITY) dead |= 1u << (c * 2 + h);
             else mx = fmaxf(mx, a * sc[c * 2 + h].x);
           }
         }
@@ -732,10 +738,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         const float off = vlog - (m == -INFINITY ? 0.f : m);
         // pass 2: P' and the sum
-#pragma unroll 1
-        for (int c = 0; c < kTok / 32; ++c) {
-          uint32_t v[32], pk[16];
-          tmem_load(s_col + c * 32, v);
+        auto probabilities = [&](int c, uint32_t(&v)[32]) {
+          uint32_t pk[16];
           const float4 g[2] = {sc[c * 2], sc[c * 2 + 1]};
           float mul[2] = {g[0].x * rscale, g[1].x * rscale};
           float add[2] = {g[0].z + off, g[1].z + off};
@@ -763,6 +767,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             if (sum != 0.f) l = fmaf(sum, g[h].w, l);
           }
           tmem_st16(s_col + c * 16, pk);
+        };
+        // the next 32 logits are on their way while these are used
+        uint32_t va[32], vb[32];
+        tmem_ld32(s_col, va);
+#pragma unroll 1
+        for (int c = 0; c < kTok / 32; c += 2) {
+          tmem_wait_into(va);
+          tmem_ld32(s_col + c * 32 + 32, vb);
+          probabilities(c, va);
+          tmem_wait_into(vb);
+          if (c + 2 < kTok / 32) tmem_ld32(s_col + c * 32 + 64, va);
+          probabilities(c + 1, vb);
         }
         tmem_wait_st();
         tc_fence_before();
