@@ -6,16 +6,20 @@
 // tile the CTA does S_i = Q_i K^T and O_i += P_i V (i = 0, 1), fp16 in, fp32
 // out, all four accumulators in tensor memory:
 //   columns [0, 128) S0, [128, 256) S1, [256, 256 + D) O0, [256 + D, 256 + 2 D) O1,
-// P_i overwriting the first half of S_i as fp16 and feeding the MMA from there.
+// the fp16 P_i of 64 tokens overwriting the first half of their S_i and feeding
+// the MMA from there.
 // While the tensor core works for one query tile the other one's softmax runs.
 //
-//   warps 0-3, 4-7   softmax of query tile 0, 1: one thread per row, no
-//                    cross-thread reduction; also load Q and write the output
-//   warps 8-11       expand codes to fp16 (exact) and store them in the
+//   warps 0-7, 8-15  softmax of query tile 0, 1: two threads per row, 64 columns
+//                    each, that exchange their maxima; also load Q and write the
+//                    output (one thread a row left the softmax of a tile at twice
+//                    the time of its MMAs: 691 us against BELOW for the
+//                    8192-token prompt)
+//   warps 16-19      expand codes to fp16 (exact) and store them in the
 //                    128-byte-swizzled layout that the MMA descriptors name:
 //                    K as K-major rows, V as rows of the MN-major B operand
-//   warp 12          issues the MMAs
-//   warp 13          walks the block table: TMA boxes of codes and the scales,
+//   warp 20          issues the MMAs
+//   warp 21          walks the block table: TMA boxes of codes and the scales,
 //                    a tile ahead of the expansion
 //
 // Three kinds of code share the SM's instruction caches, and each tile passes
@@ -43,7 +47,7 @@
 
 namespace tkv {
 
-constexpr int kManyThreads = 448;
+constexpr int kManyThreads = 704;
 constexpr int kUnitRows = 256;
 constexpr int kTok = 128;                 // tokens of a K/V tile
 constexpr int kGroups = kTok / 16;        // scale groups of a tile
@@ -64,9 +68,10 @@ struct ManyLayout {
   static constexpr int kScOff = kStOff + 2 * kCodes;      // [4][kScStride] float4 (ks, vs, log2 vs, 1 / vs)
   static constexpr int kBarOff = kScOff + 4 * kScStride * 16;
   static constexpr int kNumBars = 26;
-  static constexpr int kRowOff = kBarOff + kNumBars * 8;  // [256] logit scale of each row
-  static constexpr int kMiscOff = kRowOff + kUnitRows * 4;
-  static constexpr int kBytes = kMiscOff + 128 + 1024;    // + slack to align the base to 1024
+  static constexpr int kRowOff = kBarOff + kNumBars * 8;  // [2 tiles][2 halves][128] floats: the rows'
+                                                          // logit scales, then what their threads exchange
+  static constexpr int kMiscOff = kRowOff + 2 * kUnitRows * 4;
+  static constexpr int kBytes = kMiscOff + 128;
 };
 static_assert(ManyLayout<128>::kBytes <= 232448, "shared memory");
 
@@ -261,13 +266,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     many_rows_kernel(const __grid_constant__ AttnParams8 p, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v) {
   using L = ManyLayout<D>;
-  extern __shared__ uint8_t many_raw[];
-  const uint32_t raw = smem_u32(many_raw);
-  uint8_t* smem = many_raw + (((raw + 1023u) & ~1023u) - raw);
+  extern __shared__ __align__(1024) uint8_t many_smem[];
+  uint8_t* smem = many_smem;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
-  uint64_t* q_full = bars;          // [2] 4 warps: Q_i stored
+  uint64_t* q_full = bars;          // [2] 8 warps: Q_i stored
   uint64_t* s_full = bars + 2;      // [2] S_i written (commit)
-  uint64_t* p_full = bars + 4;      // [2] 4 warps: P_i stored, S_i read, O_i rescaled
+  uint64_t* p_full = bars + 4;      // [2] 8 warps: P_i stored, S_i read, O_i rescaled
   uint64_t* o_full = bars + 6;      // [2] O_i updated (commit)
   uint64_t* k_full = bars + 8;      // [2] 4 warps
   uint64_t* k_empty = bars + 10;    // [2] commit
@@ -286,9 +290,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full + i, 4);
+      mbar_init(q_full + i, 8);
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);
+      mbar_init(p_full + i, 8);
       mbar_init(o_full + i, 1);
       mbar_init(k_full + i, 4);
       mbar_init(k_empty + i, 1);
@@ -391,14 +395,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     walk.u.head = (int)((begin - misc[0]) / (walk.u.n + kUnitCost));
     walk.u_at = (int)(misc[0] + (int64_t)walk.u.head * (walk.u.n + kUnitCost) - begin);
   }
-  if (warp == 12) tmem_alloc(taddr_s, kManyTmem);
+  if (warp == 20) tmem_alloc(taddr_s, kManyTmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *taddr_s;
   bool ok = true;
 
-  if (warp == 12) {
+  if (warp == 20) {
     if (lane == 0) {
       // ---- MMA issuer
       constexpr uint32_t kIdescQK = umma_idesc_f16_f32(128, kTok);
@@ -427,7 +431,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const uint32_t a = tmem + i * kTok, b = v_lo + s * (L::kTile >> 4), d = tmem + 256 + i * D;
 #pragma unroll
         for (int ks = 0; ks < kTok / 16; ++ks)
-          umma_ts(d, a + ks * 8, b + ks * (2048 >> 4), mn_hi, kIdescPV, ks > 0 || !first);
+          umma_ts(d, a + (ks >> 2) * 64 + (ks & 3) * 8, b + ks * (2048 >> 4), mn_hi, kIdescPV, ks > 0 || !first);
         umma_commit(o_full + i);
       };
       int g = 0, g1 = 0;            // tiles done before this segment; query tile 1's
@@ -467,7 +471,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       ok = mbar_wait(done, 0) && ok;
     }
     __syncwarp();
-  } else if (warp == 13) {
+  } else if (warp == 21) {
     // ---- codes by TMA, scales through shared memory
     const int bs_log2 = 31 - __clz(p.block_size);
     const int box = min(p.block_size, 32), boxes = kTok / box;
@@ -541,11 +545,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       for (int kv = 0; kv < 2; ++kv)
         if (!mbar_wait(st_full + kv, (uint32_t)((j - 1) & 1))) ok = false;
     __syncwarp();
-  } else if (warp >= 8) {
+  } else if (warp >= 16) {
     // ---- codes -> fp16 tiles
     constexpr int kPerRow = D / 16;              // 16-byte chunks of a row of codes
     constexpr int kPassRows = 128 / kPerRow;     // rows that 128 threads x 16 bytes cover
-    const int t = threadIdx.x - 256;
+    const int t = threadIdx.x - 512;
     // chunk of the row and row of the pass: the eight lanes of a store phase hold
     // four chunks of two neighbouring rows of one 64-element panel, which the
     // swizzle spreads over all banks
@@ -591,11 +595,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
     }
   } else {
-    // ---- softmax: thread t owns row t of query tile i
-    const int i = warp >> 2;
+    // ---- softmax: threads t of halves 0 and 1 own row t of query tile i, and of
+    // it the columns [64 half, 64 half + 64) of S and half of the columns of O
+    const int i = warp >> 3, half = (warp >> 2) & 1;
     const int t = threadIdx.x & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    const uint32_t s_col = lane_base + i * kTok, o_col = lane_base + 256 + i * D;
+    const uint32_t s_col = lane_base + i * kTok + half * 64;
+    const uint32_t o_col = lane_base + 256 + i * D + half * (D / 2);
+    float* row_scale = row_s + i * 256;                         // [128]
+    float* mine = row_s + i * 256 + half * 128 + t;             // exchanged with the row's other thread
+    const float* other = row_s + i * 256 + (half ^ 1) * 128 + t;
     uint8_t* q_tile = smem + L::kQOff + i * L::kTile;
     const bool bf16 = p.bf16 != 0;
     auto wait = [&](uint64_t* bar, int phase) {
@@ -612,12 +621,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       // Q rows of this warp -> fp16, K-major 128-byte-swizzled; kRowLanes lanes a row
       constexpr int kRowLanes = D / 8;
       const int row0 = w.u.rt * kUnitRows + i * 128;   // the tile's first row within the request
-      const int wrow = (warp & 3) * 32;
+      const int wrow = (warp & 7) * 16;
       {
         const int ch = lane % kRowLanes;
         uint8_t* line = q_tile + (ch >> 3) * (kTok * 128);
 #pragma unroll 1
-        for (int c = 0; c < 32; c += 32 / kRowLanes) {
+        for (int c = 0; c < 16; c += 32 / kRowLanes) {
           const int tr = wrow + c + lane / kRowLanes;
           const int urow = min(row0 + tr, w.u.q_len * p.group - 1);
           const int tok = p.token_of(urow);
@@ -629,7 +638,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         float down = 1.f;
         if (bf16) {
 #pragma unroll 4
-          for (int c = 0; c < 32; c += 32 / kRowLanes) {
+          for (int c = 0; c < 16; c += 32 / kRowLanes) {
             const int tr = wrow + c + lane / kRowLanes;
             uint4* at = reinterpret_cast<uint4*>(line + tr * 128 + (((ch & 7) ^ (tr & 7)) << 4));
             uint4 v = *at;             // this lane's own copy
@@ -647,21 +656,22 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[k] = pack_half2(f[k].x * up, f[k].y * up);
             *at = v;
-            if (ch == 0) row_s[i * 128 + tr] = p.scale_log2 * down;
+            if (ch == 0) row_scale[tr] = p.scale_log2 * down;
           }
-        } else {
-          row_s[i * 128 + wrow + lane] = p.scale_log2;
+        } else if (lane < 16) {
+          row_scale[wrow + lane] = p.scale_log2;
         }
       }
       fence_proxy_async();
       tc_fence_before();
+      named_barrier(1 + i, 256);
+      const float rscale = row_scale[t];
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full + i);
       const int r = i * 128 + t;
       const bool live = r < rows;
       const int urow = min(row0 + t, w.u.q_len * p.group - 1);
       const int tok = p.token_of(urow);
-      const float rscale = row_s[r];
       const int hi = w.u.kv - w.u.q_len + tok + 1;            // keys [lo, hi) are visible
       const int lo = p.window > 0 ? hi - p.window : 0;
       // every row of the warp sees keys [all_lo, all_hi)
@@ -670,47 +680,43 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       float vlog = 0.f;                   // log2 vinv
       const int tile0 = w.first();
       for (int j = 0; j < n; ++j, ++at, ++tile) {
-        const float4* sc = scales + (tile & 3) * kScStride;
+        const float4* sc = scales + (tile & 3) * kScStride + half * 4;
         wait(s_full + i, at);
         wait(sc_full + (tile & 3), tile >> 2);   // complete by now: orders the scales' reads
         __syncwarp();
         tc_fence_after();
-        const int k0 = (tile0 + j) * kTok;
-        const bool edge = k0 + kTok > all_hi || k0 < all_lo;
+        const int k0 = (tile0 + j) * kTok + half * 64;          // this thread's first key
+        const bool edge = k0 + 64 > all_hi || k0 < all_lo;
         // pass 1: the row's maximum
         float mx = -INFINITY;
         uint32_t dead = 0;                  // edge tiles: groups that the row does not see
 #pragma unroll 1
-        for (int c = 0; c < kTok / 32; c += 2) {
-          uint32_t v[2][32];
-          tmem_ld32(s_col + c * 32, v[0]);
-          tmem_ld32(s_col + c * 32 + 32, v[1]);
-          tmem_wait_into(v[0]);
-          tmem_wait_into(v[1]);
-          if (edge) {
-            hide(v[0], hi - (k0 + c * 32), lo - (k0 + c * 32), 1.f, 1.f);
-            hide(v[1], hi - (k0 + c * 32 + 32), lo - (k0 + c * 32 + 32), 1.f, 1.f);
-          }
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[32];
+          tmem_load(s_col + c * 32, v);
+          if (edge) hide(v, hi - (k0 + c * 32), lo - (k0 + c * 32), 1.f, 1.f);
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const uint32_t(&x)[32] = v[h >> 1];
-            const int o = (h & 1) * 16;
-            float a = __uint_as_float(x[o]), a2 = __uint_as_float(x[o + 1]);
+          for (int h = 0; h < 2; ++h) {
+            float a = __uint_as_float(v[h * 16]), a2 = __uint_as_float(v[h * 16 + 1]);
 #pragma unroll
             for (int k = 2; k < 14; k += 4) {
-              a = max3(a, __uint_as_float(x[o + k]), __uint_as_float(x[o + k + 1]));
-              a2 = max3(a2, __uint_as_float(x[o + k + 2]), __uint_as_float(x[o + k + 3]));
+              a = max3(a, __uint_as_float(v[h * 16 + k]), __uint_as_float(v[h * 16 + k + 1]));
+              a2 = max3(a2, __uint_as_float(v[h * 16 + k + 2]), __uint_as_float(v[h * 16 + k + 3]));
             }
-            a = fmaxf(max3(a, __uint_as_float(x[o + 14]), __uint_as_float(x[o + 15])), a2);
+            a = fmaxf(max3(a, __uint_as_float(v[h * 16 + 14]), __uint_as_float(v[h * 16 + 15])), a2);
             // an unseen group's scale does not count (0 or NaN where nothing is stored)
             if (edge && a == -INFINITY) dead |= 1u << (c * 2 + h);
             else mx = fmaxf(mx, a * sc[c * 2 + h].x);
           }
         }
+        // the row's other half; it reads this before the next tile's S is there
+        *mine = mx;
+        named_barrier(1 + i, 256);
+        mx = fmaxf(mx, *other);
         mx *= rscale;
         // V's power of two: set by the first tile, moved when a scale outgrows it
         float shift = 0.f;                            // log2 of the factor O and l take
-        const float vtop = sc[kGroups].x;
+        const float vtop = sc[kGroups - half * 4].x;
         if (j == 0) {
           vlog = 6.f - ceilf(vtop);
         } else if (vtop + vlog > 7.f) {
@@ -728,7 +734,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
+          for (int c = 0; c < D / 32; ++c) {
             uint32_t o[16];
             tmem_load16(o_col + c * 16, o);
 #pragma unroll
@@ -768,17 +774,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
           tmem_st16(s_col + c * 16, pk);
         };
-        // the next 32 logits are on their way while these are used
-        uint32_t va[32], vb[32];
-        tmem_ld32(s_col, va);
 #pragma unroll 1
-        for (int c = 0; c < kTok / 32; c += 2) {
-          tmem_wait_into(va);
-          tmem_ld32(s_col + c * 32 + 32, vb);
-          probabilities(c, va);
-          tmem_wait_into(vb);
-          if (c + 2 < kTok / 32) tmem_ld32(s_col + c * 32 + 64, va);
-          probabilities(c + 1, vb);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[32];
+          tmem_load(s_col + c * 32, v);
+          probabilities(c, v);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -791,16 +791,21 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       tc_fence_after();
       const bool whole = w.whole();
       const int slot = w.slot();
+      *mine = l;
+      named_barrier(1 + i, 256);
+      l += *other;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (whole) {
-        // through the warp's own rows of the Q tile (its last MMA is done), so
-        // that whole rows leave together
+        // through the warp's own rows and half of the Q tile (its last MMA is
+        // done), so that whole lines leave together
         uint8_t* stage = q_tile + (warp & 3) * 32 * 128;
-        auto staged = [&](int wr, int ch) {
-          return reinterpret_cast<uint4*>(stage + ((ch >> 3) * kTok + wr) * 128 + (((ch & 7) ^ (wr & 7)) << 4));
+        constexpr int kHalfLanes = D / 16;      // 16-byte chunks of half a row
+        auto staged = [&](int wr, int ch) {     // chunk ch of the half
+          const int c = half * kHalfLanes + ch;
+          return reinterpret_cast<uint4*>(stage + ((c >> 3) * kTok + wr) * 128 + (((c & 7) ^ (wr & 7)) << 4));
         };
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < D / 64; ++c) {
           uint32_t v[32];
           tmem_load(o_col + c * 32, v);
 #pragma unroll
@@ -815,35 +820,34 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         __syncwarp();
 #pragma unroll 2
-        for (int c = 0; c < kRowLanes; ++c) {
-          const int wr = c * (32 / kRowLanes) + lane / kRowLanes, ch = lane % kRowLanes;
+        for (int c = 0; c < kHalfLanes; ++c) {
+          const int wr = c * (32 / kHalfLanes) + lane / kHalfLanes, ch = lane % kHalfLanes;
           const int tr = (warp & 3) * 32 + wr;
           const uint4 v = *staged(wr, ch);
           if (i * 128 + tr < rows) {
             const int ur = row0 + tr, tk = p.token_of(ur);
             *reinterpret_cast<uint4*>((uint16_t*)p.out + ((int64_t)(w.u.q0 + tk) * p.heads + w.u.head * p.group +
-                                                          ur - tk * p.group) * D + ch * 8) = v;
+                                                          ur - tk * p.group) * D + half * (D / 2) + ch * 8) = v;
           }
         }
-        __syncwarp();
       } else {
         // partials as shares of the row's mass: free of vinv and of the reference
         float4* part = p.part_o + ((int64_t)blockIdx.x * 2 + slot) * (D / 4) * kUnitRows + r;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < D / 64; ++c) {
           uint32_t v[32];
           tmem_load(o_col + c * 32, v);
 #pragma unroll
           for (int x = 0; x < 8; ++x)
-            part[(c * 8 + x) * kUnitRows] =
+            part[(half * (D / 8) + c * 8 + x) * kUnitRows] =
                 make_float4(__uint_as_float(v[4 * x]) * inv, __uint_as_float(v[4 * x + 1]) * inv,
                             __uint_as_float(v[4 * x + 2]) * inv, __uint_as_float(v[4 * x + 3]) * inv);
         }
       }
       const float lse2 = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + lg2(l) - vlog;
-      if (!whole) {
+      if (half == 0 && !whole) {
         p.part_lse[((int64_t)blockIdx.x * 2 + slot) * kUnitRows + r] = lse2;
-      } else if (live && p.out_lse) {
+      } else if (half == 0 && live && p.out_lse) {
         p.out_lse[(int64_t)(w.u.q0 + tok) * p.heads + w.u.head * p.group + urow - tok * p.group] = lse2 * kLn2;
       }
       if (threadIdx.x == 0 && !whole && w.skipped() == 0) {
@@ -861,6 +865,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         *merge_s = mu;
       }
       tc_fence_before();
+      named_barrier(1 + i, 256);    // both halves are done with the Q tile and the exchanged sums
     }
   }
   if (!ok) atomicOr(p.err, TKV_DEVERR_TIMEOUT);
@@ -869,7 +874,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __syncthreads();
   if (threadIdx.x == 0)
     p.merges[blockIdx.x] = *merge_s;
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     tmem_free(tmem, kManyTmem);
   }
