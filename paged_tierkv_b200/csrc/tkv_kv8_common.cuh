@@ -117,6 +117,27 @@ __device__ __forceinline__ void expand_pairs(uint32_t wa, uint32_t wb, uint32_t 
   }
 }
 
+// mbar_wait with a suspend hint: a waiting thread sleeps on the barrier instead
+// of polling it, which leaves the issue slots to the others; false on timeout.
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity), "r"(20000u)   // nanoseconds
+        : "memory");
+    if (ok) return true;
+    const uint64_t now = globaltimer();
+    if (t0 == 0) t0 = now;
+    else if (now - t0 > kWaitTimeoutNs) return false;
+  }
+}
+
 // ---- asynchronous 4-byte copies that arrive on an mbarrier
 __device__ __forceinline__ void cp_async4(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");

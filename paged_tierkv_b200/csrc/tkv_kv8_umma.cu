@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       constexpr uint32_t kIdescPV = umma_idesc_f16_f32(128, D) | (1u << 16);   // B is MN-major
       const uint32_t base = smem_u32(smem);
       auto wait = [&](uint64_t* bar, int phase) {
-        if (ok && !mbar_wait(bar, (uint32_t)(phase & 1))) ok = false;
+        if (ok && !bounded_wait(bar, (uint32_t)(phase & 1))) ok = false;
       };
       // descriptors differ in their low words (start addresses in 16-byte units):
       // steps of 16 elements move by 2 inside a 64-element panel (K-major Q, K)
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
       }
       umma_commit(done);            // every MMA issued above has completed once this phase does
-      ok = mbar_wait(done, 0) && ok;
+      ok = bounded_wait(done, 0) && ok;
     }
     __syncwarp();
   } else if (warp == 21) {
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int y = ((blk * p.kv_heads + head) << bs_log2) + ((box_grp * 16) & (p.block_size - 1));
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
-        if (ok && !mbar_wait(st_empty + kv, (uint32_t)(j & 1) ^ 1)) ok = false;
+        if (ok && !bounded_wait(st_empty + kv, (uint32_t)(j & 1) ^ 1)) ok = false;
         if (lane == 0 && ok) mbar_arrive_expect_tx(st_full + kv, bytes);
         __syncwarp();
         if (load_box && ok)
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     // no copy may still be landing when the CTA exits
     if (j > 0)
       for (int kv = 0; kv < 2; ++kv)
-        if (!mbar_wait(st_full + kv, (uint32_t)((j - 1) & 1))) ok = false;
+        if (!bounded_wait(st_full + kv, (uint32_t)((j - 1) & 1))) ok = false;
     __syncwarp();
   } else if (warp >= 16) {
     // ---- codes -> fp16 tiles
@@ -566,8 +566,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int s = j & 1;
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
-        if (ok && !mbar_wait(st_full + kv, (uint32_t)(j & 1))) ok = false;
-        if (ok && !mbar_wait((kv ? v_empty : k_empty) + s, (uint32_t)((j >> 1) & 1) ^ 1)) ok = false;
+        if (ok && !bounded_wait(st_full + kv, (uint32_t)(j & 1))) ok = false;
+        if (ok && !bounded_wait((kv ? v_empty : k_empty) + s, (uint32_t)((j >> 1) & 1) ^ 1)) ok = false;
         const float4 info = scales[(j & 3) * kScStride + kGroups];
         const int tok = __float_as_int(info.y) + row, lo = __float_as_int(info.z), hi = __float_as_int(info.w);
         const uint8_t* src = smem + L::kStOff + kv * L::kCodes + from;
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     uint8_t* q_tile = smem + L::kQOff + i * L::kTile;
     const bool bf16 = p.bf16 != 0;
     auto wait = [&](uint64_t* bar, int phase) {
-      if (ok && !mbar_wait(bar, (uint32_t)(phase & 1))) ok = false;
+      if (ok && !bounded_wait(bar, (uint32_t)(phase & 1))) ok = false;
     };
     int tile = 0;                   // tiles of the walk before this one (scale slots)
     int at = 0;                     // tiles this query tile has done
