@@ -479,15 +479,22 @@ typedef struct tkv_token_view {
 } tkv_token_view;
 
 /* Rotates q (heads) and k (kv_heads) of `tokens` tokens into q_out / k_out;
- * either may be absent (heads or kv_heads 0), and an output may be its input.
- * head_dim: a multiple of 16 up to 256.  dtype: TKV_DTYPE_F16 / BF16. */
-int32_t tkv_rotary_embed(const tkv_rotary* rotary, const tkv_token_view* q, const tkv_token_view* k,
-                         const tkv_token_view* q_out, const tkv_token_view* k_out, int32_t tokens,
-                         int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype,
-                         uint32_t* error_word, void* stream);
+ * either may be absent (heads or kv_heads 0), and an output may be its input. */
+typedef struct tkv_rotary_args {
+    tkv_rotary     rotary;
+    tkv_token_view q, k, q_out, k_out;
+    uint32_t*      error_word;     /* optional */
+    int32_t        tokens;
+    int32_t        heads;
+    int32_t        kv_heads;
+    int32_t        head_dim;       /* a multiple of 16 up to 256 */
+    int32_t        dtype;          /* TKV_DTYPE_F16 / BF16 */
+} tkv_rotary_args;
+
+int32_t tkv_rotary_embed(const tkv_rotary_args* args, void* stream);
 
 /* Writes the rows of k / v ([tokens, kv_heads, head_dim]) that `units` names
- * into the cache and, with `rotary`, rotates k on the way (in fp32, not
+ * into the cache and, with a rotary, rotates k on the way (in fp32, not
  * rounded in between) and q into q_out.  Unit (block, first, offset, rows):
  * rows [offset, offset + rows) of the block get tokens [first, first + rows).
  * Per kv head and tensor: s_new = max |x| / qmax (127 or 448) over the new
@@ -503,8 +510,8 @@ typedef struct tkv_kv8_append_args {
     tkv_token_view k, v, q, q_out;  /* q: heads 0 = none */
     const int32_t* units;           /* [units_cap][4] */
     const int32_t* num_units;       /* [1] device */
-    const tkv_rotary* rotary;       /* optional; NULL: k as is, no q */
     uint32_t*      error_word;      /* optional */
+    tkv_rotary     rotary;          /* rot_dim 0: k as is, no q */
     int32_t        units_cap;
     int32_t        tokens;
     int32_t        heads;

@@ -206,6 +206,22 @@ class TkvTokenView(ctypes.Structure):
     ]
 
 
+class TkvRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("rotary", TkvRotary),
+        ("q", TkvTokenView),
+        ("k", TkvTokenView),
+        ("q_out", TkvTokenView),
+        ("k_out", TkvTokenView),
+        ("error_word", ctypes.c_void_p),
+        ("tokens", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 class TkvKv8AppendArgs(ctypes.Structure):
     _fields_ = [
         ("k", TkvTokenView),
@@ -214,8 +230,8 @@ class TkvKv8AppendArgs(ctypes.Structure):
         ("q_out", TkvTokenView),
         ("units", ctypes.c_void_p),
         ("num_units", ctypes.c_void_p),
-        ("rotary", ctypes.POINTER(TkvRotary)),
         ("error_word", ctypes.c_void_p),
+        ("rotary", TkvRotary),
         ("units_cap", ctypes.c_int32),
         ("tokens", ctypes.c_int32),
         ("heads", ctypes.c_int32),
@@ -298,13 +314,12 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
                                       i32, vp, vp, vp], i32),
         "tkv_prefill_read_errors": ([ctypes.POINTER(ctypes.c_uint32), vp], i32),
         "tkv_store_prefill_blocks": ([ctypes.POINTER(TkvPools), vp, vp, i32, vp, i32, vp], i32),
-        "tkv_kv8_plan_step": ([ctypes.POINTER(TkvKv8PlanArgs), vp], i32),
-        "tkv_rotary_embed": ([ctypes.POINTER(TkvRotary)] + [ctypes.POINTER(TkvTokenView)] * 4
-                             + [i32] * 5 + [vp, vp], i32),
-        "tkv_kv8_append": ([ctypes.POINTER(TkvKv8Cache), ctypes.POINTER(TkvKv8AppendArgs), vp], i32),
-        "tkv_kv8_attention_workspace": ([ctypes.POINTER(TkvKv8Cache), ctypes.POINTER(TkvKv8AttentionArgs),
-                                         ctypes.POINTER(ctypes.c_size_t)], i32),
-        "tkv_kv8_attention": ([ctypes.POINTER(TkvKv8Cache), ctypes.POINTER(TkvKv8AttentionArgs), vp], i32),
+        # argument blocks of these calls are passed as packed bytes or addresses
+        "tkv_kv8_plan_step": ([vp, vp], i32),
+        "tkv_rotary_embed": ([vp, vp], i32),
+        "tkv_kv8_append": ([vp, vp, vp], i32),
+        "tkv_kv8_attention_workspace": ([vp, vp, ctypes.POINTER(ctypes.c_size_t)], i32),
+        "tkv_kv8_attention": ([vp, vp, vp], i32),
     }
     for name, (argtypes, restype) in sigs.items():
         fn = getattr(lib, name)

@@ -200,9 +200,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
 cudaError_t launch_plan_step(const tkv_kv8_plan_args& p, cudaStream_t stream) {
   const size_t smem = sizeof(int32_t) * (4 * (size_t)p.requests + 3);
   if (smem > 40 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(plan_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(sizeof(int32_t) * (4 * TKV_KV8_MAX_REQUESTS + 3)));
+    static std::atomic<uint64_t> allowed;
+    const cudaError_t e = allow_smem(plan_step_kernel, (int)(sizeof(int32_t) * (4 * TKV_KV8_MAX_REQUESTS + 3)),
+                                     allowed);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};

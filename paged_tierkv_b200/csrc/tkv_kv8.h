@@ -6,12 +6,30 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "tierkv_b200.h"
 #include "tkv_internal.h"
 
 namespace tkv {
 
 using RotaryArgs = tkv_rotary;
+
+constexpr int kKv8MaxDevices = 64;
+
+// The opt-in to more than 48 KB of shared memory is per function and device;
+// `done` (one per function) holds the devices that have it.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev >= 0 && dev < kKv8MaxDevices ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 struct RotaryParams {
   RotaryArgs rot;

@@ -1,5 +1,6 @@
 // tkv_kv8_api.cu -- the tkv_kv8_* and tkv_rotary_* entry points: argument
 // checks, workspace layout and launches.  Nothing here allocates or throws.
+#include <atomic>
 #include <cmath>
 #include <cstring>
 
@@ -56,13 +57,17 @@ inline bool fits(size_t w, size_t counters, size_t data) {
   return counter_reserve(w) >= counters && data_base(w) + data <= w;
 }
 
+// SM count of the current device, looked up once per device.
 int32_t device_sms(int* sms) {
+  static std::atomic<int> known[kKv8MaxDevices];
   int dev = 0, major = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
-      major != 10 ||
+  if (cudaGetDevice(&dev) != cudaSuccess) return TKV_ERR_NO_DEVICE;
+  const bool cached = dev >= 0 && dev < kKv8MaxDevices;
+  if (cached && (*sms = known[dev].load(std::memory_order_relaxed)) > 0) return TKV_OK;
+  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10 ||
       cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return TKV_ERR_NO_DEVICE;
+  if (cached) known[dev].store(*sms, std::memory_order_relaxed);
   return TKV_OK;
 }
 
@@ -139,34 +144,31 @@ int32_t tkv_kv8_plan_step(const tkv_kv8_plan_args* a, void* stream) {
   return cuda_status(launch_plan_step(*a, reinterpret_cast<cudaStream_t>(stream)));
 }
 
-int32_t tkv_rotary_embed(const tkv_rotary* rotary, const tkv_token_view* q, const tkv_token_view* k,
-                         const tkv_token_view* q_out, const tkv_token_view* k_out, int32_t tokens,
-                         int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype,
-                         uint32_t* error_word, void* stream) {
-  if (tokens < 0 || heads < 0 || kv_heads < 0) return TKV_ERR_INVALID;
-  if (head_dim <= 0 || head_dim % 16 || head_dim > 256) return TKV_ERR_UNSUPPORTED;
-  if (dtype != TKV_DTYPE_F16 && dtype != TKV_DTYPE_BF16) return TKV_ERR_UNSUPPORTED;
-  int32_t st = check_rotary(rotary, head_dim, tokens > 0);
+int32_t tkv_rotary_embed(const tkv_rotary_args* a, void* stream) {
+  if (!a || a->tokens < 0 || a->heads < 0 || a->kv_heads < 0) return TKV_ERR_INVALID;
+  if (a->head_dim <= 0 || a->head_dim % 16 || a->head_dim > 256) return TKV_ERR_UNSUPPORTED;
+  if (a->dtype != TKV_DTYPE_F16 && a->dtype != TKV_DTYPE_BF16) return TKV_ERR_UNSUPPORTED;
+  const int32_t st = check_rotary(&a->rotary, a->head_dim, a->tokens > 0);
   if (st != TKV_OK) return st;
   RotaryParams p;
   std::memset(&p, 0, sizeof(p));
-  p.rot = *rotary;
-  if (tokens > 0 && heads > 0) {
-    if (!q || !q_out || check_view(*q) != TKV_OK || check_view(*q_out) != TKV_OK) return TKV_ERR_INVALID;
-    p.q = *q;
-    p.q_out = *q_out;
+  p.rot = a->rotary;
+  if (a->tokens > 0 && a->heads > 0) {
+    if (check_view(a->q) != TKV_OK || check_view(a->q_out) != TKV_OK) return TKV_ERR_INVALID;
+    p.q = a->q;
+    p.q_out = a->q_out;
   }
-  if (tokens > 0 && kv_heads > 0) {
-    if (!k || !k_out || check_view(*k) != TKV_OK || check_view(*k_out) != TKV_OK) return TKV_ERR_INVALID;
-    p.k = *k;
-    p.k_out = *k_out;
+  if (a->tokens > 0 && a->kv_heads > 0) {
+    if (check_view(a->k) != TKV_OK || check_view(a->k_out) != TKV_OK) return TKV_ERR_INVALID;
+    p.k = a->k;
+    p.k_out = a->k_out;
   }
-  p.err = error_word;
-  p.tokens = tokens;
-  p.heads = heads;
-  p.kv_heads = kv_heads;
-  p.head_dim = head_dim;
-  return cuda_status(launch_rotary(p, dtype, reinterpret_cast<cudaStream_t>(stream)));
+  p.err = a->error_word;
+  p.tokens = a->tokens;
+  p.heads = a->heads;
+  p.kv_heads = a->kv_heads;
+  p.head_dim = a->head_dim;
+  return cuda_status(launch_rotary(p, a->dtype, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 int32_t tkv_kv8_append(const tkv_kv8_cache* cache, const tkv_kv8_append_args* a, void* stream) {
@@ -174,16 +176,17 @@ int32_t tkv_kv8_append(const tkv_kv8_cache* cache, const tkv_kv8_append_args* a,
   if (st != TKV_OK) return st;
   if (!a || a->tokens < 0 || a->units_cap < 0 || a->heads < 0) return TKV_ERR_INVALID;
   if (a->dtype != TKV_DTYPE_F16 && a->dtype != TKV_DTYPE_BF16) return TKV_ERR_UNSUPPORTED;
-  if (a->heads > 0 && !a->rotary) return TKV_ERR_INVALID;
-  if (a->rotary && (st = check_rotary(a->rotary, cache->head_dim, a->tokens > 0)) != TKV_OK) return st;
+  const bool rotate = a->rotary.rot_dim != 0;
+  if (a->heads > 0 && !rotate) return TKV_ERR_INVALID;
+  if (rotate && (st = check_rotary(&a->rotary, cache->head_dim, a->tokens > 0)) != TKV_OK) return st;
   if (!a->num_units || (a->units_cap > 0 && (!a->units || !aligned(a->units, 16)))) return TKV_ERR_INVALID;
   if (a->tokens == 0) return TKV_OK;
   if (check_view(a->k) != TKV_OK || check_view(a->v) != TKV_OK) return TKV_ERR_INVALID;
   if (a->heads > 0 && (check_view(a->q) != TKV_OK || check_view(a->q_out) != TKV_OK)) return TKV_ERR_INVALID;
   AppendParams8 p;
   std::memset(&p, 0, sizeof(p));
-  if (a->rotary) p.rot = *a->rotary;
-  p.has_rot = a->rotary != nullptr;
+  p.rot = a->rotary;
+  p.has_rot = rotate;
   p.k = a->k;
   p.v = a->v;
   p.q = a->q;

@@ -688,7 +688,8 @@ template <int D, int BOXES, int FMT, int NT>
 cudaError_t launch_few(const AttnParams8& p, const CUtensorMap* maps, int sms, cudaStream_t stream) {
   using L = FewLayout<D, NT>;
   auto kern = few_rows_kernel<D, BOXES, FMT, NT>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  static std::atomic<uint64_t> allowed;
+  const cudaError_t e = allow_smem(kern, L::kBytes, allowed);
   if (e != cudaSuccess) return e;
   kern<<<sms * few_ctas_per_sm(NT), kFewThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
   return cudaGetLastError();

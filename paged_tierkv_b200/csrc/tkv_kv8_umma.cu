@@ -938,7 +938,8 @@ cudaError_t launch_many(AttnParams8 p, const CUtensorMap* maps, int sms, cudaStr
   at += (size_t)sms * 2 * kUnitRows * sizeof(float);
   p.merges = reinterpret_cast<MergeUnit*>(at);
   auto kern = many_rows_kernel<D, FMT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  static std::atomic<uint64_t> allowed;
+  cudaError_t e = allow_smem(kern, L::kBytes, allowed);
   if (e != cudaSuccess) return e;
   kern<<<sms, kManyThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
   e = cudaGetLastError();

@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -32,6 +33,17 @@ from . import ops
 _FORMAT = {torch.int8: N.TKV_KV8_INT8, torch.float8_e4m3fn: N.TKV_KV8_E4M3}
 _FLOATS = {torch.float16: N.TKV_DTYPE_F16, torch.bfloat16: N.TKV_DTYPE_BF16}
 MAX_REQUESTS = N.TKV_KV8_MAX_REQUESTS
+
+# The C structs of include/tierkv_b200.h, packed in one call each: filling them
+# through ctypes field by field costs more host time than the small kernels take.
+_VIEW = "Pqq"
+_ROTARY = "PPqq9i4x"
+_ROTARY_ARGS = struct.Struct(_ROTARY + 4 * _VIEW + "P5i4x")
+_APPEND_ARGS = struct.Struct(4 * _VIEW + "PPP" + _ROTARY + "4i")
+_ATTENTION_ARGS = struct.Struct(_VIEW + "PPPqPP7ifPQ")
+_PLAN_ARGS = struct.Struct("PPPqPPPPPPPPPPPP6i")
+_NO_VIEW = (0, 0, 0)
+_NO_ROTARY = (0,) * 13
 
 
 # ---------------------------------------------------------------------------
@@ -60,9 +72,11 @@ class Kv8Cache:
         self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
         self.blocks, self.kv_heads, self.block_size, self.head_dim = (int(x) for x in k_codes.shape)
         self.device = k_codes.device
+        # the tensors are held, so the addresses stay theirs
         self._struct = N.TkvKv8Cache(k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
                                      v_scale.data_ptr(), self.blocks, self.kv_heads, self.block_size,
                                      self.head_dim, _FORMAT[k_codes.dtype])
+        self._ptr = ctypes.addressof(self._struct)
 
     @classmethod
     def allocate(cls, blocks: int, kv_heads: int, block_size: int, head_dim: int, device,
@@ -101,7 +115,7 @@ class StepPlan:
         self.block_table, self.kv_lens, self.cu_q = block_table, kv_lens, cu_q
         self.admitted = self.slot_map = self.token_request = self.positions = self.free_count = None
         self.requests = 0
-        self._args = None
+        self._outputs = None
         for name in ("units", "num_units", "kv_lens", "cu_q"):
             t = getattr(self, name)
             if t is not None and (t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous()):
@@ -137,10 +151,9 @@ class StepPlan:
         plan.kv_lens, plan.cu_q = kv, cu
         plan.slot_map, plan.token_request, plan.positions = slot, req, pos
         plan.admitted, plan.free_count = adm, free
-        plan._args = N.TkvKv8PlanArgs(
-            None, None, None, 0, None, None, kv.data_ptr(), cu.data_ptr(), adm.data_ptr(),
-            slot.data_ptr(), req.data_ptr(), pos.data_ptr(), units.data_ptr(), num.data_ptr(),
-            free.data_ptr(), None, 0, 0, 0, 0, 0, plan.block_size)
+        plan._outputs = tuple(x.data_ptr() for x in (kv, cu, adm, slot, req, pos, units, num, free))
+        plan.device = buf.device
+        plan._caps = (r, t, cap)
         return plan
 
 
@@ -168,26 +181,30 @@ class Rotary:
         sec = (half,) if self.sections is None else tuple(int(x) for x in self.sections)
         if not 1 <= len(sec) <= 4 or any(x < 0 for x in sec) or sum(sec) != half:
             raise ValueError("sections must be 1 to 4 counts that add up to rot_dim / 2.")
-        object.__setattr__(self, "_struct", N.TkvRotary(
-            t.data_ptr(), None, int(t.shape[0]), 0, 4, int(t.shape[1]), len(sec),
-            (ctypes.c_int32 * 4)(*sec), int(bool(self.interleave)), int(bool(self.pairs))))
         object.__setattr__(self, "axes", len(sec))
+        object.__setattr__(self, "rot_dim", int(t.shape[1]))
+        object.__setattr__(self, "_tail", (int(t.shape[1]), len(sec), *sec, *(0,) * (4 - len(sec)),
+                                           int(bool(self.interleave)), int(bool(self.pairs))))
+        object.__setattr__(self, "_head", (t.data_ptr(), int(t.shape[0]), t.device))
 
     def _at(self, positions: torch.Tensor, tokens: int):
-        """(the C struct with these positions, the tensor that backs them)."""
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != self.cos_sin.device:
+        """(the fields of the C struct with these positions, the tensor that backs them)."""
+        ptr, rows, device = self._head
+        size = positions.element_size()
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != device:
             raise ValueError("positions must be int32 or int64 on the table's device.")
         if positions.ndim == 1 and self.axes == 1:
-            positions = positions.unsqueeze(0)
-        if positions.ndim != 2 or positions.shape[0] != self.axes or positions.shape[1] < tokens:
+            stride, (n,), (step,) = 0, positions.shape, positions.stride()
+        else:
+            if positions.ndim != 2 or positions.shape[0] != self.axes:
+                raise ValueError("positions must have shape [axes, tokens] (or [tokens] for one axis).")
+            n, (stride, step) = positions.shape[1], positions.stride()
+        if n < tokens:
             raise ValueError("positions must have shape [axes, tokens] (or [tokens] for one axis).")
-        if positions.shape[1] > 1 and positions.stride(1) != 1:
+        if n > 1 and step != 1:
             positions = positions.contiguous()
-        st = N.TkvRotary.from_buffer_copy(self._struct)
-        st.positions = positions.data_ptr()
-        st.positions_bytes = positions.element_size()
-        st.axis_stride = positions.stride(0)
-        return st, positions
+            stride = n
+        return (ptr, positions.data_ptr(), rows, stride, size, *self._tail), positions
 
 
 # ---------------------------------------------------------------------------
@@ -209,14 +226,19 @@ def _table_stride(table: torch.Tensor) -> int:
     return int(table.stride(0)) if table.shape[0] > 1 else int(table.shape[1])
 
 
-def _view(t: torch.Tensor) -> N.TkvTokenView | None:
-    """The strided view of [tokens, heads, head_dim], None if it is not 16-byte aligned throughout."""
+def _view(t: torch.Tensor):
+    """(address, token stride, head stride) of a [tokens, heads, head_dim] view,
+    None if it is not 16-byte aligned throughout."""
     n, h, d = t.shape
     s0, s1, s2 = t.stride()
-    s0, s1 = s0 if n > 1 else 0, s1 if h > 1 else 0
-    if (d > 1 and s2 != 1) or s0 % 8 or s1 % 8 or t.data_ptr() % 16:
+    ptr = t.data_ptr()
+    if n < 2:
+        s0 = 0
+    if h < 2:
+        s1 = 0
+    if (s2 != 1 and d > 1) or (ptr | s0 * 2 | s1 * 2) & 15:
         return None
-    return N.TkvTokenView(t.data_ptr(), s0, s1)
+    return ptr, s0, s1
 
 
 def _input_view(t: torch.Tensor):
@@ -228,7 +250,7 @@ def _input_view(t: torch.Tensor):
     return v, t
 
 
-def _output_view(t: torch.Tensor, like: torch.Tensor, name: str) -> N.TkvTokenView:
+def _output_view(t: torch.Tensor, like: torch.Tensor, name: str):
     if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must match its input in shape, dtype and device.")
     v = _view(t)
@@ -263,14 +285,18 @@ def _streamed(fn):
     return call
 
 
-def _call(device: torch.device, launch) -> None:
-    """Runs ``launch(current stream of device, its workspace)`` with ``device`` current."""
+_CURRENT_DEVICE = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _on_device(device: torch.device, call):
+    """call(stream handle, its workspace) with ``device`` current."""
     index = device.index
-    if index != torch.cuda.current_device():
+    if index != _CURRENT_DEVICE():
         with torch.cuda.device(index):
-            return _call(device, launch)
-    st = ops._stream(None, index)
-    launch(st, ops.workspace_for(device, st.value or 0, 1 << 16))
+            return _on_device(device, call)
+    st = ops._RAW_STREAM(index) if ops._RAW_STREAM is not None else torch.cuda.current_stream().cuda_stream
+    ws = ops._WORKSPACES.get((index, st))
+    return call(st, ws if ws is not None else ops.workspace_for(device, st, 1 << 16))
 
 
 # ---------------------------------------------------------------------------
@@ -292,36 +318,35 @@ def plan_step(plan: StepPlan, context_lens: torch.Tensor, new_lens: torch.Tensor
     allocated for) and returns it.  ``plan.kv_lens`` and ``plan.free_count`` may
     be passed back as the next step's context_lens and free_count.  ``tokens``:
     how many entries of the token outputs to write (default: all)."""
-    a = plan._args
-    if a is None:
+    if plan._outputs is None:
         raise ValueError("plan_step fills a plan made by StepPlan.allocate.")
-    n = int(context_lens.numel())
-    for t, name in ((context_lens, "context_lens"), (new_lens, "new_lens"), (free_blocks, "free_blocks"),
-                    (free_count, "free_count")):
-        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 CUDA tensor.")
-    if not 1 <= n <= plan.admitted.numel() or new_lens.numel() != n or free_count.numel() != 1:
+    n = context_lens.numel()
+    for t in (context_lens, new_lens, free_blocks, free_count):
+        if t.dtype != torch.int32 or t.device != plan.device or not t.is_contiguous():
+            raise ValueError("context_lens, new_lens, free_blocks and free_count must be contiguous int32 "
+                             "tensors on the plan's device.")
+    max_requests, max_tokens, max_units = plan._caps
+    if not 1 <= n <= max_requests or new_lens.numel() != n or free_count.numel() != 1:
         raise ValueError("context_lens and new_lens must have 1 to the plan's max_requests entries, free_count one.")
     _check_table(block_table, n)
-    cap = int(plan.slot_map.numel())
-    tokens = cap if tokens is None else int(tokens)
-    if not 0 <= tokens <= cap:
+    if block_table.device != plan.device:
+        raise ValueError("block_table must be on the plan's device.")
+    tokens = max_tokens if tokens is None else int(tokens)
+    if not 0 <= tokens <= max_tokens:
         raise ValueError("tokens must be between 0 and the plan's max_tokens.")
-    a.context_lens = context_lens.data_ptr()
-    a.new_lens = new_lens.data_ptr()
-    a.block_table = block_table.data_ptr()
-    a.table_stride = _table_stride(block_table)
-    a.free_blocks = free_blocks.data_ptr()
-    a.free_count = free_count.data_ptr()
-    a.requests, a.tokens, a.table_width = n, tokens, int(block_table.shape[1])
-    a.units_cap = min(_units_cap(n, tokens, plan.block_size), int(plan.units.shape[0]))
-    a.free_capacity = int(free_blocks.numel())
+    out = plan._outputs
 
-    def launch(st, ws):
-        a.error_word = ws.data_ptr()
-        N.check(N.load().tkv_kv8_plan_step(ctypes.byref(a), st), "tkv_kv8_plan_step")
+    def call(st, ws):
+        args = _PLAN_ARGS.pack(
+            context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), _table_stride(block_table),
+            free_blocks.data_ptr(), free_count.data_ptr(), *out, ws.data_ptr(), n, tokens,
+            min(_units_cap(n, tokens, plan.block_size), max_units), block_table.shape[1], free_blocks.numel(),
+            plan.block_size)
+        return N.load().tkv_kv8_plan_step(args, st)
 
-    _call(plan.kv_lens.device, launch)
+    status = _on_device(plan.device, call)
+    if status:
+        N.check(status, "tkv_kv8_plan_step")
     plan.block_table, plan.requests = block_table, n
     return plan
 
@@ -334,34 +359,38 @@ def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torc
     None) by their tokens' positions [axes, tokens]; returns (q_out, k_out).
     An output may be its input."""
     x = q if q is not None else k
-    if x is None:
-        raise ValueError("rotary_embed needs q or k.")
-    tokens, _, d = x.shape if x.ndim == 3 else (0, 0, 0)
-    views, outs, inputs = [], [], []
-    for t, out, name in ((q, q_out, "q"), (k, k_out, "k")):
-        if t is None:
-            views += [None, None]
-            outs.append(None)
-            continue
-        _heads3(t, name)
-        if t.shape[0] != tokens or t.shape[2] != d or t.dtype != x.dtype or t.device != x.device:
+    if x is None or x.ndim != 3:
+        raise ValueError("rotary_embed needs q or k [tokens, heads, head_dim].")
+    tokens, _, d = x.shape
+    dtype, device = x.dtype, x.device
+    qv = kv = qov = kov = _NO_VIEW
+    heads = kv_heads = 0
+    if q is not None:
+        _heads3(q, "q")
+        heads = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
+        qov = _output_view(q_out, q, "q_out")
+        qv, q = _input_view(q)
+    if k is not None:
+        _heads3(k, "k")
+        n, kv_heads, dk = k.shape
+        if n != tokens or dk != d or k.dtype != dtype or k.device != device:
             raise ValueError("q and k must agree in tokens, head_dim, dtype and device.")
-        if out is None:
-            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        v, t = _input_view(t)
-        views += [v, _output_view(out, t, name + "_out")]
-        outs.append(out)
-        inputs.append(t)  # a copy lives until the launch
+        if k_out is None:
+            k_out = torch.empty((tokens, kv_heads, d), dtype=dtype, device=device)
+        kov = _output_view(k_out, k, "k_out")
+        kv, k = _input_view(k)
     rot, positions = rotary._at(positions, tokens)
-    qv, qov, kv, kov = (None if v is None else ctypes.byref(v) for v in views)
 
-    def launch(st, ws):
-        N.check(N.load().tkv_rotary_embed(
-            ctypes.byref(rot), qv, kv, qov, kov, tokens, 0 if q is None else q.shape[1],
-            0 if k is None else k.shape[1], d, _FLOATS[x.dtype], ws.data_ptr(), st), "tkv_rotary_embed")
+    def call(st, ws):
+        args = _ROTARY_ARGS.pack(*rot, *qv, *kv, *qov, *kov, ws.data_ptr(), tokens, heads, kv_heads, d, _FLOATS[dtype])
+        return N.load().tkv_rotary_embed(args, st)
 
-    _call(x.device, launch)
-    return outs[0], outs[1]
+    status = _on_device(device, call)
+    if status:
+        N.check(status, "tkv_rotary_embed")
+    return (q_out if q is not None else None), (k_out if k is not None else None)
 
 
 @_streamed
@@ -376,45 +405,43 @@ def append(cache: Kv8Cache, plan: StepPlan, k: torch.Tensor, v: torch.Tensor, *,
     that already holds rows gets larger ones, its scale grows and its codes are
     rounded again.  A block with a NaN or an infinity gets scale NaN."""
     _heads3(k, "k")
-    _heads3(v, "v")
-    tokens = int(k.shape[0])
-    if tuple(k.shape) != (tokens, cache.kv_heads, cache.head_dim) or v.shape != k.shape or v.dtype != k.dtype:
+    shape, dtype, device = k.shape, k.dtype, cache.device
+    tokens = shape[0]
+    if shape[1] != cache.kv_heads or shape[2] != cache.head_dim or v.shape != shape or v.dtype != dtype:
         raise ValueError("k and v must have shape [tokens, kv_heads, head_dim] of the cache and one dtype.")
-    if k.device != cache.device or v.device != cache.device:
+    if k.device != device or v.device != device:
         raise ValueError("k and v must be on the cache's device.")
     if plan.units is None or plan.block_size != cache.block_size:
         raise ValueError("append needs a plan with write units of the cache's block size.")
-    if rotary is None and q is not None:
-        raise ValueError("q is rotated only: pass rotary and positions beside it.")
-    if rotary is not None and positions is None:
-        raise ValueError("rotary needs the tokens' positions.")
-    kv_view, k = _input_view(k)
-    v_view, v = _input_view(v)
-    args = N.TkvKv8AppendArgs()
-    args.k, args.v = kv_view, v_view
-    rot = None
+    rot, qv, qov, heads = _NO_ROTARY, _NO_VIEW, _NO_VIEW, 0
     if rotary is not None:
+        if positions is None:
+            raise ValueError("rotary needs the tokens' positions.")
         rot, positions = rotary._at(positions, tokens)
-        args.rotary = ctypes.pointer(rot)
+    elif q is not None:
+        raise ValueError("q is rotated only: pass rotary and positions beside it.")
     if q is not None:
         _heads3(q, "q")
-        if q.shape[0] != tokens or q.shape[2] != cache.head_dim or q.dtype != k.dtype or q.device != k.device:
+        n, heads, d = q.shape
+        if n != tokens or d != cache.head_dim or q.dtype != dtype or q.device != device:
             raise ValueError("q must agree with k in tokens, head_dim, dtype and device.")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        args.q, q = _input_view(q)
-        args.q_out = _output_view(q_out, q, "q_out")
-        args.heads = int(q.shape[1])
-    args.units, args.num_units = plan.units.data_ptr(), plan.num_units.data_ptr()
-    # no step writes more units than tokens
-    args.units_cap = min(int(plan.units.shape[0]), tokens)
-    args.tokens, args.dtype = tokens, _FLOATS[k.dtype]
+            q_out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
+        qov = _output_view(q_out, q, "q_out")
+        qv, q = _input_view(q)
+    kv, k = _input_view(k)
+    vv, v = _input_view(v)
+    units = plan.units
 
-    def launch(st, ws):
-        args.error_word = ws.data_ptr()
-        N.check(N.load().tkv_kv8_append(ctypes.byref(cache._struct), ctypes.byref(args), st), "tkv_kv8_append")
+    def call(st, ws):
+        # no step writes more units than tokens
+        args = _APPEND_ARGS.pack(*kv, *vv, *qv, *qov, units.data_ptr(), plan.num_units.data_ptr(), ws.data_ptr(), *rot,
+                                 min(units.shape[0], tokens), tokens, heads, _FLOATS[dtype])
+        return N.load().tkv_kv8_append(cache._ptr, args, st)
 
-    _call(cache.device, launch)
+    status = _on_device(device, call)
+    if status:
+        N.check(status, "tkv_kv8_append")
     return q_out if q is not None else None
 
 
@@ -434,37 +461,38 @@ def attention(q: torch.Tensor, cache: Kv8Cache, plan: StepPlan, scaling: float, 
     to no request are not written.  A request whose table names a block outside
     the cache reads zeros there (``TKV_DEVERR_BAD_SLOT``)."""
     _heads3(q, "q")
-    tokens, heads, d = (int(x) for x in q.shape)
-    if d != cache.head_dim or q.device != cache.device or heads % cache.kv_heads:
+    tokens, heads, d = q.shape
+    dtype, device = q.dtype, cache.device
+    if d != cache.head_dim or q.device != device or heads % cache.kv_heads:
         raise ValueError("q must match the cache in head_dim and device, and heads be a multiple of kv_heads.")
-    if plan.block_table is None or plan.block_size != cache.block_size:
+    table = plan.block_table
+    if table is None or plan.block_size != cache.block_size:
         raise ValueError("attention needs a plan with block tables of the cache's block size.")
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() \
+        out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
+    elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned tensor like q.")
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
     view, q = _input_view(q)
-    table = plan.block_table
-    args = N.TkvKv8AttentionArgs(
-        view, out.data_ptr(), None if lse is None else lse.data_ptr(), table.data_ptr(), _table_stride(table),
-        plan.kv_lens.data_ptr(), plan.cu_q.data_ptr(), plan.requests, tokens, heads, _FLOATS[q.dtype],
-        int(table.shape[1]), min(tokens, tokens if max_q_len is None else int(max_q_len)), int(window),
-        float(scaling), None, 0)
+    longest = tokens if max_q_len is None else min(tokens, int(max_q_len))
 
-    def launch(st, ws):
+    def call(st, ws):
         lib = N.load()
         for attempt in range(2):
-            args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
-            status = lib.tkv_kv8_attention(ctypes.byref(cache._struct), ctypes.byref(args), st)
+            args = _ATTENTION_ARGS.pack(
+                *view, out.data_ptr(), 0 if lse is None else lse.data_ptr(), table.data_ptr(), _table_stride(table),
+                plan.kv_lens.data_ptr(), plan.cu_q.data_ptr(), plan.requests, tokens, heads, _FLOATS[dtype],
+                table.shape[1], longest, int(window), scaling, ws.data_ptr(), ws.numel())
+            status = lib.tkv_kv8_attention(cache._ptr, args, st)
             if status != N.TKV_ERR_WORKSPACE or attempt:
-                break
+                return status
             nbytes = ctypes.c_size_t()
-            N.check(lib.tkv_kv8_attention_workspace(ctypes.byref(cache._struct), ctypes.byref(args),
-                                                    ctypes.byref(nbytes)), "tkv_kv8_attention_workspace")
-            ws = ops.workspace_for(cache.device, st.value or 0, nbytes.value)
-        N.check(status, "tkv_kv8_attention")
+            N.check(lib.tkv_kv8_attention_workspace(cache._ptr, args, ctypes.byref(nbytes)),
+                    "tkv_kv8_attention_workspace")
+            ws = ops.workspace_for(device, st, nbytes.value)
 
-    _call(cache.device, launch)
+    status = _on_device(device, call)
+    if status:
+        N.check(status, "tkv_kv8_attention")
     return (out, lse) if return_lse else out
