@@ -14,12 +14,12 @@
 // the unit to arrive merges them in CTA order (the result does not depend on
 // which one is last).
 //
-// Inside a CTA every warp runs by itself: it streams its 32-token tiles (TMA
-// boxes of K and V codes, scales by 4-byte asynchronous copies) through its own
-// ring of stages, computes S^T = K Q^T and O^T += V^T P^T with mma.m16n8k16 on
-// codes expanded to fp16 (exact for int8 and e4m3), and keeps its own softmax
-// statistics; the warps meet only at the end of a unit.  A warp's issue cursor
-// runs ahead over unit boundaries, so the ring stays full across them.
+// Inside a CTA one warp produces: it walks the block table and fills a ring of
+// stages (TMA boxes of K and V codes, scales by 4-byte asynchronous copies), ahead
+// over unit boundaries.  Each of the four consumer warps takes 32 tokens of a
+// stage, computes S^T = K Q^T and O^T += V^T P^T with mma.m16n8k16 on codes
+// expanded to fp16 (exact for int8 and e4m3), and keeps its own softmax
+// statistics; they meet only at the end of a unit.
 //
 // Scales: K's multiplies the logits in fp32.  V's is folded into P, normalised
 // by a power of two (vinv) so that P stays in fp16's normal range for any
@@ -48,29 +48,36 @@ static int few_row_tiles(int group, int max_q_len) {
   const int64_t rows = std::min<int64_t>((int64_t)group * max_q_len, kFewRowsMax);
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
-constexpr int few_ctas_per_sm(int nt) { return nt == 4 ? 1 : 2; }
+constexpr int few_ctas_per_sm(int nt, int d) { return nt == 4 && d == 128 ? 1 : 2; }
 
 constexpr int kFewWarps = 4;
-constexpr int kFewThreads = 32 * kFewWarps;
+constexpr int kFewConsumers = 32 * kFewWarps;
+constexpr int kFewThreads = kFewConsumers + 32;       // and the producer warp
 constexpr int kTileTok = 32;                          // tokens of a warp's tile
 constexpr int kStepTok = kTileTok * kFewWarps;        // tokens of a step
 
 template <int D, int NT>
 struct FewLayout {
-  static constexpr int kStages = 3;
+  static constexpr int kStages = D == 64 ? 4 : NT == 2 ? 2 : 3;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kHalf = kTileTok * D;           // codes of K (or V) in a stage
+  static constexpr int kHalf = kStepTok * D;           // codes of K (or V) in a stage
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int kRing = kFewWarps * kStages * kStage;
-  static constexpr int kQOff = kRing;                  // fp16 [rows][D + 16]
-  static constexpr int kQStride = D + 16;   // 8-byte fragment reads of 4 rows hit 32 banks
-  static constexpr int kMergeOff = kQOff + kRows * kQStride * 2;   // fp32 [2][rows][D + 4]
+  static constexpr int kRing = kStages * kStage;
+  // fp16 queries, rows D + 16 apart (8-byte fragment reads of 4 rows hit 32
+  // banks), and the accumulators that the warps add up at the end of a unit;
+  // with the query fragments in registers the two share their space
+  static constexpr bool kQRegs = NT == 1;
+  static constexpr int kQStride = D + 16;
   static constexpr int kMergeStride = D + 4;
-  static constexpr int kStatOff = kMergeOff + 2 * kRows * kMergeStride * 4;  // [warps][rows][2], row scales
-  static constexpr int kScaleOff = kStatOff + (kFewWarps + 1) * kRows * 8;   // [warps][stages][4]
-  static constexpr int kBarOff = kScaleOff + kFewWarps * kStages * 16;
-  static constexpr int kMiscOff = kBarOff + kFewWarps * kStages * 8;
-  static constexpr int kBytes = kMiscOff + 64 + 1024;  // + slack to align the ring to 1024
+  static constexpr int kQBytes = kRows * kQStride * 2;
+  static constexpr int kMergeBytes = 2 * kRows * kMergeStride * 4;
+  static constexpr int kQOff = kRing;
+  static constexpr int kMergeOff = kQRegs ? kQOff : kQOff + kQBytes;
+  static constexpr int kStatOff = kMergeOff + (kMergeBytes > kQBytes ? kMergeBytes : kQBytes);  // [warps][rows][2], row scales
+  static constexpr int kScaleOff = kStatOff + (kFewWarps + 1) * kRows * 8;   // [stages][16]: K's, V's
+  static constexpr int kBarOff = kScaleOff + kStages * 64;
+  static constexpr int kMiscOff = kBarOff + kStages * 16;
+  static constexpr int kBytes = kMiscOff + 64;
 };
 
 // Where a walk over the units stands.
@@ -124,41 +131,41 @@ __device__ __forceinline__ bool next_unit(const AttnParams8& p, int bs, UnitPos&
 }
 
 template <int D, int BOXES, int FMT, int NT>
-__global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
+__global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT, D))
     few_rows_kernel(const __grid_constant__ AttnParams8 p, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v) {
   using L = FewLayout<D, NT>;
   constexpr int RT = L::kRows;
   constexpr int S = L::kStages;
-  constexpr int kBoxes = BOXES;                         // TMA boxes of a tile (K; V alike)
+  constexpr int kBoxes = BOXES;                         // TMA boxes of a warp's tile (K; V alike)
   constexpr int kBox = kTileTok / kBoxes;               // rows of a box
+  constexpr int kStepBoxes = kFewWarps * kBoxes;        // boxes of a step (K; V alike)
   const int bs = p.block_size;
   const bool bf16 = p.bf16 != 0;
-  constexpr int kBatch = 32 / kBoxes;                   // tiles whose table cells a warp holds
+  constexpr int kBatch = 32 / kStepBoxes;               // steps whose table cells the producer holds
   constexpr int kSwz = D == 128 ? 7 : 3;
-  extern __shared__ uint8_t few_raw[];
-  const uint32_t raw = smem_u32(few_raw);
-  uint8_t* smem = few_raw + (((raw + 1023u) & ~1023u) - raw);
+  extern __shared__ __align__(1024) uint8_t few_smem[];
+  uint8_t* smem = few_smem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
-  uint8_t* ring = smem + warp * S * L::kStage;
   __half* q_s = reinterpret_cast<__half*>(smem + L::kQOff);
   float* merge_s = reinterpret_cast<float*>(smem + L::kMergeOff);
   float* stat_s = reinterpret_cast<float*>(smem + L::kStatOff);
   float* rscale_s = stat_s + kFewWarps * RT * 2;         // [RT] logit scale of each row
-  float* scale_s = reinterpret_cast<float*>(smem + L::kScaleOff) + warp * S * 4;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff) + warp * S;
+  float* scale_s = reinterpret_cast<float*>(smem + L::kScaleOff);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* empty = full + S;
   int64_t* range_s = reinterpret_cast<int64_t*>(smem + L::kMiscOff);   // scan scratch
   int* flag_s = reinterpret_cast<int*>(smem + L::kMiscOff + 56);
 
-  if (lane == 0) {
-    // one expect_tx arrival and one per scale-copying lane
-    for (int s = 0; s < S; ++s) mbar_init(full + s, 1 + 2 * kBoxes);
-    fence_mbar_init();
-    if (warp == 0) {
-      prefetch_tensormap(&tm_k);
-      prefetch_tensormap(&tm_v);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full + s, 1 + 2 * kStepBoxes);   // one expect_tx arrival and one per scale-copying lane
+      mbar_init(empty + s, kFewWarps);
     }
+    fence_mbar_init();
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
   }
 
   // ---- this CTA's range of the flat step list
@@ -180,7 +187,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
     int64_t before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) {
+    for (int w = 0; w < kFewThreads / 32; ++w) {
       if (w < warp) before += range_s[w];
       total += range_s[w];
     }
@@ -208,68 +215,62 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
     unit_at = range_s[0] + in * unit.steps;
   }
 
-  // ---- the warp's issue cursor: tile `warp` of every step of the range, S ahead
-  UnitPos iu = unit;
-  int64_t i_at = unit_at;               // flat index of iu's first step
-  int64_t i_pos = begin;                // next step to issue
-  int64_t issued = 0;
-  int32_t cells = 0;                    // lane: table cell (batch tile lane / kBoxes, box lane % kBoxes)
-  int64_t cells_at = -1;                // flat step of the batch's first tile
   bool ok = true;
-  auto issue = [&]() {
-    if (i_pos >= end || !ok) return;
-    if (i_pos >= i_at + iu.steps) {
-      i_at += iu.steps;
-      next_unit<RT>(p, bs, iu);
-      cells_at = -1;
-    }
-    const int step = iu.step0 + (int)(i_pos - i_at);
-    if (cells_at < 0 || i_pos - cells_at >= kBatch) {
-      cells_at = i_pos;
-      const int tok = (step + lane / kBoxes) * kStepTok + warp * kTileTok + (lane % kBoxes) * kBox;
-      cells = -1;
-      if (tok < iu.kv) cells = p.table[iu.req * p.table_stride + tok / bs];
-    }
-    const int s = (int)(issued % S);
-    const int tok0 = step * kStepTok + warp * kTileTok;
-    const int b = (int)(i_pos - cells_at) * kBoxes;
-    uint8_t* st = ring + s * L::kStage;
-    // lanes [0, kBoxes): K boxes, [kBoxes, 2 kBoxes): V boxes
-    const int box = lane % kBoxes;
-    const int cell = __shfl_sync(~0u, cells, b + box);
-    const int tok = tok0 + box * kBox;
-    const bool in_keys = tok < iu.kv && tok + kBox > (p.window > 0 ? iu.kv - iu.q_len - p.window + 1 : 0);
-    const bool good = in_keys && cell >= 0 && cell < p.blocks;
-    if (lane == 0) {
-      int n = 0;
-#pragma unroll
-      for (int x = 0; x < kBoxes; ++x) {
-        const int tx = tok0 + x * kBox;
-        n += tx < iu.kv && tx + kBox > (p.window > 0 ? iu.kv - iu.q_len - p.window + 1 : 0);
+  if (warp == kFewWarps) {
+    // ---- producer: lane = box of the step (K in [0, kStepBoxes), V in [kStepBoxes, 2 kStepBoxes))
+    const int box = lane % kStepBoxes;
+    const bool is_v = lane >= kStepBoxes;
+    const CUtensorMap* map = is_v ? &tm_v : &tm_k;
+    const float* scales = is_v ? p.v_scale : p.k_scale;
+    const uint32_t code_off = (is_v ? L::kHalf : 0) + box * kBox * D;
+    int32_t cells = 0;                    // table cell of box lane % kStepBoxes, step lane / kStepBoxes of the batch
+    int left = 0;                         // steps left in the batch
+    int64_t issued = 0;
+    for (int64_t at = begin; at < end; ++at, ++issued) {
+      if (at >= unit_at + unit.steps) {
+        unit_at += unit.steps;
+        next_unit<RT>(p, bs, unit);
+        left = 0;
       }
-      mbar_arrive_expect_tx(full + s, n * 2 * kBox * D);
-    }
-    __syncwarp();
-    if (lane < 2 * kBoxes) {
-      const bool is_v = lane >= kBoxes;
-      const int64_t blk = good ? cell : 0;   // a bad slot loads block 0 under scale 0: zeros
-      if (in_keys) {
-        tma_load_2d(st + (is_v ? L::kHalf : 0) + box * kBox * D, is_v ? &tm_v : &tm_k, 0,
-                    (int)((blk * p.kv_heads + iu.head) * bs + tok % bs), full + s);
-        if (!good) atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
+      const int step = unit.step0 + (int)(at - unit_at);
+      if (left == 0) {
+        left = kBatch;
+        const int tok = (step + lane / kStepBoxes) * kStepTok + box * kBox;
+        cells = tok < unit.kv ? p.table[unit.req * p.table_stride + tok / bs] : -1;
       }
-      float* dst = scale_s + s * 4 + lane;
-      if (good) cp_async4(dst, (is_v ? p.v_scale : p.k_scale) + blk * p.kv_heads + iu.head);
-      else *dst = 0.f;
-      cp_async_mbar_arrive(full + s);
+      const int cell = __shfl_sync(~0u, cells, (kBatch - left) * kStepBoxes + box);
+      --left;
+      const int tok = step * kStepTok + box * kBox;
+      const int any_lo = p.window > 0 ? unit.kv - unit.q_len - p.window + 1 : 0;
+      const bool in_keys = tok < unit.kv && tok + kBox > any_lo && lane < 2 * kStepBoxes;
+      const bool good = in_keys && cell >= 0 && cell < p.blocks;
+      const int s = (int)(issued % S);
+      if (!mbar_wait(empty + s, (uint32_t)((issued / S) & 1) ^ 1)) {
+        ok = false;
+        break;
+      }
+      const uint32_t bytes = __popc(__ballot_sync(~0u, in_keys)) * kBox * D;
+      if (lane == 0) mbar_arrive_expect_tx(full + s, bytes);
+      __syncwarp();
+      if (lane < 2 * kStepBoxes) {
+        const int blk = good ? cell : 0;  // a bad slot loads block 0 under scale 0: zeros
+        if (in_keys) {
+          tma_load_2d(smem + s * L::kStage + code_off, map, 0,
+                      (blk * p.kv_heads + unit.head) * bs + (tok & (bs - 1)), full + s);
+          if (!good) atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
+        }
+        float* dst = scale_s + s * 16 + lane;
+        if (good) cp_async4(dst, scales + (int64_t)blk * p.kv_heads + unit.head);
+        else *dst = 0.f;
+        cp_async_mbar_arrive(full + s);
+      }
     }
-    __syncwarp();
-    ++issued;
-    ++i_pos;
-  };
-  __syncwarp();
-#pragma unroll 1
-  for (int s = 0; s < S; ++s) issue();
+    // no copy may still be landing when the CTA exits
+    for (int64_t i = max((int64_t)0, issued - S); i < issued; ++i)
+      ok = mbar_wait(full + i % S, (uint32_t)((i / S) & 1)) && ok;
+    if (!ok && lane == 0) atomicOr(p.err, TKV_DEVERR_TIMEOUT);
+    return;                               // the consumers' barriers do not count this warp
+  }
 
   // ---- units
   const int lm_row = (lane & 7) + ((lane >> 3) & 1) * 8;   // ldmatrix: row and 16-byte chunk of this lane
@@ -306,8 +307,8 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
             pack_half2(x[i].x * up, x[i].y * up);
       if (lane == 0) rscale_s[r] = p.scale_log2 * down;
     }
-    __syncthreads();
-    constexpr bool kQRegs = NT <= 2;     // few rows: their fragments stay in registers
+    named_barrier(1, kFewConsumers);
+    constexpr bool kQRegs = L::kQRegs;
     uint2 qf[kQRegs ? NT : 1][kQRegs ? D / 16 : 1];
     if constexpr (kQRegs) {
 #pragma unroll
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
       __syncwarp();
       const uint32_t tok_ = wait_token();
       const int tok0 = (unit.step0 + (int)(pos - unit_at)) * kStepTok + warp * kTileTok;
-      uint8_t* st = ring + s * L::kStage;
+      uint8_t* st = smem + s * L::kStage + warp * (kTileTok * D);
       if (tok0 < unit.kv && tok0 + kTileTok > any_lo) {
         const uint32_t kaddr = after(smem_u32(st), tok_);
         const bool edge = tok0 + kTileTok > all_hi || tok0 < all_lo;
@@ -368,8 +369,8 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
         float ks[kBoxes], vs[kBoxes];
 #pragma unroll
         for (int b = 0; b < kBoxes; ++b) {
-          ks[b] = scale_s[s * 4 + b];
-          vs[b] = scale_s[s * 4 + kBoxes + b];
+          ks[b] = scale_s[s * 16 + warp * kBoxes + b];
+          vs[b] = scale_s[s * 16 + kStepBoxes + warp * kBoxes + b];
         }
         // S^T: 2 x 16 tokens, 8 NT rows
         float sc[NT][2][4];
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
       for (int u = 0; u < D / 16; ++u) hold(acc[0][u][0]);
       ++consumed;
       __syncwarp();   // every lane has read the stage
-      issue();
+      if (lane == 0) mbar_arrive(empty + s);
     }
 
     // ---- the CTA's share of the unit: merge the warps' statistics and accumulators
@@ -526,7 +527,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
           stat_s[(warp * RT + n * 8 + 2 * t4 + c) * 2 + 1] = l[n][c];
         }
       }
-    __syncthreads();
+    named_barrier(1, kFewConsumers);
     float mm[NT][2], ll[NT][2];
     const float back = vinv == 0.f ? 0.f : 1.f / vinv;
 #pragma unroll
@@ -585,11 +586,11 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
     };
     float* buf = merge_s + (warp & 1) * RT * L::kMergeStride;
     if (warp >= 2) put(buf);
-    __syncthreads();
+    named_barrier(1, kFewConsumers);
     if (warp < 2) add(buf);
     __syncwarp();
     if (warp == 1) put(buf);
-    __syncthreads();
+    named_barrier(1, kFewConsumers);
     const int64_t u0 = unit_at, u1 = unit_at + unit.steps;
     const bool whole = begin <= u0 && end >= u1;
     const int slot = begin >= u0 ? 0 : 1;
@@ -630,13 +631,13 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
       // CTAs whose ranges meet this unit: start(c) = total c / ctas
       const int c0 = (int)(((u0 + 1) * ctas - 1) / total);
       const int c1 = (int)((u1 * ctas - 1) / total);
-      __syncthreads();
+      named_barrier(1, kFewConsumers);
       if (threadIdx.x == 0) {
         const uint32_t n = atom_add_acq_rel_gpu(p.counters + c0, 1u);
         *flag_s = n == (uint32_t)(c1 - c0);
         if (*flag_s) p.counters[c0] = 0;
       }
-      __syncthreads();
+      named_barrier(1, kFewConsumers);
       if (*flag_s) {
         const int64_t stride = (int64_t)2 * RT * (D + 2);
         // CTA c0's share sits in slot 0 when its range starts at the unit, else in slot 1
@@ -645,7 +646,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
         const float* rest = reinterpret_cast<const float*>(p.data) + (int64_t)c0 * stride;
         const int parts = c1 - c0 + 1;
         constexpr int kLanes = D / 4;    // threads of a row
-        for (int r = threadIdx.x / kLanes; r < rows; r += kFewThreads / kLanes) {
+        for (int r = threadIdx.x / kLanes; r < rows; r += kFewConsumers / kLanes) {
           const int d4 = (threadIdx.x % kLanes) * 4;
           float mx = -INFINITY;
           for (int i = 0; i < parts; ++i)
@@ -669,16 +670,12 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT))
         }
       }
     }
-    __syncthreads();   // the shared buffers are free for the next unit
+    named_barrier(1, kFewConsumers);   // the shared buffers are free for the next unit
     if (pos < end) {
       unit_at += unit.steps;
       next_unit<RT>(p, bs, unit);
     }
   }
-  // after a timeout: no copy may still be landing when the CTA exits
-  if (!ok)
-    for (int64_t i = max((int64_t)0, issued - S); i < issued; ++i)
-      mbar_wait(full + i % S, (uint32_t)((i / S) & 1));
 }
 
 // ---------------------------------------------------------------- host side
@@ -691,7 +688,7 @@ cudaError_t launch_few(const AttnParams8& p, const CUtensorMap* maps, int sms, c
   static std::atomic<uint64_t> allowed;
   const cudaError_t e = allow_smem(kern, L::kBytes, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<sms * few_ctas_per_sm(NT), kFewThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
+  kern<<<sms * few_ctas_per_sm(NT, D), kFewThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
   return cudaGetLastError();
 }
 
@@ -716,7 +713,7 @@ cudaError_t few_format(const AttnParams8& p, const CUtensorMap* maps, int sms, i
 
 void kv8_attention_scratch(int sms, int d, int group, int max_q_len, size_t* counters, size_t* data) {
   const int nt = few_row_tiles(group, max_q_len);
-  const size_t ctas = (size_t)sms * few_ctas_per_sm(nt);
+  const size_t ctas = (size_t)sms * few_ctas_per_sm(nt, d);
   *counters = ctas * sizeof(uint32_t);
   *data = ctas * 2 * 8 * nt * (d + 2) * sizeof(float);
   if ((int64_t)group * max_q_len > kFewRowsMax) *data = std::max(*data, many_rows_scratch(sms, d));
