@@ -2,7 +2,7 @@
 // few query rows (single tokens, drafted tokens, short chunks).
 //
 // A row is one (query token, query head); the rows of a kv head share its K/V,
-// so they are packed into tiles of 8 * NT rows and every code is read once per
+// so they are packed into tiles of 8 * NT rows (NT 1 or 2) and every code is read once per
 // tile.  At few rows the kernel is bound by HBM: 2 head_dim bytes per token and
 // kv head against 4 head_dim rows flops.
 //
@@ -39,16 +39,20 @@
 
 namespace tkv {
 
-// Rows per kv head up to which a request runs here.
-constexpr int kFewRowsMax = 64;
-
-// Row tiles of 8 that an instance of the kernel holds, by the most rows a
-// request of this kernel may have.
+// Which kernel takes a request, by its rows per kv head.  When no request has
+// more than 16, all run here, in row tiles of 8 or 16.  Otherwise requests of up
+// to 8 rows run here and the others in many_rows_kernel, whose smallest tile of
+// 128 rows still beats this kernel's 16-row instance for a batch of both (23
+// requests of 7 to 42 rows: 70 us against 89; chunks beside single tokens: 80
+// against 95), though not for 16 rows alone (32 x 32768 tokens: 170 us against
+// 300).  A 32-row instance took 594 us there.
+constexpr int kFewRowsAlone = 16;
+constexpr int kFewRowsBeside = 8;
+static bool has_many_rows(int group, int max_q_len) { return (int64_t)group * max_q_len > kFewRowsAlone; }
 static int few_row_tiles(int group, int max_q_len) {
-  const int64_t rows = std::min<int64_t>((int64_t)group * max_q_len, kFewRowsMax);
-  return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  return has_many_rows(group, max_q_len) || (int64_t)group * max_q_len <= 8 ? 1 : 2;
 }
-constexpr int few_ctas_per_sm(int nt, int d) { return nt == 4 && d == 128 ? 1 : 2; }
+constexpr int kFewCtasPerSm = 2;
 
 constexpr int kFewWarps = 4;
 constexpr int kFewConsumers = 32 * kFewWarps;
@@ -58,7 +62,7 @@ constexpr int kStepTok = kTileTok * kFewWarps;        // tokens of a step
 
 template <int D, int NT>
 struct FewLayout {
-  static constexpr int kStages = D == 64 ? 4 : NT == 2 ? 2 : 3;
+  static constexpr int kStages = D == 64 ? 5 : 3;      // what two CTAs an SM have room for
   static constexpr int kRows = 8 * NT;
   static constexpr int kHalf = kStepTok * D;           // codes of K (or V) in a stage
   static constexpr int kStage = 2 * kHalf;
@@ -70,7 +74,8 @@ struct FewLayout {
   static constexpr int kQStride = D + 16;
   static constexpr int kMergeStride = D + 4;
   static constexpr int kQBytes = kRows * kQStride * 2;
-  static constexpr int kMergeBytes = 2 * kRows * kMergeStride * 4;
+  static constexpr int kMergeBufs = NT == 1 ? 2 : 1;
+  static constexpr int kMergeBytes = kMergeBufs * kRows * kMergeStride * 4;
   static constexpr int kQOff = kRing;
   static constexpr int kMergeOff = kQRegs ? kQOff : kQOff + kQBytes;
   static constexpr int kStatOff = kMergeOff + (kMergeBytes > kQBytes ? kMergeBytes : kQBytes);  // [warps][rows][2], row scales
@@ -131,7 +136,7 @@ __device__ __forceinline__ bool next_unit(const AttnParams8& p, int bs, UnitPos&
 }
 
 template <int D, int BOXES, int FMT, int NT>
-__global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT, D))
+__global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     few_rows_kernel(const __grid_constant__ AttnParams8 p, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v) {
   using L = FewLayout<D, NT>;
@@ -553,7 +558,8 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT, D))
           acc[n][u][2 + c] *= f;
         }
       }
-    // warps 3 and 2 hand their accumulators to 1 and 0, then 1 to 0
+    // warps 3 and 2 hand their accumulators to 1 and 0, then 1 to 0; with one
+    // buffer 3 to 2, 1 to 0, 2 to 0
     auto put = [&](float* dst) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -584,19 +590,29 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas_per_sm(NT, D))
             }
           }
     };
-    float* buf = merge_s + (warp & 1) * RT * L::kMergeStride;
-    if (warp >= 2) put(buf);
-    named_barrier(1, kFewConsumers);
-    if (warp < 2) add(buf);
-    __syncwarp();
-    if (warp == 1) put(buf);
-    named_barrier(1, kFewConsumers);
+    if constexpr (L::kMergeBufs == 2) {
+      float* buf = merge_s + (warp & 1) * RT * L::kMergeStride;
+      if (warp >= 2) put(buf);
+      named_barrier(1, kFewConsumers);
+      if (warp < 2) add(buf);
+      __syncwarp();
+      if (warp == 1) put(buf);
+      named_barrier(1, kFewConsumers);
+      if (warp == 0) add(merge_s + RT * L::kMergeStride);
+    } else {
+      for (int round = 0; round < 3; ++round) {
+        const int from = round == 0 ? 3 : round == 1 ? 1 : 2, to = round == 0 ? 2 : 0;
+        if (warp == from) put(merge_s);
+        named_barrier(1, kFewConsumers);
+        if (warp == to) add(merge_s);
+        named_barrier(1, kFewConsumers);
+      }
+    }
     const int64_t u0 = unit_at, u1 = unit_at + unit.steps;
     const bool whole = begin <= u0 && end >= u1;
     const int slot = begin >= u0 ? 0 : 1;
     float* part = reinterpret_cast<float*>(p.data) + ((int64_t)blockIdx.x * 2 + slot) * RT * (D + 2);
     if (warp == 0) {
-      add(merge_s + RT * L::kMergeStride);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -688,16 +704,14 @@ cudaError_t launch_few(const AttnParams8& p, const CUtensorMap* maps, int sms, c
   static std::atomic<uint64_t> allowed;
   const cudaError_t e = allow_smem(kern, L::kBytes, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<sms * few_ctas_per_sm(NT, D), kFewThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
+  kern<<<sms * kFewCtasPerSm, kFewThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
   return cudaGetLastError();
 }
 
 template <int D, int BOXES, int FMT>
 cudaError_t few_nt(const AttnParams8& p, const CUtensorMap* maps, int sms, cudaStream_t s) {
-  const int nt = few_row_tiles(p.group, p.max_q_len);
-  if (nt == 1) return launch_few<D, BOXES, FMT, 1>(p, maps, sms, s);
-  if (nt == 2) return launch_few<D, BOXES, FMT, 2>(p, maps, sms, s);
-  return launch_few<D, BOXES, FMT, 4>(p, maps, sms, s);
+  return few_row_tiles(p.group, p.max_q_len) == 1 ? launch_few<D, BOXES, FMT, 1>(p, maps, sms, s)
+                                                  : launch_few<D, BOXES, FMT, 2>(p, maps, sms, s);
 }
 
 template <int D>
@@ -713,18 +727,18 @@ cudaError_t few_format(const AttnParams8& p, const CUtensorMap* maps, int sms, i
 
 void kv8_attention_scratch(int sms, int d, int group, int max_q_len, size_t* counters, size_t* data) {
   const int nt = few_row_tiles(group, max_q_len);
-  const size_t ctas = (size_t)sms * few_ctas_per_sm(nt, d);
+  const size_t ctas = (size_t)sms * kFewCtasPerSm;
   *counters = ctas * sizeof(uint32_t);
   *data = ctas * 2 * 8 * nt * (d + 2) * sizeof(float);
-  if ((int64_t)group * max_q_len > kFewRowsMax) *data = std::max(*data, many_rows_scratch(sms, d));
+  if (has_many_rows(group, max_q_len)) *data = std::max(*data, many_rows_scratch(sms, d));
 }
 
 cudaError_t launch_kv8_attention(const AttnParams8& args, int sms, int d, int format, cudaStream_t stream) {
   AttnParams8 p = args;
-  const bool many = (int64_t)p.group * p.max_q_len > kFewRowsMax;
+  const bool many = has_many_rows(p.group, p.max_q_len);
   // a lone request needs one kernel: the one for its largest possible size; and
   // without a request that max_q_len calls long, this kernel takes all
-  p.few_rows_max = !many ? 0x7fffffff : p.requests == 1 ? 0 : kFewRowsMax;
+  p.few_rows_max = !many ? 0x7fffffff : p.requests == 1 ? 0 : kFewRowsBeside;
   CUtensorMap maps[2];
   if (!kv8_code_maps(p, d, maps)) return cudaErrorInvalidValue;
   if (p.few_rows_max > 0) {
