@@ -31,8 +31,10 @@
 // V's go into the exponent: P' = exp2(s - m + log2(vs vinv)), vinv a power of
 // two that keeps P' in fp16's normal range, and the row sum gets p back by one
 // multiplication with 1 / vs per 16 columns.  m follows the running maximum
-// lazily: O is only rescaled when it has grown by more than 8 (a factor 2^8
-// that fp16 holds).  bf16 queries become fp16 by a power of two per row.
+// lazily: O is only rescaled when it has grown by more than 3.9 (log2; by more
+// than 2 the 8192-token prompt takes 8 % longer).  With vs vinv at most 2^12, P'
+// stays below fp16's largest number and normal down to 2^-25 of the row's largest.  bf16 queries become fp16 by a power of
+// two per row.
 //
 // Work is a flat list of (unit, K/V tile), where a unit counts kUnitCost tiles
 // more than it has (loading Q, writing the output), cut evenly over the CTAs,
@@ -54,8 +56,8 @@ constexpr int kGroups = kTok / 16;        // scale groups of a tile
 constexpr int kScStride = kGroups + 1;    // and (log2 of the largest V scale, first token, first and last key)
 constexpr int kUnitCost = 4;              // a unit's fixed cost in tiles
 constexpr uint32_t kManyTmem = 512;
-constexpr float kTinyScale = 7.8886091e-31f;   // 2^-100
-constexpr float kLazy = 8.f;              // growth of the maximum (log2) that P absorbs
+constexpr float kVLog = 12.f;             // log2 of vs vinv, at most, for the largest V scale so far
+constexpr float kLazy = 3.9f;             // growth of the maximum (log2) that P' absorbs
 
 template <int D>
 struct ManyLayout {
@@ -479,12 +481,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const int box_grp = (lane & (boxes - 1)) * (box / 16);   // and its box's first group
     Walk w = walk;
     int j = 0, i = 0, cell = 0;
-    float ks = 0.f, vs = 0.f;
+    float ks = 0.f, vs = 0.f, run_top = 0.f;
+    bool first = false;                                   // a segment's first tile
     int tok0 = 0, lo = 0, hi = 0, head = 0;               // of the tile whose cells are held
     bool seen = false;                                    // the lane's group holds keys of the unit
     auto load = [&]() {
       if (!w.more()) return;
       tok0 = (w.first() + i) * kTok;
+      first = i == 0;
       lo = w.u.req_lo;
       hi = w.u.kv;
       head = w.u.head;
@@ -508,15 +512,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     bool more = w.more();
     load();
     for (; more; ++j) {
-      // a V scale of 0 counts as 2^-100: its values stay below any output's last
-      // bit, and the row sum gets the group's p back
-      const float v1 = vs < kTinyScale ? kTinyScale : vs;
-      float top = v1 < 3e38f ? v1 : kTinyScale;           // a NaN does not move vinv
+      // the segment's largest V scale so far; a NaN does not move vinv
+      float top = vs < 3e38f ? vs : 0.f;
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+      run_top = fmaxf(first ? 0.f : run_top, top);
+      top = run_top > 0.f ? run_top : 1.f;
+      // a group whose V scale is 0 (nothing stored, a bad slot) has its codes
+      // zeroed, and takes a scale that is as good as any
+      const float v1 = vs == 0.f ? top : vs;
       float4* sc = scales + (j & 3) * kScStride;
-      if (lane < kGroups) sc[lane] = make_float4(ks, v1, lg2(v1), 1.f / v1);
+      if (lane < kGroups) sc[lane] = make_float4(ks, vs, lg2(v1), 1.f / v1);
       if (lane == 0)
         sc[kGroups] = make_float4(lg2(top), __int_as_float(tok0), __int_as_float(lo), __int_as_float(hi));
       __syncwarp();
@@ -577,7 +584,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         for (int i = 0; i < kPerRow; ++i) {
           uint4 x = *reinterpret_cast<const uint4*>(src + i * kPassRows * D);
           // rows that nobody sees may hold anything
-          if (tok + i * kPassRows < lo || tok + i * kPassRows >= hi) x = make_uint4(0, 0, 0, 0);
+          if (tok + i * kPassRows < lo || tok + i * kPassRows >= hi ||
+              (kv && scales[(j & 3) * kScStride + (row + i * kPassRows) / 16].y == 0.f))
+            x = make_uint4(0, 0, 0, 0);
           uint4 f[2];
           expand4<FMT>(x.x, f[0].x, f[0].y);
           expand4<FMT>(x.y, f[0].z, f[0].w);
@@ -718,9 +727,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         float shift = 0.f;                            // log2 of the factor O and l take
         const float vtop = sc[kGroups - half * 4].x;
         if (j == 0) {
-          vlog = 6.f - ceilf(vtop);
-        } else if (vtop + vlog > 7.f) {
-          shift = 6.f - ceilf(vtop) - vlog;
+          vlog = kVLog - ceilf(vtop);
+        } else if (vtop + vlog > kVLog + 1e-3f) {
+          shift = kVLog - ceilf(vtop) - vlog;
           vlog += shift;
         }
         if (mx > m + kLazy) {
