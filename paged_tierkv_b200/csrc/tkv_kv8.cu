@@ -7,6 +7,7 @@
 
 #include "tierkv_b200.h"
 #include "tkv_kv8.h"
+#include "tkv_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -23,8 +24,11 @@ namespace tkv {
 // scanned sums.  A cluster barrier between the last read of an input and the
 // first write lets kv_lens / free_count be updated in place.  Latency bound:
 // a launch, one round of loads, two block scans.
+// Small steps (up to 1024 requests, tokens and write units) take one CTA of 256
+// threads, whose barriers are cheaper than the cluster's; others 8 of 1024.
 constexpr int kPlanCluster = 8;
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024, kPlanSmall = 256;
+constexpr int kPlanSmallWork = 1024;
 
 struct Scan {
   int32_t warp_sum[2][32];
@@ -50,7 +54,8 @@ __device__ __forceinline__ void scan2(Scan& s, int32_t a, int32_t b, int32_t& ea
     s.warp_sum[1][warp] = ib;
   }
   __syncthreads();
-  int32_t wa = s.warp_sum[0][lane], wb = s.warp_sum[1][lane];  // kPlanThreads / 32 == 32 warps
+  const bool has = lane < (int)blockDim.x / 32;
+  int32_t wa = has ? s.warp_sum[0][lane] : 0, wb = has ? s.warp_sum[1][lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int32_t xa = __shfl_up_sync(~0u, wa, o), xb = __shfl_up_sync(~0u, wb, o);
@@ -78,16 +83,20 @@ __device__ __forceinline__ int find(const int32_t* first, int n, int32_t x) {
   return lo;
 }
 
-__device__ __forceinline__ int32_t ceil_div(int32_t x, int bs) {
-  return (int32_t)(((int64_t)x + bs - 1) / bs);
+// x / 2^log2, rounded up.
+__device__ __forceinline__ int32_t ceil_div(int32_t x, int log2) {
+  return (int32_t)(((uint32_t)x + (1u << log2) - 1) >> log2);
 }
 
-__global__ void __launch_bounds__(kPlanThreads, 1)
-    plan_step_kernel(const tkv_kv8_plan_args p) {
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads, 1)
+    plan_step_kernel(const __grid_constant__ tkv_kv8_plan_args p) {
   extern __shared__ int32_t plan_smem[];
   __shared__ Scan scan;
   const cg::cluster_group cluster = cg::this_cluster();
-  const int n = p.requests, bs = p.block_size, tid = threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int n = p.requests, bs = p.block_size, bs_log2 = 31 - __clz(bs), tid = threadIdx.x;
   int32_t* ctx = plan_smem;            // [n]      cached tokens, bit 31: not admitted
   int32_t* cu = ctx + n;               // [n + 1]  first packed token
   int32_t* need = cu + n + 1;          // [n + 1]  running sum of new blocks
@@ -95,16 +104,16 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
   const int32_t free_count = max(0, min(*p.free_count, p.free_capacity));
 
   // lengths -> running sums of the new tokens and the new blocks; a thread
-  // owns n / 1024 consecutive requests
-  const int per = (n + kPlanThreads - 1) / kPlanThreads;
+  // owns n / kThreads consecutive requests
+  const int per = (n + kThreads - 1) / kThreads;
   const int r0 = min(n, tid * per), r1 = min(n, r0 + per);
   int32_t sum_new = 0, sum_need = 0;
   for (int i = r0; i < r1; ++i) {
     const int32_t c = max(0, p.context_lens[i]), m = max(0, p.new_lens[i]);
-    const int32_t want = ceil_div(c + m, bs);
+    const int32_t want = ceil_div(c + m, bs_log2);
     ctx[i] = c;
     cu[i] = m;
-    need[i] = want <= p.table_width ? want - ceil_div(c, bs) : -1;
+    need[i] = want <= p.table_width ? want - ceil_div(c, bs_log2) : -1;
     sum_new += m;
     sum_need += max(0, need[i]);
   }
@@ -119,7 +128,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
     if (!ok && m > 0) refused = true;
     cu[i] = at_new;
     need[i] = at_need;
-    cu_unit[i] = ok && m > 0 ? ceil_div(c + m, bs) - c / bs : 0;
+    cu_unit[i] = ok && m > 0 ? ceil_div(c + m, bs_log2) - (c >> bs_log2) : 0;
     sum_units += cu_unit[i];
     at_new += m;
     at_need += max(0, k);
@@ -140,8 +149,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
   cluster.sync();  // every CTA has read its inputs; shared memory is complete
 
   const int rank = (int)cluster.block_rank();
-  const int gtid = rank * kPlanThreads + tid;
-  constexpr int kStride = kPlanCluster * kPlanThreads;
+  const int gtid = rank * kThreads + tid;
+  const int stride = (int)cluster.num_blocks() * kThreads;
+  const bool vec = ((reinterpret_cast<uintptr_t>(p.slot_map) | reinterpret_cast<uintptr_t>(p.token_request) |
+                     reinterpret_cast<uintptr_t>(p.positions)) & 15) == 0;
   if (rank == 0) {
     for (int i = r0; i < r1; ++i) {
       const int32_t c = ctx[i] & 0x7fffffff;
@@ -158,65 +169,95 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
   }
 
   // new table cells
-  for (int u = gtid; u < total_need; u += kStride) {
+  for (int u = gtid; u < total_need; u += stride) {
     const int i = find(need, n, u);
     if (ctx[i] < 0) continue;
-    p.block_table[i * p.table_stride + ceil_div(ctx[i], bs) + (u - need[i])] =
+    p.block_table[i * p.table_stride + ceil_div(ctx[i], bs_log2) + (u - need[i])] =
         p.free_blocks[free_count - 1 - u];
   }
   // block of request i's cell j: one this step takes, or one it already held
   auto block_of = [&](int i, int32_t c, int32_t j) -> int32_t {
-    const int32_t held = ceil_div(c, bs);
+    const int32_t held = ceil_div(c, bs_log2);
     return j >= held ? p.free_blocks[free_count - 1 - (need[i] + j - held)]
                      : p.block_table[i * p.table_stride + j];
   };
   // write units
-  for (int u = gtid; u < p.units_cap; u += kStride) {
+  for (int u = gtid; u < p.units_cap; u += stride) {
     int4 out = make_int4(-1, -1, -1, -1);
     if (u < total_units) {
       const int i = find(cu_unit, n, u);
       const int32_t c = ctx[i], end = c + (cu[i + 1] - cu[i]);
-      const int32_t j = c / bs + (u - cu_unit[i]);
+      const int32_t j = (c >> bs_log2) + (u - cu_unit[i]);
       const int32_t lo = max(c, j * bs), hi = min(end, (j + 1) * bs);
       out = make_int4(block_of(i, c, j), cu[i] + (lo - c), lo - j * bs, hi - lo);
     }
     reinterpret_cast<int4*>(p.units)[u] = out;
   }
-  // tokens
-  for (int t = gtid; t < p.tokens; t += kStride) {
-    int32_t slot = -1, req = -1, pos = -1;
-    if (t < total_new) {
-      req = find(cu, n, t);
-      const int32_t c = ctx[req];
-      pos = (c & 0x7fffffff) + (t - cu[req]);
-      if (c >= 0) slot = block_of(req, c, pos / bs) * bs + pos % bs;
+  // tokens, four consecutive ones at a time: they share a request or two and
+  // mostly a block, and leave as 16-byte stores
+  for (int t0 = 4 * gtid; t0 < p.tokens; t0 += 4 * stride) {
+    int4 slot = make_int4(-1, -1, -1, -1), rq = slot, ps = slot;
+    if (t0 < total_new) {
+      int req = find(cu, n, t0), end = cu[req + 1], c = ctx[req], cell = -1, cell_at = -1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = t0 + k;
+        if (t >= total_new) break;
+        if (t >= end) {
+          do ++req; while (cu[req + 1] <= t);
+          end = cu[req + 1];
+          c = ctx[req];
+          cell_at = -1;
+        }
+        const int pos = (c & 0x7fffffff) + (t - cu[req]);
+        const int j = pos >> bs_log2;
+        if (c >= 0 && j != cell_at) {
+          cell = block_of(req, c, j);
+          cell_at = j;
+        }
+        reinterpret_cast<int*>(&slot)[k] = c >= 0 ? (cell << bs_log2) + (pos & (bs - 1)) : -1;
+        reinterpret_cast<int*>(&rq)[k] = req;
+        reinterpret_cast<int*>(&ps)[k] = pos;
+      }
     }
-    p.slot_map[t] = slot;
-    p.token_request[t] = req;
-    p.positions[t] = pos;
+    if (t0 + 4 <= p.tokens && vec) {
+      *reinterpret_cast<int4*>(p.slot_map + t0) = slot;
+      *reinterpret_cast<int4*>(p.token_request + t0) = rq;
+      *reinterpret_cast<int4*>(p.positions + t0) = ps;
+    } else {
+      for (int k = 0; k < 4 && t0 + k < p.tokens; ++k) {
+        p.slot_map[t0 + k] = reinterpret_cast<int*>(&slot)[k];
+        p.token_request[t0 + k] = reinterpret_cast<int*>(&rq)[k];
+        p.positions[t0 + k] = reinterpret_cast<int*>(&ps)[k];
+      }
+    }
   }
 }
 
 cudaError_t launch_plan_step(const tkv_kv8_plan_args& p, cudaStream_t stream) {
   const size_t smem = sizeof(int32_t) * (4 * (size_t)p.requests + 3);
-  if (smem > 40 * 1024) {
+  const bool small = p.requests <= kPlanSmallWork && p.tokens <= kPlanSmallWork && p.units_cap <= kPlanSmallWork;
+  if (smem > 40 * 1024) {   // more requests than a small step has
     static std::atomic<uint64_t> allowed;
-    const cudaError_t e = allow_smem(plan_step_kernel, (int)(sizeof(int32_t) * (4 * TKV_KV8_MAX_REQUESTS + 3)),
-                                     allowed);
+    const cudaError_t e = allow_smem(plan_step_kernel<kPlanThreads>,
+                                     (int)(sizeof(int32_t) * (4 * TKV_KV8_MAX_REQUESTS + 3)), allowed);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kPlanCluster);
-  cfg.blockDim = dim3(kPlanThreads);
+  cfg.gridDim = dim3(small ? 1 : kPlanCluster);
+  cfg.blockDim = dim3(small ? kPlanSmall : kPlanThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = kPlanCluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cfg.gridDim.x;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, plan_step_kernel, p);
+  cfg.numAttrs = small ? 1 : 2;
+  return small ? cudaLaunchKernelEx(&cfg, plan_step_kernel<kPlanSmall>, p)
+               : cudaLaunchKernelEx(&cfg, plan_step_kernel<kPlanThreads>, p);
 }
 
 // ---------------------------------------------------------------- element types
@@ -394,6 +435,8 @@ __device__ __forceinline__ void rotate_token(const RotaryArgs& r, int64_t token,
 template <typename T>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ float cs[kMaxRotDim];
+  pdl_launch_dependents();
+  pdl_wait();
   const int64_t t = blockIdx.x;
   rotate_token<T>(p.rot, t, (const T*)p.q.data + t * p.q.token_stride,
                   (const T*)p.k.data + t * p.k.token_stride,
@@ -405,9 +448,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
 
 cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream) {
   if (p.tokens == 0 || p.heads + p.kv_heads == 0) return cudaSuccess;
-  if (dtype == kDtF16) rotary_kernel<__half><<<p.tokens, kRotThreads, 0, stream>>>(p);
-  else rotary_kernel<__nv_bfloat16><<<p.tokens, kRotThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(dtype == kDtF16 ? rotary_kernel<__half> : rotary_kernel<__nv_bfloat16>, dim3(p.tokens),
+                          kRotThreads, 0, stream, p);
 }
 
 // ---------------------------------------------------------------- append
@@ -428,11 +470,27 @@ __device__ __forceinline__ float decode(uint32_t b) {
 template <int FMT>
 constexpr float kQMax = FMT == TKV_KV8_INT8 ? 127.f : 448.f;
 
+// Codes of x / s.  x (1 / s) is within 2^-22 of the quotient, so the codes of the
+// two ends of that interval agree unless the quotient lies next to a rounding
+// boundary; only then (about once in 10^4 elements) it is divided.
 template <int FMT>
-__device__ __forceinline__ uint2 encode8(const float* x, float s) {
+__device__ __forceinline__ uint32_t encode_quotient(float x, float s, float inv) {
+  const float q = x * inv;
+  if (!(inv < INFINITY)) return encode<FMT>(__fdiv_rn(x, s));   // 1 / s overflows for a subnormal s
+  if (FMT == TKV_KV8_INT8) {
+    const float n = rintf(q);
+    if (fabsf(fabsf(q - n) - 0.5f) > 1e-4f) return (uint32_t)(int32_t)fminf(fmaxf(n, -127.f), 127.f) & 0xffu;
+    return encode<FMT>(__fdiv_rn(x, s));
+  }
+  const uint32_t a = encode<FMT>(q * (1.f - 0x1p-21f)), b = encode<FMT>(q * (1.f + 0x1p-21f));
+  return a == b ? a : encode<FMT>(__fdiv_rn(x, s));
+}
+
+template <int FMT>
+__device__ __forceinline__ uint2 encode8(const float* x, float s, float inv) {
   uint32_t w[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i >> 2] |= encode<FMT>(__fdiv_rn(x[i], s)) << (8 * (i & 3));
+  for (int i = 0; i < 8; ++i) w[i >> 2] |= encode_quotient<FMT>(x[i], s, inv) << (8 * (i & 3));
   return make_uint2(w[0], w[1]);
 }
 
@@ -455,6 +513,8 @@ __global__ void __launch_bounds__(128) append_kernel8(const __grid_constant__ Ap
   using S = AppendShape<D, BS>;
   __shared__ float cs[kMaxRotDim];
   __shared__ float warp_max[4];
+  pdl_launch_dependents();
+  pdl_wait();
   const int tiles_per_unit = 2 * p.kv_heads;
   const int ctas_per_unit = (tiles_per_unit + S::kTiles - 1) / S::kTiles;
   const int64_t unit_ctas = (int64_t)p.units_cap * ctas_per_unit;
@@ -492,6 +552,14 @@ __global__ void __launch_bounds__(128) append_kernel8(const __grid_constant__ Ap
   const tkv_token_view& view = is_v ? p.v : p.k;
   const T* src = (const T*)view.data + h * view.head_stride;
 
+  // the axes of the item's 8 frequencies, 4 bits each; one for all in most layouts
+  uint32_t axes = 0;
+  bool one_axis = true;
+  if (rotate && w.f0 >= 0 && p.rot.axes > 1) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) axes |= (uint32_t)freq_axis(p.rot, w.f0 + j) << (4 * j);
+    one_axis = axes == (axes & 15u) * 0x11111111u;
+  }
   float x[S::kItems][16];
   float amax = 0.f;
   bool odd = false;  // a NaN or an infinity among the new rows
@@ -504,8 +572,8 @@ __global__ void __launch_bounds__(128) append_kernel8(const __grid_constant__ Ap
       if (rotate && w.f0 >= 0) {
         const int half = p.rot.rot_dim / 2;
         if (p.rot.pairs) split_pairs(x[i]);
-        if (p.rot.axes == 1) {
-          const float* c = p.rot.cos_sin + load_position(p.rot, 0, token, p.err) * p.rot.rot_dim + w.f0;
+        if (one_axis) {
+          const float* c = p.rot.cos_sin + load_position(p.rot, axes & 15, token, p.err) * p.rot.rot_dim + w.f0;
 #pragma unroll
           for (int j = 0; j < 8; j += 4) {
             const float4 c4 = *reinterpret_cast<const float4*>(c + j);
@@ -516,12 +584,17 @@ __global__ void __launch_bounds__(128) append_kernel8(const __grid_constant__ Ap
             turn(x[i][j + 3], x[i][11 + j], c4.w, s4.w);
           }
         } else {
+          const float* row_of[4];
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
+            row_of[a] = a < p.rot.axes
+                            ? p.rot.cos_sin + load_position(p.rot, a, token, p.err) * p.rot.rot_dim + w.f0
+                            : nullptr;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const int f = w.f0 + j;
-            const int64_t pos = load_position(p.rot, freq_axis(p.rot, f), token, p.err);
-            turn(x[i][j], x[i][8 + j], p.rot.cos_sin[pos * p.rot.rot_dim + f],
-                 p.rot.cos_sin[pos * p.rot.rot_dim + half + f]);
+            const uint32_t a = axes >> (4 * j) & 15;
+            const float* c = a == 0 ? row_of[0] : a == 1 ? row_of[1] : a == 2 ? row_of[2] : row_of[3];
+            turn(x[i][j], x[i][8 + j], c[j], c[half + j]);
           }
         }
         if (p.rot.pairs) join_pairs(x[i]);
@@ -551,7 +624,7 @@ __global__ void __launch_bounds__(128) append_kernel8(const __grid_constant__ Ap
   uint8_t* codes = (is_v ? p.v_codes : p.k_codes) + ((int64_t)unit.x * p.kv_heads + h) * (BS * D);
   if (S::kWarps > 1) __syncthreads();  // every warp has read the old scale
   if (part == 0 && lane == 0) *scale = poisoned ? __int_as_float(0x7fc00000) : s;
-  const float shrink = __fdiv_rn(s_old, s);
+  const float shrink = __fdiv_rn(s_old, s), inv = __fdiv_rn(1.f, s);
 #pragma unroll
   for (int i = 0; i < S::kItems; ++i) {
     const int row = row0 + i * kRowStep;
@@ -559,8 +632,8 @@ __global__ void __launch_bounds__(128) append_kernel8(const __grid_constant__ Ap
     if (row >= off && row < off + rows) {
       uint2 a = make_uint2(0, 0), b = a;
       if (!poisoned) {
-        a = encode8<FMT>(x[i], s);
-        b = encode8<FMT>(x[i] + 8, s);
+        a = encode8<FMT>(x[i], s, inv);
+        b = encode8<FMT>(x[i] + 8, s, inv);
       }
       *reinterpret_cast<uint2*>(dst + w.lo) = a;
       *reinterpret_cast<uint2*>(dst + w.hi) = b;
@@ -587,8 +660,7 @@ static cudaError_t launch_append8(const AppendParams8& p, cudaStream_t stream) {
                        (p.heads > 0 ? p.tokens : 0);
   if (ctas == 0) return cudaSuccess;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
-  append_kernel8<T, D, BS, FMT><<<(unsigned)ctas, 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(append_kernel8<T, D, BS, FMT>, dim3((unsigned)ctas), 128, 0, stream, p);
 }
 
 template <typename T, int FMT>

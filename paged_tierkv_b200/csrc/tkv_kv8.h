@@ -53,6 +53,25 @@ struct AppendParams8 {
   int32_t has_rot;
 };
 
+// A launch with programmatic dependent launch: the kernel's CTAs may start while
+// the previous kernel of the stream drains, and wait for it (griddepcontrol.wait)
+// before they touch memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kern)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                             const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, Params(args)...);
+}
+
 // A unit of many_rows_kernel split over `parts` CTAs; parts 0: none.
 struct MergeUnit {
   int32_t parts, slot0;   // the first part's slot in its CTA

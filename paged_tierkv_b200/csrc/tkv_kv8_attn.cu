@@ -97,6 +97,12 @@ struct UnitPos {
   int steps;      // steps of each of its units
 };
 
+// floor(total c / ctas), in 32 bits where that fits.
+__device__ __forceinline__ int64_t share_of(int64_t total, int64_t c, int64_t ctas) {
+  if (total < (1 << 21) && ctas < (1 << 10)) return (uint32_t)total * (uint32_t)c / (uint32_t)ctas;
+  return total * c / ctas;
+}
+
 template <int RT>
 __device__ __forceinline__ bool load_request(const AttnParams8& p, int bs, int req, UnitPos& u) {
   u.req = req;
@@ -173,6 +179,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     prefetch_tensormap(&tm_v);
   }
 
+  pdl_launch_dependents();
+  pdl_wait();   // everything below reads what the kernels before may have written
+
   // ---- this CTA's range of the flat step list
   UnitPos unit;
   int64_t total, ctas, begin, end, unit_at;   // unit_at: flat index of the unit's first step
@@ -198,8 +207,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     }
     ctas = min((int64_t)gridDim.x, total);   // every range holds a step
     if (blockIdx.x >= ctas) return;
-    begin = total * blockIdx.x / ctas;
-    end = total * (blockIdx.x + 1) / ctas;
+    begin = share_of(total, blockIdx.x, ctas);
+    end = share_of(total, blockIdx.x + 1, ctas);
     int64_t at = before + inc - sum;
     __syncthreads();
     if (at <= begin && begin < at + sum) {
@@ -665,10 +674,11 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
         for (int r = threadIdx.x / kLanes; r < rows; r += kFewConsumers / kLanes) {
           const int d4 = (threadIdx.x % kLanes) * 4;
           float mx = -INFINITY;
+#pragma unroll 8
           for (int i = 0; i < parts; ++i)
             mx = fmaxf(mx, __ldcg((i ? rest + i * stride : first) + RT * D + r * 2));
           float sum = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
-#pragma unroll 4
+#pragma unroll 8
           for (int i = 0; i < parts; ++i) {
             const float* src = i ? rest + i * stride : first;
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + RT * D + r * 2));
@@ -704,8 +714,7 @@ cudaError_t launch_few(const AttnParams8& p, const CUtensorMap* maps, int sms, c
   static std::atomic<uint64_t> allowed;
   const cudaError_t e = allow_smem(kern, L::kBytes, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<sms * kFewCtasPerSm, kFewThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
-  return cudaGetLastError();
+  return launch_dependent(kern, dim3(sms * kFewCtasPerSm), kFewThreads, L::kBytes, stream, p, maps[0], maps[1]);
 }
 
 template <int D, int BOXES, int FMT>

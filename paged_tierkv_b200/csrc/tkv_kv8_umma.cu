@@ -311,6 +311,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     prefetch_tensormap(&tm_v);
   }
 
+  pdl_launch_dependents();
+  pdl_wait();   // everything below reads what the kernels before may have written
+
   // ---- this CTA's range of the flat list
   Walk walk;
   {
@@ -889,45 +892,47 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   }
 }
 
-// Joins the partial rows of a split unit: CTA (c, y) takes 32 elements of every
-// row of the unit that starts in CTA c of many_rows_kernel and ends in a later one.
+// Joins the partial rows of a split unit: CTA (c, y) takes 8 elements of every
+// row of the unit that starts in CTA c of many_rows_kernel and ends in a later
+// one.  Latency bound: the parts' loads do not depend on one another, and are
+// spread over as many CTAs as the row has 32-byte pieces (with 128-byte pieces,
+// one part after the other, 21 us for a batch of drafted tokens; 8 us so).
+constexpr int kMergeCols = 8;
 template <int D>
 __global__ void __launch_bounds__(kUnitRows) merge_rows_kernel(const __grid_constant__ AttnParams8 p) {
+  pdl_wait();
   const MergeUnit u = p.merges[blockIdx.x];
   const int r = threadIdx.x;
   if (u.parts == 0 || r >= u.rows) return;
   // part 0 sits in slot0 of CTA c, the others in slot 0 of theirs
   auto at = [&](int i) { return ((int64_t)(blockIdx.x + i) * 2 + (i ? 0 : u.slot0)); };
   float mx = -INFINITY;
-  for (int i = 0; i < u.parts; ++i) mx = fmaxf(mx, p.part_lse[at(i) * kUnitRows + r]);
-  float4 o[8] = {};
+#pragma unroll 8
+  for (int i = 0; i < u.parts; ++i) mx = fmaxf(mx, __ldcg(p.part_lse + at(i) * kUnitRows + r));
+  float o[kMergeCols] = {};
   float sum = 0.f;
+#pragma unroll 4
   for (int i = 0; i < u.parts; ++i) {
-    const float lse = p.part_lse[at(i) * kUnitRows + r];
+    const float lse = __ldcg(p.part_lse + at(i) * kUnitRows + r);
+    const float4* src = p.part_o + (at(i) * (D / 4) + blockIdx.y * (kMergeCols / 4)) * kUnitRows + r;
     const float f = lse == -INFINITY ? 0.f : ex2(lse - mx);
     sum += f;
-    if (f == 0.f) continue;       // also skips NaN-free empties; a NaN weight is not 0
-    const float4* src = p.part_o + (at(i) * (D / 4) + blockIdx.y * 8) * kUnitRows + r;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const float4 v = src[x * kUnitRows];
-      o[x].x += v.x * f;
-      o[x].y += v.y * f;
-      o[x].z += v.z * f;
-      o[x].w += v.w * f;
+    for (int x = 0; x < kMergeCols / 4; ++x) {
+      const float4 v = __ldcg(src + x * kUnitRows);
+      o[4 * x] += v.x * f;
+      o[4 * x + 1] += v.y * f;
+      o[4 * x + 2] += v.z * f;
+      o[4 * x + 3] += v.w * f;
     }
   }
   const int urow = u.row0 + r, tok = p.token_of(urow);
   const int64_t orow = (int64_t)(u.q0 + tok) * p.heads + u.head * p.group + urow - tok * p.group;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const bool bf16 = p.bf16 != 0;
-  uint4* dst = reinterpret_cast<uint4*>((uint16_t*)p.out + orow * D + blockIdx.y * 32);
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-    dst[x] = make_uint4(pack_out(bf16, o[2 * x].x * inv, o[2 * x].y * inv),
-                        pack_out(bf16, o[2 * x].z * inv, o[2 * x].w * inv),
-                        pack_out(bf16, o[2 * x + 1].x * inv, o[2 * x + 1].y * inv),
-                        pack_out(bf16, o[2 * x + 1].z * inv, o[2 * x + 1].w * inv));
+  *reinterpret_cast<uint4*>((uint16_t*)p.out + orow * D + blockIdx.y * kMergeCols) =
+      make_uint4(pack_out(bf16, o[0] * inv, o[1] * inv), pack_out(bf16, o[2] * inv, o[3] * inv),
+                 pack_out(bf16, o[4] * inv, o[5] * inv), pack_out(bf16, o[6] * inv, o[7] * inv));
   if (blockIdx.y == 0 && p.out_lse) p.out_lse[orow] = sum == 0.f ? -INFINITY : (mx + lg2(sum)) * kLn2;
 }
 
@@ -950,11 +955,9 @@ cudaError_t launch_many(AttnParams8 p, const CUtensorMap* maps, int sms, cudaStr
   static std::atomic<uint64_t> allowed;
   cudaError_t e = allow_smem(kern, L::kBytes, allowed);
   if (e != cudaSuccess) return e;
-  kern<<<sms, kManyThreads, L::kBytes, stream>>>(p, maps[0], maps[1]);
-  e = cudaGetLastError();
+  e = launch_dependent(kern, dim3(sms), kManyThreads, L::kBytes, stream, p, maps[0], maps[1]);
   if (e != cudaSuccess) return e;
-  merge_rows_kernel<D><<<dim3(sms, D / 32), kUnitRows, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(merge_rows_kernel<D>, dim3(sms, D / kMergeCols), kUnitRows, 0, stream, p);
 }
 }  // namespace
 

@@ -706,3 +706,24 @@ def test_refusals():
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("amax", [2.0 ** -130, 2.0 ** -120, 2.0 ** -60, 1.0, 2.0 ** 100])
+def test_append_of_any_magnitude(fmt, amax):
+    """Scales down to subnormal ones, and quotients on rounding boundaries."""
+    from paged_tierkv_b200 import kv8
+    rng = np.random.default_rng(18)
+    qmax = float(kv8o.QMAX[fmt])
+    cache = kv8.Kv8Cache.allocate(1, 1, 64, 128, "cuda", CODES[fmt])
+    x = rng.uniform(-1, 1, (64, 1, 128)) * amax
+    half = np.arange(128) - 63.5 if fmt == "int8" else np.concatenate([kv8o.E4M3[:64] + kv8o.E4M3[1:65], -kv8o.E4M3[:64]]) / 2
+    x[1, 0] = half * (amax / qmax)                       # on, or next to, boundaries
+    x[0, 0, 0] = amax
+    t = torch.from_numpy(x).to(torch.bfloat16).cuda()
+    kv8.append(cache, kv8.StepPlan(block_size=64, units=_i32([(0, 0, 0, 64)]), num_units=_i32([1])), t, t)
+    c = np.zeros((1, 1, 64, 128), np.int8 if fmt == "int8" else np.uint8)
+    s = np.ones((1, 1), np.float32)
+    kv8o.write_units(t.float().cpu().numpy(), c, s, [(0, 0, 0, 64)], fmt)
+    np.testing.assert_array_equal(_np(cache.k_scale), s)
+    np.testing.assert_array_equal(_np(cache.k_codes), c)
