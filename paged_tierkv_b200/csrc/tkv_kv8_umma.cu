@@ -13,8 +13,8 @@
 //   warps 0-7, 8-15  softmax of query tile 0, 1: two threads per row, 64 columns
 //                    each, that exchange their maxima; also load Q and write the
 //                    output (one thread a row left the softmax of a tile at twice
-//                    the time of its MMAs: 691 us against BELOW for the
-//                    8192-token prompt)
+//                    the time of its MMAs: 691 us against 686 for the
+//                    8192-token prompt, 678 against 668 with e4m3 codes)
 //   warps 16-19      expand codes to fp16 (exact) and store them in the
 //                    128-byte-swizzled layout that the MMA descriptors name:
 //                    K as K-major rows, V as rows of the MN-major B operand
@@ -25,7 +25,7 @@
 // Three kinds of code share the SM's instruction caches, and each tile passes
 // through all of it: the loops over a tile's columns and over the MMAs of a
 // product stay rolled (unrolled, the instruction fetch of every role stalled:
-// 1530 us against BELOW for the 8192-token prompt).
+// 1141 us against 807 for the 8192-token prompt at that stage).
 //
 // Scales.  A tile's K scales multiply the logits of their 16 columns in fp32.
 // V's go into the exponent: P' = exp2(s - m + log2(vs vinv)), vinv a power of
@@ -166,11 +166,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
-               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_wait_into(uint32_t (&v)[32]) {
@@ -227,11 +222,6 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(kTok * 128 >> 4) << 16) |
          ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-
-// Exponentials of each 16 that run on the FMA pipe instead of the MUFU unit
-// (16 a clock per SM, which 128 x 128 logits keep busy for as long as the tile's
-// two MMAs take the tensor core).
-constexpr int kFmaExps = 0;
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -777,7 +767,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               const float2 x = fma2(make_float2(__uint_as_float(v[h * 16 + 2 * k]),
                                                 __uint_as_float(v[h * 16 + 2 * k + 1])),
                                     make_float2(mul[h], mul[h]), make_float2(add[h], add[h]));
-              const float2 e = make_float2(ex2(x.x), k >= 8 - kFmaExps ? ex2_fma(x.y) : ex2(x.y));
+              const float2 e = make_float2(ex2(x.x), ex2(x.y));
               s2 = k ? add2(s2, e) : e;
               pk[h * 8 + k] = pack_half2(e.x, e.y);
             }
