@@ -90,38 +90,10 @@ int32_t check_attention(const tkv_kv8_cache* c, const tkv_kv8_attention_args* a)
 
 }  // namespace
 
-// Encoding costs host time on every call and a serving loop attends the same
-// few caches layer after layer, so this thread's last encodings are kept, keyed
-// by every input of the encoding.
 bool tkv::kv8_code_maps(const AttnParams8& p, int d, CUtensorMap maps[2]) {
-  struct Entry {
-    const void *k, *v;
-    int64_t rows;
-    int d, box;
-    CUtensorMap maps[2];
-  };
-  thread_local Entry cache[8] = {};
-  thread_local int next = 0;
   const int64_t rows = p.blocks * p.kv_heads * p.block_size;
   const int box = p.block_size < 32 ? p.block_size : 32;
-  for (const Entry& e : cache) {
-    if (e.k == p.k_codes && e.v == p.v_codes && e.rows == rows && e.d == d && e.box == box) {
-      std::memcpy(maps, e.maps, sizeof(e.maps));
-      return true;
-    }
-  }
-  if (!encode_code_map(&maps[0], p.k_codes, rows, d, box) ||
-      !encode_code_map(&maps[1], p.v_codes, rows, d, box))
-    return false;
-  Entry& e = cache[next];
-  next = (next + 1) % 8;
-  e.k = p.k_codes;
-  e.v = p.v_codes;
-  e.rows = rows;
-  e.d = d;
-  e.box = box;
-  std::memcpy(e.maps, maps, sizeof(e.maps));
-  return true;
+  return encode_code_map(&maps[0], p.k_codes, rows, d, box) && encode_code_map(&maps[1], p.v_codes, rows, d, box);
 }
 
 extern "C" {

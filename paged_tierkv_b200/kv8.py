@@ -21,7 +21,6 @@ reference has no counterpart: its 8-bit blocks are filled by demotion only.
 from __future__ import annotations
 
 import ctypes
-import functools
 import struct
 from dataclasses import dataclass
 
@@ -32,6 +31,7 @@ from . import ops
 
 _FORMAT = {torch.int8: N.TKV_KV8_INT8, torch.float8_e4m3fn: N.TKV_KV8_E4M3}
 _FLOATS = {torch.float16: N.TKV_DTYPE_F16, torch.bfloat16: N.TKV_DTYPE_BF16}
+_POSITIONS = {torch.int32: 4, torch.int64: 8}
 MAX_REQUESTS = N.TKV_KV8_MAX_REQUESTS
 
 # The C structs of include/tierkv_b200.h, packed in one call each: filling them
@@ -44,6 +44,8 @@ _ATTENTION_ARGS = struct.Struct(_VIEW + "PPPqPP7ifPQ")
 _PLAN_ARGS = struct.Struct("PPPqPPPPPPPPPPPP6i")
 _NO_VIEW = (0, 0, 0)
 _NO_ROTARY = (0,) * 13
+_INT32 = torch.int32
+_CONTIGUOUS = torch.contiguous_format
 
 
 # ---------------------------------------------------------------------------
@@ -71,7 +73,7 @@ class Kv8Cache:
                 raise ValueError("cache tensors must be contiguous and on one device.")
         self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
         self.blocks, self.kv_heads, self.block_size, self.head_dim = (int(x) for x in k_codes.shape)
-        self.device = k_codes.device
+        self.device, self._index = k_codes.device, k_codes.get_device()
         # the tensors are held, so the addresses stay theirs
         self._struct = N.TkvKv8Cache(k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
                                      v_scale.data_ptr(), self.blocks, self.kv_heads, self.block_size,
@@ -152,7 +154,7 @@ class StepPlan:
         plan.slot_map, plan.token_request, plan.positions = slot, req, pos
         plan.admitted, plan.free_count = adm, free
         plan._outputs = tuple(x.data_ptr() for x in (kv, cu, adm, slot, req, pos, units, num, free))
-        plan.device = buf.device
+        plan.device, plan._index = buf.device, buf.get_device()
         plan._caps = (r, t, cap)
         return plan
 
@@ -185,23 +187,24 @@ class Rotary:
         object.__setattr__(self, "rot_dim", int(t.shape[1]))
         object.__setattr__(self, "_tail", (int(t.shape[1]), len(sec), *sec, *(0,) * (4 - len(sec)),
                                            int(bool(self.interleave)), int(bool(self.pairs))))
-        object.__setattr__(self, "_head", (t.data_ptr(), int(t.shape[0]), t.device))
+        object.__setattr__(self, "_head", (t.data_ptr(), int(t.shape[0]), t.get_device()))
 
     def _at(self, positions: torch.Tensor, tokens: int):
         """(the fields of the C struct with these positions, the tensor that backs them)."""
-        ptr, rows, device = self._head
-        size = positions.element_size()
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != device:
+        ptr, rows, index = self._head
+        size = _POSITIONS.get(positions.dtype)
+        if size is None or positions.get_device() != index:
             raise ValueError("positions must be int32 or int64 on the table's device.")
-        if positions.ndim == 1 and self.axes == 1:
-            stride, (n,), (step,) = 0, positions.shape, positions.stride()
-        else:
-            if positions.ndim != 2 or positions.shape[0] != self.axes:
-                raise ValueError("positions must have shape [axes, tokens] (or [tokens] for one axis).")
+        nd = positions.ndim
+        if nd == 1 and self.axes == 1:
+            n, stride, step = positions.numel(), 0, positions.stride()[0]
+        elif nd == 2 and positions.shape[0] == self.axes:
             n, (stride, step) = positions.shape[1], positions.stride()
+        else:
+            raise ValueError("positions must have shape [axes, tokens] (or [tokens] for one axis).")
         if n < tokens:
             raise ValueError("positions must have shape [axes, tokens] (or [tokens] for one axis).")
-        if n > 1 and step != 1:
+        if step != 1 and n > 1:
             positions = positions.contiguous()
             stride = n
         return (ptr, positions.data_ptr(), rows, stride, size, *self._tail), positions
@@ -215,97 +218,101 @@ def _units_cap(requests: int, tokens: int, block_size: int) -> int:
     return min(tokens, tokens // block_size + 2 * requests)
 
 
-def _check_table(table: torch.Tensor, requests: int) -> None:
-    if table.dtype != torch.int32 or not table.is_cuda or table.ndim != 2 or table.shape[0] < requests:
+def _check_table(table: torch.Tensor, requests: int):
+    """(row stride, width) of a block table."""
+    if table.dtype != _INT32 or not table.is_cuda or table.ndim != 2:
         raise ValueError("block_table must be an int32 CUDA tensor [requests, width].")
-    if table.shape[1] > 1 and table.stride(1) != 1 or table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+    rows, width = table.shape
+    s0, s1 = table.stride()
+    if rows < requests:
+        raise ValueError("block_table must be an int32 CUDA tensor [requests, width].")
+    if width > 1 and s1 != 1 or rows > 1 and s0 < width:
         raise ValueError("block_table rows must be contiguous and must not overlap.")
+    return (s0 if rows > 1 else width), width
 
 
-def _table_stride(table: torch.Tensor) -> int:
-    return int(table.stride(0)) if table.shape[0] > 1 else int(table.shape[1])
+# A view is (address, token stride, head stride) of a [n, h, head_dim] tensor.
+# These run on every call, and small calls cost what the host spends on them:
+# device indices instead of device objects, shapes read once.
 
-
-def _view(t: torch.Tensor):
-    """(address, token stride, head stride) of a [tokens, heads, head_dim] view,
-    None if it is not 16-byte aligned throughout."""
-    n, h, d = t.shape
+def _view(t: torch.Tensor, n: int, h: int):
+    """None if it is not 16-byte aligned throughout."""
     s0, s1, s2 = t.stride()
     ptr = t.data_ptr()
     if n < 2:
         s0 = 0
     if h < 2:
         s1 = 0
-    if (s2 != 1 and d > 1) or (ptr | s0 * 2 | s1 * 2) & 15:
+    if (ptr | s0 * 2 | s1 * 2) & 15 or s2 != 1 and t.shape[2] > 1:
         return None
     return ptr, s0, s1
 
 
-def _input_view(t: torch.Tensor):
+def _input_view(t: torch.Tensor, n: int, h: int):
     """(view, tensor that backs it): strided as it is, or through a compact copy."""
-    v = _view(t)
+    v = _view(t, n, h)
     if v is None:
-        t = t.clone(memory_format=torch.contiguous_format)
-        v = _view(t)
+        t = t.clone(memory_format=_CONTIGUOUS)
+        v = _view(t, n, h)
     return v, t
 
 
-def _output_view(t: torch.Tensor, like: torch.Tensor, name: str):
+def _output_view(t: torch.Tensor | None, like: torch.Tensor, n: int, h: int, name: str):
+    """(output, view): the caller's, or a new contiguous one."""
+    if t is None:
+        t = torch.empty_like(like, memory_format=_CONTIGUOUS)
+        d = like.shape[2]
+        return t, (t.data_ptr(), h * d, d)
     if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must match its input in shape, dtype and device.")
-    v = _view(t)
+    v = _view(t, n, h)
     if v is None:
         raise ValueError(f"{name} must be 16-byte aligned with head_dim contiguous.")
-    return v
+    return t, v
 
 
-def _heads3(t: torch.Tensor, name: str) -> None:
-    if t.ndim != 3 or t.dtype not in _FLOATS:
+def _heads3(t: torch.Tensor, name: str):
+    """(dtype code, device index) of a tensor [tokens, heads, head_dim]."""
+    code, index = _FLOATS.get(t.dtype), t.get_device()
+    if code is None or t.ndim != 3:
         raise ValueError(f"{name} must be an fp16 or bf16 tensor [tokens, heads, head_dim].")
-    if not t.is_cuda:
+    if index < 0:
         raise ValueError(f"{name} must be a CUDA tensor.")
+    return code, index
 
 
-def _streamed(fn):
+def _on_stream(stream, fn, *args, **kwargs):
     """``stream=``: the whole call -- its copies, outputs and workspace too -- runs
     on that stream, and the caching allocator learns that its inputs are used
     there.  Ordering it after the inputs' producers is the caller's part."""
-
-    @functools.wraps(fn)
-    def call(*args, stream=None, **kwargs):
-        if stream is None:
-            return fn(*args, **kwargs)
-        for x in (*args, *kwargs.values()):
-            for t in (x,) if isinstance(x, torch.Tensor) else getattr(x, "__dict__", {}).values():
-                if isinstance(t, torch.Tensor) and t.is_cuda:
-                    t.record_stream(stream)
-        with torch.cuda.stream(stream):
-            return fn(*args, **kwargs)
-
-    return call
+    for x in (*args, *kwargs.values()):
+        for t in (x,) if isinstance(x, torch.Tensor) else getattr(x, "__dict__", {}).values():
+            if isinstance(t, torch.Tensor) and t.is_cuda:
+                t.record_stream(stream)
+    with torch.cuda.stream(stream):
+        return fn(*args, **kwargs)
 
 
 _CURRENT_DEVICE = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
-def _on_device(device: torch.device, call):
-    """call(stream handle, its workspace) with ``device`` current."""
-    index = device.index
+def _launch(index: int, fn):
+    """fn(stream handle, its workspace) with device ``index`` current."""
     if index != _CURRENT_DEVICE():
         with torch.cuda.device(index):
-            return _on_device(device, call)
+            return _launch(index, fn)
     st = ops._RAW_STREAM(index) if ops._RAW_STREAM is not None else torch.cuda.current_stream().cuda_stream
     ws = ops._WORKSPACES.get((index, st))
-    return call(st, ws if ws is not None else ops.workspace_for(device, st, 1 << 16))
+    return fn(st, ws if ws is not None else ops.workspace_for(torch.device("cuda", index), st, 1 << 16))
 
 
 # ---------------------------------------------------------------------------
 # the operators
 # ---------------------------------------------------------------------------
 
-@_streamed
 def plan_step(plan: StepPlan, context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
-              free_blocks: torch.Tensor, free_count: torch.Tensor, *, tokens: int | None = None) -> StepPlan:
+              free_blocks: torch.Tensor, free_count: torch.Tensor, *, tokens: int | None = None,
+              stream=None) -> StepPlan:
     """Plans one step on the GPU: request i holds context_lens[i] tokens and gets
     new_lens[i] more, packed one request after the other.
 
@@ -318,18 +325,21 @@ def plan_step(plan: StepPlan, context_lens: torch.Tensor, new_lens: torch.Tensor
     allocated for) and returns it.  ``plan.kv_lens`` and ``plan.free_count`` may
     be passed back as the next step's context_lens and free_count.  ``tokens``:
     how many entries of the token outputs to write (default: all)."""
+    if stream is not None:
+        return _on_stream(stream, plan_step, plan, context_lens, new_lens, block_table, free_blocks, free_count,
+                          tokens=tokens)
     if plan._outputs is None:
         raise ValueError("plan_step fills a plan made by StepPlan.allocate.")
-    n = context_lens.numel()
+    n, index = context_lens.numel(), plan._index
     for t in (context_lens, new_lens, free_blocks, free_count):
-        if t.dtype != torch.int32 or t.device != plan.device or not t.is_contiguous():
+        if t.dtype != _INT32 or t.get_device() != index or not t.is_contiguous():
             raise ValueError("context_lens, new_lens, free_blocks and free_count must be contiguous int32 "
                              "tensors on the plan's device.")
     max_requests, max_tokens, max_units = plan._caps
     if not 1 <= n <= max_requests or new_lens.numel() != n or free_count.numel() != 1:
         raise ValueError("context_lens and new_lens must have 1 to the plan's max_requests entries, free_count one.")
-    _check_table(block_table, n)
-    if block_table.device != plan.device:
+    stride, width = _check_table(block_table, n)
+    if block_table.get_device() != index:
         raise ValueError("block_table must be on the plan's device.")
     tokens = max_tokens if tokens is None else int(tokens)
     if not 0 <= tokens <= max_tokens:
@@ -338,65 +348,60 @@ def plan_step(plan: StepPlan, context_lens: torch.Tensor, new_lens: torch.Tensor
 
     def call(st, ws):
         args = _PLAN_ARGS.pack(
-            context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), _table_stride(block_table),
+            context_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), stride,
             free_blocks.data_ptr(), free_count.data_ptr(), *out, ws.data_ptr(), n, tokens,
-            min(_units_cap(n, tokens, plan.block_size), max_units), block_table.shape[1], free_blocks.numel(),
+            min(_units_cap(n, tokens, plan.block_size), max_units), width, free_blocks.numel(),
             plan.block_size)
         return N.load().tkv_kv8_plan_step(args, st)
 
-    status = _on_device(plan.device, call)
+    status = _launch(index, call)
     if status:
         N.check(status, "tkv_kv8_plan_step")
     plan.block_table, plan.requests = block_table, n
     return plan
 
 
-@_streamed
 def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, rotary: Rotary, *,
-                 q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+                 q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None, stream=None):
     """Rotates q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim]
     (fp16 / bf16, any 16-byte aligned token and head strides; either may be
     None) by their tokens' positions [axes, tokens]; returns (q_out, k_out).
     An output may be its input."""
-    x = q if q is not None else k
-    if x is None or x.ndim != 3:
-        raise ValueError("rotary_embed needs q or k [tokens, heads, head_dim].")
-    tokens, _, d = x.shape
-    dtype, device = x.dtype, x.device
+    if stream is not None:
+        return _on_stream(stream, rotary_embed, q, k, positions, rotary, q_out=q_out, k_out=k_out)
     qv = kv = qov = kov = _NO_VIEW
     heads = kv_heads = 0
     if q is not None:
-        _heads3(q, "q")
-        heads = q.shape[1]
-        if q_out is None:
-            q_out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
-        qov = _output_view(q_out, q, "q_out")
-        qv, q = _input_view(q)
+        code, index = _heads3(q, "q")
+        tokens, heads, d = q.shape
+        q_out, qov = _output_view(q_out, q, tokens, heads, "q_out")
+        qv, q = _input_view(q, tokens, heads)
+    elif k is None:
+        raise ValueError("rotary_embed needs q or k [tokens, heads, head_dim].")
     if k is not None:
-        _heads3(k, "k")
+        k_code, k_index = _heads3(k, "k")
         n, kv_heads, dk = k.shape
-        if n != tokens or dk != d or k.dtype != dtype or k.device != device:
+        if q is None:
+            code, index, tokens, d = k_code, k_index, n, dk
+        elif n != tokens or dk != d or k_code != code or k_index != index:
             raise ValueError("q and k must agree in tokens, head_dim, dtype and device.")
-        if k_out is None:
-            k_out = torch.empty((tokens, kv_heads, d), dtype=dtype, device=device)
-        kov = _output_view(k_out, k, "k_out")
-        kv, k = _input_view(k)
+        k_out, kov = _output_view(k_out, k, n, kv_heads, "k_out")
+        kv, k = _input_view(k, n, kv_heads)
     rot, positions = rotary._at(positions, tokens)
 
     def call(st, ws):
-        args = _ROTARY_ARGS.pack(*rot, *qv, *kv, *qov, *kov, ws.data_ptr(), tokens, heads, kv_heads, d, _FLOATS[dtype])
+        args = _ROTARY_ARGS.pack(*rot, *qv, *kv, *qov, *kov, ws.data_ptr(), tokens, heads, kv_heads, d, code)
         return N.load().tkv_rotary_embed(args, st)
 
-    status = _on_device(device, call)
+    status = _launch(index, call)
     if status:
         N.check(status, "tkv_rotary_embed")
     return (q_out if q is not None else None), (k_out if k is not None else None)
 
 
-@_streamed
 def append(cache: Kv8Cache, plan: StepPlan, k: torch.Tensor, v: torch.Tensor, *, q: torch.Tensor | None = None,
            positions: torch.Tensor | None = None, rotary: Rotary | None = None,
-           q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+           q_out: torch.Tensor | None = None, stream=None) -> torch.Tensor | None:
     """Quantizes the step's new keys and values [tokens, kv_heads, head_dim] into
     the blocks of ``plan.units``; with ``rotary``, k is rotated on the way (in
     fp32) and q, when given, into q_out, which is returned.
@@ -404,12 +409,14 @@ def append(cache: Kv8Cache, plan: StepPlan, k: torch.Tensor, v: torch.Tensor, *,
     A block's scale is max |x| / 127 (448 for e4m3) of its rows; when a block
     that already holds rows gets larger ones, its scale grows and its codes are
     rounded again.  A block with a NaN or an infinity gets scale NaN."""
-    _heads3(k, "k")
-    shape, dtype, device = k.shape, k.dtype, cache.device
-    tokens = shape[0]
-    if shape[1] != cache.kv_heads or shape[2] != cache.head_dim or v.shape != shape or v.dtype != dtype:
+    if stream is not None:
+        return _on_stream(stream, append, cache, plan, k, v, q=q, positions=positions, rotary=rotary, q_out=q_out)
+    code, index = _heads3(k, "k")
+    shape = k.shape
+    tokens, kv_heads, d = shape
+    if kv_heads != cache.kv_heads or d != cache.head_dim or v.shape != shape or v.dtype != k.dtype:
         raise ValueError("k and v must have shape [tokens, kv_heads, head_dim] of the cache and one dtype.")
-    if k.device != device or v.device != device:
+    if index != cache._index or v.get_device() != index:
         raise ValueError("k and v must be on the cache's device.")
     if plan.units is None or plan.block_size != cache.block_size:
         raise ValueError("append needs a plan with write units of the cache's block size.")
@@ -421,34 +428,31 @@ def append(cache: Kv8Cache, plan: StepPlan, k: torch.Tensor, v: torch.Tensor, *,
     elif q is not None:
         raise ValueError("q is rotated only: pass rotary and positions beside it.")
     if q is not None:
-        _heads3(q, "q")
-        n, heads, d = q.shape
-        if n != tokens or d != cache.head_dim or q.dtype != dtype or q.device != device:
+        q_code, q_index = _heads3(q, "q")
+        n, heads, dq = q.shape
+        if n != tokens or dq != d or q_code != code or q_index != index:
             raise ValueError("q must agree with k in tokens, head_dim, dtype and device.")
-        if q_out is None:
-            q_out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
-        qov = _output_view(q_out, q, "q_out")
-        qv, q = _input_view(q)
-    kv, k = _input_view(k)
-    vv, v = _input_view(v)
+        q_out, qov = _output_view(q_out, q, n, heads, "q_out")
+        qv, q = _input_view(q, n, heads)
+    kv, k = _input_view(k, tokens, kv_heads)
+    vv, v = _input_view(v, tokens, kv_heads)
     units = plan.units
 
     def call(st, ws):
         # no step writes more units than tokens
         args = _APPEND_ARGS.pack(*kv, *vv, *qv, *qov, units.data_ptr(), plan.num_units.data_ptr(), ws.data_ptr(), *rot,
-                                 min(units.shape[0], tokens), tokens, heads, _FLOATS[dtype])
+                                 min(units.shape[0], tokens), tokens, heads, code)
         return N.load().tkv_kv8_append(cache._ptr, args, st)
 
-    status = _on_device(device, call)
+    status = _launch(index, call)
     if status:
         N.check(status, "tkv_kv8_append")
     return q_out if q is not None else None
 
 
-@_streamed
 def attention(q: torch.Tensor, cache: Kv8Cache, plan: StepPlan, scaling: float, *,
               max_q_len: int | None = None, window: int = 0, out: torch.Tensor | None = None,
-              return_lse: bool = False):
+              return_lse: bool = False, stream=None):
     """Causal attention of the step's query tokens q [tokens, heads, head_dim]
     over the cache: request i's tokens are q[cu_q[i]:cu_q[i + 1]], the last of
     its kv_lens[i] tokens; each sees the keys up to its own position, with
@@ -460,39 +464,42 @@ def attention(q: torch.Tensor, cache: Kv8Cache, plan: StepPlan, scaling: float, 
     natural log).  A token that sees nothing gets 0 and -inf; tokens that belong
     to no request are not written.  A request whose table names a block outside
     the cache reads zeros there (``TKV_DEVERR_BAD_SLOT``)."""
-    _heads3(q, "q")
+    if stream is not None:
+        return _on_stream(stream, attention, q, cache, plan, scaling, max_q_len=max_q_len, window=window, out=out,
+                          return_lse=return_lse)
+    code, index = _heads3(q, "q")
     tokens, heads, d = q.shape
-    dtype, device = q.dtype, cache.device
-    if d != cache.head_dim or q.device != device or heads % cache.kv_heads:
+    if d != cache.head_dim or index != cache._index or heads % cache.kv_heads:
         raise ValueError("q must match the cache in head_dim and device, and heads be a multiple of kv_heads.")
     table = plan.block_table
     if table is None or plan.block_size != cache.block_size:
         raise ValueError("attention needs a plan with block tables of the cache's block size.")
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=dtype, device=device)
-    elif out.shape != q.shape or out.dtype != dtype or out.device != device or not out.is_contiguous() \
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned tensor like q.")
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
-    view, q = _input_view(q)
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
+    stride, width = _check_table(table, plan.requests)
+    view, q = _input_view(q, tokens, heads)
     longest = tokens if max_q_len is None else min(tokens, int(max_q_len))
 
     def call(st, ws):
         lib = N.load()
         for attempt in range(2):
             args = _ATTENTION_ARGS.pack(
-                *view, out.data_ptr(), 0 if lse is None else lse.data_ptr(), table.data_ptr(), _table_stride(table),
-                plan.kv_lens.data_ptr(), plan.cu_q.data_ptr(), plan.requests, tokens, heads, _FLOATS[dtype],
-                table.shape[1], longest, int(window), scaling, ws.data_ptr(), ws.numel())
+                *view, out.data_ptr(), 0 if lse is None else lse.data_ptr(), table.data_ptr(), stride,
+                plan.kv_lens.data_ptr(), plan.cu_q.data_ptr(), plan.requests, tokens, heads, code,
+                width, longest, int(window), scaling, ws.data_ptr(), ws.numel())
             status = lib.tkv_kv8_attention(cache._ptr, args, st)
             if status != N.TKV_ERR_WORKSPACE or attempt:
                 return status
             nbytes = ctypes.c_size_t()
             N.check(lib.tkv_kv8_attention_workspace(cache._ptr, args, ctypes.byref(nbytes)),
                     "tkv_kv8_attention_workspace")
-            ws = ops.workspace_for(device, st, nbytes.value)
+            ws = ops.workspace_for(cache.device, st, nbytes.value)
 
-    status = _on_device(device, call)
+    status = _launch(index, call)
     if status:
         N.check(status, "tkv_kv8_attention")
     return (out, lse) if return_lse else out
