@@ -9,7 +9,8 @@
 // Work is a flat list of steps -- 128 tokens (4 warps x 32) of one (request, kv
 // head, row tile) unit, units in order -- cut into one contiguous range per
 // resident CTA, so ragged batches and single long contexts load every SM
-// alike.  A CTA that covers a whole unit writes the output; otherwise it
+// alike; where there is little work, each CTA gets a part of one unit instead,
+// so that none ends a unit twice.  A CTA that covers a whole unit writes the output; otherwise it
 // leaves (max, sum, accumulator) partials in the workspace and the last CTA of
 // the unit to arrive merges them in CTA order (the result does not depend on
 // which one is last).
@@ -59,6 +60,15 @@ constexpr int kFewConsumers = 32 * kFewWarps;
 constexpr int kFewThreads = kFewConsumers + 32;       // and the producer warp
 constexpr int kTileTok = 32;                          // tokens of a warp's tile
 constexpr int kStepTok = kTileTok * kFewWarps;        // tokens of a step
+// What ending one unit and starting the next costs a CTA, in steps: up to this
+// many more steps than an even share, each CTA takes a part of one unit only
+// (4 requests of 2048 tokens: 11.7 us against 14.4; drafted tokens 45 against
+// 50; a 131071-token context the same; with up to 16 steps more, 16 requests of
+// 2048 tokens take 31 us against 24).
+constexpr int kBoundarySteps = 2;
+// Parts of a unit that one trip to L2 fetches when they are joined (a trip for
+// the maxima and one for every 8 parts: a 131071-token context 56.6 us, 52.7 so).
+constexpr int kJoin = 12;
 
 template <int D, int NT>
 struct FewLayout {
@@ -82,7 +92,7 @@ struct FewLayout {
   static constexpr int kScaleOff = kStatOff + (kFewWarps + 1) * kRows * 8;   // [stages][16]: K's, V's
   static constexpr int kBarOff = kScaleOff + kStages * 64;
   static constexpr int kMiscOff = kBarOff + kStages * 16;
-  static constexpr int kBytes = kMiscOff + 64;
+  static constexpr int kBytes = kMiscOff + 88;
 };
 
 // Where a walk over the units stands.
@@ -123,10 +133,15 @@ __device__ __forceinline__ bool load_request(const AttnParams8& p, int bs, int r
   return u.tiles_r > 0;
 }
 
+// Places of a request in the list that the CTAs share: its steps (chunk 0), or
+// its parts of up to `chunk` steps.
 template <int RT>
-__device__ __forceinline__ int64_t request_steps(const AttnParams8& p, int bs, int req) {
+__device__ __forceinline__ int64_t request_places(const AttnParams8& p, int bs, int req, int chunk, int64_t& units) {
   UnitPos u;
-  return load_request<RT>(p, bs, req, u) ? (int64_t)u.steps * u.tiles_r * p.kv_heads : 0;
+  if (!load_request<RT>(p, bs, req, u)) return 0;
+  const int64_t n = (int64_t)u.tiles_r * p.kv_heads;
+  units += n;
+  return n * (chunk ? (u.steps + chunk - 1) / chunk : u.steps);
 }
 
 // Next unit in order; false past the last request.
@@ -166,8 +181,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
   float* scale_s = reinterpret_cast<float*>(smem + L::kScaleOff);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   uint64_t* empty = full + S;
-  int64_t* range_s = reinterpret_cast<int64_t*>(smem + L::kMiscOff);   // scan scratch
-  int* flag_s = reinterpret_cast<int*>(smem + L::kMiscOff + 56);
+  int64_t* range_s = reinterpret_cast<int64_t*>(smem + L::kMiscOff);   // [5] scan scratch
+  int64_t* units_s = range_s + 5;                                       // [5]
+  int* flag_s = reinterpret_cast<int*>(smem + L::kMiscOff + 80);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -182,39 +198,58 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
   pdl_launch_dependents();
   pdl_wait();   // everything below reads what the kernels before may have written
 
-  // ---- this CTA's range of the flat step list
+  // ---- this CTA's range of the flat step list, or its part of one unit
   UnitPos unit;
   int64_t total, ctas, begin, end, unit_at;   // unit_at: flat index of the unit's first step
+  int chunk = 0;                              // steps of a part, 0: ranges over unit boundaries
+  int part0 = 0, parts0 = 0;                  // first CTA and count of the unit's parts
   {
     const int per = (p.requests + kFewThreads - 1) / kFewThreads;
     const int r0 = min(p.requests, (int)threadIdx.x * per), r1 = min(p.requests, r0 + per);
-    int64_t sum = 0;
-    for (int r = r0; r < r1; ++r) sum += request_steps<RT>(p, bs, r);
-    int64_t inc = sum;
+    int64_t at, mine;                         // first place and places of this thread's requests
+    auto scan = [&](int64_t& units) {
+      mine = 0;
+      for (int r = r0; r < r1; ++r) mine += request_places<RT>(p, bs, r, chunk, units);
+      int64_t inc = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(~0u, inc, o);
-      if (lane >= o) inc += x;
-    }
-    if (lane == 31) range_s[warp] = inc;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(~0u, inc, o);
+        if (lane >= o) inc += x;
+      }
+      units = warp_sum(units);
+      if (lane == 31) {
+        range_s[warp] = inc;
+        units_s[warp] = units;
+      }
+      __syncthreads();
+      at = inc - mine;
+      total = units = 0;
 #pragma unroll
-    for (int w = 0; w < kFewThreads / 32; ++w) {
-      if (w < warp) before += range_s[w];
-      total += range_s[w];
+      for (int w = 0; w < kFewThreads / 32; ++w) {
+        if (w < warp) at += range_s[w];
+        total += range_s[w];
+        units += units_s[w];
+      }
+      __syncthreads();
+    };
+    int64_t units = 0;
+    scan(units);
+    const int64_t grid = gridDim.x;
+    if (units < grid) {
+      const int64_t c = (total + grid - units - 1) / (grid - units);
+      if (c * grid <= total + kBoundarySteps * grid) {
+        chunk = (int)c;                       // total / c + units parts at most
+        scan(units);
+      }
     }
-    ctas = min((int64_t)gridDim.x, total);   // every range holds a step
+    ctas = min(grid, total);                  // every range holds a place
     if (blockIdx.x >= ctas) return;
-    begin = share_of(total, blockIdx.x, ctas);
-    end = share_of(total, blockIdx.x + 1, ctas);
-    int64_t at = before + inc - sum;
-    __syncthreads();
-    if (at <= begin && begin < at + sum) {
+    begin = chunk ? blockIdx.x : share_of(total, blockIdx.x, ctas);
+    end = chunk ? 0 : share_of(total, blockIdx.x + 1, ctas);
+    if (at <= begin && begin < at + mine) {
       int r = r0;
       for (;; ++r) {
-        const int64_t n = request_steps<RT>(p, bs, r);
+        const int64_t n = request_places<RT>(p, bs, r, chunk, units);
         if (begin < at + n) break;
         at += n;
       }
@@ -223,10 +258,21 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     }
     __syncthreads();
     load_request<RT>(p, bs, (int)range_s[1], unit);
-    const int64_t in = (begin - range_s[0]) / unit.steps;   // unit of the request
-    unit.head = (int)(in / unit.tiles_r);
-    unit.rt = (int)(in % unit.tiles_r);
-    unit_at = range_s[0] + in * unit.steps;
+    int in;                                   // unit of the request
+    if (chunk) {
+      const int place = (int)(begin - range_s[0]);
+      parts0 = (unit.steps + chunk - 1) / chunk;
+      in = place / parts0;
+      part0 = blockIdx.x - (place - in * parts0);
+      begin = (int64_t)(place - in * parts0) * chunk;
+      end = min(begin + chunk, (int64_t)unit.steps);
+      unit_at = 0;
+    } else {
+      in = (int)((begin - range_s[0]) / unit.steps);
+      unit_at = range_s[0] + (int64_t)in * unit.steps;
+    }
+    unit.head = in / unit.tiles_r;
+    unit.rt = in - unit.head * unit.tiles_r;
   }
 
   bool ok = true;
@@ -654,8 +700,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     }
     if (!whole) {
       // CTAs whose ranges meet this unit: start(c) = total c / ctas
-      const int c0 = (int)(((u0 + 1) * ctas - 1) / total);
-      const int c1 = (int)((u1 * ctas - 1) / total);
+      const int c0 = chunk ? part0 : (int)(((u0 + 1) * ctas - 1) / total);
+      const int c1 = chunk ? part0 + parts0 - 1 : (int)((u1 * ctas - 1) / total);
       named_barrier(1, kFewConsumers);
       if (threadIdx.x == 0) {
         const uint32_t n = atom_add_acq_rel_gpu(p.counters + c0, 1u);
@@ -667,25 +713,40 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
         const int64_t stride = (int64_t)2 * RT * (D + 2);
         // CTA c0's share sits in slot 0 when its range starts at the unit, else in slot 1
         const float* first = reinterpret_cast<const float*>(p.data) +
-                             ((int64_t)c0 * 2 + (total * c0 / ctas >= u0 ? 0 : 1)) * RT * (D + 2);
+                             ((int64_t)c0 * 2 + (chunk || total * c0 / ctas >= u0 ? 0 : 1)) * RT * (D + 2);
         const float* rest = reinterpret_cast<const float*>(p.data) + (int64_t)c0 * stride;
         const int parts = c1 - c0 + 1;
         constexpr int kLanes = D / 4;    // threads of a row
         for (int r = threadIdx.x / kLanes; r < rows; r += kFewConsumers / kLanes) {
           const int d4 = (threadIdx.x % kLanes) * 4;
-          float mx = -INFINITY;
-#pragma unroll 8
-          for (int i = 0; i < parts; ++i)
-            mx = fmaxf(mx, __ldcg((i ? rest + i * stride : first) + RT * D + r * 2));
-          float sum = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
-#pragma unroll 8
-          for (int i = 0; i < parts; ++i) {
-            const float* src = i ? rest + i * stride : first;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + RT * D + r * 2));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(src + r * D + d4));
-            const float f = mx == -INFINITY ? 1.f : ex2(ml.x - mx);
-            sum += ml.y * f;
-            o0 += v.x * f, o1 += v.y * f, o2 += v.z * f, o3 += v.w * f;
+          float mx = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
+#pragma unroll 1
+          for (int i = 0; i < parts; i += kJoin) {
+            float2 ml[kJoin];
+            float4 v[kJoin];
+#pragma unroll
+            for (int j = 0; j < kJoin; ++j) {
+              ml[j] = make_float2(-INFINITY, 0.f);
+              v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (i + j < parts) {
+                const float* src = i + j ? rest + (i + j) * stride : first;
+                ml[j] = __ldcg(reinterpret_cast<const float2*>(src + RT * D + r * 2));
+                v[j] = __ldcg(reinterpret_cast<const float4*>(src + r * D + d4));
+              }
+            }
+            float mn = mx;
+#pragma unroll
+            for (int j = 0; j < kJoin; ++j) mn = fmaxf(mn, ml[j].x);
+            const float base = mn == -INFINITY ? 0.f : mn;
+            const float back = mx == -INFINITY && mn == -INFINITY ? 1.f : ex2(mx - base);
+            mx = mn;
+            sum *= back, o0 *= back, o1 *= back, o2 *= back, o3 *= back;
+#pragma unroll
+            for (int j = 0; j < kJoin; ++j) {
+              const float f = mx == -INFINITY ? 1.f : ex2(ml[j].x - base);
+              sum += ml[j].y * f;
+              o0 += v[j].x * f, o1 += v[j].y * f, o2 += v[j].z * f, o3 += v[j].w * f;
+            }
           }
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           const int64_t orow = (int64_t)(unit.q0 + (row0 + r) / p.group) * p.heads + unit.head * p.group +

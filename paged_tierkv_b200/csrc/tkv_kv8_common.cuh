@@ -52,6 +52,12 @@ __device__ __forceinline__ float warp_max(float x) {
   return x;
 }
 
+__device__ __forceinline__ int64_t warp_sum(int64_t x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+  return x;
+}
+
 // Power of two that brings a row whose largest magnitude is amax into fp16
 // with its maximum in [2^14, 2^15), and its inverse.
 __device__ __forceinline__ void fp16_scale(float amax, float& up, float& down) {

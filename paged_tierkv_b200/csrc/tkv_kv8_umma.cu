@@ -886,8 +886,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 // row of the unit that starts in CTA c of many_rows_kernel and ends in a later
 // one.  Latency bound: the parts' loads do not depend on one another, and are
 // spread over as many CTAs as the row has 32-byte pieces (with 128-byte pieces,
-// one part after the other, 21 us for a batch of drafted tokens; 8 us so).
+// one part after the other, 21 us for a batch of drafted tokens; 9 us so), a trip
+// to L2 for each kMergeParts parts (2 and 8 parts a trip take as long).
 constexpr int kMergeCols = 8;
+constexpr int kMergeParts = 4;
 template <int D>
 __global__ void __launch_bounds__(kUnitRows) merge_rows_kernel(const __grid_constant__ AttnParams8 p) {
   pdl_wait();
@@ -896,24 +898,40 @@ __global__ void __launch_bounds__(kUnitRows) merge_rows_kernel(const __grid_cons
   if (u.parts == 0 || r >= u.rows) return;
   // part 0 sits in slot0 of CTA c, the others in slot 0 of theirs
   auto at = [&](int i) { return ((int64_t)(blockIdx.x + i) * 2 + (i ? 0 : u.slot0)); };
-  float mx = -INFINITY;
-#pragma unroll 8
-  for (int i = 0; i < u.parts; ++i) mx = fmaxf(mx, __ldcg(p.part_lse + at(i) * kUnitRows + r));
+  float mx = -INFINITY, sum = 0.f;
   float o[kMergeCols] = {};
-  float sum = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < u.parts; ++i) {
-    const float lse = __ldcg(p.part_lse + at(i) * kUnitRows + r);
-    const float4* src = p.part_o + (at(i) * (D / 4) + blockIdx.y * (kMergeCols / 4)) * kUnitRows + r;
-    const float f = lse == -INFINITY ? 0.f : ex2(lse - mx);
-    sum += f;
+#pragma unroll 1
+  for (int i = 0; i < u.parts; i += kMergeParts) {
+    float lse[kMergeParts];
+    float4 v[kMergeParts][kMergeCols / 4];
 #pragma unroll
-    for (int x = 0; x < kMergeCols / 4; ++x) {
-      const float4 v = __ldcg(src + x * kUnitRows);
-      o[4 * x] += v.x * f;
-      o[4 * x + 1] += v.y * f;
-      o[4 * x + 2] += v.z * f;
-      o[4 * x + 3] += v.w * f;
+    for (int j = 0; j < kMergeParts; ++j) {   // past the last part: the last part again, dropped below
+      const int64_t k = at(min(i + j, u.parts - 1));
+      lse[j] = __ldcg(p.part_lse + k * kUnitRows + r);
+      const float4* src = p.part_o + (k * (D / 4) + blockIdx.y * (kMergeCols / 4)) * kUnitRows + r;
+#pragma unroll
+      for (int x = 0; x < kMergeCols / 4; ++x) v[j][x] = __ldcg(src + x * kUnitRows);
+    }
+    float mn = mx;
+#pragma unroll
+    for (int j = 0; j < kMergeParts; ++j) mn = fmaxf(mn, lse[j]);
+    const float back = mx == -INFINITY ? 0.f : ex2(mx - mn);
+    mx = mn;
+    sum *= back;
+#pragma unroll
+    for (int x = 0; x < kMergeCols; ++x) o[x] *= back;
+#pragma unroll
+    for (int j = 0; j < kMergeParts; ++j) {
+      if (i + j >= u.parts) break;
+      const float f = lse[j] == -INFINITY ? 0.f : ex2(lse[j] - mx);
+      sum += f;
+#pragma unroll
+      for (int x = 0; x < kMergeCols / 4; ++x) {
+        o[4 * x] += v[j][x].x * f;
+        o[4 * x + 1] += v[j][x].y * f;
+        o[4 * x + 2] += v[j][x].z * f;
+        o[4 * x + 3] += v[j][x].w * f;
+      }
     }
   }
   const int urow = u.row0 + r, tok = p.token_of(urow);
