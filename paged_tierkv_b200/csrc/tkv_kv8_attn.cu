@@ -4,7 +4,9 @@
 // A row is one (query token, query head); the rows of a kv head share its K/V,
 // so they are packed into tiles of 8 * NT rows (NT 1 or 2) and every code is read once per
 // tile.  At few rows the kernel is bound by HBM: 2 head_dim bytes per token and
-// kv head against 4 head_dim rows flops.
+// kv head against 4 head_dim rows flops.  32 x 32768 tokens, 8 kv heads of 128:
+// 378 us with int8 codes, 5.7 TB/s, whose expansion takes twice the
+// instructions of e4m3's: 334 us, 6.4 TB/s.
 //
 // Work is a flat list of steps -- 128 tokens (4 warps x 32) of one (request, kv
 // head, row tile) unit, units in order -- cut into one contiguous range per

@@ -9,6 +9,9 @@
 // the fp16 P_i of 64 tokens overwriting the first half of their S_i and feeding
 // the MMA from there.
 // While the tensor core works for one query tile the other one's softmax runs.
+// A prompt of 8192 tokens, 32 / 8 heads of 128: 691 us, 796 TFLOP/s.  Bound by
+// shared memory, which the MMAs of S alone read at its full bandwidth and the
+// expansion writes, and by the tensor-memory reads of the softmax.
 //
 //   warps 0-7, 8-15  softmax of query tile 0, 1: two threads per row, 64 columns
 //                    each, that exchange their maxima; also load Q and write the

@@ -570,6 +570,19 @@ def test_repeated_calls_give_the_same_bits():
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("kv,kvh", [
+    ([5000], 1),                                          # one unit in more parts than a join takes at once
+    ([1700, 1, 0, 2600], 2),                              # every CTA a part of one unit
+    ([100 + 41 * r for r in range(20)], 16),              # more units than CTAs
+    ([6000 + 7 * r for r in range(9)], 8),                # ranges over the boundaries of split units
+])
+@pytest.mark.parametrize("window", [0, 1000])
+def test_how_single_tokens_are_split_over_ctas(kv, kvh, window):
+    rng = np.random.default_rng(len(kv))
+    scene = _scene(rng, kv, [1] * len(kv), kvh, kvh, 64, 16, "int8", "fp16")
+    _check_attention(scene, kv, 16, "int8", "fp16", 0.125, window, max_q_len=1)
+
+
 def test_another_stream_and_a_graph():
     from paged_tierkv_b200 import kv8
     rng = np.random.default_rng(15)
