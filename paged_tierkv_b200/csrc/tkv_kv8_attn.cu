@@ -46,15 +46,19 @@ namespace tkv {
 // more than 16, all run here, in row tiles of 8 or 16.  Otherwise requests of up
 // to 8 rows run here and the others in many_rows_kernel, whose smallest tile of
 // 128 rows still beats this kernel's 16-row instance for a batch of both (23
-// requests of 7 to 42 rows: 70 us against 89; chunks beside single tokens: 80
-// against 95), though not for 16 rows alone (32 x 32768 tokens: 170 us against
-// 300).  A 32-row instance took 594 us there.
+// requests of up to 9001 tokens with 28 rows each: 49 us against 56, with 35: 49
+// against 78; chunks beside single tokens: 80 against 95), though not for 16 rows
+// alone (32 x 32768 tokens: 170 us against 300).  A 32-row instance took 594 us
+// there.
+// Small batches are the exception: up to 48 rows, and as long as the tables leave
+// every CTA at most 32 steps, all run here, which saves the second kernel and the
+// join (42 rows over 3000 tokens, 4 requests: 20 us against 31, 16 requests: 43
+// against 48, 32 requests: 72 both; 64 rows, 4 requests: 53 against 42).
 constexpr int kFewRowsAlone = 16;
 constexpr int kFewRowsBeside = 8;
-static bool has_many_rows(int group, int max_q_len) { return (int64_t)group * max_q_len > kFewRowsAlone; }
-static int few_row_tiles(int group, int max_q_len) {
-  return has_many_rows(group, max_q_len) || (int64_t)group * max_q_len <= 8 ? 1 : 2;
-}
+constexpr int kFewRowsShort = 48;
+constexpr int kShortSteps = 32;
+static int few_row_tiles(int64_t rows) { return rows <= 8 ? 1 : 2; }
 constexpr int kFewCtasPerSm = 2;
 
 constexpr int kFewWarps = 4;
@@ -768,6 +772,20 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
 }
 
 // ---------------------------------------------------------------- host side
+static bool has_many_rows(const AttnParams8& p, int sms) {
+  const int64_t rows = (int64_t)p.group * p.max_q_len;
+  if (rows <= kFewRowsAlone) return false;
+  if (rows > kFewRowsShort) return true;
+  // what the step may hold at most: its row tiles, and the keys that a table has
+  // room for or a window leaves
+  const int64_t tiles = std::min<int64_t>(p.requests * ((rows + 15) / 16),
+                                          (int64_t)p.tokens * p.group / 16 + p.requests);
+  int64_t keys = (int64_t)p.table_width * p.block_size;
+  if (p.window > 0) keys = std::min<int64_t>(keys, (int64_t)p.window + p.max_q_len + kStepTok);
+  const int64_t steps = tiles * p.kv_heads * ((keys + kStepTok - 1) / kStepTok);
+  return steps > (int64_t)kShortSteps * sms * kFewCtasPerSm;
+}
+
 namespace {
 
 template <int D, int BOXES, int FMT, int NT>
@@ -782,8 +800,9 @@ cudaError_t launch_few(const AttnParams8& p, const CUtensorMap* maps, int sms, c
 
 template <int D, int BOXES, int FMT>
 cudaError_t few_nt(const AttnParams8& p, const CUtensorMap* maps, int sms, cudaStream_t s) {
-  return few_row_tiles(p.group, p.max_q_len) == 1 ? launch_few<D, BOXES, FMT, 1>(p, maps, sms, s)
-                                                  : launch_few<D, BOXES, FMT, 2>(p, maps, sms, s);
+  const int64_t rows = std::min<int64_t>((int64_t)p.group * p.max_q_len, p.few_rows_max);
+  return few_row_tiles(rows) == 1 ? launch_few<D, BOXES, FMT, 1>(p, maps, sms, s)
+                                  : launch_few<D, BOXES, FMT, 2>(p, maps, sms, s);
 }
 
 template <int D>
@@ -798,16 +817,17 @@ cudaError_t few_format(const AttnParams8& p, const CUtensorMap* maps, int sms, i
 }  // namespace
 
 void kv8_attention_scratch(int sms, int d, int group, int max_q_len, size_t* counters, size_t* data) {
-  const int nt = few_row_tiles(group, max_q_len);
+  const int64_t rows = (int64_t)group * max_q_len;
+  const int nt = few_row_tiles(rows);
   const size_t ctas = (size_t)sms * kFewCtasPerSm;
   *counters = ctas * sizeof(uint32_t);
   *data = ctas * 2 * 8 * nt * (d + 2) * sizeof(float);
-  if (has_many_rows(group, max_q_len)) *data = std::max(*data, many_rows_scratch(sms, d));
+  if (rows > kFewRowsAlone) *data = std::max(*data, many_rows_scratch(sms, d));
 }
 
 cudaError_t launch_kv8_attention(const AttnParams8& args, int sms, int d, int format, cudaStream_t stream) {
   AttnParams8 p = args;
-  const bool many = has_many_rows(p.group, p.max_q_len);
+  const bool many = has_many_rows(p, sms);
   // a lone request needs one kernel: the one for its largest possible size; and
   // without a request that max_q_len calls long, this kernel takes all
   p.few_rows_max = !many ? 0x7fffffff : p.requests == 1 ? 0 : kFewRowsBeside;

@@ -570,6 +570,20 @@ def test_repeated_calls_give_the_same_bits():
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("d,bs", SHAPES)
+@pytest.mark.parametrize("fmt,dtype", [("int8", "bf16"), ("e4m3", "fp16")])
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("room", [0, 700000])
+def test_few_rows_under_narrow_and_wide_tables(d, bs, fmt, dtype, window, room):
+    """20 to 48 rows a kv head: tables with room for long contexts take the kernel
+    for many rows, narrow ones the kernel for few."""
+    kv, ql = [5, 64, 300, 3, 777, 130], [5, 6, 12, 1, 2, 0]
+    rng = np.random.default_rng(bs + window)
+    scene = list(_scene(rng, kv, ql, 8, 2, d, bs, fmt, dtype))
+    scene[4] = np.concatenate([scene[4], rng.integers(-5, 10 ** 6, (len(kv), room // bs))], 1).astype(np.int32)
+    _check_attention(tuple(scene), kv, bs, fmt, dtype, d ** -0.5, window, max_q_len=12)
+
+
 @pytest.mark.parametrize("kv,kvh", [
     ([5000], 1),                                          # one unit in more parts than a join takes at once
     ([1700, 1, 0, 2600], 2),                              # every CTA a part of one unit
