@@ -113,12 +113,6 @@ struct UnitPos {
   int steps;      // steps of each of its units
 };
 
-// floor(total c / ctas), in 32 bits where that fits.
-__device__ __forceinline__ int64_t share_of(int64_t total, int64_t c, int64_t ctas) {
-  if (total < (1 << 21) && ctas < (1 << 10)) return (uint32_t)total * (uint32_t)c / (uint32_t)ctas;
-  return total * c / ctas;
-}
-
 template <int RT>
 __device__ __forceinline__ bool load_request(const AttnParams8& p, int bs, int req, UnitPos& u) {
   u.req = req;
@@ -242,7 +236,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     scan(units);
     const int64_t grid = gridDim.x;
     if (units < grid) {
-      const int64_t c = (total + grid - units - 1) / (grid - units);
+      const int64_t c = quotient(total + grid - units - 1, grid - units);
       if (c * grid <= total + kBoundarySteps * grid) {
         chunk = (int)c;                       // total / c + units parts at most
         scan(units);
@@ -250,8 +244,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     }
     ctas = min(grid, total);                  // every range holds a place
     if (blockIdx.x >= ctas) return;
-    begin = chunk ? blockIdx.x : share_of(total, blockIdx.x, ctas);
-    end = chunk ? 0 : share_of(total, blockIdx.x + 1, ctas);
+    begin = chunk ? blockIdx.x : quotient(total * blockIdx.x, ctas);
+    end = chunk ? 0 : quotient(total * (blockIdx.x + 1), ctas);
     if (at <= begin && begin < at + mine) {
       int r = r0;
       for (;; ++r) {
@@ -274,7 +268,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
       end = min(begin + chunk, (int64_t)unit.steps);
       unit_at = 0;
     } else {
-      in = (int)((begin - range_s[0]) / unit.steps);
+      in = (int)quotient(begin - range_s[0], unit.steps);
       unit_at = range_s[0] + (int64_t)in * unit.steps;
     }
     unit.head = in / unit.tiles_r;
@@ -706,8 +700,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     }
     if (!whole) {
       // CTAs whose ranges meet this unit: start(c) = total c / ctas
-      const int c0 = chunk ? part0 : (int)(((u0 + 1) * ctas - 1) / total);
-      const int c1 = chunk ? part0 + parts0 - 1 : (int)((u1 * ctas - 1) / total);
+      const int c0 = chunk ? part0 : (int)quotient((u0 + 1) * ctas - 1, total);
+      const int c1 = chunk ? part0 + parts0 - 1 : (int)quotient(u1 * ctas - 1, total);
       named_barrier(1, kFewConsumers);
       if (threadIdx.x == 0) {
         const uint32_t n = atom_add_acq_rel_gpu(p.counters + c0, 1u);
@@ -719,7 +713,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
         const int64_t stride = (int64_t)2 * RT * (D + 2);
         // CTA c0's share sits in slot 0 when its range starts at the unit, else in slot 1
         const float* first = reinterpret_cast<const float*>(p.data) +
-                             ((int64_t)c0 * 2 + (chunk || total * c0 / ctas >= u0 ? 0 : 1)) * RT * (D + 2);
+                             ((int64_t)c0 * 2 + (chunk || quotient(total * c0, ctas) >= u0 ? 0 : 1)) * RT * (D + 2);
         const float* rest = reinterpret_cast<const float*>(p.data) + (int64_t)c0 * stride;
         const int parts = c1 - c0 + 1;
         constexpr int kLanes = D / 4;    // threads of a row

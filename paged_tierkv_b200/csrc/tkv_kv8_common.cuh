@@ -52,6 +52,13 @@ __device__ __forceinline__ float warp_max(float x) {
   return x;
 }
 
+// a / b for a >= 0, b > 0: the 64-bit division is a subroutine of some 500
+// clocks, and small steps have several in a row.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((uint64_t)(a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
+
 __device__ __forceinline__ int64_t warp_sum(int64_t x) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(~0u, x, o);

@@ -317,30 +317,28 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     while (lanes > 1 && lanes * p.requests > kScan) lanes >>= 1;
     const int sub = tid & (lanes - 1), per_round = kScan / lanes;
     const bool scans = tid < kScan;
-    int64_t sum = 0;
-    for (int r = tid / lanes; scans && r - tid / lanes < p.requests; r += per_round) {
-      const int64_t n = many_places(p, r, sub, lanes);
-      if (sub == 0) sum += n;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (scans && lane == 0) misc[warp] = sum;
-    __syncthreads();
-    int64_t total = 0;
-    for (int w = 0; w < kScan / 32; ++w) total += misc[w];
-    const int64_t ctas = min((int64_t)gridDim.x, total);
-    if (blockIdx.x >= ctas) {
-      if (tid == 0) p.merges[blockIdx.x].parts = 0;
-      return;                       // CTA-uniform
-    }
-    const int64_t begin = total * blockIdx.x / ctas;
-    walk.end = (int)(total * (blockIdx.x + 1) / ctas - begin);
-    // the request that holds `begin`, then its row tile
-    __syncthreads();
-    int64_t at = 0;
-    for (int r0 = 0; r0 < p.requests; r0 += per_round) {
-      const int64_t n = scans ? many_places(p, r0 + tid / lanes, sub, lanes) : 0;
-      int64_t inc = sub == 0 && scans ? n : 0;
+    // most steps have a thread for every row tile: one scan finds the tile
+    ManyUnit own;
+    own.rts = 0;
+    const int own_req = tid / lanes;
+    if (scans && own_req < p.requests) load_many(p, own_req, own);
+    own.rt = sub;
+    if (sub < own.rts) unit_tiles(p, own);
+    const int64_t mine = sub < own.rts ? (int64_t)(own.n + kUnitCost) * p.kv_heads : 0;
+    const bool one_scan = !__syncthreads_or(per_round < p.requests || own.rts > lanes);
+    int64_t total = 0, begin, ctas;
+    auto share = [&]() {            // this CTA's part of the list; false without one
+      ctas = min((int64_t)gridDim.x, total);
+      if (blockIdx.x >= ctas) {
+        if (tid == 0) p.merges[blockIdx.x].parts = 0;
+        return false;               // CTA-uniform
+      }
+      begin = quotient(total * blockIdx.x, ctas);
+      walk.end = (int)(quotient(total * (blockIdx.x + 1), ctas) - begin);
+      return true;
+    };
+    if (one_scan) {
+      int64_t inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t x = __shfl_up_sync(~0u, inc, o);
@@ -348,49 +346,87 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
       if (scans && lane == 31) misc[warp] = inc;
       __syncthreads();
-      int64_t first = at + inc - n, next = at;
+      int64_t first = inc - mine;
       for (int w = 0; w < kScan / 32; ++w) {
         if (w < warp) first += misc[w];
-        next += misc[w];
+        total += misc[w];
       }
-      if (scans && sub == 0 && first <= begin && begin < first + n) {
-        misc[8] = first;
-        misc[9] = r0 + tid / lanes;
-      }
+      if (!share()) return;
       __syncthreads();
-      at = next;
-      if (begin < at) break;        // CTA-uniform
-    }
-    if (warp == 0) {
-      ManyUnit u;
-      load_many(p, (int)misc[9], u);
-      int64_t first = misc[8];
-      for (int rt0 = 0;; rt0 += 32) {
-        u.rt = min(rt0 + lane, u.rts - 1);
-        unit_tiles(p, u);
-        int64_t inc = rt0 + lane < u.rts ? (int64_t)(u.n + kUnitCost) * p.kv_heads : 0;
-        const int64_t n = inc;
+      if (first <= begin && begin < first + mine) {
+        misc[0] = first;
+        misc[1] = own.req;
+        misc[2] = own.rt;
+        misc[3] = total;
+      }
+    } else {
+      int64_t sum = 0;
+      for (int r = tid / lanes; scans && r - tid / lanes < p.requests; r += per_round) {
+        const int64_t n = many_places(p, r, sub, lanes);
+        if (sub == 0) sum += n;
+      }
+      sum = warp_sum(sum);
+      if (scans && lane == 0) misc[warp] = sum;
+      __syncthreads();
+      for (int w = 0; w < kScan / 32; ++w) total += misc[w];
+      if (!share()) return;
+      // the request that holds `begin`, then its row tile
+      __syncthreads();
+      int64_t at = 0;
+      for (int r0 = 0; r0 < p.requests; r0 += per_round) {
+        const int64_t n = scans ? many_places(p, r0 + tid / lanes, sub, lanes) : 0;
+        int64_t inc = sub == 0 && scans ? n : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int64_t x = __shfl_up_sync(~0u, inc, o);
           if (lane >= o) inc += x;
         }
-        const int64_t mine = first + inc - n;
-        if (mine <= begin && begin < mine + n) {
-          misc[0] = mine;
-          misc[1] = u.req;
-          misc[2] = u.rt;
-          misc[3] = total;
+        if (scans && lane == 31) misc[warp] = inc;
+        __syncthreads();
+        int64_t first = at + inc - n, next = at;
+        for (int w = 0; w < kScan / 32; ++w) {
+          if (w < warp) first += misc[w];
+          next += misc[w];
         }
-        first += __shfl_sync(~0u, inc, 31);
-        if (begin < first) break;
+        if (scans && sub == 0 && first <= begin && begin < first + n) {
+          misc[8] = first;
+          misc[9] = r0 + tid / lanes;
+        }
+        __syncthreads();
+        at = next;
+        if (begin < at) break;      // CTA-uniform
+      }
+      if (warp == 0) {
+        ManyUnit u;
+        load_many(p, (int)misc[9], u);
+        int64_t first = misc[8];
+        for (int rt0 = 0;; rt0 += 32) {
+          u.rt = min(rt0 + lane, u.rts - 1);
+          unit_tiles(p, u);
+          int64_t inc = rt0 + lane < u.rts ? (int64_t)(u.n + kUnitCost) * p.kv_heads : 0;
+          const int64_t n = inc;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(~0u, inc, o);
+            if (lane >= o) inc += x;
+          }
+          const int64_t here = first + inc - n;
+          if (here <= begin && begin < here + n) {
+            misc[0] = here;
+            misc[1] = u.req;
+            misc[2] = u.rt;
+            misc[3] = total;
+          }
+          first += __shfl_sync(~0u, inc, 31);
+          if (begin < first) break;
+        }
       }
     }
     __syncthreads();
     load_many(p, (int)misc[1], walk.u);
     walk.u.rt = (int)misc[2];
     unit_tiles(p, walk.u);
-    walk.u.head = (int)((begin - misc[0]) / (walk.u.n + kUnitCost));
+    walk.u.head = (int)quotient(begin - misc[0], walk.u.n + kUnitCost);
     walk.u_at = (int)(misc[0] + (int64_t)walk.u.head * (walk.u.n + kUnitCost) - begin);
   }
   if (warp == 20) tmem_alloc(taddr_s, kManyTmem);
@@ -860,8 +896,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         // the one whose range (start(c) = total c / ctas) holds its last tile
         MergeUnit mu;
         const int64_t total = misc[3], ctas = min((int64_t)gridDim.x, total);
-        const int64_t u_end = total * blockIdx.x / ctas + w.u_end();
-        mu.parts = (int)((u_end * ctas - 1) / total) - (int)blockIdx.x + 1;
+        const int64_t u_end = quotient(total * blockIdx.x, ctas) + w.u_end();
+        mu.parts = (int)quotient(u_end * ctas - 1, total) - (int)blockIdx.x + 1;
         mu.slot0 = slot;
         mu.q0 = w.u.q0;
         mu.row0 = w.u.rt * kUnitRows;
