@@ -24,10 +24,12 @@ namespace tkv {
 // scanned sums.  A cluster barrier between the last read of an input and the
 // first write lets kv_lens / free_count be updated in place.  Latency bound:
 // a launch, one round of loads, two block scans (64 requests of one token: 4.3
-// us; 1024 requests with 130000 tokens: 13.4 us for 1.7 MB of outputs).
+// us; 1024 requests with 130000 tokens: 9.9 us for 1.7 MB of outputs).
 // Small steps (up to 1024 requests, tokens and write units) take one CTA of 256
-// threads, whose barriers are cheaper than the cluster's; others 8 of 1024.
-constexpr int kPlanCluster = 8;
+// threads, whose barriers are cheaper than the cluster's; others 16 of 1024, the
+// largest cluster there is (8: 13.3 us for those 130000 tokens, 16 of 512: 10.8;
+// 2000 tokens the same).
+constexpr int kPlanCluster = 16;
 constexpr int kPlanThreads = 1024, kPlanSmall = 256;
 constexpr int kPlanSmallWork = 1024;
 
@@ -238,10 +240,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 cudaError_t launch_plan_step(const tkv_kv8_plan_args& p, cudaStream_t stream) {
   const size_t smem = sizeof(int32_t) * (4 * (size_t)p.requests + 3);
   const bool small = p.requests <= kPlanSmallWork && p.tokens <= kPlanSmallWork && p.units_cap <= kPlanSmallWork;
-  if (smem > 40 * 1024) {   // more requests than a small step has
-    static std::atomic<uint64_t> allowed;
-    const cudaError_t e = allow_smem(plan_step_kernel<kPlanThreads>,
-                                     (int)(sizeof(int32_t) * (4 * TKV_KV8_MAX_REQUESTS + 3)), allowed);
+  if (!small) {
+    static std::atomic<uint64_t> allowed, wide;
+    cudaError_t e = allow_smem(plan_step_kernel<kPlanThreads>,
+                               (int)(sizeof(int32_t) * (4 * TKV_KV8_MAX_REQUESTS + 3)), allowed);
+    if (e == cudaSuccess)
+      e = allow(plan_step_kernel<kPlanThreads>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, wide);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};

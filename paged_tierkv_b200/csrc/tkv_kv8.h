@@ -17,18 +17,22 @@ using RotaryArgs = tkv_rotary;
 
 constexpr int kKv8MaxDevices = 64;
 
-// The opt-in to more than 48 KB of shared memory is per function and device;
-// `done` (one per function) holds the devices that have it.
+// Opt-ins (more than 48 KB of shared memory, clusters of 16) are per function and
+// device; `done` (one per function and opt-in) holds the devices that have it.
 template <typename Kernel>
-cudaError_t allow_smem(Kernel kern, int bytes, std::atomic<uint64_t>& done) {
+cudaError_t allow(Kernel kern, cudaFuncAttribute what, int value, std::atomic<uint64_t>& done) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev >= 0 && dev < kKv8MaxDevices ? uint64_t(1) << dev : 0;
   if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  e = cudaFuncSetAttribute(kern, what, value);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
+}
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kern, int bytes, std::atomic<uint64_t>& done) {
+  return allow(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes, done);
 }
 
 struct RotaryParams {
