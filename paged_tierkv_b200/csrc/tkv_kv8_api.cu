@@ -236,7 +236,9 @@ int32_t tkv_kv8_attention(const tkv_kv8_cache* cache, const tkv_kv8_attention_ar
   p.group = group;
   p.table_width = a->table_width;
   p.max_q_len = a->max_q_len;
-  p.window = a->window;
+  // no context reaches 2^30 keys, so a window of that many hides none; the
+  // kernels' position arithmetic (keys - query tokens - window) stays in 32 bits
+  p.window = a->window < (1 << 30) ? a->window : 0;
   p.scale_log2 = a->scaling * kLog2e;
   p.group_inv = group > 1 ? (uint32_t)(((uint64_t(1) << 32) + group - 1) / group) : 0;
   p.block_size = cache->block_size;
