@@ -416,7 +416,8 @@ typedef struct tkv_kv8_cache {
  * 0 or C(i) <= free_count; a row without room counts need 0.  A request that
  * is not admitted keeps its context, its tokens get slot -1, and the launch
  * records TKV_DEVERR_NO_BLOCKS.  Nothing is written to table cells other than
- * those of the new blocks.
+ * those of the new blocks.  Running sums and a refused request's positions end
+ * at 2^31 - 1.
  * Inputs may alias the outputs of the same meaning (context_lens / kv_lens,
  * free_count / free_count_out). */
 typedef struct tkv_kv8_plan_args {

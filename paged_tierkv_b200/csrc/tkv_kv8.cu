@@ -38,7 +38,13 @@ struct Scan {
   int32_t carry[2];
 };
 
-// Exclusive sums over the CTA's threads of (a, b); every thread also gets the totals.
+// a + b for a, b >= 0, at most 2^31 - 1: sums over lengths that make no sense
+// (8192 prompts of 2^30 tokens) stay sums that no step can hold.
+__device__ __forceinline__ int32_t sat_add(int32_t a, int32_t b) {
+  return (int32_t)min((uint32_t)a + (uint32_t)b, 0x7fffffffu);
+}
+
+// Exclusive saturated sums over the CTA's threads of (a, b); every thread also gets the totals.
 __device__ __forceinline__ void scan2(Scan& s, int32_t a, int32_t b, int32_t& ea, int32_t& eb,
                                       int32_t& ta, int32_t& tb) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -47,8 +53,8 @@ __device__ __forceinline__ void scan2(Scan& s, int32_t a, int32_t b, int32_t& ea
   for (int o = 1; o < 32; o <<= 1) {
     const int32_t xa = __shfl_up_sync(~0u, ia, o), xb = __shfl_up_sync(~0u, ib, o);
     if (lane >= o) {
-      ia += xa;
-      ib += xb;
+      ia = sat_add(ia, xa);
+      ib = sat_add(ib, xb);
     }
   }
   __syncthreads();  // the previous scan's readers are done
@@ -63,16 +69,17 @@ __device__ __forceinline__ void scan2(Scan& s, int32_t a, int32_t b, int32_t& ea
   for (int o = 1; o < 32; o <<= 1) {
     const int32_t xa = __shfl_up_sync(~0u, wa, o), xb = __shfl_up_sync(~0u, wb, o);
     if (lane >= o) {
-      wa += xa;
-      wb += xb;
+      wa = sat_add(wa, xa);
+      wb = sat_add(wb, xb);
     }
   }
   ta = __shfl_sync(~0u, wa, 31);
   tb = __shfl_sync(~0u, wb, 31);
   const int32_t before_a = __shfl_sync(~0u, wa, warp ? warp - 1 : 0);
   const int32_t before_b = __shfl_sync(~0u, wb, warp ? warp - 1 : 0);
-  ea = (warp ? before_a : 0) + ia - a;
-  eb = (warp ? before_b : 0) + ib - b;
+  const int32_t lane_a = __shfl_up_sync(~0u, ia, 1), lane_b = __shfl_up_sync(~0u, ib, 1);
+  ea = sat_add(warp ? before_a : 0, lane ? lane_a : 0);
+  eb = sat_add(warp ? before_b : 0, lane ? lane_b : 0);
 }
 
 // Largest i with first[i] <= x, for a non-decreasing first[0 .. n] with first[0] = 0 <= x < first[n].
@@ -86,9 +93,9 @@ __device__ __forceinline__ int find(const int32_t* first, int n, int32_t x) {
   return lo;
 }
 
-// x / 2^log2, rounded up.
-__device__ __forceinline__ int32_t ceil_div(int32_t x, int log2) {
-  return (int32_t)(((uint32_t)x + (1u << log2) - 1) >> log2);
+// x / 2^log2, rounded up, for any x below 2^32.
+__device__ __forceinline__ int32_t ceil_div(uint32_t x, int log2) {
+  return (int32_t)((x >> log2) + ((x & ((1u << log2) - 1)) != 0));
 }
 
 template <int kThreads>
@@ -113,12 +120,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   int32_t sum_new = 0, sum_need = 0;
   for (int i = r0; i < r1; ++i) {
     const int32_t c = max(0, p.context_lens[i]), m = max(0, p.new_lens[i]);
-    const int32_t want = ceil_div(c + m, bs_log2);
+    const int32_t want = ceil_div((uint32_t)c + (uint32_t)m, bs_log2);
     ctx[i] = c;
     cu[i] = m;
     need[i] = want <= p.table_width ? want - ceil_div(c, bs_log2) : -1;
-    sum_new += m;
-    sum_need += max(0, need[i]);
+    sum_new = sat_add(sum_new, m);
+    sum_need = sat_add(sum_need, max(0, need[i]));
   }
   int32_t at_new, at_need, total_new, total_need;
   scan2(scan, sum_new, sum_need, at_new, at_need, total_new, total_need);
@@ -126,23 +133,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool refused = false;
   for (int i = r0; i < r1; ++i) {
     const int32_t m = cu[i], k = need[i], c = ctx[i];
-    const bool ok = k >= 0 && (k == 0 || at_need + k <= free_count);
+    const bool ok = k >= 0 && (k == 0 || (uint32_t)at_need + (uint32_t)k <= (uint32_t)free_count);
     if (!ok) ctx[i] = c | (int32_t)0x80000000;
     if (!ok && m > 0) refused = true;
     cu[i] = at_new;
     need[i] = at_need;
     cu_unit[i] = ok && m > 0 ? ceil_div(c + m, bs_log2) - (c >> bs_log2) : 0;
-    sum_units += cu_unit[i];
-    at_new += m;
-    at_need += max(0, k);
-    if (ok) taken += k;
+    sum_units = sat_add(sum_units, cu_unit[i]);
+    at_new = sat_add(at_new, m);
+    at_need = sat_add(at_need, max(0, k));
+    if (ok) taken += k;                   // free_count at most, in sum
   }
   int32_t at_unit, at_taken, total_units, total_taken;
   scan2(scan, sum_units, taken, at_unit, at_taken, total_units, total_taken);
   for (int i = r0; i < r1; ++i) {
     const int32_t u = cu_unit[i];
     cu_unit[i] = at_unit;
-    at_unit += u;
+    at_unit = sat_add(at_unit, u);
   }
   if (tid == 0) {
     cu[n] = total_new;
@@ -152,14 +159,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster.sync();  // every CTA has read its inputs; shared memory is complete
 
   const int rank = (int)cluster.block_rank();
-  const int gtid = rank * kThreads + tid;
-  const int stride = (int)cluster.num_blocks() * kThreads;
+  const uint32_t gtid = rank * kThreads + tid;
+  const uint32_t stride = cluster.num_blocks() * kThreads;
   const bool vec = ((reinterpret_cast<uintptr_t>(p.slot_map) | reinterpret_cast<uintptr_t>(p.token_request) |
                      reinterpret_cast<uintptr_t>(p.positions)) & 15) == 0;
   if (rank == 0) {
     for (int i = r0; i < r1; ++i) {
       const int32_t c = ctx[i] & 0x7fffffff;
-      p.kv_lens[i] = ctx[i] >= 0 ? c + (cu[i + 1] - cu[i]) : c;
+      const int32_t m = cu[i + 1] < 0x7fffffff ? cu[i + 1] - cu[i] : max(0, p.new_lens[i]);
+      p.kv_lens[i] = ctx[i] >= 0 ? c + m : c;
       p.cu_q[i] = cu[i];
       p.admitted[i] = ctx[i] >= 0;
     }
@@ -171,8 +179,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (refused && p.error_word) atomicOr(p.error_word, TKV_DEVERR_NO_BLOCKS);
   }
 
-  // new table cells
-  for (int u = gtid; u < total_need; u += stride) {
+  // new table cells; blocks past the free list are nobody's
+  for (uint32_t u = gtid; u < (uint32_t)min(total_need, free_count); u += stride) {
     const int i = find(need, n, u);
     if (ctx[i] < 0) continue;
     p.block_table[i * p.table_stride + ceil_div(ctx[i], bs_log2) + (u - need[i])] =
@@ -185,9 +193,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                      : p.block_table[i * p.table_stride + j];
   };
   // write units
-  for (int u = gtid; u < p.units_cap; u += stride) {
+  for (uint32_t u = gtid; u < (uint32_t)p.units_cap; u += stride) {
     int4 out = make_int4(-1, -1, -1, -1);
-    if (u < total_units) {
+    if (u < (uint32_t)total_units) {
       const int i = find(cu_unit, n, u);
       const int32_t c = ctx[i], end = c + (cu[i + 1] - cu[i]);
       const int32_t j = (c >> bs_log2) + (u - cu_unit[i]);
@@ -198,21 +206,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   // tokens, four consecutive ones at a time: they share a request or two and
   // mostly a block, and leave as 16-byte stores
-  for (int t0 = 4 * gtid; t0 < p.tokens; t0 += 4 * stride) {
+  for (uint32_t t0 = 4 * gtid; t0 < (uint32_t)p.tokens; t0 += 4 * stride) {
     int4 slot = make_int4(-1, -1, -1, -1), rq = slot, ps = slot;
-    if (t0 < total_new) {
+    if (t0 < (uint32_t)total_new) {
       int req = find(cu, n, t0), end = cu[req + 1], c = ctx[req], cell = -1, cell_at = -1;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int t = t0 + k;
-        if (t >= total_new) break;
+        const int t = (int)t0 + k;
+        if (t0 + k >= (uint32_t)total_new) break;
         if (t >= end) {
           do ++req; while (cu[req + 1] <= t);
           end = cu[req + 1];
           c = ctx[req];
           cell_at = -1;
         }
-        const int pos = (c & 0x7fffffff) + (t - cu[req]);
+        const int pos = sat_add(c & 0x7fffffff, t - cu[req]);   // a refused request's context is any number
         const int j = pos >> bs_log2;
         if (c >= 0 && j != cell_at) {
           cell = block_of(req, c, j);
@@ -223,12 +231,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         reinterpret_cast<int*>(&ps)[k] = pos;
       }
     }
-    if (t0 + 4 <= p.tokens && vec) {
+    if (t0 + 4 <= (uint32_t)p.tokens && vec) {
       *reinterpret_cast<int4*>(p.slot_map + t0) = slot;
       *reinterpret_cast<int4*>(p.token_request + t0) = rq;
       *reinterpret_cast<int4*>(p.positions + t0) = ps;
     } else {
-      for (int k = 0; k < 4 && t0 + k < p.tokens; ++k) {
+      for (int k = 0; k < 4 && t0 + k < (uint32_t)p.tokens; ++k) {
         p.slot_map[t0 + k] = reinterpret_cast<int*>(&slot)[k];
         p.token_request[t0 + k] = reinterpret_cast<int*>(&rq)[k];
         p.positions[t0 + k] = reinterpret_cast<int*>(&ps)[k];

@@ -36,3 +36,50 @@ def test_a_window_as_wide_as_an_int_is_no_window(q, window):
     rng = np.random.default_rng(q)
     scene = _scene(rng, kv, [q, q, q], 2, 1, 128, 16, "int8", "fp16")
     _check_attention(scene, kv, 16, "int8", "fp16", 0.1, window)
+
+
+# ---------------------------------------------------------------------------
+# plans
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens", [64, 2000])                   # one CTA, a cluster
+def test_plans_of_lengths_near_the_end_of_an_int(tokens):
+    """Lengths whose sums pass 2^31: refused, and the requests around them planned."""
+    from paged_tierkv_b200 import kv8
+    big = 2 ** 31 - 1
+    ctx, new = [0, big, 5, 0, big - 3], [big, big, 7, 20, 30]
+    plan = kv8.StepPlan.allocate(5, tokens, 16, "cuda")
+    table = torch.full((5, 4), 77, dtype=torch.int32, device="cuda")
+    kv8.plan_step(plan, _i32(ctx), _i32(new), table, _i32([10, 11, 12, 13]), _i32([4]))
+    assert _errors() & 4
+    assert _np(plan.admitted).tolist() == [0, 0, 1, 1, 0]
+    assert _np(plan.kv_lens).tolist()[:3] == [0, big, 12]
+    assert _np(plan.cu_q).tolist() == [0, big, big, big, big, big]
+    assert int(plan.free_count) == 2 and (_np(plan.slot_map) == -1).all() and (_np(plan.token_request) == 0).all()
+    np.testing.assert_array_equal(_np(plan.positions), np.arange(tokens))
+    np.testing.assert_array_equal(_np(table), np.array([[77] * 4] * 3 + [[13, 12, 77, 77]] + [[77] * 4]))
+    # a refused request at the end of the range, first in the batch
+    kv8.plan_step(plan, _i32([big - 3, 5]), _i32([30, 7]), table, _i32([10]), _i32([1]))
+    assert _errors() & 4
+    assert _np(plan.cu_q)[:3].tolist() == [0, 30, 37] and _np(plan.kv_lens)[:2].tolist() == [big - 3, 12]
+    want = np.full(tokens, -1)
+    want[:37] = np.concatenate([np.minimum(big - 3 + np.arange(30), big), 5 + np.arange(7)])
+    np.testing.assert_array_equal(_np(plan.positions), want)
+
+
+@pytest.mark.parametrize("tokens", [64, 2000])
+def test_plans_of_more_blocks_than_an_int_counts(tokens):
+    """Forty requests that would take 2^26 - 1 blocks each: what they ask for
+    never wraps into blocks that the free list holds."""
+    from paged_tierkv_b200 import kv8
+    n, width = 43, 2 ** 26 - 1
+    new = [20] + [16 * width] * 40 + [1, 0]
+    plan = kv8.StepPlan.allocate(n, tokens, 16, "cuda")
+    table = torch.empty((n, width), dtype=torch.int32, device="cuda")
+    kv8.plan_step(plan, _i32([0] * n), _i32(new), table, _i32(np.arange(50, 60)), _i32([10]))
+    assert _errors() & 4
+    assert _np(plan.admitted).tolist() == [1] + [0] * 41 + [1]
+    assert _np(plan.kv_lens).tolist() == [20] + [0] * 42 and int(plan.free_count) == 8 and int(plan.num_units) == 2
+    assert _np(table[0, :2]).tolist() == [59, 58]
+    cu = _np(plan.cu_q)
+    assert cu[:3].tolist() == [0, 20, 20 + 16 * width] and (np.diff(cu) >= 0).all() and cu[-1] == 2 ** 31 - 1
