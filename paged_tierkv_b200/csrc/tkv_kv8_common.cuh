@@ -75,10 +75,21 @@ __device__ __forceinline__ void fp16_scale(float amax, float& up, float& down) {
   down = __uint_as_float((uint32_t)(e - 14) << 23);            // 2^((e - 127) - 14)
 }
 
-// 2^14 over the power of two at or above s: s times it lies in (2^13, 2^14].
+// 2^14 over the power of two at or above s: s times it lies in (2^13, 2^14]; for
+// an s below 2^-114 2^127, the largest power of two.
 __device__ __forceinline__ float scale_inverse(float s) {
-  const int e = max((int)(__float_as_uint(s) >> 23), 20);
+  const int e = max((int)(__float_as_uint(s) >> 23), 13);
   return __uint_as_float((uint32_t)(267 - e) << 23);
+}
+
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Smallest e with x <= 2^e, for a finite x > 0 (subnormal ones too).
+__device__ __forceinline__ int ceil_log2(float x) {
+  const uint32_t b = __float_as_uint(x);
+  if (b < 0x00800000u) return (b > 1 ? 32 - __clz(b - 1) : 0) - 149;
+  return (int)(b >> 23) - 127 + ((b & 0x007fffffu) != 0);
 }
 
 __device__ __forceinline__ float row_lse(float m, float sum) { return (m + lg2(sum)) * kLn2; }

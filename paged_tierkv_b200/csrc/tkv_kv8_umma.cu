@@ -31,13 +31,17 @@
 // 1141 us against 807 for the 8192-token prompt at that stage).
 //
 // Scales.  A tile's K scales multiply the logits of their 16 columns in fp32.
-// V's go into the exponent: P' = exp2(s - m + log2(vs vinv)), vinv a power of
-// two that keeps P' in fp16's normal range, and the row sum gets p back by one
-// multiplication with 1 / vs per 16 columns.  m follows the running maximum
-// lazily: O is only rescaled when it has grown by more than 3.9 (log2; by more
-// than 2 the 8192-token prompt takes 8 % longer).  With vs vinv at most 2^12, P'
-// stays below fp16's largest number and normal down to 2^-25 of the row's largest.  bf16 queries become fp16 by a power of
-// two per row.
+// V's go into the exponent: P' = exp2(s - m + 12 + log2(vs / 2^E)), 2^E the power
+// of two at or above the largest V scale of the segment so far.  O is in units
+// of 2^(E - 12) and is rescaled when E grows; the row sum gets p back by one
+// multiplication with 2^E / vs per 16 columns and is in units of 2^-12 whatever
+// E is, so it neither passes fp32's range nor loses a key for the sake of V's
+// scales.  m follows the running maximum lazily: O is only rescaled when it has
+// grown by more than 3.9 (log2; by more than 2 the 8192-token prompt takes 8 %
+// longer).  With vs / 2^E at most 1, P' stays below fp16's largest number and
+// normal down to 2^-25 of the row's largest.  A scale below 2^-60 of 2^E (or 0)
+// is beyond what P' can hold: its keys count in the row sum, its values as
+// zeros.  bf16 queries become fp16 by a power of two per row.
 //
 // Work is a flat list of (unit, K/V tile), where a unit counts kUnitCost tiles
 // more than it has (loading Q, writing the output), cut evenly over the CTAs,
@@ -56,10 +60,11 @@ constexpr int kManyThreads = 704;
 constexpr int kUnitRows = 256;
 constexpr int kTok = 128;                 // tokens of a K/V tile
 constexpr int kGroups = kTok / 16;        // scale groups of a tile
-constexpr int kScStride = kGroups + 1;    // and (log2 of the largest V scale, first token, first and last key)
+constexpr int kScStride = kGroups + 1;    // and (E, first token, first and last key)
 constexpr int kUnitCost = 4;              // a unit's fixed cost in tiles
 constexpr uint32_t kManyTmem = 512;
-constexpr float kVLog = 12.f;             // log2 of vs vinv, at most, for the largest V scale so far
+constexpr float kVLog = 12.f;             // log2 of P' at the row's reference and the scale 2^E
+constexpr float kVLeast = 0x1p-60f;       // smallest vs / 2^E whose values count
 constexpr float kLazy = 3.9f;             // growth of the maximum (log2) that P' absorbs
 
 template <int D>
@@ -70,7 +75,7 @@ struct ManyLayout {
   static constexpr int kVOff = 4 * kTile;                 // [2] stages
   static constexpr int kCodes = kTok * D;                 // staged codes of a tile
   static constexpr int kStOff = 6 * kTile;                // K, V
-  static constexpr int kScOff = kStOff + 2 * kCodes;      // [4][kScStride] float4 (ks, vs, log2 vs, 1 / vs)
+  static constexpr int kScOff = kStOff + 2 * kCodes;      // [4][kScStride] float4 (ks, vs, log2 (vs / 2^E), 2^E / vs)
   static constexpr int kBarOff = kScOff + 4 * kScStride * 16;
   static constexpr int kNumBars = 26;
   static constexpr int kRowOff = kBarOff + kNumBars * 8;  // [2 tiles][2 halves][128] floats: the rows'
@@ -544,20 +549,22 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     bool more = w.more();
     load();
     for (; more; ++j) {
-      // the segment's largest V scale so far; a NaN does not move vinv
-      float top = vs < 3e38f ? vs : 0.f;
+      // the segment's largest V scale so far; a NaN does not move E
+      float top = vs <= 0x1p127f ? vs : 0.f;
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
       run_top = fmaxf(first ? 0.f : run_top, top);
-      top = run_top > 0.f ? run_top : 1.f;
-      // a group whose V scale is 0 (nothing stored, a bad slot) has its codes
-      // zeroed, and takes a scale that is as good as any
-      const float v1 = vs == 0.f ? top : vs;
+      const int e = run_top > 0.f ? ceil_log2(run_top) : 0;
+      // a group without a V scale to speak of (0: nothing stored, a bad slot)
+      // has its codes zeroed, and takes a scale that is as good as any
+      float v1 = vs * exp2_int((-e) >> 1) * exp2_int(-e - ((-e) >> 1));   // exact, or far below kVLeast
+      const bool none = fabsf(v1) < kVLeast;
+      if (none) v1 = 1.f;
       float4* sc = scales + (j & 3) * kScStride;
-      if (lane < kGroups) sc[lane] = make_float4(ks, vs, lg2(v1), 1.f / v1);
+      if (lane < kGroups) sc[lane] = make_float4(ks, none ? 0.f : vs, lg2(v1), 1.f / v1);
       if (lane == 0)
-        sc[kGroups] = make_float4(lg2(top), __int_as_float(tok0), __int_as_float(lo), __int_as_float(hi));
+        sc[kGroups] = make_float4((float)e, __int_as_float(tok0), __int_as_float(lo), __int_as_float(hi));
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_full + (j & 3));
       const uint32_t live = __ballot_sync(~0u, seen) & ((1u << kGroups) - 1);
@@ -717,8 +724,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int lo = p.window > 0 ? hi - p.window : 0;
       // every row of the warp sees keys [all_lo, all_hi)
       const int all_hi = __shfl_sync(~0u, hi, 0), all_lo = __shfl_sync(~0u, lo, 31);
-      float m = -INFINITY, l = 0.f;       // reference of the exponents (log2), sum in units of vinv
-      float vlog = 0.f;                   // log2 vinv
+      float m = -INFINITY, l = 0.f;       // reference of the exponents (log2), sum in units of 2^-kVLog
+      float e_v = 0.f;                    // E
       const int tile0 = w.first();
       for (int j = 0; j < n; ++j, ++at, ++tile) {
         const float4* sc = scales + (tile & 3) * kScStride + half * 4;
@@ -756,21 +763,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         mx = fmaxf(mx, *other);
         mx *= rscale;
         // V's power of two: set by the first tile, moved when a scale outgrows it
-        float shift = 0.f;                            // log2 of the factor O and l take
-        const float vtop = sc[kGroups - half * 4].x;
-        if (j == 0) {
-          vlog = kVLog - ceilf(vtop);
-        } else if (vtop + vlog > kVLog + 1e-3f) {
-          shift = kVLog - ceilf(vtop) - vlog;
-          vlog += shift;
-        }
+        float shift = 0.f;                            // log2 of the factor that O takes
+        const float e_tile = sc[kGroups - half * 4].x;
+        if (j > 0) shift = e_v - e_tile;
+        e_v = e_tile;
         if (mx > m + kLazy) {
-          if (m != -INFINITY) shift += m - mx;        // nothing summed yet: nothing to rescale
+          if (m != -INFINITY) {                       // nothing summed yet: nothing to rescale
+            shift += m - mx;
+            l *= ex2(m - mx);
+          }
           m = mx;
         }
         if (__any_sync(~0u, shift != 0.f)) {
           const float f = ex2(shift);
-          l *= f;
           wait(o_full + i, at - 1);
           __syncwarp();
           tc_fence_after();
@@ -783,7 +788,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             tmem_st16(o_col + c * 16, o);
           }
         }
-        const float off = vlog - (m == -INFINITY ? 0.f : m);
+        const float off = kVLog - (m == -INFINITY ? 0.f : m);
         // pass 2: P' and the sum
         auto probabilities = [&](int c, uint32_t(&v)[32]) {
           uint32_t pk[16];
@@ -836,6 +841,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       named_barrier(1 + i, 256);
       l += *other;
       const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int e_o = (int)e_v;                       // 2^E down to 2^-149; apart from inv: the product may leave fp32's range
+      const float unit = exp2_int(e_o >> 1) * exp2_int(e_o - (e_o >> 1));
       if (whole) {
         // through the warp's own rows and half of the Q tile (its last MMA is
         // done), so that whole lines leave together
@@ -854,8 +861,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             uint32_t o[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              o[k] = pack_out(bf16, __uint_as_float(v[x * 8 + 2 * k]) * inv,
-                              __uint_as_float(v[x * 8 + 2 * k + 1]) * inv);
+              o[k] = pack_out(bf16, __uint_as_float(v[x * 8 + 2 * k]) * inv * unit,
+                              __uint_as_float(v[x * 8 + 2 * k + 1]) * inv * unit);
             *staged(lane, c * 4 + x) = make_uint4(o[0], o[1], o[2], o[3]);
           }
         }
@@ -872,7 +879,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
         }
       } else {
-        // partials as shares of the row's mass: free of vinv and of the reference
+        // partials as shares of the row's mass: free of E and of the reference
         float4* part = p.part_o + ((int64_t)blockIdx.x * 2 + slot) * (D / 4) * kUnitRows + r;
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {
@@ -881,11 +888,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
           for (int x = 0; x < 8; ++x)
             part[(half * (D / 8) + c * 8 + x) * kUnitRows] =
-                make_float4(__uint_as_float(v[4 * x]) * inv, __uint_as_float(v[4 * x + 1]) * inv,
-                            __uint_as_float(v[4 * x + 2]) * inv, __uint_as_float(v[4 * x + 3]) * inv);
+                make_float4(__uint_as_float(v[4 * x]) * inv * unit, __uint_as_float(v[4 * x + 1]) * inv * unit,
+                            __uint_as_float(v[4 * x + 2]) * inv * unit, __uint_as_float(v[4 * x + 3]) * inv * unit);
         }
       }
-      const float lse2 = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + lg2(l) - vlog;
+      const float lse2 = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + lg2(l) - kVLog;
       if (half == 0 && !whole) {
         p.part_lse[((int64_t)blockIdx.x * 2 + slot) * kUnitRows + r] = lse2;
       } else if (half == 0 && live && p.out_lse) {

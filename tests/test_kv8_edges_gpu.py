@@ -83,3 +83,36 @@ def test_plans_of_more_blocks_than_an_int_counts(tokens):
     assert _np(table[0, :2]).tolist() == [59, 58]
     cu = _np(plan.cu_q)
     assert cu[:3].tolist() == [0, 20, 20 + 16 * width] and (np.diff(cu) >= 0).all() and cu[-1] == 2 ** 31 - 1
+# ---------------------------------------------------------------------------
+# scales
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("exponent", [-110, -124])
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("kv,ql,heads", [
+    ([500, 300], [1, 1], 1),            # few rows
+    ([500, 300], [200, 66], 1),         # many rows, units split over CTAs
+    ([60, 50, 55], [49] * 3, 100),      # many rows, whole units
+])
+def test_tiny_v_scales_leave_the_row_sums_alone(exponent, mixed, fmt, kv, ql, heads):
+    """V scales that append writes for tiny values (2^-116 and below, subnormal
+    ones too): the LSE depends on K alone, and the values stay what they are.
+    Mixed: beside ordinary blocks."""
+    rng = np.random.default_rng(200 + exponent)
+    scene = _scene(rng, kv, ql, heads, heads, 64, 16, fmt, "bf16")
+    vs = scene[3]
+    live = np.isfinite(vs[:, 0])
+    if mixed:
+        live &= rng.integers(0, 2, len(live)).astype(bool)
+    vs[live] *= np.float32(2.0 ** exponent)
+    kc, ks, vc, vs, table, cu, q = scene
+    out, lse = _attend(scene, kv, 16, fmt, 0.125)
+    ref, rl, mass, size = kv8o.attention(q.double().cpu().numpy(), kc, vc, ks, vs, table, kv, cu, 0.125, fmt)
+    got, gl = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    assert np.all(np.abs(gl - rl) <= 2.0 ** -18 * size + 2.0 ** -19 * (1 + np.abs(rl)))
+    eps, biggest = 2.0 ** -8, np.nanmax(vs) * float(kv8o.QMAX[fmt])
+    tol = (mass * (2.0 ** -11 + 2.0 ** -17 * size[..., None] + 2.0 ** -18) * (1 + eps) + eps * np.abs(ref) + 2.0 ** -134
+           + max(kv) * 2.0 ** -21 * biggest)
+    err = np.abs(got - ref)
+    assert np.all(err <= tol), (np.nanmax(err / tol), np.argwhere(~(err <= tol))[:3])
