@@ -313,14 +313,14 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
       if (lane == 0) mbar_arrive_expect_tx(full + s, bytes);
       __syncwarp();
       if (lane < 2 * kStepBoxes) {
-        const int blk = good ? cell : 0;  // a bad slot loads block 0 under scale 0: zeros
         if (in_keys) {
+          // a bad slot's box lies before the cache, which TMA fills with zeros
           tma_load_2d(smem + s * L::kStage + code_off, map, 0,
-                      (blk * p.kv_heads + unit.head) * bs + (tok & (bs - 1)), full + s);
+                      good ? (cell * p.kv_heads + unit.head) * bs + (tok & (bs - 1)) : -kBox, full + s);
           if (!good) atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
         }
         float* dst = scale_s + s * 16 + lane;
-        if (good) cp_async4(dst, scales + (int64_t)blk * p.kv_heads + unit.head);
+        if (good) cp_async4(dst, scales + (int64_t)cell * p.kv_heads + unit.head);
         else *dst = 0.f;
         cp_async_mbar_arrive(full + s);
       }

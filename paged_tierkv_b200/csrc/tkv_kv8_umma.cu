@@ -534,9 +534,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       cell = seen ? p.table[w.u.req * p.table_stride + (tok >> bs_log2)] : 0;
       const bool good = cell >= 0 && cell < p.blocks;
       if (seen && !good) atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
-      // a bad slot loads block 0's codes under scale 0
       ks = vs = 0.f;
-      if (!good) cell = 0;
+      if (!good) cell = -1;
       else if (seen) {
         ks = p.k_scale[(int64_t)cell * p.kv_heads + head];
         vs = p.v_scale[(int64_t)cell * p.kv_heads + head];
@@ -574,7 +573,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       // a box's block: that of its first group with keys
       const int src = box_grp + (load_box ? __ffs(live >> box_grp & mask) - 1 : 0);
       const int blk = __shfl_sync(~0u, cell, src);
-      const int y = ((blk * p.kv_heads + head) << bs_log2) + ((box_grp * 16) & (p.block_size - 1));
+      // a bad slot's box lies before the cache, which TMA fills with zeros
+      const int y = blk < 0 ? -box : ((blk * p.kv_heads + head) << bs_log2) + ((box_grp * 16) & (p.block_size - 1));
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
         if (ok && !bounded_wait(st_empty + kv, (uint32_t)(j & 1) ^ 1)) ok = false;

@@ -116,3 +116,22 @@ def test_tiny_v_scales_leave_the_row_sums_alone(exponent, mixed, fmt, kv, ql, he
            + max(kv) * 2.0 ** -21 * biggest)
     err = np.abs(got - ref)
     assert np.all(err <= tol), (np.nanmax(err / tol), np.argwhere(~(err <= tol))[:3])
+
+
+# ---------------------------------------------------------------------------
+# blocks that are not there
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("ql", [[1, 1], [40, 70]])
+@pytest.mark.parametrize("d,bs", [(128, 16), (64, 32), (128, 64)])
+def test_cells_outside_the_cache_read_zeros_whatever_block_0_holds(ql, d, bs):
+    """Block 0 is nobody's and full of e4m3 NaN codes."""
+    kv = [4 * bs + 5, 150]
+    rng = np.random.default_rng(31)
+    kc, ks, vc, vs, table, cu, q = _scene(rng, kv, ql, 2, 1, d, bs, "e4m3", "fp16")
+    table = table + 1
+    kc, vc = (np.concatenate([np.full_like(x[:1], 0x7F), x]) for x in (kc, vc))
+    ks, vs = (np.concatenate([np.ones_like(x[:1]), x]) for x in (ks, vs))
+    table[0, 2], table[1, 0] = -1, kc.shape[0]
+    _check_attention((kc, ks, vc, vs, table, cu, q), kv, bs, "e4m3", "fp16", 0.09)
+    assert _errors() == 1
