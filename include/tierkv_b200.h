@@ -457,7 +457,8 @@ int32_t tkv_kv8_plan_step(const tkv_kv8_plan_args* args, void* stream);
  * after the other, or with `interleave` f belongs to axis f % axes while f /
  * axes < sections[f % axes] and to axis 0 otherwise.  Elements past rot_dim
  * pass through.  Positions outside [0, rows) are clamped and recorded
- * (TKV_DEVERR_BAD_POS). */
+ * (TKV_DEVERR_BAD_POS); -1, which tkv_kv8_plan_step leaves past the last token,
+ * is clamped and not recorded. */
 typedef struct tkv_rotary {
     const float* cos_sin;          /* [rows, rot_dim], 16-byte aligned */
     const void*  positions;        /* [axes, tokens] int32 or int64 */

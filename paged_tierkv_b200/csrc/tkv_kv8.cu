@@ -354,7 +354,7 @@ __device__ __forceinline__ int64_t load_position(const RotaryArgs& r, int axis, 
   const int64_t p = r.positions_bytes == 8 ? reinterpret_cast<const int64_t*>(r.positions)[at]
                                            : (int64_t)reinterpret_cast<const int32_t*>(r.positions)[at];
   if (p >= 0 && p < r.rows) return p;
-  if (err) atomicOr(err, TKV_DEVERR_BAD_POS);
+  if (p != -1 && err) atomicOr(err, TKV_DEVERR_BAD_POS);   // -1: a step's padding
   return p < 0 ? 0 : r.rows - 1;
 }
 

@@ -366,7 +366,8 @@ def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torc
     """Rotates q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim]
     (fp16 / bf16, any 16-byte aligned token and head strides; either may be
     None) by their tokens' positions [axes, tokens]; returns (q_out, k_out).
-    An output may be its input."""
+    An output may be its input.  Position -1 (a step's padding) counts as 0;
+    others outside the table are clamped too, and recorded."""
     if stream is not None:
         return _on_stream(stream, rotary_embed, q, k, positions, rotary, q_out=q_out, k_out=k_out)
     qv = kv = qov = kov = _NO_VIEW

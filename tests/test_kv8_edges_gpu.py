@@ -135,3 +135,45 @@ def test_cells_outside_the_cache_read_zeros_whatever_block_0_holds(ql, d, bs):
     table[0, 2], table[1, 0] = -1, kc.shape[0]
     _check_attention((kc, ks, vc, vs, table, cu, q), kv, bs, "e4m3", "fp16", 0.09)
     assert _errors() == 1
+
+
+# ---------------------------------------------------------------------------
+# error bits
+# ---------------------------------------------------------------------------
+
+def _step(new, free, bs=16, capacity=None, width=4):
+    """A plan over an empty cache of ``free`` blocks, and a batch for it."""
+    from paged_tierkv_b200 import kv8
+    tokens = capacity or sum(new)
+    cache = kv8.Kv8Cache.allocate(max(free, 1), 1, bs, 64, "cuda")
+    plan = kv8.StepPlan.allocate(len(new), tokens, bs, "cuda")
+    kv8.plan_step(plan, _i32([0] * len(new)), _i32(new), torch.full((len(new), width), -1, dtype=torch.int32, device="cuda"),
+                  _i32(np.arange(free)), _i32([free]))
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(tokens, 1, 64, generator=gen, device="cuda").half()
+    return cache, plan, x
+
+
+@pytest.mark.parametrize("axes", [1, 3])
+@pytest.mark.parametrize("wide", [False, True])
+def test_padding_tokens_are_no_error(axes, wide):
+    """A step padded to a fixed number of tokens: positions past the last token
+    are -1, which every operator takes without an error; others still count."""
+    from paged_tierkv_b200 import kv8
+    cache, plan, x = _step([10, 3], free=2, capacity=20)
+    angle = torch.rand(16, 32, device="cuda")
+    rotary = kv8.Rotary(torch.cat([angle.cos(), angle.sin()], 1), (32,) if axes == 1 else (10, 11, 11))
+    pos = plan.positions.expand(axes, -1)
+    pos = pos.long() if wide else pos
+    q = kv8.append(cache, plan, x, x, q=x, positions=pos, rotary=rotary)
+    both = kv8.rotary_embed(x, x, pos, rotary)
+    assert torch.equal(both[0], q) and torch.equal(both[1], q)
+    kv8.attention(q, cache, plan, 0.125)
+    assert _errors() == 0
+    for bad in (-2, 16):
+        pos = pos.clone()
+        pos[:, 12] = bad
+        kv8.append(cache, plan, x, x, q=x, positions=pos, rotary=rotary)
+        assert _errors() == 8
+        kv8.rotary_embed(x, None, pos, rotary)
+        assert _errors() == 8
