@@ -172,7 +172,8 @@ class TieredPools:
 
 
 # ---------------------------------------------------------------------------
-# workspace: one zero-filled buffer per (device, stream), grown on demand
+# workspace: one zero-filled buffer per (device, stream), grown on demand; its
+# first word collects the stream's device errors and moves along
 # ---------------------------------------------------------------------------
 _WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 
@@ -181,8 +182,11 @@ def workspace_for(device: torch.device, stream_handle: int, nbytes: int) -> torc
     key = (device.index if device.index is not None else torch.cuda.current_device(), stream_handle)
     ws = _WORKSPACES.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
-        _WORKSPACES[key] = ws
+        with torch.cuda.device(key[0]), torch.cuda.stream(torch.cuda.ExternalStream(stream_handle)):
+            new = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
+            if ws is not None:
+                new[:4].copy_(ws[:4])
+        _WORKSPACES[key] = ws = new
     return ws
 
 
@@ -364,7 +368,7 @@ class DeviceErrorWatch:
         self.period = max(1, int(period))
         self.what = what
         self._host = None
-        self._slots: list = []      # (event, slot index, call number, error word)
+        self._slots: list = []      # (event, slot index, call number, error word, workspace key)
         self._next_slot = 0
         self.calls = 0
 
@@ -374,6 +378,7 @@ class DeviceErrorWatch:
             return
         if self._host is None:
             self._host = torch.zeros(self.depth, dtype=torch.int32).pin_memory()
+        key = (word.device.index, _stream(None, word.device.index).value or 0)
         if len(self._slots) >= self.depth:   # the GPU is `depth` recorded calls behind
             self._slots[0][0].synchronize()
             self.poll()
@@ -384,16 +389,18 @@ class DeviceErrorWatch:
         self._host[slot:slot + 1].copy_(word, non_blocking=True)
         ev = torch.cuda.Event()
         ev.record()
-        self._slots.append((ev, slot, self.calls, word))
+        self._slots.append((ev, slot, self.calls, word, key))
 
     def poll(self) -> None:
         if not self._slots or torch.cuda.is_current_stream_capturing():
             return  # event queries are not permitted while a graph is captured
         while self._slots and self._slots[0][0].query():
-            _, slot, call, word = self._slots.pop(0)
+            _, slot, call, word, key = self._slots.pop(0)
             bits = int(self._host[slot])
             if bits:
                 word.zero_()
+                if key in _WORKSPACES:       # a workspace that has grown since took the bits along
+                    _WORKSPACES[key][:4].zero_()
                 self._slots.clear()
                 raise TierKVDeviceError(bits, call, self.what)
 

@@ -177,3 +177,40 @@ def test_padding_tokens_are_no_error(axes, wide):
         assert _errors() == 8
         kv8.rotary_embed(x, None, pos, rotary)
         assert _errors() == 8
+
+
+def test_error_bits_survive_a_growing_workspace():
+    """The first step of a fresh stream refuses a request; attention then needs a
+    larger workspace, and after it a chunk a still larger one."""
+    from paged_tierkv_b200 import kv8, ops
+    torch.cuda.synchronize()
+    ops._WORKSPACES.clear()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        cache, plan, x = _step([10, 30], free=1)
+        kv8.append(cache, plan, x, x)
+        kv8.attention(x, cache, plan, 0.125, max_q_len=1)
+        assert ops.read_device_errors() == 4
+        kv8.plan_step(plan, _i32([0, 0]), _i32([30, 1]), torch.full((2, 4), -1, dtype=torch.int32, device="cuda"),
+                      _i32([0]), _i32([1]))
+        big = torch.zeros(200, 1, 64, dtype=torch.float16, device="cuda")
+        table = torch.zeros(1, 20, dtype=torch.int32, device="cuda")
+        kv8.attention(big, cache, kv8.StepPlan(block_size=16, block_table=table, kv_lens=_i32([200]), cu_q=_i32([0, 200])), 0.125)
+        assert ops.read_device_errors() == 4
+        assert ops.read_device_errors() == 0
+
+
+def test_one_error_is_raised_once_though_the_workspace_grows():
+    """A watch that recorded the word before the growth clears the bits after it too."""
+    from paged_tierkv_b200 import kv8, ops
+    torch.cuda.synchronize()
+    ops._WORKSPACES.clear()
+    watch = ops.DeviceErrorWatch()
+    cache, plan, x = _step([10, 30], free=1)
+    watch.record(ops.workspace_error_word())
+    kv8.attention(x, cache, plan, 0.125)
+    with pytest.raises(ops.TierKVDeviceError):
+        watch.check()
+    watch.record(ops.workspace_error_word())
+    watch.check()
+    assert ops.read_device_errors() == 0
