@@ -334,6 +334,18 @@ int32_t tkv_prefill_read_errors(uint32_t* bits_out, void* stream);
  * using this workspace have recorded.  Synchronizes the stream. */
 int32_t tkv_read_device_errors(void* workspace, uint32_t* bits_out, void* stream);
 
+/* The stream capture that `stream` is part of (CUDA's id of it), 0 outside of
+ * one.  A workspace must belong to one capture, or to none: see
+ * tkv_exchange_capture_mode. */
+int32_t tkv_stream_capture_id(void* stream, uint64_t* id_out);
+
+/* Swaps the calling thread's capture mode (cudaStreamCaptureMode) with *mode.
+ * In the relaxed mode (2) a host may allocate and zero a workspace on another
+ * stream while this one is captured: a workspace's counters must be zero before
+ * the first replay, and zeroing them as a node of one graph does not serve a
+ * second graph that shares them. */
+int32_t tkv_exchange_capture_mode(int32_t* mode);
+
 /* Decode attention for callers that cannot allocate device memory -- a serving
  * runtime that has handed (nearly) all of HBM to its own pools and forbids side
  * allocations, or a host that reaches this library only through this C ABI

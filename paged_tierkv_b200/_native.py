@@ -47,6 +47,8 @@ EXPORTED_SYMBOLS = (
     "tkv_demote_to_warm",
     "tkv_promote_to_hot",
     "tkv_read_device_errors",
+    "tkv_stream_capture_id",
+    "tkv_exchange_capture_mode",
     "tkv_decode_attention_noalloc",
     "tkv_noalloc_prepare",
     "tkv_noalloc_read_device_errors",
@@ -296,6 +298,8 @@ def load(build_if_missing: bool = False) -> ctypes.CDLL:
         "tkv_demote_to_warm": ([ctypes.POINTER(TkvPools), vp, vp, vp, i32, i32, vp], i32),
         "tkv_promote_to_hot": ([ctypes.POINTER(TkvPools), vp, vp, vp, i32, vp], i32),
         "tkv_read_device_errors": ([vp, ctypes.POINTER(ctypes.c_uint32), vp], i32),
+        "tkv_stream_capture_id": ([vp, ctypes.POINTER(ctypes.c_uint64)], i32),
+        "tkv_exchange_capture_mode": ([ctypes.POINTER(i32)], i32),
         "tkv_decode_attention_noalloc": ([ctypes.POINTER(TkvPools), ctypes.POINTER(TkvDecodeArgs),
                                           vp], i32),
         "tkv_noalloc_prepare": ([i32], i32),

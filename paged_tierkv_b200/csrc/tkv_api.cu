@@ -821,6 +821,24 @@ int32_t tkv_read_device_errors(void* workspace, uint32_t* bits_out, void* stream
   return TKV_OK;
 }
 
+int32_t tkv_stream_capture_id(void* stream, uint64_t* id_out) {
+  if (!id_out) return TKV_ERR_INVALID;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess)
+    return TKV_ERR_CUDA;
+  *id_out = status == cudaStreamCaptureStatusNone ? 0 : id;
+  return TKV_OK;
+}
+
+int32_t tkv_exchange_capture_mode(int32_t* mode) {
+  if (!mode || *mode < cudaStreamCaptureModeGlobal || *mode > cudaStreamCaptureModeRelaxed) return TKV_ERR_INVALID;
+  cudaStreamCaptureMode m = static_cast<cudaStreamCaptureMode>(*mode);
+  if (cudaThreadExchangeStreamCaptureMode(&m) != cudaSuccess) return TKV_ERR_CUDA;
+  *mode = static_cast<int32_t>(m);
+  return TKV_OK;
+}
+
 }  // extern "C"
 
 // ---------------------------------------------------------------------------

@@ -293,16 +293,13 @@ def _on_stream(stream, fn, *args, **kwargs):
         return fn(*args, **kwargs)
 
 
-_CURRENT_DEVICE = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
-
-
 def _launch(index: int, fn):
     """fn(stream handle, its workspace) with device ``index`` current."""
-    if index != _CURRENT_DEVICE():
+    if index != ops._CURRENT_DEVICE():
         with torch.cuda.device(index):
             return _launch(index, fn)
     st = ops._RAW_STREAM(index) if ops._RAW_STREAM is not None else torch.cuda.current_stream().cuda_stream
-    ws = ops._WORKSPACES.get((index, st))
+    ws = None if ops._CAPTURING() else ops._WORKSPACES.get((index, st))
     return fn(st, ws if ws is not None else ops.workspace_for(torch.device("cuda", index), st, 1 << 16))
 
 

@@ -173,21 +173,79 @@ class TieredPools:
 
 # ---------------------------------------------------------------------------
 # workspace: one zero-filled buffer per (device, stream), grown on demand; its
-# first word collects the stream's device errors and moves along
+# first word collects the stream's device errors and moves along.  Calls that a
+# CUDA graph captures have workspaces of their own, one per capture and stream:
+# replays then share no counter with eager calls or with other graphs, whatever
+# the order and the streams they run on.
 # ---------------------------------------------------------------------------
 _WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
+# (device, stream, capture id) -> its workspaces, the largest last; kept because
+# nothing tells when a graph is gone
+_GRAPH_WORKSPACES: dict[tuple[int, int, int], list[torch.Tensor]] = {}
+_CAPTURING = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+_CURRENT_DEVICE = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _capture_id(index: int, stream_handle: int) -> int:
+    """The graph capture that calls on this stream belong to, 0 outside of one."""
+    if (not _CAPTURING() and _RAW_STREAM is not None
+            and index == _CURRENT_DEVICE() and stream_handle == _RAW_STREAM(index)):
+        return 0
+    capture = ctypes.c_uint64()
+    N.check(N.load().tkv_stream_capture_id(stream_handle, ctypes.byref(capture)), "tkv_stream_capture_id")
+    return capture.value
+
+
+def _zeros_during_capture(device: torch.device, nbytes: int) -> torch.Tensor:
+    """Zeros that are there before any replay: filled on a stream outside of the
+    capture, in memory that is not the graph's."""
+    lib, mode = N.load(), ctypes.c_int32(2)            # cudaStreamCaptureModeRelaxed
+    N.check(lib.tkv_exchange_capture_mode(ctypes.byref(mode)), "tkv_exchange_capture_mode")
+    try:
+        side = torch.cuda.Stream(device)
+        while _capture_id(device.index, side.cuda_stream):   # torch hands out a few streams in turn
+            side = torch.cuda.Stream(device)
+        with torch.cuda.stream(side):
+            buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        side.synchronize()
+    finally:
+        N.check(lib.tkv_exchange_capture_mode(ctypes.byref(mode)), "tkv_exchange_capture_mode")
+    return buf
+
+
+def stream_workspace(index: int, stream_handle: int) -> torch.Tensor | None:
+    """The workspace that calls on this stream use now, if there is one."""
+    capture = _capture_id(index, stream_handle)
+    if not capture:
+        return _WORKSPACES.get((index, stream_handle))
+    held = _GRAPH_WORKSPACES.get((index, stream_handle, capture))
+    return held[-1] if held else None
 
 
 def workspace_for(device: torch.device, stream_handle: int, nbytes: int) -> torch.Tensor:
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream_handle)
-    ws = _WORKSPACES.get(key)
-    if ws is None or ws.numel() < nbytes:
-        with torch.cuda.device(key[0]), torch.cuda.stream(torch.cuda.ExternalStream(stream_handle)):
-            new = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
-            if ws is not None:
-                new[:4].copy_(ws[:4])
-        _WORKSPACES[key] = ws = new
-    return ws
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    ws = stream_workspace(index, stream_handle)
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
+    nbytes = max(nbytes, 1 << 16)
+    capture = _capture_id(index, stream_handle)
+    if capture:
+        new = _zeros_during_capture(torch.device("cuda", index), nbytes)
+        _GRAPH_WORKSPACES.setdefault((index, stream_handle, capture), []).append(new)
+        return new
+    with torch.cuda.device(index), torch.cuda.stream(torch.cuda.ExternalStream(stream_handle)):
+        new = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        if ws is not None:
+            new[:4].copy_(ws[:4])
+    _WORKSPACES[index, stream_handle] = new
+    return new
+
+
+def release_graph_workspaces(device: int | None = None) -> None:
+    """Frees the workspaces of captured calls (of one device, or all).  Only once
+    every graph that holds such calls has been destroyed."""
+    for key in [k for k in _GRAPH_WORKSPACES if device is None or k[0] == device]:
+        del _GRAPH_WORKSPACES[key]
 
 
 def _as_table(t: torch.Tensor, batch: int, name: str) -> torch.Tensor:
@@ -280,7 +338,7 @@ def decode_attention(query: torch.Tensor, block_table: torch.Tensor, block_state
         int(chunk_blocks), None, 0)
     # The stream's workspace usually fits already; the plan (and a larger
     # workspace) is only needed when the library reports that it does not.
-    ws = _WORKSPACES.get((dev_index, st.value or 0))
+    ws = stream_workspace(dev_index, st.value or 0)
     for attempt in range(2):
         if ws is None or attempt:
             splits = ctypes.c_int32()
@@ -411,14 +469,19 @@ class DeviceErrorWatch:
 
 
 def read_device_errors(device=None, stream=None) -> int:
-    """Read and clear the device error bits of the current stream's workspace."""
+    """Read and clear the device error bits of the current stream's workspace, and
+    those that replayed graphs have recorded on the device (whole once the
+    replays have completed)."""
     st = _stream(stream)
     dev = torch.device("cuda", torch.cuda.current_device() if device is None else device)
-    ws = workspace_for(dev, st.value or 0, 1 << 16)
-    bits = ctypes.c_uint32()
-    N.check(N.load().tkv_read_device_errors(ws.data_ptr(), ctypes.byref(bits), st),
-            "tkv_read_device_errors")
-    return int(bits.value)
+    found = 0
+    held = [ws for key, kept in _GRAPH_WORKSPACES.items() if key[0] == dev.index for ws in kept]
+    for ws in (workspace_for(dev, st.value or 0, 1 << 16), *held):
+        bits = ctypes.c_uint32()
+        N.check(N.load().tkv_read_device_errors(ws.data_ptr(), ctypes.byref(bits), st),
+                "tkv_read_device_errors")
+        found |= bits.value
+    return int(found)
 
 
 def read_prefill_errors(stream=None) -> int:

@@ -214,3 +214,118 @@ def test_one_error_is_raised_once_though_the_workspace_grows():
     watch.record(ops.workspace_error_word())
     watch.check()
     assert ops.read_device_errors() == 0
+
+
+# ---------------------------------------------------------------------------
+# graphs
+# ---------------------------------------------------------------------------
+
+def _decode(seed, kv=(3000, 17, 900), ql=(1, 1, 1)):
+    """(call, expected output): units split over CTAs, so that the arrival
+    counters of the workspace are used."""
+    from paged_tierkv_b200 import kv8
+    rng = np.random.default_rng(seed)
+    kc, ks, vc, vs, table, cu, q = scene = _scene(rng, list(kv), list(ql), 4, 2, 128, 16, "int8", "fp16")
+    want, _ = _attend(scene, list(kv), 16, "int8", 0.09)
+    cache = kv8.Kv8Cache(*(torch.from_numpy(x).cuda() for x in (kc, vc, ks, vs)))
+    plan = kv8.StepPlan(block_size=16, block_table=_i32(table), kv_lens=_i32(kv), cu_q=_i32(cu))
+    return (lambda: kv8.attention(q, cache, plan, 0.09)), want
+
+
+def _captured(call, stream=None):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        out = call()
+    return g, out
+
+
+@pytest.mark.parametrize("cold", [False, True])
+def test_graphs_of_one_stream_replay_in_any_order(cold):
+    from paged_tierkv_b200 import ops
+    calls = [_decode(40), _decode(41, (2500, 300), (1, 30))]
+    torch.cuda.synchronize()
+    if cold:                                   # the captures come before any call on their stream
+        ops._WORKSPACES.clear()
+    graphs = [_captured(call) for call, _ in calls]
+    for i in (1, 0, 0, 1, 1):
+        graphs[i][1].zero_()
+        graphs[i][0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[i][1], calls[i][1])
+
+
+def test_a_graph_keeps_its_workspace_when_the_stream_needs_a_larger_one():
+    from paged_tierkv_b200 import ops
+    side = torch.cuda.Stream()
+    (decode, want), (chunk, want_chunk) = _decode(42), _decode(43, (400, 900), (60, 200))
+    torch.cuda.synchronize()
+    ops._WORKSPACES.clear()
+    with torch.cuda.stream(side):
+        decode()
+    g, out = _captured(decode, side)
+    with torch.cuda.stream(side):
+        assert torch.equal(chunk(), want_chunk)
+        filler = [torch.full((n,), 77, dtype=torch.uint8, device="cuda") for n in [1 << 16, 1 << 20, 2 << 20, 3 << 20] * 8]
+        for _ in range(3):
+            out.zero_()
+            g.replay()
+            side.synchronize()
+            assert torch.equal(out, want)
+        assert all(bool((f == 77).all()) for f in filler)
+        assert torch.equal(decode(), want)
+
+
+def test_graphs_replay_beside_one_another():
+    calls = [_decode(44), _decode(45), _decode(46, (1800, 800), (40, 1))]
+    graphs = [_captured(call) for call, _ in calls]
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(50):
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for (_, out), (_, want) in zip(graphs, calls):
+        assert torch.equal(out, want)
+
+
+def test_tiered_decode_graphs_replay_in_any_order():
+    from paged_tierkv_b200 import ops
+    from tierkv_cases import make_case, to_device
+    cases = [make_case(seed=s, batch=2, q_heads=32, kv_heads=8, head_dim=128, num_blocks=70, max_blocks=72) for s in (1, 2)]
+    data = [to_device(c) for c in cases]
+
+    def call(c, d):
+        return ops.decode_attention(d["query"], d["block_table"], d["block_states"], d["block_lengths"], d["pools"],
+                                    d["num_blocks"], c["groups"], c["scaling"], num_splits=6)[0]
+    want = [call(c, d) for c, d in zip(cases, data)]
+    torch.cuda.synchronize()
+    ops._WORKSPACES.clear()
+    graphs = [_captured(lambda c=c, d=d: call(c, d)) for c, d in zip(cases, data)]
+    for i in (1, 0, 1):
+        graphs[i][1].zero_()
+        graphs[i][0].replay()
+        torch.cuda.synchronize()
+        assert torch.allclose(graphs[i][1].float(), want[i].float(), atol=2e-3)
+
+
+def test_errors_of_replays_are_read():
+    from paged_tierkv_b200 import kv8, ops
+    cache = kv8.Kv8Cache.allocate(4, 1, 16, 64, "cuda")
+    table = _i32([[0, 9]])
+    plan = kv8.StepPlan(block_size=16, block_table=table, kv_lens=_i32([20]), cu_q=_i32([0, 1]))
+    q = torch.zeros(1, 1, 64, dtype=torch.float16, device="cuda")
+    assert _errors() == 0
+    g, _ = _captured(lambda: kv8.attention(q, cache, plan, 0.1))
+    assert _errors() == 0
+    g.replay()
+    g.replay()
+    torch.cuda.synchronize()
+    assert _errors() == 1 and _errors() == 0
+    table[0, 1] = 2
+    g.replay()
+    torch.cuda.synchronize()
+    assert _errors() == 0
+    del g
+    ops.release_graph_workspaces()
+    assert not ops._GRAPH_WORKSPACES and _errors() == 0
