@@ -122,8 +122,12 @@ class StepPlan:
             t = getattr(self, name)
             if t is not None and (t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous int32 CUDA tensor.")
-        if units is not None and (units.ndim != 2 or units.shape[1] != 4 or num_units is None):
+        if units is not None and (units.ndim != 2 or units.shape[1] != 4 or num_units is None or num_units.numel() != 1):
             raise ValueError("units must be [count, 4] beside num_units [1].")
+        devices = {t.get_device() for t in (units, num_units, block_table, kv_lens, cu_q) if t is not None}
+        if len(devices) > 1:
+            raise ValueError("a plan's tensors must be on one device.")
+        self._index = devices.pop() if devices else None
         if block_table is not None:
             if kv_lens is None or cu_q is None:
                 raise ValueError("a block_table needs kv_lens and cu_q.")
@@ -372,6 +376,8 @@ def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torc
     if q is not None:
         code, index = _heads3(q, "q")
         tokens, heads, d = q.shape
+        if index != rotary._head[2]:
+            raise ValueError("q must be on the cos / sin table's device.")
         q_out, qov = _output_view(q_out, q, tokens, heads, "q_out")
         qv, q = _input_view(q, tokens, heads)
     elif k is None:
@@ -379,6 +385,8 @@ def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torc
     if k is not None:
         k_code, k_index = _heads3(k, "k")
         n, kv_heads, dk = k.shape
+        if k_index != rotary._head[2]:
+            raise ValueError("k must be on the cos / sin table's device.")
         if q is None:
             code, index, tokens, d = k_code, k_index, n, dk
         elif n != tokens or dk != d or k_code != code or k_index != index:
@@ -416,12 +424,14 @@ def append(cache: Kv8Cache, plan: StepPlan, k: torch.Tensor, v: torch.Tensor, *,
         raise ValueError("k and v must have shape [tokens, kv_heads, head_dim] of the cache and one dtype.")
     if index != cache._index or v.get_device() != index:
         raise ValueError("k and v must be on the cache's device.")
-    if plan.units is None or plan.block_size != cache.block_size:
-        raise ValueError("append needs a plan with write units of the cache's block size.")
+    if plan.units is None or plan.block_size != cache.block_size or plan._index != index:
+        raise ValueError("append needs a plan with write units of the cache's block size, on its device.")
     rot, qv, qov, heads = _NO_ROTARY, _NO_VIEW, _NO_VIEW, 0
     if rotary is not None:
         if positions is None:
             raise ValueError("rotary needs the tokens' positions.")
+        if rotary._head[2] != index:
+            raise ValueError("the cos / sin table must be on the cache's device.")
         rot, positions = rotary._at(positions, tokens)
     elif q is not None:
         raise ValueError("q is rotated only: pass rotary and positions beside it.")
@@ -470,8 +480,8 @@ def attention(q: torch.Tensor, cache: Kv8Cache, plan: StepPlan, scaling: float, 
     if d != cache.head_dim or index != cache._index or heads % cache.kv_heads:
         raise ValueError("q must match the cache in head_dim and device, and heads be a multiple of kv_heads.")
     table = plan.block_table
-    if table is None or plan.block_size != cache.block_size:
-        raise ValueError("attention needs a plan with block tables of the cache's block size.")
+    if table is None or plan.block_size != cache.block_size or plan._index != index:
+        raise ValueError("attention needs a plan with block tables of the cache's block size, on its device.")
     if out is None:
         out = torch.empty_like(q, memory_format=_CONTIGUOUS)
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous() \

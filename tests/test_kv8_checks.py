@@ -1,0 +1,87 @@
+"""Checks of the 8-bit cache's front end that need no GPU: tensors are stand-ins
+with a device, a type and a shape, and nothing is launched."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from paged_tierkv_b200 import kv8  # noqa: E402
+
+
+class FakeTensor:
+    """What the checks read of a CUDA tensor."""
+
+    def __init__(self, *shape, dtype=torch.int32, device=0, at=0x1000):
+        self.shape, self.ndim, self.dtype, self._device, self._at = torch.Size(shape), len(shape), dtype, device, at
+        self.is_cuda, self.device, self.requires_grad = True, torch.device("cuda", device), False
+
+    def get_device(self):
+        return self._device
+
+    def numel(self):
+        return self.shape.numel()
+
+    def is_contiguous(self):
+        return True
+
+    def stride(self):
+        s, out = 1, []
+        for n in reversed(self.shape):
+            out.append(s)
+            s *= n
+        return tuple(reversed(out))
+
+    def data_ptr(self):
+        return self._at
+
+
+def _never(*_):
+    raise AssertionError("launched")
+
+
+def _cache(device=0):
+    codes, scale = (FakeTensor(4, 2, 16, 64, dtype=torch.int8, device=device), FakeTensor(4, 2, dtype=torch.float32, device=device))
+    return kv8.Kv8Cache(codes, codes, scale, scale)
+
+
+def _plan(device=0, **other):
+    t = {"units": FakeTensor(3, 4), "num_units": FakeTensor(1), "block_table": FakeTensor(1, 2), "kv_lens": FakeTensor(1),
+         "cu_q": FakeTensor(2)}
+    for name, x in t.items():
+        x._device = other.get(name, device)
+    return kv8.StepPlan(block_size=16, **t)
+
+
+@pytest.mark.parametrize("name", ["units", "num_units", "block_table", "kv_lens", "cu_q"])
+def test_a_plan_lives_on_one_device(name):
+    _plan(1)
+    with pytest.raises(ValueError, match="one device"):
+        _plan(0, **{name: 1})
+
+
+def test_num_units_is_one_number():
+    with pytest.raises(ValueError, match="num_units"):
+        kv8.StepPlan(block_size=16, units=FakeTensor(3, 4), num_units=FakeTensor(2))
+    with pytest.raises(ValueError, match="num_units"):
+        kv8.StepPlan(block_size=16, units=FakeTensor(3, 4), num_units=FakeTensor(0))
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    monkeypatch.setattr(kv8, "_launch", _never)
+    half = {"dtype": torch.float16}
+    x, kv, pos = FakeTensor(3, 4, 64, **half), FakeTensor(3, 2, 64, **half), FakeTensor(3)
+    there = kv8.Rotary(FakeTensor(8, 64, dtype=torch.float32, device=1))
+    pos_there = FakeTensor(3, device=1)
+    for call in (lambda: kv8.append(_cache(), _plan(1), kv, kv),
+                 lambda: kv8.append(_cache(), _plan(0), kv, kv, q=x, positions=pos_there, rotary=there, q_out=x),
+                 lambda: kv8.append(_cache(1), _plan(1), kv, kv),
+                 lambda: kv8.attention(x, _cache(), _plan(1), 0.1, out=x),
+                 lambda: kv8.attention(x, _cache(1), _plan(1), 0.1, out=x),
+                 lambda: kv8.rotary_embed(x, None, pos_there, there, q_out=x),
+                 lambda: kv8.rotary_embed(None, kv, pos_there, there, k_out=kv),
+                 lambda: kv8.rotary_embed(x, None, pos, there, q_out=x)):
+        with pytest.raises(ValueError, match="device"):
+            call()
+    for call in (lambda: kv8.append(_cache(), _plan(0), kv, kv), lambda: kv8.attention(x, _cache(), _plan(0), 0.1, out=x)):
+        with pytest.raises(AssertionError, match="launched"):
+            call()
