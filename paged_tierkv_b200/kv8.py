@@ -21,6 +21,7 @@ reference has no counterpart: its 8-bit blocks are filled by demotion only.
 from __future__ import annotations
 
 import ctypes
+import operator
 import struct
 from dataclasses import dataclass
 
@@ -52,10 +53,17 @@ _CONTIGUOUS = torch.contiguous_format
 # handles
 # ---------------------------------------------------------------------------
 
+def _held(name: str) -> property:
+    """A tensor that calls use by its address: it can be written, not exchanged."""
+    return property(operator.attrgetter("_" + name))
+
+
 class Kv8Cache:
     """One layer's 8-bit cache: k_codes / v_codes [blocks, kv_heads, block_size,
     head_dim] int8 or float8_e4m3fn, k_scale / v_scale [blocks, kv_heads] fp32;
     value = code * scale.  block_size 16, 32 or 64; head_dim 64 or 128."""
+
+    k_codes, v_codes, k_scale, v_scale = map(_held, ("k_codes", "v_codes", "k_scale", "v_scale"))
 
     def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
                  v_scale: torch.Tensor):
@@ -71,7 +79,7 @@ class Kv8Cache:
         for t in (k_codes, v_codes, k_scale, v_scale):
             if not t.is_contiguous() or t.device != k_codes.device:
                 raise ValueError("cache tensors must be contiguous and on one device.")
-        self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
+        self._k_codes, self._v_codes, self._k_scale, self._v_scale = k_codes, v_codes, k_scale, v_scale
         self.blocks, self.kv_heads, self.block_size, self.head_dim = (int(x) for x in k_codes.shape)
         self.device, self._index = k_codes.device, k_codes.get_device()
         # the tensors are held, so the addresses stay theirs
@@ -110,12 +118,16 @@ class StepPlan:
     (block, first token, row offset, rows; -1 past the last), num_units [1],
     free_count [1]; all int32."""
 
+    kv_lens, cu_q, admitted, slot_map, token_request, positions, units, num_units, free_count, block_table = map(
+        _held, ("kv_lens", "cu_q", "admitted", "slot_map", "token_request", "positions", "units", "num_units",
+                "free_count", "block_table"))
+
     def __init__(self, *, block_size: int, units=None, num_units=None, block_table=None, kv_lens=None,
                  cu_q=None):
         self.block_size = int(block_size)
-        self.units, self.num_units = units, num_units
-        self.block_table, self.kv_lens, self.cu_q = block_table, kv_lens, cu_q
-        self.admitted = self.slot_map = self.token_request = self.positions = self.free_count = None
+        self._units, self._num_units = units, num_units
+        self._block_table, self._kv_lens, self._cu_q = block_table, kv_lens, cu_q
+        self._admitted = self._slot_map = self._token_request = self._positions = self._free_count = None
         self.requests = 0
         self._outputs = None
         for name in ("units", "num_units", "kv_lens", "cu_q"):
@@ -154,9 +166,9 @@ class StepPlan:
             at += (n + 3) // 4 * 4
         units, slot, req, pos, kv, adm, cu, num, free = parts
         plan = cls(block_size=block_size, units=units.view(cap, 4), num_units=num)
-        plan.kv_lens, plan.cu_q = kv, cu
-        plan.slot_map, plan.token_request, plan.positions = slot, req, pos
-        plan.admitted, plan.free_count = adm, free
+        plan._kv_lens, plan._cu_q = kv, cu
+        plan._slot_map, plan._token_request, plan._positions = slot, req, pos
+        plan._admitted, plan._free_count = adm, free
         plan._outputs = tuple(x.data_ptr() for x in (kv, cu, adm, slot, req, pos, units, num, free))
         plan.device, plan._index = buf.device, buf.get_device()
         plan._caps = (r, t, cap)
@@ -358,7 +370,7 @@ def plan_step(plan: StepPlan, context_lens: torch.Tensor, new_lens: torch.Tensor
     status = _launch(index, call)
     if status:
         N.check(status, "tkv_kv8_plan_step")
-    plan.block_table, plan.requests = block_table, n
+    plan._block_table, plan.requests = block_table, n
     return plan
 
 

@@ -85,3 +85,16 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
     for call in (lambda: kv8.append(_cache(), _plan(0), kv, kv), lambda: kv8.attention(x, _cache(), _plan(0), 0.1, out=x)):
         with pytest.raises(AssertionError, match="launched"):
             call()
+
+
+def test_tensors_whose_addresses_are_kept_cannot_be_exchanged():
+    cache, plan = _cache(), _plan()
+    for holder, names in ((cache, ("k_codes", "v_codes", "k_scale", "v_scale")),
+                          (plan, ("kv_lens", "cu_q", "admitted", "slot_map", "token_request", "positions", "units",
+                                  "num_units", "free_count", "block_table"))):
+        for name in names:
+            with pytest.raises(AttributeError):
+                setattr(holder, name, None)
+    rotary = kv8.Rotary(FakeTensor(8, 64, dtype=torch.float32))
+    with pytest.raises(AttributeError):
+        rotary.cos_sin = None
