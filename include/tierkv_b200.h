@@ -99,6 +99,7 @@ extern "C" {
 #define TKV_DEVERR_TIMEOUT   0x2u  /* a bounded pipeline wait gave up            */
 #define TKV_DEVERR_NO_BLOCKS 0x4u  /* a planned request found no free block or no table room */
 #define TKV_DEVERR_BAD_POS   0x8u  /* rotary position outside the cos / sin table (clamped) */
+#define TKV_DEVERR_DROPPED   0x10u /* a planned step has more tokens than its outputs hold */
 
 /* tkv_decode_args.flags: blocks per work chunk (0 = chosen by the planner) */
 #define TKV_FLAG_CHUNK_MASK  0xff
@@ -451,7 +452,9 @@ typedef struct tkv_kv8_plan_args {
     int32_t*       free_count_out; /* [1] */
     uint32_t*      error_word;     /* optional */
     int32_t        requests;       /* 1 .. TKV_KV8_MAX_REQUESTS */
-    int32_t        tokens;         /* capacity of the token outputs; tokens past it are dropped */
+    int32_t        tokens;         /* capacity of the token outputs; tokens past it are dropped
+                                      (0: none wanted; else recorded, TKV_DEVERR_DROPPED: they
+                                      count in kv_lens, but nothing will write them) */
     int32_t        units_cap;      /* min(tokens, tokens / block_size + 2 * requests) suffices */
     int32_t        table_width;    /* cells of a row that may be used */
     int32_t        free_capacity;

@@ -31,6 +31,7 @@ TKV_DEVERR_BAD_SLOT = 0x1
 TKV_DEVERR_TIMEOUT = 0x2
 TKV_DEVERR_NO_BLOCKS = 0x4
 TKV_DEVERR_BAD_POS = 0x8
+TKV_DEVERR_DROPPED = 0x10
 
 TKV_KV8_INT8 = 0
 TKV_KV8_E4M3 = 1

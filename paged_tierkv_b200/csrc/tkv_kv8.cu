@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       *p.free_count_out = free_count - total_taken;
     }
     if (refused && p.error_word) atomicOr(p.error_word, TKV_DEVERR_NO_BLOCKS);
+    if (tid == 0 && p.tokens > 0 && total_new > p.tokens && p.error_word) atomicOr(p.error_word, TKV_DEVERR_DROPPED);
   }
 
   // new table cells; blocks past the free list are nobody's

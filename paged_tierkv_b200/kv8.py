@@ -337,7 +337,8 @@ def plan_step(plan: StepPlan, context_lens: torch.Tensor, new_lens: torch.Tensor
     Fills ``plan`` (its buffers' first entries, for fewer requests than it was
     allocated for) and returns it.  ``plan.kv_lens`` and ``plan.free_count`` may
     be passed back as the next step's context_lens and free_count.  ``tokens``:
-    how many entries of the token outputs to write (default: all)."""
+    how many entries of the token outputs to write (default: all; 0: none are
+    wanted); a step of more tokens records ``TKV_DEVERR_DROPPED``."""
     if stream is not None:
         return _on_stream(stream, plan_step, plan, context_lens, new_lens, block_table, free_blocks, free_count,
                           tokens=tokens)

@@ -398,7 +398,8 @@ class TierKVDeviceError(N.TierKVError):
         names = [n for b, n in ((N.TKV_DEVERR_BAD_SLOT, "out-of-pool slot"),
                                 (N.TKV_DEVERR_TIMEOUT, "bounded wait timed out"),
                                 (N.TKV_DEVERR_NO_BLOCKS, "request without free blocks or table room"),
-                                (N.TKV_DEVERR_BAD_POS, "rotary position outside its table"))
+                                (N.TKV_DEVERR_BAD_POS, "rotary position outside its table"),
+                                (N.TKV_DEVERR_DROPPED, "step of more tokens than its plan holds"))
                  if self.bits & b]
         super().__init__(f"{what} call {self.call} recorded device error 0x{self.bits:x} "
                          f"({', '.join(names) or 'unknown'})")

@@ -329,3 +329,13 @@ def test_errors_of_replays_are_read():
     del g
     ops.release_graph_workspaces()
     assert not ops._GRAPH_WORKSPACES and _errors() == 0
+
+
+@pytest.mark.parametrize("tokens,bits", [(None, 0), (23, 0), (22, 16), (0, 0)])
+def test_a_step_of_more_tokens_than_its_outputs_hold_is_reported(tokens, bits):
+    """The dropped tokens are counted in kv_lens but have no slot and no unit."""
+    from paged_tierkv_b200 import kv8
+    plan = kv8.StepPlan.allocate(2, 40, 16, "cuda")
+    kv8.plan_step(plan, _i32([0, 0]), _i32([20, 3]), torch.full((2, 4), -1, dtype=torch.int32, device="cuda"),
+                  _i32(np.arange(9)), _i32([9]), tokens=tokens)
+    assert _errors() == bits
