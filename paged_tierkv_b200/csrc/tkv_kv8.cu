@@ -28,8 +28,12 @@ namespace tkv {
 // Small steps (up to 1024 requests, tokens and write units) take one CTA of 256
 // threads, whose barriers are cheaper than the cluster's; others 16 of 1024, the
 // largest cluster there is (8: 13.3 us for those 130000 tokens, 16 of 512: 10.8;
-// 2000 tokens the same).
-constexpr int kPlanCluster = 16;
+// 2000 tokens the same), or 8, which every device can place, where a part of a
+// GPU has no room for 16.
+#ifndef TKV_PLAN_CLUSTER
+#define TKV_PLAN_CLUSTER 16
+#endif
+constexpr int kPlanCluster = TKV_PLAN_CLUSTER, kPlanPortable = 8;
 constexpr int kPlanThreads = 1024, kPlanSmall = 256;
 constexpr int kPlanSmallWork = 1024;
 
@@ -246,19 +250,48 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// CTAs of the current device's plan cluster, with the kernel's opt-ins made.
+static cudaError_t plan_cluster(int* ctas) {
+  static std::atomic<int> known[kKv8MaxDevices];
+  static std::atomic<uint64_t> allowed, wide;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const bool cached = dev >= 0 && dev < kKv8MaxDevices;
+  if (cached && (*ctas = known[dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  const int smem = (int)(sizeof(int32_t) * (4 * TKV_KV8_MAX_REQUESTS + 3));
+  if ((e = allow_smem(plan_step_kernel<kPlanThreads>, smem, allowed)) != cudaSuccess) return e;
+  *ctas = kPlanPortable;
+  if (allow(plan_step_kernel<kPlanThreads>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, wide) == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kPlanCluster);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = kPlanCluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int fit = 0;
+    if (cudaOccupancyMaxActiveClusters(&fit, plan_step_kernel<kPlanThreads>, &cfg) == cudaSuccess && fit > 0)
+      *ctas = kPlanCluster;
+  }
+  cudaGetLastError();   // a size that does not fit is no error of this call
+  if (cached) known[dev].store(*ctas, std::memory_order_relaxed);
+  return cudaSuccess;
+}
+
 cudaError_t launch_plan_step(const tkv_kv8_plan_args& p, cudaStream_t stream) {
   const size_t smem = sizeof(int32_t) * (4 * (size_t)p.requests + 3);
   const bool small = p.requests <= kPlanSmallWork && p.tokens <= kPlanSmallWork && p.units_cap <= kPlanSmallWork;
+  int ctas = 1;
   if (!small) {
-    static std::atomic<uint64_t> allowed, wide;
-    cudaError_t e = allow_smem(plan_step_kernel<kPlanThreads>,
-                               (int)(sizeof(int32_t) * (4 * TKV_KV8_MAX_REQUESTS + 3)), allowed);
-    if (e == cudaSuccess)
-      e = allow(plan_step_kernel<kPlanThreads>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, wide);
+    const cudaError_t e = plan_cluster(&ctas);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(small ? 1 : kPlanCluster);
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(small ? kPlanSmall : kPlanThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
