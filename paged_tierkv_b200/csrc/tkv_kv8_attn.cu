@@ -310,6 +310,11 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
         break;
       }
       const uint32_t bytes = __popc(__ballot_sync(~0u, in_keys)) * kBox * D;
+      // zero scales are plain stores, which lane 0's arrival (a release, unlike
+      // those of the asynchronous copies) makes visible to the consumers
+      float* dst = scale_s + s * 16 + lane;
+      if (lane < 2 * kStepBoxes && !good) *dst = 0.f;
+      __syncwarp();
       if (lane == 0) mbar_arrive_expect_tx(full + s, bytes);
       __syncwarp();
       if (lane < 2 * kStepBoxes) {
@@ -319,9 +324,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
                       good ? (cell * p.kv_heads + unit.head) * bs + (tok & (bs - 1)) : -kBox, full + s);
           if (!good) atomicOr(p.err, TKV_DEVERR_BAD_SLOT);
         }
-        float* dst = scale_s + s * 16 + lane;
         if (good) cp_async4(dst, scales + (int64_t)cell * p.kv_heads + unit.head);
-        else *dst = 0.f;
         cp_async_mbar_arrive(full + s);
       }
     }
