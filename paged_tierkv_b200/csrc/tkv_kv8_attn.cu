@@ -305,7 +305,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
       const bool in_keys = tok < unit.kv && tok + kBox > any_lo && lane < 2 * kStepBoxes;
       const bool good = in_keys && cell >= 0 && cell < p.blocks;
       const int s = (int)(issued % S);
-      if (!mbar_wait(empty + s, (uint32_t)((issued / S) & 1) ^ 1)) {
+      // one lane's timeout is the warp's: the votes below want all of it
+      if (!__all_sync(~0u, mbar_wait(empty + s, (uint32_t)((issued / S) & 1) ^ 1))) {
         ok = false;
         break;
       }

@@ -577,7 +577,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int y = blk < 0 ? -box : ((blk * p.kv_heads + head) << bs_log2) + ((box_grp * 16) & (p.block_size - 1));
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
-        if (ok && !bounded_wait(st_empty + kv, (uint32_t)(j & 1) ^ 1)) ok = false;
+        // one lane's timeout is the warp's: what the boxes announce is what they load
+        ok = __all_sync(~0u, ok && bounded_wait(st_empty + kv, (uint32_t)(j & 1) ^ 1));
         if (lane == 0 && ok) mbar_arrive_expect_tx(st_full + kv, bytes);
         __syncwarp();
         if (load_box && ok)
