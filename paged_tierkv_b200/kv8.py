@@ -284,6 +284,9 @@ def _output_view(t: torch.Tensor | None, like: torch.Tensor, n: int, h: int, nam
     v = _view(t, n, h)
     if v is None:
         raise ValueError(f"{name} must be 16-byte aligned with head_dim contiguous.")
+    d = t.shape[2]
+    if n > 1 and v[1] < d or h > 1 and v[2] < d:
+        raise ValueError(f"{name} must not name one element for two tokens or heads.")
     return t, v
 
 
@@ -380,7 +383,7 @@ def rotary_embed(q: torch.Tensor | None, k: torch.Tensor | None, positions: torc
     """Rotates q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim]
     (fp16 / bf16, any 16-byte aligned token and head strides; either may be
     None) by their tokens' positions [axes, tokens]; returns (q_out, k_out).
-    An output may be its input.  Position -1 (a step's padding) counts as 0;
+    An output may be its input, but not overlap it otherwise.  Position -1 (a step's padding) counts as 0;
     others outside the table are clamped too, and recorded."""
     if stream is not None:
         return _on_stream(stream, rotary_embed, q, k, positions, rotary, q_out=q_out, k_out=k_out)

@@ -11,8 +11,9 @@ from paged_tierkv_b200 import kv8  # noqa: E402
 class FakeTensor:
     """What the checks read of a CUDA tensor."""
 
-    def __init__(self, *shape, dtype=torch.int32, device=0, at=0x1000):
+    def __init__(self, *shape, dtype=torch.int32, device=0, at=0x1000, stride=None):
         self.shape, self.ndim, self.dtype, self._device, self._at = torch.Size(shape), len(shape), dtype, device, at
+        self._stride = stride
         self.is_cuda, self.device, self.requires_grad = True, torch.device("cuda", device), False
 
     def get_device(self):
@@ -25,6 +26,8 @@ class FakeTensor:
         return True
 
     def stride(self):
+        if self._stride is not None:
+            return self._stride
         s, out = 1, []
         for n in reversed(self.shape):
             out.append(s)
@@ -98,3 +101,22 @@ def test_tensors_whose_addresses_are_kept_cannot_be_exchanged():
     rotary = kv8.Rotary(FakeTensor(8, 64, dtype=torch.float32))
     with pytest.raises(AttributeError):
         rotary.cos_sin = None
+
+
+def test_outputs_that_name_one_element_twice_are_refused(monkeypatch):
+    monkeypatch.setattr(kv8, "_launch", _never)
+    half = {"dtype": torch.float16}
+    x, pos, rotary = FakeTensor(3, 4, 64, **half), FakeTensor(3), kv8.Rotary(FakeTensor(8, 64, dtype=torch.float32))
+    for stride in ((0, 64, 1), (256, 0, 1), (32, 64, 1), (256, 32, 1)):
+        out = FakeTensor(3, 4, 64, stride=stride, **half)
+        with pytest.raises(ValueError, match="one element"):
+            kv8.rotary_embed(x, None, pos, rotary, q_out=out)
+        with pytest.raises(ValueError, match="one element"):
+            kv8.append(_cache(), _plan(), FakeTensor(3, 2, 64, **half), FakeTensor(3, 2, 64, **half), q=x, positions=pos,
+                       rotary=rotary, q_out=out)
+    for stride in ((256, 64, 1), (64, 192, 1), (1024, 128, 1)):      # packed, heads outermost, with room between
+        with pytest.raises(AssertionError, match="launched"):
+            kv8.rotary_embed(x, None, pos, rotary, q_out=FakeTensor(3, 4, 64, stride=stride, **half))
+    one = FakeTensor(1, 1, 64, stride=(0, 0, 1), **half)
+    with pytest.raises(AssertionError, match="launched"):
+        kv8.rotary_embed(one, None, pos, rotary, q_out=one)
