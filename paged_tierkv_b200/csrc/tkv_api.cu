@@ -22,11 +22,6 @@ using namespace tkv;
 
 namespace {
 
-constexpr size_t kAlign = 256;
-inline size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
-
-bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
-
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
@@ -145,24 +140,6 @@ bool encode_hot_map_3d(CUtensorMap* map, void* base, int64_t rows, int head_dim,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
-}
-
-// Workspace layout, a function of the workspace's size W alone: [0, 256) the
-// device error word, [256, 256 + R) the counters with R = W / 8 rounded down
-// to 256 bytes, then the data regions (partials, per-block LSE).  Every launch
-// returns its counters to zero and no data region reaches below 256 + R, so
-// one workspace, zero-filled once, serves calls of any shape in any order.
-inline size_t counter_reserve(size_t w) { return (w / 8) / kAlign * kAlign; }
-inline size_t data_base(size_t w) { return kAlign + counter_reserve(w); }
-inline bool layout_fits(size_t w, size_t counters, size_t data) {
-  return counter_reserve(w) >= counters && data_base(w) + data <= w;
-}
-size_t required_workspace(size_t counters, size_t data) {
-  constexpr size_t kStep = 8 * kAlign;
-  size_t w = std::max(8 * align_up(counters), (data + kAlign) * 8 / 7 + kAlign);
-  w = (w + kStep - 1) / kStep * kStep;
-  while (!layout_fits(w, counters, data)) w += kStep;
-  return w;
 }
 
 struct Plan {

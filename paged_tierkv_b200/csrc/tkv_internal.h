@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 // HOT tiles: one 3-D TMA box per K/V tile instead of head_dim/64 2-D boxes.
 #ifndef TKV_HOT_3D
 #define TKV_HOT_3D 1
@@ -32,6 +34,29 @@ constexpr int kMaxGroups = 8;      // query heads per KV head handled by one CTA
 constexpr int kMaxSplits = 512;    // split-KV partitions per (sequence, kv head)
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.442695040888963387f;
+
+inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+constexpr size_t kAlign = 256;
+inline size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+
+// Workspace layout, a function of the workspace's size W alone: [0, 256) the
+// device error word, [256, 256 + R) the counters with R = W / 8 rounded down
+// to 256 bytes, then the data regions (partials, per-block LSE).  Every launch
+// returns its counters to zero and no data region reaches below 256 + R, so
+// one workspace, zero-filled once, serves calls of any shape in any order.
+inline size_t counter_reserve(size_t w) { return (w / 8) / kAlign * kAlign; }
+inline size_t data_base(size_t w) { return kAlign + counter_reserve(w); }
+inline bool layout_fits(size_t w, size_t counters, size_t data) {
+  return counter_reserve(w) >= counters && data_base(w) + data <= w;
+}
+inline size_t required_workspace(size_t counters, size_t data) {
+  constexpr size_t kStep = 8 * kAlign;
+  size_t w = std::max(8 * align_up(counters), (data + kAlign) * 8 / 7 + kAlign);
+  w = (w + kStep - 1) / kStep * kStep;
+  while (!layout_fits(w, counters, data)) w += kStep;
+  return w;
+}
 
 // Everything one decode launch needs besides the four TMA descriptors.
 struct DecodeParams {

@@ -10,7 +10,6 @@ using namespace tkv;
 
 namespace {
 
-bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 inline int32_t cuda_status(cudaError_t e) { return e == cudaSuccess ? TKV_OK : TKV_ERR_CUDA; }
 
 bool block_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64; }
@@ -46,15 +45,6 @@ int32_t check_rotary(const tkv_rotary* r, int head_dim, bool any_token) {
     sum += r->sections[a];
   }
   return sum == r->rot_dim / 2 ? TKV_OK : TKV_ERR_INVALID;
-}
-
-// The decode workspace's convention: the error word in the first 256 bytes,
-// counters in the first eighth, data above.
-constexpr size_t kAlign = 256;
-inline size_t counter_reserve(size_t w) { return (w / 8) / kAlign * kAlign; }
-inline size_t data_base(size_t w) { return kAlign + counter_reserve(w); }
-inline bool fits(size_t w, size_t counters, size_t data) {
-  return counter_reserve(w) >= counters && data_base(w) + data <= w;
 }
 
 // SM count of the current device, looked up once per device.
@@ -189,12 +179,7 @@ int32_t tkv_kv8_attention_workspace(const tkv_kv8_cache* cache, const tkv_kv8_at
   size_t counters = 0, data = 0;
   kv8_attention_scratch(sms, cache->head_dim, a->heads / cache->kv_heads, a->max_q_len,
                         &counters, &data);
-  size_t w = 8 * ((counters + kAlign - 1) / kAlign * kAlign);
-  const size_t by_data = (data + 2 * kAlign) * 8 / 7 + 8 * kAlign;
-  if (by_data > w) w = by_data;
-  w = (w + 8 * kAlign - 1) / (8 * kAlign) * (8 * kAlign);
-  while (!fits(w, counters, data)) w += 8 * kAlign;
-  *workspace_bytes_out = w;
+  *workspace_bytes_out = required_workspace(counters, data);
   return TKV_OK;
 }
 
@@ -209,7 +194,7 @@ int32_t tkv_kv8_attention(const tkv_kv8_cache* cache, const tkv_kv8_attention_ar
   size_t counters = 0, data = 0;
   const int group = a->heads / cache->kv_heads;
   kv8_attention_scratch(sms, cache->head_dim, group, a->max_q_len, &counters, &data);
-  if (!a->workspace || !aligned(a->workspace, 256) || !fits(a->workspace_bytes, counters, data))
+  if (!a->workspace || !aligned(a->workspace, 256) || !layout_fits(a->workspace_bytes, counters, data))
     return TKV_ERR_WORKSPACE;
   uint8_t* ws = reinterpret_cast<uint8_t*>(a->workspace);
   AttnParams8 p;

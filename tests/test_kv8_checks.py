@@ -1,11 +1,20 @@
 """Checks of the 8-bit cache's front end that need no GPU: tensors are stand-ins
 with a device, a type and a shape, and nothing is launched."""
 
+import ctypes
+import os
+import re
+import struct
+import subprocess
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
+from paged_tierkv_b200 import _native as N  # noqa: E402
 from paged_tierkv_b200 import kv8  # noqa: E402
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 class FakeTensor:
@@ -120,3 +129,41 @@ def test_outputs_that_name_one_element_twice_are_refused(monkeypatch):
     one = FakeTensor(1, 1, 64, stride=(0, 0, 1), **half)
     with pytest.raises(AssertionError, match="launched"):
         kv8.rotary_embed(one, None, pos, rotary, q_out=one)
+
+
+def _leaves(struct_type, base=0):
+    """(offset, size) of every scalar of a ctypes structure, in order."""
+    for name, kind in struct_type._fields_:
+        at = base + getattr(struct_type, name).offset
+        if hasattr(kind, "_fields_"):
+            yield from _leaves(kind, at)
+        elif hasattr(kind, "_length_"):
+            yield from ((at + i * ctypes.sizeof(kind._type_), ctypes.sizeof(kind._type_)) for i in range(kind._length_))
+        else:
+            yield at, ctypes.sizeof(kind)
+
+
+def _packed(fmt):
+    """The same of a native struct format."""
+    codes = [c for n, c in re.findall(r"(\d*)([A-Za-z])", fmt) for _ in range(int(n or 1))]
+    for i, c in enumerate(codes):
+        if c != "x":
+            yield struct.calcsize("".join(codes[:i + 1])) - struct.calcsize(c), struct.calcsize(c)
+
+
+def test_packed_argument_blocks_have_the_structs_offsets():
+    for fmt, kind in ((kv8._ROTARY_ARGS, N.TkvRotaryArgs), (kv8._APPEND_ARGS, N.TkvKv8AppendArgs),
+                      (kv8._ATTENTION_ARGS, N.TkvKv8AttentionArgs), (kv8._PLAN_ARGS, N.TkvKv8PlanArgs)):
+        assert list(_packed(fmt.format)) == list(_leaves(kind)), kind
+
+
+def test_structs_have_the_headers_offsets(tmp_path):
+    pairs = (("tkv_kv8_cache", N.TkvKv8Cache), ("tkv_kv8_plan_args", N.TkvKv8PlanArgs), ("tkv_rotary", N.TkvRotary),
+             ("tkv_token_view", N.TkvTokenView), ("tkv_rotary_args", N.TkvRotaryArgs),
+             ("tkv_kv8_append_args", N.TkvKv8AppendArgs), ("tkv_kv8_attention_args", N.TkvKv8AttentionArgs))
+    checks = "".join(f"_Static_assert(sizeof({c}) == {ctypes.sizeof(k)}, \"{c}\");\n" for c, k in pairs)
+    checks += "".join(f"_Static_assert(offsetof({c}, {n}) == {getattr(k, n).offset}, \"{c}.{n}\");\n"
+                      for c, k in pairs for n, _ in k._fields_)
+    src = tmp_path / "offsets.c"
+    src.write_text('#include <stddef.h>\n#include "tierkv_b200.h"\n' + checks)
+    subprocess.run(["gcc", "-std=c11", "-fsyntax-only", "-I", os.path.join(ROOT, "include"), str(src)], check=True)
