@@ -514,7 +514,7 @@ def attention(q: torch.Tensor, cache: Kv8Cache, plan: StepPlan, scaling: float, 
             args = _ATTENTION_ARGS.pack(
                 *view, out.data_ptr(), 0 if lse is None else lse.data_ptr(), table.data_ptr(), stride,
                 plan.kv_lens.data_ptr(), plan.cu_q.data_ptr(), plan.requests, tokens, heads, code,
-                width, longest, int(window), scaling, ws.data_ptr(), ws.numel())
+                width, longest, min(int(window), 0x7fffffff), scaling, ws.data_ptr(), ws.numel())
             status = lib.tkv_kv8_attention(cache._ptr, args, st)
             if status != N.TKV_ERR_WORKSPACE or attempt:
                 return status

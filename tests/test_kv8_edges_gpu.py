@@ -339,3 +339,10 @@ def test_a_step_of_more_tokens_than_its_outputs_hold_is_reported(tokens, bits):
     kv8.plan_step(plan, _i32([0, 0]), _i32([20, 3]), torch.full((2, 4), -1, dtype=torch.int32, device="cuda"),
                   _i32(np.arange(9)), _i32([9]), tokens=tokens)
     assert _errors() == bits
+
+
+def test_a_window_past_an_int_is_no_window():
+    rng = np.random.default_rng(50)
+    scene = _scene(rng, [200], [3], 2, 1, 128, 16, "int8", "fp16")
+    a, b = _attend(scene, [200], 16, "int8", 0.1), _attend(scene, [200], 16, "int8", 0.1, 2 ** 40)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
