@@ -16,6 +16,9 @@ Every computation is one call into the C-ABI library (``tkv_kv8_*`` and
 (out-of-cache slots, exhausted free blocks, positions outside the cos / sin
 table) go to the stream's error word, ``ops.read_device_errors``.  The
 reference has no counterpart: its 8-bit blocks are filled by demotion only.
+
+These are serving operators without a backward pass: inputs that require a
+gradient are taken as they are, and no output carries one.
 """
 
 from __future__ import annotations

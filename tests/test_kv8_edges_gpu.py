@@ -346,3 +346,13 @@ def test_a_window_past_an_int_is_no_window():
     scene = _scene(rng, [200], [3], 2, 1, 128, 16, "int8", "fp16")
     a, b = _attend(scene, [200], 16, "int8", 0.1), _attend(scene, [200], 16, "int8", 0.1, 2 ** 40)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_inputs_that_require_a_gradient_give_outputs_without_one():
+    from paged_tierkv_b200 import kv8
+    rng = np.random.default_rng(51)
+    scene = _scene(rng, [40], [3], 2, 1, 64, 16, "int8", "fp16")
+    out, lse = _attend(scene, [40], 16, "int8", 0.1, q=scene[6].requires_grad_())
+    rotary = kv8.Rotary(torch.ones(4, 64, device="cuda"))
+    turned, _ = kv8.rotary_embed(scene[6], None, _i32([0, 1, 2]), rotary)
+    assert not (out.requires_grad or lse.requires_grad or turned.requires_grad)
