@@ -5,8 +5,9 @@
 // so they are packed into tiles of 8 * NT rows (NT 1 or 2) and every code is read once per
 // tile.  At few rows the kernel is bound by HBM: 2 head_dim bytes per token and
 // kv head against 4 head_dim rows flops.  32 x 32768 tokens, 8 kv heads of 128:
-// 378 us with int8 codes, 5.7 TB/s, whose expansion takes twice the
-// instructions of e4m3's: 334 us, 6.4 TB/s.
+// 389 us with int8 codes, 5.5 TB/s, whose expansion takes twice the
+// instructions of e4m3's: 334 us, 6.4 TB/s (from a graph, in runs of some 10 ms;
+// under the power limit of longer ones 416-442 and 360-373 us).
 //
 // Work is a flat list of steps -- 128 tokens (4 warps x 32) of one (request, kv
 // head, row tile) unit, units in order -- cut into one contiguous range per
@@ -27,9 +28,15 @@
 // Scales: K's multiplies the logits in fp32.  V's is folded into P, normalised
 // by a power of two (vinv) so that P stays in fp16's normal range for any
 // scale; queries in bf16 become fp16 through a power of two per row, which
-// only drops bits 2^-28 below the row's maximum.  fp16 P (11 bits) rounds 8
-// times finer than the bf16 of the usual fused kernels; sums, maxima and
-// accumulators are fp32.
+// only drops bits 2^-28 below the row's maximum.  P is rounded to fp16 (11 bits,
+// 8 times finer than the bf16 of the usual fused kernels).  Where that would show
+// beside the output's own rounding, with fp16 outputs, and the tile has idle
+// columns, at up to 4 rows, those take what the rounding left over, and the two
+// sums meet at the end of the unit: 22 bits without another MMA (error against 64
+// bits of the 32 x 32768 tokens 0.0002, that of the output's rounding, instead of
+// 0.0003; 389 us against 378 in short runs, the same under the power limit).  A
+// second product for tiles of more rows took 22 % longer at 16 rows and was left
+// out.  Sums, maxima and accumulators are fp32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -48,8 +55,8 @@ namespace tkv {
 // 128 rows still beats this kernel's 16-row instance for a batch of both (23
 // requests of up to 9001 tokens with 28 rows each: 49 us against 56, with 35: 49
 // against 78; chunks beside single tokens: 80 against 95), though not for 16 rows
-// alone (32 x 32768 tokens: 170 us against 300).  A 32-row instance took 594 us
-// there.
+// alone (32 requests of 4 tokens over 32768, 32 / 8 heads of 128: 577 us here
+// against 1071, with e4m3 codes 476 against 1032).
 // Small batches are the exception: up to 48 rows, and as long as the tables leave
 // every CTA at most 32 steps, all run here, which saves the second kernel and the
 // join (42 rows over 3000 tokens, 4 requests: 20 us against 31, 16 requests: 43
@@ -72,8 +79,9 @@ constexpr int kStepTok = kTileTok * kFewWarps;        // tokens of a step
 // 50; a 131071-token context the same; with up to 16 steps more, 16 requests of
 // 2048 tokens take 31 us against 24).
 constexpr int kBoundarySteps = 2;
-// Parts of a unit that one trip to L2 fetches when they are joined (a trip for
-// the maxima and one for every 8 parts: a 131071-token context 56.6 us, 52.7 so).
+// Parts of a unit that one trip to L2 fetches when they are joined, maxima and
+// accumulators together (a 131071-token context, 36 parts: 52.7 us; a first trip
+// for all maxima and then 8 accumulators a trip: 56.6).
 constexpr int kJoin = 12;
 
 template <int D, int NT>
@@ -346,6 +354,11 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     const int rows = min(RT, unit.q_len * p.group - unit.rt * RT);
     const int nact = (rows + 7) / 8;
     const int row0 = unit.rt * RT;       // first row of the tile within the request
+    // Up to 4 rows leave half of the tile's columns idle: columns 4-7 repeat rows
+    // 0-3, and take what the rounding of P to fp16 leaves over in columns 0-3.
+    const bool twin = NT == 1 && !bf16 && rows <= 4;
+    const float rest = t4 >= 2 ? -1.f : 0.f;
+    const auto row_of = [&](int r) { return twin ? r & 3 : r; };
     // the rows' queries as fp16, and their logit scales
     for (int r = warp; r < RT; r += kFewWarps) {
       constexpr int E = D / 64;            // words per lane
@@ -353,8 +366,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
       float amax = 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) x[i] = make_float2(0.f, 0.f);
-      if (r < rows) {
-        const int tok = unit.q0 + (row0 + r) / p.group, h = unit.head * p.group + (row0 + r) % p.group;
+      if (row_of(r) < rows) {
+        const int row = row0 + row_of(r);
+        const int tok = unit.q0 + row / p.group, h = unit.head * p.group + row % p.group;
         const uint32_t* src = reinterpret_cast<const uint32_t*>(
             (const uint16_t*)p.q.data + tok * p.q.token_stride + h * p.q.head_stride);
 #pragma unroll
@@ -389,7 +403,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
       for (int c = 0; c < 2; ++c) {
         const int r = n * 8 + 2 * t4 + c;
         rs[n][c] = rscale_s[r];
-        limit[n][c] = unit.kv - unit.q_len + (row0 + min(r, rows - 1)) / p.group + 1;
+        limit[n][c] = unit.kv - unit.q_len + (row0 + min(row_of(r), rows - 1)) / p.group + 1;
       }
     // every row sees keys [all_lo, all_hi)
     const int all_hi = unit.kv - unit.q_len + row0 / p.group + 1;
@@ -535,8 +549,14 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
               e[x] = w * vn[h * kBoxes / 2];
               if (edge && sc[n][h][x] == -INFINITY) e[x] = 0.f;   // also under a NaN scale
             }
-            pb[n][h][0] = movmatrix_t(pack_half2(e[0], e[1]));
-            pb[n][h][1] = movmatrix_t(pack_half2(e[2], e[3]));
+            uint32_t p0 = pack_half2(e[0], e[1]), p1 = pack_half2(e[2], e[3]);
+            if (twin) {
+              const float2 r0 = unpack_in(false, p0), r1 = unpack_in(false, p1);
+              p0 = pack_half2(fmaf(rest, r0.x, e[0]), fmaf(rest, r0.y, e[1]));
+              p1 = pack_half2(fmaf(rest, r1.x, e[2]), fmaf(rest, r1.y, e[3]));
+            }
+            pb[n][h][0] = movmatrix_t(p0);
+            pb[n][h][1] = movmatrix_t(p1);
           }
         }
         // O^T += V^T P^T: lane (g, t4) owns head_dim elements [g D / 8, (g + 1) D / 8)
@@ -580,6 +600,12 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtasPerSm)
     }
 
     // ---- the CTA's share of the unit: merge the warps' statistics and accumulators
+    if (twin) {
+#pragma unroll
+      for (int u = 0; u < D / 16; ++u)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[0][u][x] += __shfl_xor_sync(~0u, acc[0][u][x], 2);
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -9,7 +9,8 @@
 // the fp16 P_i of 64 tokens overwriting the first half of their S_i and feeding
 // the MMA from there.
 // While the tensor core works for one query tile the other one's softmax runs.
-// A prompt of 8192 tokens, 32 / 8 heads of 128: 679 us, 810 TFLOP/s.  Bound by
+// A prompt of 8192 tokens, 32 / 8 heads of 128: 675 us, 814 TFLOP/s (from a
+// graph, in runs of some 10 ms; 696-708 us under the power limit).  Bound by
 // shared memory, which the MMAs of S alone read at its full bandwidth and the
 // expansion writes, and by the tensor-memory reads of the softmax.
 //

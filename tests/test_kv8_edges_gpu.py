@@ -356,3 +356,25 @@ def test_inputs_that_require_a_gradient_give_outputs_without_one():
     rotary = kv8.Rotary(torch.ones(4, 64, device="cuda"))
     turned, _ = kv8.rotary_embed(scene[6], None, _i32([0, 1, 2]), rotary)
     assert not (out.requires_grad or lse.requires_grad or turned.requires_grad)
+
+
+# ---------------------------------------------------------------------------
+# precision
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("group,ql", [(4, 1), (3, 1), (1, 4), (2, 2), (1, 1)])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("d,bs", [(128, 16), (64, 32)])
+def test_up_to_four_rows_keep_what_fp16_drops_of_p(group, ql, fmt, d, bs):
+    """fp16 queries with up to 4 rows a kv head: P counts with two fp16 numbers,
+    2^-21 of it instead of 2^-11 in the bound of the other tests."""
+    kv = [700, 40, 3000]
+    rng = np.random.default_rng(60 + group)
+    scene = _scene(rng, kv, [ql] * 3, 2 * group, 2, d, bs, fmt, "fp16")
+    kc, ks, vc, vs, table, cu, q = scene
+    out, _ = _attend(scene, kv, bs, fmt, d ** -0.5, max_q_len=ql)
+    ref, _, mass, size = kv8o.attention(q.double().cpu().numpy(), kc, vc, ks, vs, table, kv, cu, d ** -0.5, fmt)
+    eps = 2.0 ** -11
+    tol = mass * (2.0 ** -21 + 2.0 ** -17 * size[..., None] + 2.0 ** -18) * (1 + eps) + eps * np.abs(ref) + 2.0 ** -25
+    err = np.abs(out.double().cpu().numpy() - ref)
+    assert np.all(err <= tol), (np.nanmax(err / tol), np.argwhere(~(err <= tol))[:3])
