@@ -23,8 +23,8 @@ namespace tkv {
 // cells and write units and find each one's request by bisection of the
 // scanned sums.  A cluster barrier between the last read of an input and the
 // first write lets kv_lens / free_count be updated in place.  Latency bound:
-// a launch, one round of loads, two block scans (64 requests of one token: 4.3
-// us; 1024 requests with 130000 tokens: 9.9 us for 1.7 MB of outputs).
+// a launch, one round of loads, two block scans (64 requests of one token: 4.5
+// us; 1024 requests with 130000 tokens: 10.1 us for 1.7 MB of outputs).
 // Small steps (up to 1024 requests, tokens and write units) take one CTA of 256
 // threads, whose barriers are cheaper than the cluster's; others 16 of 1024, the
 // largest cluster there is (8: 13.3 us for those 130000 tokens, 16 of 512: 10.8;
