@@ -557,7 +557,8 @@ typedef struct tkv_kv8_attention_args {
     int32_t        heads;           /* a multiple of the cache's kv_heads, up to 64 each */
     int32_t        dtype;           /* TKV_DTYPE_F16 / BF16 */
     int32_t        table_width;     /* cells of a row */
-    int32_t        max_q_len;       /* upper bound of the requests' query tokens */
+    int32_t        max_q_len;       /* upper bound of the requests' query tokens; a lower
+                                       number costs time only */
     int32_t        window;          /* 0 = none; 2^30 and more hide nothing either */
     float          scaling;         /* finite, > 0 */
     void*          workspace;       /* as tkv_decode_args.workspace */

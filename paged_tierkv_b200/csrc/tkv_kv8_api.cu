@@ -187,7 +187,7 @@ int32_t tkv_kv8_attention(const tkv_kv8_cache* cache, const tkv_kv8_attention_ar
   int32_t st = check_attention(cache, a);
   if (st != TKV_OK) return st;
   if (!a->kv_lens || !a->cu_q || (a->table_width > 0 && !a->block_table)) return TKV_ERR_INVALID;
-  if (a->tokens == 0 || a->max_q_len == 0) return TKV_OK;
+  if (a->tokens == 0) return TKV_OK;
   if (check_view(a->q) != TKV_OK || !a->out || !aligned(a->out, 16)) return TKV_ERR_INVALID;
   int sms = 0;
   if ((st = device_sms(&sms)) != TKV_OK) return st;

@@ -378,3 +378,12 @@ def test_up_to_four_rows_keep_what_fp16_drops_of_p(group, ql, fmt, d, bs):
     tol = mass * (2.0 ** -21 + 2.0 ** -17 * size[..., None] + 2.0 ** -18) * (1 + eps) + eps * np.abs(ref) + 2.0 ** -25
     err = np.abs(out.double().cpu().numpy() - ref)
     assert np.all(err <= tol), (np.nanmax(err / tol), np.argwhere(~(err <= tol))[:3])
+
+
+@pytest.mark.parametrize("ql", [[1] * 3, [60, 1, 45]])
+def test_a_bound_of_zero_query_tokens_costs_time_only(ql):
+    kv = [100, 7, 64]
+    rng = np.random.default_rng(70)
+    scene = _scene(rng, kv, ql, 4, 2, 64, 16, "int8", "fp16")
+    out = torch.full(scene[6].shape, 9.0, dtype=torch.float16, device="cuda")
+    _check_attention(scene, kv, 16, "int8", "fp16", 0.125, max_q_len=0, out=out)
